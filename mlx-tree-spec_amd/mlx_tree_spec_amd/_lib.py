@@ -26,10 +26,12 @@ QMM4_EPILOGUE_SILU_MUL = 1
 # Size of qmm4_affine_bf16_noalloc's static device array per GPU (QMM4_NOALLOC_SCRATCH_BYTES).
 QMM4_NOALLOC_SCRATCH_BYTES = 136 * 1024 * 1024
 
-# name -> (restype, argtypes); the symbols include/qmm4.h and include/qmm_general.h declare.
+# name -> (restype, argtypes); the symbols that the headers in include/ declare.
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
+_i32 = ctypes.c_int32
+_f32 = ctypes.c_float
 SIGNATURES = {
     "qmm4_affine_bf16": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _int, _vp]),
     "qmm4_affine_bf16_noalloc": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _int, _vp]),
@@ -39,6 +41,14 @@ SIGNATURES = {
     "qmm4_add_rms_norm_qmm_bf16": (_int, [_vp, _vp, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _vp,
                                           _i64, _i64, _i64, _int, _int, _int, _int, _vp]),
     "qmm_affine_general_bf16": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp]),
+    "qmm4_lora_workspace": (_i64, [_i64, _i64]),
+    "qmm4_lora_add_bf16": (_int, [_vp] * 5 + [_int, _vp, _vp] + [_i64] * 5 + [_vp]),
+    "qmm4_affine_lora_bf16": (_int, [_vp] * 8 + [_int, _vp, _vp] + [_i64] * 5 + [_int, _int, _int, _vp]),
+    "qmm4_qk_norm_rope_bf16": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _f32, _vp, _int, _vp, _int, _vp, _vp]
+                               + [_i64] * 5 + [_int, _vp]),
+    "qmm4_sample_workspace": (_i64, [_i64, _i64]),
+    "qmm4_sample_bf16": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _f32, _vp, _i32, _vp, _f32, _vp, _f32, _vp, _vp, _vp,
+                                _vp]),
     "qmm4_last_error": (ctypes.c_char_p, []),
     "qmm4_abi_version": (_int, []),
 }
