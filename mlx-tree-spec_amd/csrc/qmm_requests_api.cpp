@@ -67,6 +67,24 @@ int run_lora(const qmm4::LoraTables& lora, const void* x, void* y, void* workspa
   return QMM4_OK;
 }
 
+int check_sample_shape(int64_t M, int64_t V) {
+  if (M < 0 || M > (1LL << 20) || V < 1 || V > QMM4_SAMPLE_MAX_VOCAB)
+    return set_error(QMM4_ERR_INVALID, "invalid shape M=%lld V=%lld (at most 2^20 rows, 1 to %d tokens)", (long long)M,
+                     (long long)V, QMM4_SAMPLE_MAX_VOCAB);
+  return QMM4_OK;
+}
+
+int current_cus(int* cus) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return hip_error(e, "hipGetDevice");
+  std::lock_guard<std::mutex> lock(qmm4::api_mutex());
+  qmm4::DeviceInfo* di = nullptr;
+  if (int rc = qmm4::device_info(dev, &di)) return rc;
+  *cus = qmm4::device_cus(di);
+  return QMM4_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -139,16 +157,24 @@ int qmm4_qk_norm_rope_bf16(const void* q, int64_t q_row, int64_t q_head, const v
   });
 }
 
-int64_t qmm4_sample_workspace(int64_t M, int64_t V) { return qmm4::sample_workspace(M, V); }
+int64_t qmm4_sample_workspace(int64_t M, int64_t V) {
+  int64_t bytes = 0;
+  const int rc = guarded([&] {
+    if (int bad = check_sample_shape(M, V)) return bad;
+    int cus = 0;
+    if (int bad = current_cus(&cus)) return bad;
+    bytes = qmm4::sample_workspace(M, V, cus);
+    return (int)QMM4_OK;
+  });
+  return rc ? rc : bytes;
+}
 
 int qmm4_sample_bf16(const void* logits, int64_t M, int64_t V, int64_t row_stride, const float* uniform,
                      const float* temperature, float temperature_value, const int32_t* top_k, int32_t top_k_value,
                      const float* top_p, float top_p_value, const float* min_p, float min_p_value, int64_t* tokens,
                      float* logprobs, void* workspace, void* hip_stream) {
   return guarded([&] {
-    if (M < 0 || M > (1LL << 20) || V < 1 || V > QMM4_SAMPLE_MAX_VOCAB)
-      return set_error(QMM4_ERR_INVALID, "invalid shape M=%lld V=%lld (at most 2^20 rows, 1 to %d tokens)", (long long)M,
-                       (long long)V, QMM4_SAMPLE_MAX_VOCAB);
+    if (int rc = check_sample_shape(M, V)) return rc;
     if (M > 1 && row_stride < V)
       return set_error(QMM4_ERR_INVALID, "row_stride=%lld is less than V=%lld", (long long)row_stride, (long long)V);
     if (M == 0) return (int)QMM4_OK;
@@ -159,7 +185,9 @@ int qmm4_sample_bf16(const void* logits, int64_t M, int64_t V, int64_t row_strid
     const qmm4::SampleParams p{static_cast<const uint16_t*>(logits), row_stride, uniform,
                                {temperature, temperature_value}, {top_p, top_p_value}, {min_p, min_p_value},
                                {top_k, top_k_value}, tokens, logprobs, (int)V};
-    hipError_t e = qmm4::launch_sample(p, M, workspace, static_cast<hipStream_t>(hip_stream));
+    int cus = 0;
+    if (int rc = current_cus(&cus)) return rc;
+    hipError_t e = qmm4::launch_sample(p, M, workspace, cus, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return hip_error(e, "sampling kernel launch");
     return (int)QMM4_OK;
   });

@@ -65,7 +65,8 @@ struct SampleParams {
   float* logprobs;
   int V;
 };
-int64_t sample_workspace(int64_t M, int64_t V);
-hipError_t launch_sample(const SampleParams& p, int64_t M, void* workspace, hipStream_t stream);
+// The workspace for M rows on a GPU of `cus` CUs, in bytes.
+int64_t sample_workspace(int64_t M, int64_t V, int cus);
+hipError_t launch_sample(const SampleParams& p, int64_t M, void* workspace, int cus, hipStream_t stream);
 
 }  // namespace qmm4

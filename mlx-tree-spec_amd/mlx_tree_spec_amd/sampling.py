@@ -69,9 +69,11 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0
     tokens = torch.empty(lead, dtype=torch.int64, device=dev)
     logprobs = torch.empty(lead, dtype=torch.float32, device=dev)
     lib = _lib.load()
-    workspace = torch.empty(lib.qmm4_sample_workspace(m, v), dtype=torch.uint8, device=dev)
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     with torch.cuda.device(dev):
+        size = lib.qmm4_sample_workspace(m, v)
+        _lib.check(min(size, 0), what)
+        workspace = torch.empty(size, dtype=torch.uint8, device=dev)
         stream = torch.cuda.current_stream(dev).cuda_stream
         rc = lib.qmm4_sample_bf16(rows.data_ptr(), m, v, rows.stride(0), uniform.data_ptr(), ptr(temps), float(temp),
                                   ptr(ks), min(int(k), 2**31 - 1), ptr(ps), float(p), ptr(mins), float(mn),
