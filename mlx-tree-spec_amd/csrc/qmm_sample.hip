@@ -13,9 +13,16 @@
 //   pick    one workgroup per row: the slices' lists added into one histogram (32-bit counts) over the range of
 //           values that occur, then the sums over it; the slice that holds the occurrence is found in the lists
 //           again, and only that slice is read.
-// Up to 65535 logits one pick kernel counts its row itself. The sums go over blocks of the histogram, one per wave
-// and turn (neighbouring blocks on different waves: the values that occur lie close together): a block's count
-// and masses, a prefix over the blocks, then only the two blocks with the borders value by value.
+// Up to 65535 logits one pick kernel counts its row itself.
+//
+// The sums run over the values that occur, up to 4096 of them (a page) listed in LDS, 4 neighbours to a thread: a
+// prefix over the workgroup gives the count before each thread, its counts within top-k, their masses; another the
+// mass before it, what top-p and min-p keep of it; a third the kept mass before it, and with it the value that
+// passes the target. More values (152k logits of a model have about 3500; past 4096 they lie many octaves apart)
+// take their pages in turn, once per sum.
+//
+// What bounds it: a row's steps follow each other in one workgroup, and its 16 waves get through about 150
+// instructions each a microsecond; the steps are kept to few instructions per value and wave.
 #include "qmm4_common.h"
 #include "qmm4_lds.h"
 #include "qmm_requests_kernels.h"
@@ -32,90 +39,138 @@ constexpr int kMinSlice = 4096;
 constexpr int kMaxSlices = 512;
 constexpr int kMaxBatch = 256;     // rows per launch: bounds the workspace
 
-// Rank of a bf16 value in falling order (0: +infinity, -0 equal to +0), or -1 for -infinity and NaN.
+// Rank of a bf16 value in falling order (0: +infinity, -0 equal to +0); outside 0 .. kValues - 1 for -infinity and
+// NaN.
 __device__ __forceinline__ int rank_of(uint32_t b) {
   const int mag = (int)(b & 0x7FFFu);
-  const int r = (b & 0x8000u) && mag != 0 ? 0x7F80 + mag : 0x7F80 - mag;
-  return mag > 0x7F80 || b == 0xFF80u ? -1 : r;
+  return 0x7F80 + (b & 0x8000u ? mag : -mag);
 }
 __device__ __forceinline__ double value_of(int rank) {
   return (double)bf16_to_f32(rank <= 0x7F80 ? 0x7F80 - rank : 0x8000 | (rank - 0x7F80));
 }
 
-// Logits [begin, end) of a row in groups of 8 within 16-byte lines: group 0 up to the first line's start, the last
-// one up to the end (single loads), whole lines between. Places outside hold -infinity.
-struct Groups {
+// Logits [begin, end) of a row: whole 16-byte lines of 8 (line g from index first(g)), and up to 7 logits either side
+// of them, which `edge` holds for threads 0 .. 15 in index order around the lines. Places outside hold -infinity.
+constexpr uint32_t kNone = 0xFF80u;
+struct Lines {
   const uint16_t* row;
   int begin, end, line0, count;
-  __device__ Groups(const uint16_t* r, int b, int e) : row(r), begin(b), end(e) {
+  __device__ Lines(const uint16_t* r, int b, int e) : row(r), begin(b), end(e) {
     const int past = (int)((reinterpret_cast<uintptr_t>(r + b) >> 1) & 7);
-    line0 = b + (past ? 8 - past : 0);
-    count = e > line0 ? 1 + (e - line0 + 7) / 8 : 1;
+    line0 = min(e, b + (past ? 8 - past : 0));
+    count = (e - line0) / 8;
   }
-  __device__ int first(int g) const { return line0 + (g - 1) * 8; }  // index of the group's place 0
+  __device__ int first(int g) const { return line0 + g * 8; }
+  // Lines past the last are loads of the last one, made -infinity: no branch keeps loads apart.
   __device__ u32x4 load(int g) const {
-    const int i0 = first(g);
-    if (g > 0 && i0 + 8 <= end) return *reinterpret_cast<const u32x4*>(row + i0);
-    u32x4 v;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = i0 + e;
-      const uint32_t b = i >= begin && i < end ? row[i] : 0xFF80u;
-      if (e & 1) v[e / 2] |= b << 16;
-      else v[e / 2] = b;
-    }
-    return v;
+    const u32x4 none = {kNone << 16 | kNone, kNone << 16 | kNone, kNone << 16 | kNone, kNone << 16 | kNone};
+    if (count == 0) return none;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(row + first(min(g, count - 1)));
+    return g < count ? v : none;
   }
+  __device__ int edge_index(int t) const { return t < 8 ? begin + t : first(count) + t - 8; }
+  __device__ bool has_edge(int t) const { return t < 8 ? begin + t < line0 : t < 16 && first(count) + t - 8 < end; }
+  __device__ uint32_t edge(int t) const { return has_edge(t) ? row[edge_index(t)] : kNone; }
 };
 __device__ __forceinline__ uint32_t place(u32x4 v, int e) { return e & 1 ? v[e / 2] >> 16 : v[e / 2] & 0xFFFFu; }
 
-// Inclusive prefix over the 64 lanes.
+// v of the lane that the DPP control names, 0 where there is none or its row is masked out.
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T dpp(T v) {
+  if constexpr (sizeof(T) == 8) {
+    const u32x2 p = __builtin_bit_cast(u32x2, v);
+    return __builtin_bit_cast(T, u32x2{dpp<CTRL, ROWS>(p.x), dpp<CTRL, ROWS>(p.y)});
+  } else {
+    return (T)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+  }
+}
+template <class T>
+__device__ __forceinline__ T lane_value(T v, int lane) {  // lane: the same in all lanes
+  if constexpr (sizeof(T) == 8) {
+    const u32x2 p = __builtin_bit_cast(u32x2, v);
+    return __builtin_bit_cast(T, u32x2{lane_value(p.x, lane), lane_value(p.y, lane)});
+  } else {
+    return (T)__builtin_amdgcn_readlane((int)v, lane);
+  }
+}
+// Inclusive prefix over the 64 lanes: within rows of 16 by shifts of 1, 2, 4 and 8 lanes, then the last lane of rows
+// 0 and 2 to the row behind, and of the first half to the second. (Register moves: the same through LDS permutes
+// cost 6 round trips of about 50 ns each, a tenth of the pick kernel.)
 template <class T>
 __device__ __forceinline__ T wave_prefix(T v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const T o = __shfl_up(v, off);
-    if (lane >= off) v += o;
-  }
+  v += dpp<0x111, 0xF>(v);
+  v += dpp<0x112, 0xF>(v);
+  v += dpp<0x114, 0xF>(v);
+  v += dpp<0x118, 0xF>(v);
+  v += dpp<0x142, 0xA>(v);
+  v += dpp<0x143, 0xC>(v);
+  return v;
+}
+// Over the first 16 lanes (of other lanes: anything).
+template <class T>
+__device__ __forceinline__ T row_prefix(T v) {
+  v += dpp<0x111, 0xF>(v);
+  v += dpp<0x112, 0xF>(v);
+  v += dpp<0x114, 0xF>(v);
+  v += dpp<0x118, 0xF>(v);
   return v;
 }
 template <class T>
-__device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-  return v;
+__device__ __forceinline__ T wave_sum(T v) { return lane_value(wave_prefix(v), 63); }
+// The largest of values >= -1 over the first 16 lanes, or all.
+__device__ __forceinline__ int row_max(int v) {
+  v += 1;  // (a DPP without a source lane gives 0)
+  v = max(v, dpp<0x111, 0xF>(v));
+  v = max(v, dpp<0x112, 0xF>(v));
+  v = max(v, dpp<0x114, 0xF>(v));
+  v = max(v, dpp<0x118, 0xF>(v));
+  return lane_value(v, 15) - 1;
 }
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = min(v, __shfl_xor(v, off));
-  return v;
+__device__ __forceinline__ int wave_max(int v) {
+  v += 1;
+  v = max(v, dpp<0x111, 0xF>(v));
+  v = max(v, dpp<0x112, 0xF>(v));
+  v = max(v, dpp<0x114, 0xF>(v));
+  v = max(v, dpp<0x118, 0xF>(v));
+  v = max(v, dpp<0x142, 0xA>(v));
+  v = max(v, dpp<0x143, 0xC>(v));
+  return lane_value(v, 63) - 1;
 }
-__device__ __forceinline__ int wave_max(int v) { return -wave_min(-v); }
+// The smallest of values up to kValues.
+__device__ __forceinline__ int row_min(int v) { return kValues - row_max(kValues - v); }
+__device__ __forceinline__ int wave_min(int v) { return kValues - wave_max(kValues - v); }
 
-// 16-bit counts of the logits in groups, two to a word; returns the smallest rank this thread saw.
-__device__ __forceinline__ int count_groups(const Groups& G, uint32_t* hist) {
+// 16-bit counts of the logits, two to a word; returns the smallest rank this thread saw. `held`: the lines loaded
+// last (lines threadIdx.x + i kThreads where there are at most kBatch * kThreads of them). `between` runs while the
+// first loads are under way.
+constexpr int kBatch = 4;
+template <class F>
+__device__ __forceinline__ int count_lines(const Lines& G, uint32_t* hist, u32x4 (&held)[kBatch], F&& between) {
   int lowest = kValues;
-  constexpr int kBatch = 4;
-  for (int g0 = threadIdx.x; g0 < G.count; g0 += kBatch * kThreads) {
-    u32x4 v[kBatch];
+  auto count = [&](uint32_t b) {  // -infinity and NaN go to bins past the values, one for each lane
+    int r = rank_of(b);
+    r = (uint32_t)r < (uint32_t)kValues ? r : kValues + (int)(threadIdx.x & 63);
+    atomicAdd(&hist[r >> 1], r & 1 ? 0x10000u : 1u);
+    lowest = min(lowest, r);
+  };
+  const uint32_t edge = G.edge(threadIdx.x);
+  for (int g0 = threadIdx.x, at = 0; at < max(G.count, 1); g0 += kBatch * kThreads, at += kBatch * kThreads) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int g = g0 + i * kThreads;
-      v[i] = g < G.count ? G.load(g) : u32x4{0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u};
+    for (int i = 0; i < kBatch; ++i) held[i] = G.load(g0 + i * kThreads);
+    if (at == 0) {
+      __builtin_amdgcn_sched_barrier(0);
+      between();
+      count(edge);
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
+      if (at + i * kThreads >= G.count) break;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int r = rank_of(place(v[i], e));
-        if (r >= 0) {
-          atomicAdd(&hist[r >> 1], r & 1 ? 0x10000u : 1u);
-          lowest = min(lowest, r);
-        }
-      }
+      for (int e = 0; e < 8; ++e) count(place(held[i], e));
     }
   }
+  __syncthreads();
+  if (threadIdx.x < 32) hist[kValues / 2 + threadIdx.x] = 0;
   return lowest;
 }
 
@@ -136,49 +191,44 @@ struct Lists {
 constexpr int kBytes16 = 65536 * 2;
 
 __global__ __launch_bounds__(kThreads) void sample_count_kernel(SampleParams S, Lists L) {
-  extern __shared__ uint32_t hist[];
+  extern __shared__ __attribute__((aligned(16))) uint32_t hist[];
   __shared__ uint32_t s_n[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t m = blockIdx.y;
   const int begin = blockIdx.x * L.slice, end = min(S.V, begin + L.slice);
-  zero_lds<kBytes16>(hist);
+  u32x4 held[kBatch];
+  count_lines(Lines(S.logits + m * S.row_stride, begin, end), hist, held, [&] {
+    zero_lds<kBytes16>(hist);
+    __syncthreads();
+  });
   __syncthreads();
-  count_groups(Groups(S.logits + m * S.row_stride, begin, end), hist);
-  __syncthreads();
-  // Each wave lists 4096 neighbouring values, 8 to a lane and turn.
-  constexpr int kTurns = 8;
-  const u32x4* h = reinterpret_cast<const u32x4*>(hist) + wave * (kTurns * 64);
-  uint32_t mine = 0;
-  for (int t = 0; t < kTurns; ++t) {
-    const u32x4 v = h[t * 64 + lane];
+  // Each wave lists 4096 neighbouring values, 64 words of two at a time: a comparison is a mask of the lanes, and a
+  // lane's place in the list the number of values below it.
+  constexpr int kLooks = 32;
+  const uint32_t* h = hist + wave * (kLooks * 64) + lane;
+  uint32_t mine = 0, looks = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) mine += place(v, e) != 0;
+  for (int t = 0; t < kLooks; ++t) {
+    const uint32_t v = h[t * 64];
+    const int seen = __popcll(__ballot((v & 0xFFFFu) != 0)) + __popcll(__ballot(v > 0xFFFFu));
+    mine += seen;
+    looks |= seen != 0 ? 1u << t : 0;
   }
-  mine = wave_sum(mine);
   if (lane == 0) s_n[wave] = mine;
   __syncthreads();
-  uint32_t at = 0, total = 0;
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    if (i == wave) at = total;
-    total += s_n[i];
-  }
+  const uint32_t waves = row_prefix(s_n[lane & 15]), total = lane_value(waves, 15);
+  uint32_t at = wave ? lane_value(waves, wave - 1) : 0u;
   uint32_t* list = L.list(m, blockIdx.x);
-  for (int t = 0; t < kTurns; ++t) {
-    const u32x4 v = h[t * 64 + lane];
-    uint32_t c = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) c += place(v, e) != 0;
-    if (__ballot(c != 0) == 0) continue;
-    const uint32_t inc = wave_prefix(c);
-    uint32_t o = at + inc - c;
-    const uint32_t rank = (uint32_t)((wave * kTurns + t) * 512 + lane * 8);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t n = place(v, e);
-      if (n != 0) list[o++] = (rank + e) << 16 | n;
-    }
-    at += __shfl(inc, 63);
+  for (; looks != 0; looks &= looks - 1) {
+    const int t = __ffs((int)looks) - 1;
+    const uint32_t v = h[t * 64];
+    const unsigned long long lo = __ballot((v & 0xFFFFu) != 0), hi = __ballot(v > 0xFFFFu);
+    uint32_t o = __builtin_amdgcn_mbcnt_hi((uint32_t)(lo >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lo, at));
+    o = __builtin_amdgcn_mbcnt_hi((uint32_t)(hi >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hi, o));
+    const uint32_t r = (uint32_t)((wave * kLooks + t) * 64 + lane) * 2;
+    if ((v & 0xFFFFu) != 0) list[o++] = r << 16 | (v & 0xFFFFu);
+    if (v > 0xFFFFu) list[o] = (r + 1) << 16 | v >> 16;
+    at += __popcll(lo) + __popcll(hi);
   }
   if (tid == 0) L.n[m * L.slices + blockIdx.x] = total;
   if (tid < 4 && (total & 3) != 0 && tid >= (int)(total & 3)) list[(total & ~3u) + tid] = 0;
@@ -187,24 +237,21 @@ __global__ __launch_bounds__(kThreads) void sample_count_kernel(SampleParams S, 
 // One row. MERGE: from the slices' lists, else from the row itself.
 template <bool MERGE>
 __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams S, Lists L) {
-  constexpr int kPerLane = MERGE ? 4 : 8;        // values of a block to a lane (16 bytes of the histogram)
-  constexpr int kBlock = 64 * kPerLane;
-  constexpr int kTurns = MERGE ? 9 : 8;          // blocks of each wave
-  constexpr int kBlocks = kTurns * kWaves;
-  constexpr int kSpan = kBlocks * kBlock;        // values of one histogram: 36864, or all 65536
-  constexpr int kParts = MERGE ? 2 : 1;          // histograms that cover the values
-  constexpr int kPerScan = (kParts * kBlocks + 63) / 64;
-  extern __shared__ uint32_t hist[];
-  __shared__ uint32_t s_count[kPerScan * 64], s_before[kPerScan * 64];
-  __shared__ double s_mass[kPerScan * 64], s_kept[kPerScan * 64];
+  constexpr int kSpan = MERGE ? 36 * kThreads : 65536;  // values of one histogram: +-512 with all between, or all
+  constexpr int kPer = 4;                         // listed values of a page to a thread
+  constexpr int kPage = kPer * kThreads;
+  extern __shared__ __attribute__((aligned(16))) uint32_t hist[];
+  __shared__ uint16_t s_page[kPage];
   __shared__ int s_lo[kWaves], s_hi[kWaves];
-  __shared__ uint32_t s_u[kWaves], s_occ[MERGE ? kMaxSlices : 1];
+  __shared__ double s_d[2][kWaves];
+  __shared__ uint32_t s_u[kBatch][kWaves], s_n[MERGE ? kMaxSlices : 1], s_occ[MERGE ? kMaxSlices : 1];
+  __shared__ uint32_t s_hit[2];
+  __shared__ double s_weight;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t m = blockIdx.x;
   const uint16_t* row = S.logits + m * S.row_stride;
 
-  float temp = S.temperature[m];
-  float top_p = S.top_p[m], min_p = S.min_p[m];
+  float temp = S.temperature[m], top_p = S.top_p[m], min_p = S.min_p[m];
   const float u = S.uniform[m];
   const int32_t top_k = S.top_k[m];
   // Settings that leave the first of the order only: as top-k 1.
@@ -215,45 +262,15 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams S, L
     min_p = 0.0f;
   }
 
-  for (int i = tid; i < kPerScan * 64; i += kThreads) {
-    s_count[i] = 0;
-    s_mass[i] = s_kept[i] = 0.0;
-  }
-  // The histogram of values base + part * kSpan ..; `lowest`: the first value that occurs, parts: histograms
-  // that the values which occur span.
-  int base = 0, lowest, parts = 1;
-  auto build = [&](int part) {
-    if constexpr (MERGE) {
-      __syncthreads();
-      zero_lds<kSpan * 4>(hist);
-      __syncthreads();
-      const int from = base + part * kSpan;
-      for (int s = wave; s < L.slices; s += kWaves) {
-        const int n4 = ((int)L.n[m * L.slices + s] + 3) / 4;
-        const u32x4* list = reinterpret_cast<const u32x4*>(L.list(m, s));
-        constexpr int kBatch = 8;
-        for (int i0 = lane; i0 < n4; i0 += kBatch * 64) {
-          u32x4 v[kBatch];
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) v[i] = i0 + i * 64 < n4 ? list[i0 + i * 64] : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = (int)(v[i][e] >> 16) - from;
-              if (r >= 0 && r < kSpan && (v[i][e] & 0xFFFFu) != 0) atomicAdd(&hist[r], v[i][e] & 0xFFFFu);
-            }
-          }
-        }
-      }
-      __syncthreads();
-    }
-  };
-  int last = -1;
+  // `lowest`: the first value that occurs. The histogram holds values from `base`; a second one (part 1) those past
+  // its end, where there are any.
+  int lowest = kValues, base = 0, parts = 1;
+  u32x4 held[kBatch];
   if constexpr (MERGE) {
     int lo = kValues, hi = -1;
     for (int s = tid; s < L.slices; s += kThreads) {
       const uint32_t n = L.n[m * L.slices + s];
+      s_n[s] = n;
       if (n == 0) continue;
       const uint32_t* list = L.list(m, s);
       lo = min(lo, (int)(list[0] >> 16));
@@ -266,21 +283,17 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams S, L
       s_hi[wave] = hi;
     }
     __syncthreads();
-    lowest = kValues;
-    for (int i = 0; i < kWaves; ++i) {
-      lowest = min(lowest, s_lo[i]);
-      last = max(last, s_hi[i]);
-    }
+    lowest = row_min(s_lo[lane & 15]);
     base = lowest & ~3;
-    parts = last - base >= kSpan ? 2 : 1;
+    parts = row_max(s_hi[lane & 15]) - base >= kSpan ? 2 : 1;
   } else {
-    zero_lds<kBytes16>(hist);
-    __syncthreads();
-    const int lo = wave_min(count_groups(Groups(row, 0, S.V), hist));
+    const int lo = wave_min(count_lines(Lines(row, 0, S.V), hist, held, [&] {
+      zero_lds<kBytes16>(hist);
+      __syncthreads();
+    }));
     if (lane == 0) s_lo[wave] = lo;
     __syncthreads();
-    lowest = kValues;
-    for (int i = 0; i < kWaves; ++i) lowest = min(lowest, s_lo[i]);
+    lowest = row_min(s_lo[lane & 15]);
   }
   if (lowest == kValues) {
     if (tid == 0) {
@@ -289,204 +302,210 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams S, L
     }
     return;
   }
+  const double largest = value_of(lowest), per_temp = 1.0 / (double)temp;
 
-  const double largest = value_of(lowest);
-  auto weight = [&](int rank) {  // (the largest value itself has 1, also where it is infinite)
-    const double d = value_of(rank) - largest;
-    return rank == lowest ? 1.0 : largest == __builtin_inf() ? 0.0 : exp(d / (double)temp);
-  };
-  auto counts = [&](int b, uint32_t (&c)[kPerLane]) {
-    const u32x4 v = reinterpret_cast<const u32x4*>(hist)[(b % kBlocks) * 64 + lane];
-#pragma unroll
-    for (int e = 0; e < kPerLane; ++e) c[e] = MERGE ? v[e % 4] : place(v, e);
-  };
-  auto rank_at = [&](int b, int e) { return base + b * kBlock + lane * kPerLane + e; };
-  // Counts within top-k, from the count before the lane's values.
-  auto within = [&](uint32_t (&c)[kPerLane], uint32_t before) {
-#pragma unroll
-    for (int e = 0; e < kPerLane; ++e) {
-      const uint32_t all = c[e];
-      c[e] = before >= limit ? 0u : min(all, limit - before);
-      before += all;
-    }
-  };
-  auto lane_before = [&](const uint32_t (&c)[kPerLane]) {
-    uint32_t n = 0;
-#pragma unroll
-    for (int e = 0; e < kPerLane; ++e) n += c[e];
-    return wave_prefix(n) - n;
-  };
-
-  // Each block's count, then its mass within top-k and the part of it with a weight of at least min_p.
-  for (int part = 0; part < parts; ++part) {
-    build(part);
-    for (int t = 0; t < kTurns; ++t) {
-      const int b = part * kBlocks + t * kWaves + wave;
-      uint32_t c[kPerLane], n = 0;
-      counts(b, c);
-#pragma unroll
-      for (int e = 0; e < kPerLane; ++e) n += c[e];
-      if (__ballot(n != 0) == 0) continue;
-      n = wave_sum(n);
-      if (lane == 0) s_count[b] = n;
-    }
+  // Prefix of v over the workgroup's threads, and its total. `slot` alternates between calls.
+  auto block_prefix = [&](auto v, auto* slot, auto* total) __attribute__((always_inline)) {
+    const auto inc = wave_prefix(v);
+    if (lane == 63) slot[wave] = inc;
     __syncthreads();
-    if (wave == 0) {
-      uint32_t v[kPerScan], sum = 0;
-#pragma unroll
-      for (int i = 0; i < kPerScan; ++i) sum += v[i] = s_count[lane * kPerScan + i];
-      uint32_t before = wave_prefix(sum) - sum;
-#pragma unroll
-      for (int i = 0; i < kPerScan; ++i) {
-        s_before[lane * kPerScan + i] = before;
-        before += v[i];
-      }
-    }
-    __syncthreads();
-    for (int t = 0; t < kTurns; ++t) {
-      const int b = part * kBlocks + t * kWaves + wave;
-      if (s_count[b] == 0 || s_before[b] >= limit) continue;
-      uint32_t c[kPerLane];
-      counts(b, c);
-      if (s_before[b] + s_count[b] > limit) within(c, s_before[b] + lane_before(c));
-      double mass = 0.0, kept = 0.0;
-#pragma unroll
-      for (int e = 0; e < kPerLane; ++e) {
-        if (c[e] == 0) continue;
-        const double w = weight(rank_at(b, e)), mw = c[e] * w;
-        mass += mw;
-        kept += w < (double)min_p ? 0.0 : mw;
-      }
-      mass = wave_sum(mass);
-      kept = wave_sum(kept);
-      if (lane == 0) {
-        s_mass[b] = mass;
-        s_kept[b] = kept;
-      }
-    }
-  }
-  __syncthreads();
+    const auto waves = row_prefix(slot[lane & 15]);
+    *total = lane_value(waves, 15);
+    return (wave ? lane_value(waves, wave - 1) : decltype(v)(0)) + (inc - v);
+  };
 
-  // Every wave finds the same: the block in which the mass before reaches top_p of the whole, what is kept, and the
-  // block in which the kept mass passes the target.
-  double mass_before[kPerScan], kept_before[kPerScan], total, kept_total;
-  {
-    double a = 0.0, k = 0.0;
+  // Three sums over the pages: the mass within top-k, the part of it that is kept, and up to the target. With one page
+  // the threads keep their values from sum to sum.
+  double total = 0.0, kept_total = 0.0, target = 0.0;
+  int built = MERGE ? -1 : 0;
+  bool one_page = true;
+  uint32_t c[kPer], n[kPer];
+  double w[kPer], mass = 0.0, mass_before = 0.0, kept = 0.0, kept_before = 0.0;
+  int rank[kPer], per = 0;
+  for (int sum = 0; sum < 3; ++sum) {
+    uint32_t count_sum = 0;
+    double mass_sum = 0.0, kept_sum = 0.0;
+    for (int part = 0; part < parts; ++part) {
+      const int from = base + part * kSpan;
+      if (MERGE && built != part) {
+        __syncthreads();
+        zero_lds<kSpan * 4>(hist);
+        __syncthreads();
+        built = part;
+        for (int s = wave; s < L.slices; s += kWaves) {
+          const int n4 = ((int)s_n[s] + 3) / 4;
+          const u32x4* list = reinterpret_cast<const u32x4*>(L.list(m, s));
+          constexpr int kAhead = 8;
+          for (int i0 = lane; i0 < n4; i0 += kAhead * 64) {
+            u32x4 v[kAhead];
 #pragma unroll
-    for (int i = 0; i < kPerScan; ++i) {
-      mass_before[i] = a;
-      kept_before[i] = k;
-      a += s_mass[lane * kPerScan + i];
-      k += s_kept[lane * kPerScan + i];
+            for (int i = 0; i < kAhead; ++i) v[i] = list[min(i0 + i * 64, n4 - 1)];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {  // (what is not for this histogram goes behind it, one word for each lane)
+                const int r = (int)(v[i][e] >> 16) - from;
+                const bool in = i0 + i * 64 < n4 && (uint32_t)r < (uint32_t)kSpan;
+                atomicAdd(&hist[in ? r : kSpan + lane], v[i][e] & 0xFFFFu);
+              }
+            }
+          }
+        }
+        __syncthreads();
+      }
+      uint32_t entries = 0;
+      for (uint32_t first = 0; first == 0 || first < entries; first += kPage) {
+        if (sum == 0 || !one_page) {
+          // The page's values: those that occur, the first-th and on. A wave lists kLooks * 64 neighbouring words of the
+          // histogram, 64 at a time: a comparison is a mask of the lanes, and a lane's place in the list the number of
+          // them below it. (Neighbouring groups of 64 to different waves took two more barriers and 0.4 us.)
+          constexpr int kLooks = kSpan / (MERGE ? 1 : 2) / kThreads;
+          const uint32_t* h = hist + wave * (kLooks * 64) + lane;
+          uint32_t here = 0;
+#pragma unroll 9
+          for (int t = 0; t < kLooks; ++t) {
+            const uint32_t v = h[t * 64];
+            if constexpr (MERGE) here += __popcll(__ballot(v != 0));
+            else here += __popcll(__ballot((v & 0xFFFFu) != 0)) + __popcll(__ballot(v > 0xFFFFu));
+          }
+          __syncthreads();  // (the page before is read)
+          uint32_t at = block_prefix(lane == 0 ? here : 0u, s_u[0], &entries);
+          at = lane_value(at, 0) - first;
+          if (sum == 0 && part == 0 && first == 0) one_page = parts == 1 && entries <= kPage;
+#pragma unroll 9
+          for (int t = 0; t < kLooks; ++t) {
+            const uint32_t v = h[t * 64];
+            const unsigned long long lo = __ballot(MERGE ? v != 0 : (v & 0xFFFFu) != 0), hi = MERGE ? 0 : __ballot(v > 0xFFFFu);
+            if ((lo | hi) == 0) continue;
+            uint32_t o = __builtin_amdgcn_mbcnt_hi((uint32_t)(lo >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lo, at));
+            const uint32_t r = (uint32_t)((wave * kLooks + t) * 64 + lane) * (MERGE ? 1 : 2);
+            if constexpr (!MERGE)
+              o = __builtin_amdgcn_mbcnt_hi((uint32_t)(hi >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hi, o));
+            if ((MERGE ? v != 0 : (v & 0xFFFFu) != 0) && o < (uint32_t)kPage) s_page[o] = (uint16_t)r;
+            if constexpr (!MERGE) {
+              o += (v & 0xFFFFu) != 0;
+              if (v > 0xFFFFu && o < (uint32_t)kPage) s_page[o] = (uint16_t)(r + 1);
+            }
+            at += __popcll(lo) + __popcll(hi);
+          }
+          __syncthreads();
+          // Counts within top-k and their masses. (Equal weights of neighbours: none of the values is taken twice.)
+          const uint32_t in_page = min(entries - first, (uint32_t)kPage);
+          per = (int)((in_page + kThreads - 1) / kThreads);
+          uint32_t own = 0, page_count, all[kPer];
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            all[e] = c[e] = n[e] = 0;
+            w[e] = 0.0;
+            if (e >= per) continue;
+            const uint32_t i = tid * per + e;
+            const bool is = i < in_page;
+            const uint32_t r = is ? s_page[i] : 0u;
+            rank[e] = from + (int)r;
+            all[e] = !is ? 0u : MERGE ? hist[r] : r & 1 ? hist[r >> 1] >> 16 : hist[r >> 1] & 0xFFFFu;
+            own += all[e];
+          }
+          uint32_t before = count_sum + block_prefix(own, s_u[1], &page_count);
+          count_sum += page_count;
+          double page_mass;
+          mass = 0.0;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            if (e >= per) break;
+            c[e] = before >= limit ? 0u : min(all[e], limit - before);
+            before += all[e];
+            // (The largest value itself has 1, also where it is infinite.)
+            const double d = value_of(rank[e]) - largest;
+            w[e] = rank[e] == lowest ? 1.0 : largest == __builtin_inf() ? 0.0 : exp(d * per_temp);
+            if (c[e] == 0) w[e] = 0.0;
+            mass += c[e] * w[e];
+          }
+          mass_before = mass_sum + block_prefix(mass, s_d[0], &page_mass);
+          mass_sum += page_mass;
+        }
+        if (sum == 1 || (sum == 2 && !one_page)) {
+          // Kept of a value: those with less mass before them than the bound, and a weight of at least min_p.
+          if (top_p < 1.0f || min_p > 0.0f) {
+            const double bound = (double)top_p * total;
+            double mb = mass_before, page_kept;
+            kept = 0.0;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+              if (e >= per) break;
+              const double end = mb + c[e] * w[e];
+              n[e] = c[e];
+              if (top_p < 1.0f && end > bound) {  // (the division is for one value of all: 4 in each thread took 0.7 us)
+                n[e] = 0;
+                if (mb < bound) n[e] = min(c[e], (uint32_t)ceil((bound - mb) / w[e]));
+              }
+              if (w[e] < (double)min_p) n[e] = 0;
+              mb = end;
+              kept += n[e] * w[e];
+            }
+            kept_before = kept_sum + block_prefix(kept, s_d[1], &page_kept);
+            kept_sum += page_kept;
+          } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) n[e] = c[e];
+            kept = mass;
+            kept_before = mass_before;
+            kept_sum = one_page ? total : mass_sum;
+          }
+        }
+        if (sum == 2) {
+          // The last thread with some kept mass that starts at or before the target holds the value that passes it (up
+          // to rounding: then its last one).
+          const int thread = wave_max(kept > 0.0 && kept_before <= target ? tid : -1);
+          if (lane == 0) s_hi[wave] = thread;
+          __syncthreads();
+          if (tid == row_max(s_hi[lane & 15])) {
+            uint32_t hit_n = 1, hit_rank = 0;
+            double kb = kept_before, hit_before = 0.0, hit_weight = 1.0;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+              if (n[e] != 0 && w[e] > 0.0 && kb <= target) {
+                hit_n = n[e];
+                hit_rank = (uint32_t)rank[e];
+                hit_before = kb;
+                hit_weight = w[e];
+              }
+              kb += n[e] * w[e];
+            }
+            const double j = floor((target - hit_before) / hit_weight);
+            s_hit[0] = hit_rank;
+            s_hit[1] = j < (double)(hit_n - 1) ? (uint32_t)j : hit_n - 1;
+            s_weight = hit_weight;
+          }
+          __syncthreads();
+        }
+        if (one_page) break;
+      }
     }
-    const double ia = wave_prefix(a), ik = wave_prefix(k);
-    total = __shfl(ia, 63);
-    kept_total = __shfl(ik, 63);
-#pragma unroll
-    for (int i = 0; i < kPerScan; ++i) {
-      mass_before[i] += ia - a;
-      kept_before[i] += ik - k;
+    if (sum == 0) total = mass_sum;
+    if (sum == 1) {
+      kept_total = kept_sum;
+      target = (double)(u > 0.0f ? u : 0.0f) * kept_total;
     }
   }
-  // One block value by value: counts kept (c), weights, and the kept mass before each of the lane's values.
-  const double bound = (double)top_p * total;
-  const bool has_bound = top_p < 1.0f;
-  int built = parts - 1;
-  auto open_block = [&](int b, double mass0, double kept0, uint32_t (&c)[kPerLane], double (&w)[kPerLane],
-                        double (&before)[kPerLane]) {
-    if (b / kBlocks != built) {
-      built = b / kBlocks;
-      build(built);
-    }
-    counts(b, c);
-    within(c, s_before[b] + lane_before(c));
-    double mass = 0.0;
-#pragma unroll
-    for (int e = 0; e < kPerLane; ++e) {
-      w[e] = c[e] != 0 ? weight(rank_at(b, e)) : 0.0;
-      mass += c[e] * w[e];
-    }
-    double mb = mass0 + (wave_prefix(mass) - mass), kept = 0.0;
-#pragma unroll
-    for (int e = 0; e < kPerLane; ++e) {
-      const double all = c[e] * w[e];
-      if (has_bound && c[e] != 0) {  // of a value, those with less than the bound before them
-        const double fit = ceil((bound - mb) / w[e]);
-        c[e] = fit <= 0.0 ? 0u : fit < (double)c[e] ? (uint32_t)fit : c[e];
-      }
-      if (w[e] < (double)min_p) c[e] = 0;
-      mb += all;
-      before[e] = kept;
-      kept += c[e] * w[e];
-    }
-    const double inc = wave_prefix(kept);
-#pragma unroll
-    for (int e = 0; e < kPerLane; ++e) before[e] += kept0 + (inc - kept);
-    return kept0 + __shfl(inc, 63);  // kept up to the block's end
-  };
-  // The last block with some kept mass for which `before` lies below a limit (or at it).
-  auto find = [&](auto&& ok, double* mass0, double* kept0) {
-    int b = -1;
-#pragma unroll
-    for (int i = 0; i < kPerScan; ++i)
-      if (s_kept[lane * kPerScan + i] > 0.0 && ok(i)) b = lane * kPerScan + i;
-    b = wave_max(b);
-    double mm = 0.0, kk = 0.0;
-#pragma unroll
-    for (int i = 0; i < kPerScan; ++i)
-      if (i == b % kPerScan) {
-        mm = mass_before[i];
-        kk = kept_before[i];
-      }
-    *mass0 = __shfl(mm, b / kPerScan);
-    *kept0 = __shfl(kk, b / kPerScan);
-    return b;
-  };
-  uint32_t c[kPerLane];
-  double w[kPerLane], before[kPerLane], mass0, kept0;
-  int border = kParts * kBlocks;
-  if (has_bound) {
-    border = find([&](int i) { return mass_before[i] < bound; }, &mass0, &kept0);
-    kept_total = open_block(border, mass0, kept0, c, w, before);
-  }
-  const double target = (double)(u > 0.0f ? u : 0.0f) * kept_total;
-  const int block = find([&](int i) { return lane * kPerScan + i <= border && kept_before[i] <= target; }, &mass0, &kept0);
-  if (block != border) open_block(block, mass0, kept0, c, w, before);
-  // The last value with some mass that starts at or before the target, and the occurrence of it that passes it.
-  int slot = -1;
-#pragma unroll
-  for (int e = 0; e < kPerLane; ++e)
-    if (c[e] != 0 && w[e] > 0.0 && before[e] <= target) slot = e;
-  const unsigned long long lanes = __ballot(slot >= 0);
-  const int owner = 63 - __builtin_clzll(lanes | 1);
-  slot = __shfl(slot, owner);
-  uint32_t index = 0;
-  double hit_weight = 1.0;
-#pragma unroll
-  for (int e = 0; e < kPerLane; ++e)
-    if (e == slot) {
-      const double j = floor((target - before[e]) / w[e]);
-      index = j < (double)(c[e] - 1) ? (uint32_t)j : c[e] - 1;
-      hit_weight = w[e];
-    }
-  uint32_t left = __shfl(index, owner);
-  hit_weight = __shfl(hit_weight, owner);
-  const int rank = base + block * kBlock + owner * kPerLane + max(slot, 0);
+  const int hit = (int)s_hit[0];
+  uint32_t left = s_hit[1];
+  const double hit_weight = s_weight;
 
   // The slice with the occurrence: the value's count in each list, found by two looks of a wave.
   int begin = 0, end = S.V;
   if constexpr (MERGE) {
     for (int s = wave; s < L.slices; s += kWaves) {
-      const int n = (int)L.n[m * L.slices + s];
+      const int n = (int)s_n[s];
       const uint32_t* list = L.list(m, s);
       const int step = (n + 63) / 64;
-      const unsigned long long le = __ballot(lane * step < n && (int)(list[min(lane * step, max(n - 1, 0))] >> 16) <= rank);
+      const unsigned long long le = __ballot(lane * step < n && (int)(list[min(lane * step, max(n - 1, 0))] >> 16) <= hit);
       uint32_t occ = 0;
       if (le != 0) {
         const int from = (63 - __builtin_clzll(le)) * step;
         for (int i = lane; i < step; i += 64) {
           const uint32_t v = from + i < n ? list[from + i] : 0xFFFFFFFFu;
-          if ((int)(v >> 16) == rank) occ = v & 0xFFFFu;
+          if ((int)(v >> 16) == hit) occ = v & 0xFFFFu;
         }
       }
       occ = wave_sum(occ);
@@ -494,48 +513,78 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams S, L
     }
     __syncthreads();
     int slice = L.slices - 1;
-    for (int s = 0; s < L.slices; ++s) {
-      if (left < s_occ[s]) {
-        slice = s;
+    for (int s0 = 0; s0 < L.slices; s0 += 64) {
+      const uint32_t occ = s0 + lane < L.slices ? s_occ[s0 + lane] : 0, inc = wave_prefix(occ);
+      const unsigned long long past = __ballot(left < inc);
+      if (past != 0) {
+        const int at = __ffsll(past) - 1;
+        slice = s0 + at;
+        left -= lane_value(inc - occ, at);
         break;
       }
-      left -= s_occ[s];
+      left -= lane_value(inc, 63);
     }
     begin = slice * L.slice;
     end = min(S.V, begin + L.slice);
   }
-  const Groups G(row, begin, end);
-  for (int g0 = 0; g0 < G.count; g0 += kThreads) {
-    const int g = g0 + tid;
-    uint32_t hits = 0;
-    if (g < G.count) {
-      const u32x4 v = G.load(g);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) hits |= (rank_of(place(v, e)) == rank ? 1u : 0u) << e;
-    }
-    const uint32_t n = __popc(hits), inc = wave_prefix(n);
-    __syncthreads();
-    if (lane == 63) s_u[wave] = inc;
-    __syncthreads();
-    uint32_t ahead = inc - n, all = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      if (i < wave) ahead += s_u[i];
-      all += s_u[i];
-    }
-    if (left >= ahead && left < ahead + n) {
-      for (uint32_t skip = left - ahead; skip > 0; --skip) hits &= hits - 1;
-      S.tokens[m] = G.first(g) + (__ffs((int)hits) - 1);
-      S.logprobs[m] = (float)log(hit_weight / kept_total);
-    }
-    if (left < all) break;
-    left -= all;
+  auto found = [&](int index) {
+    S.tokens[m] = index;
+    S.logprobs[m] = (float)log(hit_weight / kept_total);
+  };
+  // The value's bits; zero has two forms.
+  const uint32_t bits = hit <= 0x7F80 ? 0x7F80 - hit : 0x8000 | (hit - 0x7F80), other = bits == 0 ? 0x8000u : bits;
+  auto matches = [&](uint32_t b) { return b == bits || b == other; };
+  // Occurrences in index order: the logits before the lines, the lines, the logits behind them.
+  const Lines G(row, begin, end);
+  const unsigned long long edges = __ballot(matches(G.edge(lane)));  // (of lanes 0 .. 15, in every wave)
+  const uint32_t head = __popcll(edges & 0xFF);
+  if (left < head) {
+    unsigned long long e = edges & 0xFF;
+    for (; left > 0; --left) e &= e - 1;
+    if (tid == 0) found(G.edge_index(__ffsll(e) - 1));
+    return;
   }
+  left -= head;
+  const bool in_registers = !MERGE && G.count <= kBatch * kThreads;
+  for (int g0 = 0; g0 < G.count; g0 += kBatch * kThreads) {
+    uint32_t hits[kBatch], inc[kBatch];
+    if (!in_registers) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) held[i] = G.load(g0 + i * kThreads + tid);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      hits[i] = 0;
+      if (g0 + i * kThreads >= G.count) break;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) hits[i] |= (matches(place(held[i], e)) ? 1u : 0u) << e;
+      inc[i] = wave_prefix((uint32_t)__popc(hits[i]));
+      if (lane == 63) s_u[i][wave] = inc[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (g0 + i * kThreads >= G.count) break;
+      const uint32_t waves = row_prefix(s_u[i][lane & 15]);
+      const uint32_t n = __popc(hits[i]);
+      const uint32_t ahead = (wave ? lane_value(waves, wave - 1) : 0u) + inc[i] - n, all = lane_value(waves, 15);
+      if (left >= ahead && left < ahead + n) {
+        for (uint32_t skip = left - ahead; skip > 0; --skip) hits[i] &= hits[i] - 1;
+        found(G.first(g0 + i * kThreads + tid) + __ffs((int)hits[i]) - 1);
+      }
+      if (left < all) return;
+      left -= all;
+    }
+  }
+  unsigned long long e = edges >> 8 & 0xFF;
+  for (; left > 0 && (e & (e - 1)) != 0; --left) e &= e - 1;
+  if (tid == 0) found(G.edge_index(8 + max(__ffsll(e) - 1, 0)));
 }
 
 LdsAllowance g_count, g_pick, g_merge;
 
-constexpr size_t kMergeBytes = 36864 * sizeof(uint32_t);
+constexpr size_t kMergeBytes = (36864 + 64) * sizeof(uint32_t);
 
 struct Plan {
   int slice, slices;
@@ -546,6 +595,7 @@ struct Plan {
 Plan plan_of(int64_t M, int V, int cus) {
   const int64_t batch = M < kMaxBatch ? M : kMaxBatch;
   int64_t s = cus / batch;
+  if (s > kWaves) s = kWaves;  // (a list to each wave of the merge: 37 slices of one row took it 7 us, 16 take 3)
   if (s > V / kMinSlice) s = V / kMinSlice;
   if (s < (V + kMaxSlice - 1) / kMaxSlice) s = (V + kMaxSlice - 1) / kMaxSlice;
   if (s > kMaxSlices) s = kMaxSlices;

@@ -61,6 +61,26 @@ def test_settings_of_each_row(m, v):
     check(logits, u, **{k: t.to(DEV) for k, t in settings.items()})
 
 
+@pytest.mark.parametrize("settings", [dict(), dict(temperature=3e4), dict(temperature=1e5, top_p=0.99, min_p=1e-9),
+                                      dict(temperature=1e38, top_k=9000), dict(temperature=1e38, top_p=0.7)], ids=str)
+@pytest.mark.parametrize("v", [30000, 65535, 65536, 100003])
+def test_more_values_than_a_page(v, settings):
+    """Logits spread over many octaves: more than 4096 different values, over more than one histogram."""
+    g = torch.Generator().manual_seed(v)
+    l = torch.randn(6, v, generator=g) * 2.0 ** torch.randint(-60, 60, (6, v), generator=g)
+    l[3:] = torch.randn(3, v, generator=g) * 2.0 ** torch.randint(-12, 9, (3, v), generator=g)  # one histogram
+    logits = l.to(torch.bfloat16).to(DEV)
+    logits[1, ::3] = torch.finfo(torch.bfloat16).min
+    logits[4, 5::7] = -float("inf")
+    check(logits, torch.tensor([0.0, 0.99, 0.5, 0.3, 0.7, 0.9], device=DEV), **settings)
+
+
+def test_more_rows_than_a_batch():
+    logits, u = logits_of(300, 65601, 8, boosted=9)
+    g = torch.Generator().manual_seed(1)
+    check(logits, u, temperature=(torch.rand(300, generator=g) * 1.5).to(DEV), top_p=0.97)
+
+
 @pytest.mark.parametrize("settings", [dict(), dict(top_k=7), dict(top_p=0.4), dict(top_k=5000, top_p=0.77, min_p=0.5)], ids=str)
 def test_every_border_of_a_small_vocabulary(settings):
     """512 random numbers walk through the whole order: falling logits, equal ones by index, -0 with +0."""
