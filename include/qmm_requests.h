@@ -25,27 +25,29 @@ extern "C" {
 #define QMM4_SAMPLE_MAX_VOCAB (1 << 24)
 
 /*
- * y[m] += scale[a] * (x[m] A[a]^T) B[a]^T for a = adapters[m]: low-rank adapters of many requests, added to a
- * projection's output. Rows whose adapter lies outside 0 .. L - 1 (-1 by convention) are left as they are.
- *   x: bf16 [M, K]; lora_a: bf16 [L, R, K]; lora_b: bf16 [L, N, R]; lora_scale: fp32 [L]; adapters: int32 or
- *   int64 [M] (adapter_bits 32 or 64); y: bf16 [M, N], added to in fp32 and rounded once.
- *   x A^T is kept in fp32 in `workspace`. Requires K % 8 == 0, R % 8 == 0, 8 <= R <= QMM4_LORA_MAX_RANK,
- *   M, N, K, L <= 2^30, x, lora_a, lora_b 16-byte aligned, lora_scale 4-byte, adapters by their own size, y
- *   2-byte aligned. M == 0, N == 0 or L == 0 is a no-op. Deterministic.
+ * y[m] = x[m] dequant(w)^T + scale[a] * (x[m] A[a]^T) B[a]^T for a = adapters[m]: a shared quantized projection with
+ * each row's low-rank adapter. Rows whose adapter lies outside 0 .. L - 1 (-1 by convention) have the projection alone,
+ * with its bits.
+ *   x, w, scales, biases, y and their requirements: those of qmm4_affine_bf16 (bits 4, group_size 64, K % 128 == 0,
+ *   N % 16 == 0), else of qmm_affine_general_bf16; lora_a: bf16 [L, R, K]; lora_b: bf16 [L, N, R]; lora_scale: fp32
+ *   [L]; adapters: int32 or int64 [M] (adapter_bits 32 or 64).
+ *   The sums of both products are fp32 and rounded once; between its factors the second one is kept (in `workspace`) to
+ *   2^-18 of its value. Requires R % 8 == 0, 8 <= R <= QMM4_LORA_MAX_RANK, L <= 2^30, lora_a, lora_b and workspace
+ *   16-byte aligned, lora_scale 4-byte, adapters by their own size. M == 0 or N == 0 is a no-op. Deterministic.
  */
 int64_t qmm4_lora_workspace(int64_t M, int64_t R);
-int qmm4_lora_add_bf16(const void* x, const void* lora_a, const void* lora_b, const float* lora_scale,
-                       const void* adapters, int adapter_bits, void* y, void* workspace, int64_t M, int64_t N,
-                       int64_t K, int64_t L, int64_t R, void* hip_stream);
-
-/*
- * y[m] = x[m] dequant(w)^T + scale[a] * (x[m] A[a]^T) B[a]^T: the shared 4-bit projection of qmm4_affine_bf16
- * with each row's adapter. The requirements of both calls.
- */
 int qmm4_affine_lora_bf16(const void* x, const uint32_t* w, const void* scales, const void* biases,
                           const void* lora_a, const void* lora_b, const float* lora_scale, const void* adapters,
                           int adapter_bits, void* y, void* workspace, int64_t M, int64_t N, int64_t K, int64_t L,
                           int64_t R, int group_size, int bits, int transpose, void* hip_stream);
+
+/*
+ * y[m] += scale[a] * (x[m] A[a]^T) B[a]^T in place, for a projection that ran elsewhere: the same arguments (K % 8 == 0,
+ * any N, each dimension at most 2^30), y added to in fp32 and rounded again. L == 0 is a no-op.
+ */
+int qmm4_lora_add_bf16(const void* x, const void* lora_a, const void* lora_b, const float* lora_scale,
+                       const void* adapters, int adapter_bits, void* y, void* workspace, int64_t M, int64_t N,
+                       int64_t K, int64_t L, int64_t R, void* hip_stream);
 
 /*
  * The RMS norms of the query and key heads and their rotation at each row's position, in one pass: the step

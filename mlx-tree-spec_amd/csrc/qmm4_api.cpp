@@ -269,6 +269,17 @@ int qmm4_gate_up_silu_bf16(const void* x, const uint32_t* w, const void* scales,
 
 namespace qmm4 {
 
+int with_stream_workspace(hipStream_t stream, const std::function<int(DeviceInfo*, WorkspaceSource&)>& f) {
+  int dev = 0;
+  int rc = current_device(&dev);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lock(api_mutex());
+  DeviceInfo* di = nullptr;
+  if ((rc = device_info(dev, &di))) return rc;
+  StreamWorkspace ws(dev, stream);
+  return f(di, ws);
+}
+
 int check_qmm_args(const void* x, const uint32_t* w, const void* scales, const void* biases, const void* y,
                    int64_t M, int64_t N, int64_t K, int group_size, int bits, int transpose) {
   int rc = check_format(group_size, bits, transpose);
@@ -297,6 +308,31 @@ int check_qmm_args(const void* x, const uint32_t* w, const void* scales, const v
       (unsigned long long)(M + 256) * (unsigned long long)N * 2 >= (1ULL << 32))
     return set_error(QMM4_ERR_INVALID, "x [%lld, %lld] or y [%lld, %lld] exceeds 4 GiB", (long long)M,
                      (long long)K, (long long)M, (long long)N);
+  return QMM4_OK;
+}
+
+int check_general_args(const void* x, const uint32_t* w, const void* scales, const void* biases, const void* y,
+                       int64_t M, int64_t N, int64_t K, int group_size, int bits) {
+  if (bits != 2 && bits != 4 && bits != 8)
+    return set_error(QMM4_ERR_UNSUPPORTED, "bits=%d: 2-, 4- and 8-bit codes are supported", bits);
+  if (group_size != 32 && group_size != 64 && group_size != 128)
+    return set_error(QMM4_ERR_UNSUPPORTED, "group_size=%d: groups of 32, 64 and 128 are supported", group_size);
+  if (M < 0 || N < 0 || K <= 0 || K % 64 != 0 || K % group_size != 0)
+    return set_error(QMM4_ERR_INVALID, "invalid shape M=%lld N=%lld K=%lld (K must be a positive multiple of 64 and of "
+                     "group_size=%d)", (long long)M, (long long)N, (long long)K, group_size);
+  if (M > (1LL << 20) || N > (1LL << 30) || K > (1LL << 24))
+    return set_error(QMM4_ERR_INVALID, "shape M=%lld N=%lld K=%lld is too large", (long long)M, (long long)N, (long long)K);
+  if (M == 0 || N == 0) return QMM4_OK;
+  if (!x || !w || !scales || !biases || !y) return set_error(QMM4_ERR_INVALID, "null pointer argument");
+  if (!aligned(x, 16) || !aligned(w, 16)) return set_error(QMM4_ERR_INVALID, "x and w must be 16-byte aligned");
+  if (!aligned(scales, 2) || !aligned(biases, 2) || !aligned(y, 2))
+    return set_error(QMM4_ERR_INVALID, "scales, biases and y must be 2-byte aligned");
+  // Byte offsets (which may reach 64 rows or columns past the end) stay below 2 GiB.
+  constexpr unsigned long long kMax = 1ULL << 31;
+  if ((unsigned long long)(M + 64) * K * 2 >= kMax || (unsigned long long)(N + 64) * (K / 8 * bits) >= kMax ||
+      (unsigned long long)(N + 64) * (K / 32) * 2 >= kMax)
+    return set_error(QMM4_ERR_INVALID, "x [%lld, %lld] or w [%lld, %lld] exceeds 2 GiB", (long long)M, (long long)K,
+                     (long long)N, (long long)K);
   return QMM4_OK;
 }
 
@@ -388,7 +424,8 @@ int dispatch_gate_up_silu(DeviceInfo* di, const void* x, const uint32_t* w, cons
 
 // The kernel choice for y = x @ dequant(w)^T (arguments already checked, M and N > 0, api_mutex held).
 int dispatch_qmm(DeviceInfo* di, const void* x, const uint32_t* w, const void* scales, const void* biases,
-                 void* y, int64_t M, int64_t N, int64_t K, hipStream_t stream, WorkspaceSource& ws) {
+                 void* y, int64_t M, int64_t N, int64_t K, hipStream_t stream, WorkspaceSource& ws,
+                 const LoraAdd* lora) {
   const uint16_t* xb = static_cast<const uint16_t*>(x);
   const uint16_t* sb = static_cast<const uint16_t*>(scales);
   const uint16_t* bb = static_cast<const uint16_t*>(biases);
@@ -404,7 +441,7 @@ int dispatch_qmm(DeviceInfo* di, const void* x, const uint32_t* w, const void* s
       int rc2 = ws.get(0, pplan.part_bytes, &pcnt, &ppart);
       if (rc2) return rc2;
     }
-    hipError_t e2 = launch_rowphase(pplan, xb, w, sb, bb, yb, ppart, (int)M, (int)N, (int)K, stream);
+    hipError_t e2 = launch_rowphase(pplan, xb, w, sb, bb, yb, ppart, (int)M, (int)N, (int)K, stream, lora);
     if (e2 != hipSuccess) return hip_error(e2, "row-phase kernel launch");
     return QMM4_OK;
   };
@@ -429,7 +466,7 @@ int dispatch_qmm(DeviceInfo* di, const void* x, const uint32_t* w, const void* s
       rc = ws.get(0, gplan.part_bytes, &gcnt, &gpart);
       if (rc) return rc;
     }
-    e = launch_gemm(gplan, xb, w, sb, bb, yb, gpart, (int)M, (int)N, (int)K, di->cus, stream);
+    e = launch_gemm(gplan, xb, w, sb, bb, yb, gpart, (int)M, (int)N, (int)K, di->cus, stream, lora);
     if (e != hipSuccess) return hip_error(e, "gemm kernel launch");
     return QMM4_OK;
   }
@@ -438,7 +475,7 @@ int dispatch_qmm(DeviceInfo* di, const void* x, const uint32_t* w, const void* s
   // kernel's form with one wave per K chunk, every load in flight from the start.
   RowSplitPlan rplan;
   if (M >= 9 && rowsplit_xreg_plan((int)M, (int)N, (int)K, di->cus, &rplan)) {
-    e = launch_rowsplit(rplan, xb, w, sb, bb, yb, nullptr, nullptr, (int)M, (int)N, (int)K, stream);
+    e = launch_rowsplit(rplan, xb, w, sb, bb, yb, nullptr, nullptr, (int)M, (int)N, (int)K, stream, nullptr, lora);
     if (e != hipSuccess) return hip_error(e, "row-split kernel launch");
     return QMM4_OK;
   }
@@ -451,7 +488,7 @@ int dispatch_qmm(DeviceInfo* di, const void* x, const uint32_t* w, const void* s
       rc = ws.get((size_t)rplan.ranges * sizeof(uint32_t), rplan.part_bytes, &rcnt, &rpart);
       if (rc) return rc;
     }
-    e = launch_rowsplit(rplan, xb, w, sb, bb, yb, rpart, rcnt, (int)M, (int)N, (int)K, stream);
+    e = launch_rowsplit(rplan, xb, w, sb, bb, yb, rpart, rcnt, (int)M, (int)N, (int)K, stream, nullptr, lora);
     if (e != hipSuccess) return hip_error(e, "row-split kernel launch");
     return QMM4_OK;
   }
@@ -479,7 +516,7 @@ int dispatch_qmm(DeviceInfo* di, const void* x, const uint32_t* w, const void* s
       float* vpart = nullptr;
       rc = ws.get((size_t)vplan.tiles * sizeof(uint32_t), vplan.part_bytes, &vcnt, &vpart);
       if (rc) return rc;
-      e = launch_verify(vplan, xb, w, sb, bb, yb, vpart, vcnt, (int)M, (int)N, (int)K, stream);
+      e = launch_verify(vplan, xb, w, sb, bb, yb, vpart, vcnt, (int)M, (int)N, (int)K, stream, lora);
       if (e != hipSuccess) return hip_error(e, "verify kernel launch");
       return QMM4_OK;
     }
@@ -519,7 +556,7 @@ int dispatch_qmm(DeviceInfo* di, const void* x, const uint32_t* w, const void* s
   rc = ws.get((size_t)plan.tiles * sizeof(uint32_t),
               (size_t)plan.blocks * 2 * (size_t)M * plan.tile_cols * sizeof(float), &cnt, &part);
   if (rc) return rc;
-  e = launch_skinny(plan, xb, w, sb, bb, yb, part, cnt, (int)M, (int)N, (int)K, stream);
+  e = launch_skinny(plan, xb, w, sb, bb, yb, part, cnt, (int)M, (int)N, (int)K, stream, lora);
   if (e != hipSuccess) return hip_error(e, "skinny kernel launch");
   return QMM4_OK;
 }
@@ -638,29 +675,10 @@ int qmm4_add_rms_norm_bf16(const void* x, const void* r, const void* weight, voi
 int qmm_affine_general_bf16(const void* x, const uint32_t* w, const void* scales, const void* biases, void* y,
                             int64_t M, int64_t N, int64_t K, int group_size, int bits, void* hip_stream) {
   qmm4::clear_error();
-  if (bits != 2 && bits != 4 && bits != 8)
-    return set_error(QMM4_ERR_UNSUPPORTED, "bits=%d: 2-, 4- and 8-bit codes are supported", bits);
-  if (group_size != 32 && group_size != 64 && group_size != 128)
-    return set_error(QMM4_ERR_UNSUPPORTED, "group_size=%d: groups of 32, 64 and 128 are supported", group_size);
-  if (M < 0 || N < 0 || K <= 0 || K % 64 != 0 || K % group_size != 0)
-    return set_error(QMM4_ERR_INVALID, "invalid shape M=%lld N=%lld K=%lld (K must be a positive multiple of 64 and of "
-                     "group_size=%d)", (long long)M, (long long)N, (long long)K, group_size);
-  if (M > (1LL << 20) || N > (1LL << 30) || K > (1LL << 24))
-    return set_error(QMM4_ERR_INVALID, "shape M=%lld N=%lld K=%lld is too large", (long long)M, (long long)N, (long long)K);
-  if (M == 0 || N == 0) return QMM4_OK;
-  if (!x || !w || !scales || !biases || !y) return set_error(QMM4_ERR_INVALID, "null pointer argument");
-  if (!aligned(x, 16) || !aligned(w, 16)) return set_error(QMM4_ERR_INVALID, "x and w must be 16-byte aligned");
-  if (!aligned(scales, 2) || !aligned(biases, 2) || !aligned(y, 2))
-    return set_error(QMM4_ERR_INVALID, "scales, biases and y must be 2-byte aligned");
-  // Byte offsets (which may reach 64 rows or columns past the end) stay below 2 GiB.
-  constexpr unsigned long long kMax = 1ULL << 31;
-  if ((unsigned long long)(M + 64) * K * 2 >= kMax || (unsigned long long)(N + 64) * (K / 8 * bits) >= kMax ||
-      (unsigned long long)(N + 64) * (K / 32) * 2 >= kMax)
-    return set_error(QMM4_ERR_INVALID, "x [%lld, %lld] or w [%lld, %lld] exceeds 2 GiB", (long long)M, (long long)K,
-                     (long long)N, (long long)K);
+  int rc = qmm4::check_general_args(x, w, scales, biases, y, M, N, K, group_size, bits);
+  if (rc || M == 0 || N == 0) return rc;
   int dev = 0;
-  int rc = current_device(&dev);
-  if (rc) return rc;
+  if ((rc = current_device(&dev))) return rc;
   int cus = 0;
   {
     std::lock_guard<std::mutex> lock(qmm4::api_mutex());

@@ -6,6 +6,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <functional>
 #include <mutex>
 
 namespace qmm4 {
@@ -41,10 +42,19 @@ class WorkspaceSource {
 int check_qmm_args(const void* x, const uint32_t* w, const void* scales, const void* biases, const void* y,
                    int64_t M, int64_t N, int64_t K, int group_size, int bits, int transpose);
 
+// The same of the general kernel (qmm_affine_general_bf16).
+int check_general_args(const void* x, const uint32_t* w, const void* scales, const void* biases, const void* y,
+                       int64_t M, int64_t N, int64_t K, int group_size, int bits);
+
 // The kernel choice and launches of y = x @ dequant(w)^T (arguments checked, M and N > 0,
-// api_mutex held).
+// api_mutex held). `lora` (optional) is added to the sums.
+struct LoraAdd;
 int dispatch_qmm(DeviceInfo* di, const void* x, const uint32_t* w, const void* scales, const void* biases,
-                 void* y, int64_t M, int64_t N, int64_t K, hipStream_t stream, WorkspaceSource& ws);
+                 void* y, int64_t M, int64_t N, int64_t K, hipStream_t stream, WorkspaceSource& ws,
+                 const LoraAdd* lora = nullptr);
+
+// f with the workspace of the current device and `stream`, api_mutex held.
+int with_stream_workspace(hipStream_t stream, const std::function<int(DeviceInfo*, WorkspaceSource&)>& f);
 
 // The fused gate+up projection with its SiLU·mul epilogue (same preconditions, N % 32 == 0).
 int dispatch_gate_up_silu(DeviceInfo* di, const void* x, const uint32_t* w, const void* scales,

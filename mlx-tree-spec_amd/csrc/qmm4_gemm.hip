@@ -43,6 +43,7 @@
 
 #include "qmm4_common.h"
 #include "qmm4_kernels.h"
+#include "qmm_lora.h"
 #include "qmm4_lds.h"
 #include "qmm4_offsets.h"
 
@@ -80,6 +81,7 @@ struct GemmParams {
   int ups;           // K steps (BK) per unit
   long long U;       // tiles * upt
   float* part;
+  LoraAdd lora;   // LORA: added to the sums
 };
 
 // Stream-K range of workgroup p: units [p U / G, (p + 1) U / G).
@@ -113,6 +115,189 @@ struct Raw {
   uint32_t s, b;      // that group's scale and bias (bf16 bits)
 };
 
+// LORA: sum_j t[m, j] B[a, n, j] of a BM x BN tile as matrix products like those of K: for one adapter of the tile's rows
+// after another and 64 j at a time, t (high and low parts; zero for rows of other adapters) takes the place of the
+// two activation stages in LDS and B that of the first weight stage. One round trip to memory per 64 j, where loads
+// straight into fragments took one per 16 (and 150 us of 2000 x 5120 -> 17408 in spilled registers).
+// A tile of several adapters holds rows whose t is zero beside a B that is not theirs, and a product of zero with an
+// infinity would reach them: what is not finite in B is zeroed and its column noted, and a last step of two products
+// that overflow to both infinities makes those columns of the adapter's own rows NaN. (Only matrix products touch the
+// accumulators: selections on them spilled the registers of the whole kernel.)
+constexpr int kLoraK = BK;
+template <int BM, int BN>
+struct LoraLds {
+  int adapter[BM];  // of the tile's rows: -1 none, -2 past M
+  int bad[BN];      // columns with a B that is not finite (zero between adapters)
+  int any[2];       // whether this stage (by its parity) saw one
+  // Rows r and columns c < max(BM, BN), before the first stage.
+  __device__ __forceinline__ void init(const LoraAdd& E, int i, int m0, int M) {
+    if (i < BM) adapter[i] = m0 + i < M ? lora_adapter(E, m0 + i, M) : -2;
+    if (i < BN) bad[i] = 0;
+    if (i < 2) any[i] = 0;
+  }
+};
+
+// The adapters of a tile's rows one after another, the same in every wave.
+template <int BM>
+struct TileAdapters {
+  int a[BM / 64];
+  unsigned long long todo[BM / 64];
+  __device__ __forceinline__ explicit TileAdapters(const int* adapter) {
+#pragma unroll
+    for (int q = 0; q < BM / 64; ++q) {
+      a[q] = adapter[q * 64 + (threadIdx.x & 63)];
+      todo[q] = __ballot(a[q] >= 0);
+    }
+  }
+  __device__ __forceinline__ bool next(int* d, bool* mixed) {
+    *d = -1;
+    *mixed = false;
+#pragma unroll
+    for (int q = BM / 64 - 1; q >= 0; --q)
+      if (todo[q] != 0) *d = __builtin_amdgcn_readlane(a[q], __ffsll(todo[q]) - 1);
+    if (*d < 0) return false;
+#pragma unroll
+    for (int q = 0; q < BM / 64; ++q) {
+      const unsigned long long mine = __ballot(a[q] == *d);
+      todo[q] &= ~mine;
+      *mixed |= (mine | __ballot(a[q] == -2)) != ~0ull;
+    }
+    return true;
+  }
+};
+
+// Threads 0 .. NT - 1 stage j0 .. j0 + 63 of adapter d into LDS (to the next 16 past R with zeros); `stage` counts.
+template <int BM, int BN, int NT, int AHEAD>
+__device__ __forceinline__ void lora_stage(const LoraAdd& E, LoraLds<BM, BN>& S, uint16_t* As, uint16_t* Bs, int tid, int d,
+                                           bool mixed, int j0, int stage, int m0, int n0, int M, int N) {
+  constexpr uint32_t kOut = 0x80000000u;  // past the end of a tile's rows or columns: reads zero
+  // (A quarter of a 256 x 256 tile may begin past M or N: no rows or columns then.)
+  const int rows = max(0, min(BM, M - m0)), cols = max(0, min(BN, N - n0));
+  const int width = min(E.R - j0, kLoraK), pieces = (width + 15) / 16 * 2;
+  const int pc = tid & 7, r0 = tid >> 3;
+  const bool in = pc * 8 < width;
+  if (tid == 0) S.any[~stage & 1] = 0;  // (the stage before is read)
+  const __amdgpu_buffer_rsrc_t rt = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint32_t*>(E.t + (int64_t)m0 * E.R), 0, rows * E.R * 4, kBufferRsrcWord3);
+  const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint16_t*>(E.b + ((int64_t)d * N + n0) * E.R), 0, cols * E.R * 2, kBufferRsrcWord3);
+#pragma unroll
+  for (int i0 = 0; i0 < BM * 8 / NT; i0 += AHEAD) {
+    u32x4 t0[AHEAD], t1[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int r = (i0 + i) * (NT / 8) + r0;
+      const uint32_t o = in && S.adapter[r] == d ? (uint32_t)(r * E.R + j0 + pc * 8) * 4u : kOut;
+      t0[i] = __builtin_amdgcn_raw_buffer_load_b128(rt, o, 0, 0);
+      t1[i] = __builtin_amdgcn_raw_buffer_load_b128(rt, o + 16u, 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (pc < pieces) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int r = (i0 + i) * (NT / 8) + r0;
+        bf16x8 hi, lo;
+        lora_split(t0[i], t1[i], &hi, &lo);
+        *reinterpret_cast<u32x4*>(As + r * LDK + pc * 8) = __builtin_bit_cast(u32x4, hi);
+        *reinterpret_cast<u32x4*>(As + (BM + r) * LDK + pc * 8) = __builtin_bit_cast(u32x4, lo);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int i0 = 0; i0 < BN * 8 / NT; i0 += AHEAD) {
+    u32x4 b[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int c = (i0 + i) * (NT / 8) + r0;
+      b[i] = __builtin_amdgcn_raw_buffer_load_b128(rb, in ? (uint32_t)(c * E.R + j0 + pc * 8) * 2u : kOut, 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int c = (i0 + i) * (NT / 8) + r0;
+      if (mixed) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool lo = (b[i][e] & 0x7F80u) == 0x7F80u, hi = (b[i][e] & 0x7F800000u) == 0x7F800000u;
+          if (lo || hi) {
+            S.bad[c] = 1;
+            S.any[stage & 1] = 1;
+            b[i][e] = (lo ? 0u : b[i][e] & 0xFFFFu) | (hi ? 0u : b[i][e] & 0xFFFF0000u);
+          }
+        }
+      }
+      if (pc < pieces) *reinterpret_cast<u32x4*>(Bs + c * LDK + pc * 8) = b[i];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// The last step of an adapter with columns noted.
+template <int BM, int BN, int NT>
+__device__ __forceinline__ void lora_stage_bad(LoraLds<BM, BN>& S, uint16_t* As, uint16_t* Bs, int tid, int d) {
+  constexpr uint32_t kBig = 0x7F7Fu;  // the largest bf16
+  for (int i = tid; i < 2 * BM; i += NT) {
+    const u32x4 v = {i < BM && S.adapter[i] == d ? (kBig | 0x8000u) << 16 | kBig : 0u, 0u, 0u, 0u};
+    *reinterpret_cast<u32x4*>(As + i * LDK) = v;
+    *reinterpret_cast<u32x4*>(As + i * LDK + 8) = u32x4{0u, 0u, 0u, 0u};
+  }
+  for (int i = tid; i < BN; i += NT) {
+    const u32x4 v = {S.bad[i] ? kBig << 16 | kBig : 0u, 0u, 0u, 0u};
+    S.bad[i] = 0;
+    *reinterpret_cast<u32x4*>(Bs + i * LDK) = v;
+    *reinterpret_cast<u32x4*>(Bs + i * LDK + 8) = u32x4{0u, 0u, 0u, 0u};
+  }
+}
+
+// Every wave's walk over the tile's adapters: stage(d, mixed, j0, n) (j0 < 0: lora_stage_bad), a barrier, take(steps of 16), a
+// barrier. Roles that do not stage or take pass functions that do nothing.
+template <int BM, int BN, class Stage, class Take>
+__device__ __forceinline__ void lora_walk(const LoraLds<BM, BN>& S, int R, Stage&& stage, Take&& take) {
+  TileAdapters<BM> list(S.adapter);
+  int d, n = 0;
+  bool mixed;
+  while (list.next(&d, &mixed)) {
+    int bad = 0;
+    for (int j0 = 0; j0 < R; j0 += kLoraK, ++n) {
+      stage(d, mixed, j0, n);
+      __syncthreads();
+      bad |= *const_cast<const volatile int*>(&S.any[n & 1]);
+      take((min(R - j0, kLoraK) + 15) / 16);
+      __syncthreads();
+    }
+    if (__builtin_amdgcn_readfirstlane(bad)) {
+      stage(d, mixed, -1, n);
+      __syncthreads();
+      take(1);
+      __syncthreads();
+    }
+  }
+}
+
+// A wave's part of the tile (I x J blocks of 32 from its row wr and column wc) takes the staged products.
+template <int BM, int I, int J>
+__device__ __forceinline__ void lora_take(const uint16_t* As, const uint16_t* Bs, f32x16 (&acc)[I][J], int steps, int wr,
+                                          int wc) {
+  const int lane = threadIdx.x & 63, lrow = lane & 31, lk = (lane >> 5) * 8;
+#pragma unroll 1
+  for (int ks = 0; ks < steps; ++ks) {
+    bf16x8 Bf[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) Bf[j] = as_bf16x8(*reinterpret_cast<const u32x4*>(Bs + (wc + j * 32 + lrow) * LDK + ks * 16 + lk));
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        const bf16x8 Af =
+            as_bf16x8(*reinterpret_cast<const u32x4*>(As + (half * BM + wr + i * 32 + lrow) * LDK + ks * 16 + lk));
+#pragma unroll
+        for (int j = 0; j < J; ++j) acc[i][j] = Mfma<32>::mma(Af, Bf[j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);  // (fragments read far ahead would spill accumulators)
+      }
+  }
+}
+
 // Partial-tile item e (f32x4) of a wave's accumulators: item ((((wave * I + i) * J + j) * 4 + rq)
 // * 64 + lane) holds acc[i][j][4 rq .. 4 rq + 3] of that lane.
 template <class C>
@@ -136,12 +321,13 @@ __device__ __forceinline__ void part_item_coords(int e, int* m, int* n) {
 // out). The 128 x 128 configuration with D = 2 is held to 128 VGPRs so that two workgroups share a
 // CU (the quarter tiles of full-tile launches); stream-K launches with SB8 use D = 4 at one
 // workgroup per CU.
-template <int BM, int BN, bool SB8, int D = 2>
+template <int BM, int BN, bool SB8, int D, bool LORA>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(BM == 128 && D == 2 ? 4 : 2)))
 void gemm_kernel(GemmParams P) {
   static_assert(D == 2 || (SB8 && D == 4), "raw ring depth: its index must be static in the loop unrolled by 8");
   using C = GemmCfg<BM, BN>;
   constexpr int I = C::I, J = C::J, AJ = C::AJ, WPT = C::WPT, LDC = C::LDC;
+  __shared__ int s_lora[LORA ? sizeof(LoraLds<BM, BN>) / sizeof(int) : 1];
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   uint16_t* As = smem;                    // [2][BM * LDK]
   uint16_t* Bs = smem + 2 * BM * LDK;     // [2][BN * LDK]
@@ -398,6 +584,21 @@ void gemm_kernel(GemmParams P) {
   // so a chunk is entirely inside or outside).
   auto write_tile = [&](int m0, int n0) __attribute__((always_inline)) {
     uint16_t* Cs = smem;
+    if constexpr (LORA) {
+      LoraLds<BM, BN>& S = *reinterpret_cast<LoraLds<BM, BN>*>(s_lora);
+      static_assert(kThreads >= BM && kThreads >= BN, "a thread per row and column of the tile");
+      S.init(P.lora, tid, m0, P.M);
+      __syncthreads();
+      lora_walk<BM, BN>(
+          S, P.lora.R,
+          [&](int d, bool mixed, int j0, int n) __attribute__((always_inline)) {
+            if (j0 < 0) lora_stage_bad<BM, BN, kThreads>(S, As, Bs, tid, d);
+            else lora_stage<BM, BN, kThreads, 2>(P.lora, S, As, Bs, tid, d, mixed, j0, n, m0, n0, P.M, P.N);
+          },
+          [&](int steps) __attribute__((always_inline)) {
+            lora_take<BM, I, J>(As, Bs, acc, steps, wm * C::WM, wn * C::WN);
+          });
+    }
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
@@ -479,7 +680,7 @@ void gemm_kernel(GemmParams P) {
 // checks the range): 64-bit divisions per thread and contributor took part of its time:
 // 203 x 5120 -> 17408 69.6 -> 68.0 us, 333 x 5120 -> 5120 42.4 -> 41.6, others within 1%.
 constexpr int kSkRedThreads = 256;
-template <int BM, int BN>
+template <int BM, int BN, bool LORA>
 __global__ __launch_bounds__(kSkRedThreads) void gemm_sk_reduce_kernel(GemmParams P, int G) {
   using C = GemmCfg<BM, BN>;
   static_assert(C::kPartF4 % kSkRedThreads == 0, "whole blocks per tile");
@@ -502,6 +703,11 @@ __global__ __launch_bounds__(kSkRedThreads) void gemm_sk_reduce_kernel(GemmParam
   int mi, ni;
   part_item_coords<C>(e, &mi, &ni);
   const int n = n0 + ni;
+  f32x4 add = {0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (LORA) {
+    const int lane = threadIdx.x & 63, rq = e >> 6 & 3;
+    add = lora_part32(P.lora, m0 + mi - 8 * rq - 4 * (lane >> 5), rq, n, P.M, P.N);
+  }
   if (n >= P.N || m0 + mi >= P.M) return;
   const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc(
       P.part, 0, rsrc_bytes((unsigned long long)G * 2 * C::kPartF4 * 16), kBufferRsrcWord3);
@@ -515,6 +721,9 @@ __global__ __launch_bounds__(kSkRedThreads) void gemm_sk_reduce_kernel(GemmParam
         f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, (uint32_t)e * 16u, (int)(slot * (uint32_t)(C::kPartF4 * 16)), 0));
     sum[0] += v[0]; sum[1] += v[1]; sum[2] += v[2]; sum[3] += v[3];
   }
+  if constexpr (LORA) {
+    sum[0] += add[0]; sum[1] += add[1]; sum[2] += add[2]; sum[3] += add[3];
+  }
   const __amdgpu_buffer_rsrc_t ry = __builtin_amdgcn_make_buffer_rsrc(
       P.y, 0, rsrc_bytes((unsigned long long)P.M * P.N * 2), kBufferRsrcWord3);
 #pragma unroll
@@ -526,14 +735,20 @@ __global__ __launch_bounds__(kSkRedThreads) void gemm_sk_reduce_kernel(GemmParam
   }
 }
 
-template <int BM, int BN, bool SB8, int D = 2>
-hipError_t launch_tiles(const GemmParams& P, int blocks, hipStream_t stream) {
+template <int BM, int BN, bool SB8, int D, bool LORA>
+hipError_t launch_tiles_l(const GemmParams& P, int blocks, hipStream_t stream) {
   constexpr size_t smem = GemmCfg<BM, BN>::kSmem;
   static LdsAllowance lds;
-  const hipError_t e = lds.allow(reinterpret_cast<const void*>(&gemm_kernel<BM, BN, SB8, D>), smem);
+  const hipError_t e = lds.allow(reinterpret_cast<const void*>(&gemm_kernel<BM, BN, SB8, D, LORA>), smem);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((gemm_kernel<BM, BN, SB8, D>), dim3(blocks), dim3(kThreads), smem, stream, P);
+  hipLaunchKernelGGL((gemm_kernel<BM, BN, SB8, D, LORA>), dim3(blocks), dim3(kThreads), smem, stream, P);
   return hipGetLastError();
+}
+
+template <int BM, int BN, bool SB8, int D = 2>
+hipError_t launch_tiles(const GemmParams& P, int blocks, hipStream_t stream) {
+  return P.lora.t ? launch_tiles_l<BM, BN, SB8, D, true>(P, blocks, stream)
+                  : launch_tiles_l<BM, BN, SB8, D, false>(P, blocks, stream);
 }
 
 // 256 x 256 tiles with K % 512 == 0 (whole, or stream-K segments), waves split by role: waves 0-7
@@ -549,10 +764,14 @@ hipError_t launch_tiles(const GemmParams& P, int blocks, hipStream_t stream) {
 constexpr int kWsProd = 4;                                  // producer waves
 constexpr int kWsThreads = 64 * (kWaves + kWsProd);
 constexpr int kWsD = 2;                                     // K steps of raw inputs in registers
+template <bool LORA>
 __global__ __launch_bounds__(kWsThreads) __attribute__((amdgpu_waves_per_eu(3)))
 void gemm_ws_kernel(GemmParams P) {
   using C = GemmCfg<256, 256>;
   constexpr int BM = 256, BN = 256, I = C::I, J = C::J, LDC = C::LDC;
+  __shared__ int s_lora[LORA ? sizeof(LoraLds<BM, BN>) / sizeof(int) : 1];
+  [[maybe_unused]] LoraLds<BM, BN>& S = *reinterpret_cast<LoraLds<BM, BN>*>(s_lora);
+  static_assert(64 * kWsProd == BM, "a producer thread per row of the tile");
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   uint16_t* As = smem;
   uint16_t* Bs = smem + 2 * BM * LDK;
@@ -624,7 +843,7 @@ void gemm_ws_kernel(GemmParams P) {
     }
   };
   // Every segment passes the same barriers in both roles: one after the producers' prologue, one
-  // per K step, one between the bf16 tile's LDS writes and its stores (whole tiles), one at the end
+  // per K step, (LORA: one and those of lora_walk,) one between the bf16 tile's LDS writes and its stores (whole tiles), one at the end
   // (the next segment's prologue reuses the LDS stages and the output tile).
 
   if (mma) {
@@ -669,6 +888,14 @@ void gemm_ws_kernel(GemmParams P) {
       if (kb == 0 && ke == nk) {
         // The tile as bf16 into LDS (every wave is past the last step's reads).
         uint16_t* Cs = smem;
+        if constexpr (LORA) {
+          __syncthreads();  // the producers have noted the rows' adapters
+          lora_walk<BM, BN>(
+              S, P.lora.R, [](int, bool, int, int) {},
+              [&](int steps) __attribute__((always_inline)) {
+                lora_take<BM, I, J>(As, Bs, acc, steps, wm * C::WM, wn * C::WN);
+              });
+        }
 #pragma unroll
         for (int i = 0; i < I; ++i)
 #pragma unroll
@@ -791,6 +1018,17 @@ void gemm_ws_kernel(GemmParams P) {
       bcur = bnext;
     }
     if (kb == 0 && ke == nk) {
+      if constexpr (LORA) {
+        S.init(P.lora, pt, m0, P.M);
+        __syncthreads();
+        lora_walk<BM, BN>(
+            S, P.lora.R,
+            [&](int d, bool mixed, int j0, int n) __attribute__((always_inline)) {
+              if (j0 < 0) lora_stage_bad<BM, BN, 64 * kWsProd>(S, As, Bs, pt, d);
+              else lora_stage<BM, BN, 64 * kWsProd, 8>(P.lora, S, As, Bs, pt, d, mixed, j0, n, m0, n0, P.M, P.N);
+            },
+            [](int) {});
+      }
       __syncthreads();  // the MFMA waves' bf16 tile is in LDS
       store_chunks(m0, n0);
     }
@@ -798,13 +1036,18 @@ void gemm_ws_kernel(GemmParams P) {
   });
 }
 
-hipError_t launch_ws(const GemmParams& P, int blocks, hipStream_t stream) {
+template <bool LORA>
+hipError_t launch_ws_l(const GemmParams& P, int blocks, hipStream_t stream) {
   constexpr size_t smem = GemmCfg<256, 256>::kSmem;
   static LdsAllowance lds;
-  const hipError_t e = lds.allow(reinterpret_cast<const void*>(&gemm_ws_kernel), smem);
+  const hipError_t e = lds.allow(reinterpret_cast<const void*>(&gemm_ws_kernel<LORA>), smem);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(gemm_ws_kernel, dim3(blocks), dim3(kWsThreads), smem, stream, P);
+  hipLaunchKernelGGL(gemm_ws_kernel<LORA>, dim3(blocks), dim3(kWsThreads), smem, stream, P);
   return hipGetLastError();
+}
+
+hipError_t launch_ws(const GemmParams& P, int blocks, hipStream_t stream) {
+  return P.lora.t ? launch_ws_l<true>(P, blocks, stream) : launch_ws_l<false>(P, blocks, stream);
 }
 
 template <int BM, int BN>
@@ -812,7 +1055,11 @@ hipError_t launch_sk_reduce(const GemmParams& P, int G, hipStream_t stream) {
   // The kernel's 32-bit owner arithmetic: (U + 1) (G + 1) below 2^32.
   if ((unsigned long long)(P.U + 1) * (unsigned long long)(G + 1) >= 1ULL << 32) return hipErrorInvalidValue;
   const long long blocks = (long long)P.sk_tiles * (GemmCfg<BM, BN>::kPartF4 / kSkRedThreads);
-  hipLaunchKernelGGL((gemm_sk_reduce_kernel<BM, BN>), dim3((unsigned)blocks), dim3(kSkRedThreads), 0, stream, P, G);
+  const dim3 grid((unsigned)blocks);
+  if (P.lora.t)
+    hipLaunchKernelGGL((gemm_sk_reduce_kernel<BM, BN, true>), grid, dim3(kSkRedThreads), 0, stream, P, G);
+  else
+    hipLaunchKernelGGL((gemm_sk_reduce_kernel<BM, BN, false>), grid, dim3(kSkRedThreads), 0, stream, P, G);
   return hipGetLastError();
 }
 
@@ -830,8 +1077,8 @@ int sk_occupancy(bool sb8) {
   static int occ[2] = {0, 0};
   int& o = occ[sb8 ? 1 : 0];
   if (o == 0)
-    o = resident_per_cu(sb8 ? reinterpret_cast<const void*>(&gemm_kernel<128, 128, true, kSkRing>)
-                            : reinterpret_cast<const void*>(&gemm_kernel<128, 128, false>),
+    o = resident_per_cu(sb8 ? reinterpret_cast<const void*>(&gemm_kernel<128, 128, true, kSkRing, false>)
+                            : reinterpret_cast<const void*>(&gemm_kernel<128, 128, false, 2, false>),
                         GemmCfg<128, 128>::kSmem);
   return o;
 }
@@ -840,7 +1087,7 @@ int sk_occupancy(bool sb8) {
 int sk_wide_occupancy() {
   static int o = 0;
   if (o == 0)
-    o = resident_per_cu(reinterpret_cast<const void*>(&gemm_kernel<128, 256, true, kSkRing>), GemmCfg<128, 256>::kSmem);
+    o = resident_per_cu(reinterpret_cast<const void*>(&gemm_kernel<128, 256, true, kSkRing, false>), GemmCfg<128, 256>::kSmem);
   return o;
 }
 
@@ -983,8 +1230,10 @@ bool gemm_plan(int M, int N, int K, int cus, size_t ws_capacity, const uint16_t*
 }
 
 hipError_t launch_gemm(const GemmPlan& plan, const uint16_t* x, const uint32_t* w, const uint16_t* s, const uint16_t* b,
-                       uint16_t* y, float* part, int M, int N, int K, int cus, hipStream_t stream) {
+                       uint16_t* y, float* part, int M, int N, int K, int cus, hipStream_t stream,
+                       const LoraAdd* lora) {
   GemmParams P;
+  P.lora = lora ? *lora : LoraAdd{};
   P.x = x; P.w = w; P.s = s; P.b = b; P.y = y;
   P.M = M; P.N = N; P.K = K;
   P.sk = 0; P.sk_tiles = 0; P.upt = 0; P.ups = 0; P.U = 0; P.part = part;

@@ -7,6 +7,10 @@
 
 namespace qmm4 {
 
+// A low-rank product added to the fp32 sums of y = x @ dequant(w)^T before they are rounded (qmm_requests_kernels.h);
+// the launches below take one, or null.
+struct LoraAdd;
+
 // Skinny (M <= 64) stream-K kernel geometry, chosen by M, K and the scale/bias alignment.
 struct SkinnyPlan {
   int variant;      // index into the kernel table (see qmm4_skinny.hip)
@@ -29,7 +33,7 @@ int skinny_occupancy(int variant);
 // Enqueue the skinny kernel. `part` holds blocks*2*M*tile_cols floats, `cnt` tiles zeroed uint32s.
 hipError_t launch_skinny(const SkinnyPlan& plan, const uint16_t* x, const uint32_t* w,
                          const uint16_t* s, const uint16_t* b, uint16_t* y, float* part,
-                         uint32_t* cnt, int M, int N, int K, hipStream_t stream);
+                         uint32_t* cnt, int M, int N, int K, hipStream_t stream, const LoraAdd* lora = nullptr);
 
 // Verify-shape kernel (M <= 64): tiles of output columns shared by the waves of a workgroup, which
 // split each tile's k-steps round-robin; stream-K ranges over (tile, step) units.
@@ -54,7 +58,7 @@ bool verify_plan(int M, int N, int K, int vmax, int cus, int occ, VerifyPlan* pl
 // `part` holds plan.part_bytes, `cnt` tiles zeroed uint32s.
 hipError_t launch_verify(const VerifyPlan& plan, const uint16_t* x, const uint32_t* w, const uint16_t* s,
                          const uint16_t* b, uint16_t* y, float* part, uint32_t* cnt, int M, int N, int K,
-                         hipStream_t stream);
+                         hipStream_t stream, const LoraAdd* lora = nullptr);
 
 // Row-phase kernel (M <= 64): each workgroup owns a range of 16-row weight blocks and a range of
 // K phases; x and the scales are staged per phase in LDS; K is split when N is small.
@@ -72,9 +76,10 @@ struct RowPhasePlan {
 };
 bool rowphase_plan(int M, int N, int K, int cus, RowPhasePlan* plan, bool fused = false);
 // `part` holds plan.part_bytes (used when plan.S > 1: the partial tiles, added by a second kernel
-// launched behind the first on the same stream). A fused plan writes y as [M, N / 2].
+// launched behind the first on the same stream). A fused plan writes y as [M, N / 2] (no `lora`).
 hipError_t launch_rowphase(const RowPhasePlan& plan, const uint16_t* x, const uint32_t* w, const uint16_t* s,
-                           const uint16_t* b, uint16_t* y, float* part, int M, int N, int K, hipStream_t stream);
+                           const uint16_t* b, uint16_t* y, float* part, int M, int N, int K, hipStream_t stream,
+                           const LoraAdd* lora = nullptr);
 
 // Row-split kernel (up to 16 rows, output columns split evenly over one workgroup per CU, K whole
 // or in a few slices).
@@ -117,10 +122,10 @@ struct RowSplitNorm {
 // the 9-16-row form).
 bool rowsplit_norm_ok(const RowSplitPlan& plan, int M, int K);
 // part / cnt: the workspace (plan.part_bytes, plan.ranges counters at zero) when plan.KS > 1.
-// `norm` (optional, rowsplit_norm_ok): x is normalised as it is staged.
+// `norm` (optional, rowsplit_norm_ok): x is normalised as it is staged. `lora`: not with `norm` or a fused plan.
 hipError_t launch_rowsplit(const RowSplitPlan& plan, const uint16_t* x, const uint32_t* w, const uint16_t* s,
                            const uint16_t* b, uint16_t* y, float* part, uint32_t* cnt, int M, int N, int K,
-                           hipStream_t stream, const RowSplitNorm* norm = nullptr);
+                           hipStream_t stream, const RowSplitNorm* norm = nullptr, const LoraAdd* lora = nullptr);
 
 // y[m, j] = silu_mul_bf16(t[m, j], t[m, n + j]) for t bf16 [M, 2n] (the unfused gate+up epilogue).
 hipError_t launch_silu_mul(const uint16_t* t, uint16_t* y, int M, int n, hipStream_t stream);
@@ -153,7 +158,7 @@ bool gemm_plan(int M, int N, int K, int cus, size_t ws_capacity, const uint16_t*
                GemmPlan* plan);
 hipError_t launch_gemm(const GemmPlan& plan, const uint16_t* x, const uint32_t* w, const uint16_t* s,
                        const uint16_t* b, uint16_t* y, float* part, int M, int N, int K, int cus,
-                       hipStream_t stream);
+                       hipStream_t stream, const LoraAdd* lora = nullptr);
 
 // Bit-exact dequantization to bf16 [N, K]: 4-bit codes in groups of 64 (the packed kernels'
 // format), or 2-, 4- or 8-bit codes in groups of 32, 64 or 128 (K % group_size == 0).
@@ -163,6 +168,7 @@ hipError_t launch_dequant(const uint32_t* w, const uint16_t* s, const uint16_t* 
 // y = x @ dequant(w)^T in the formats and shapes the packed kernels do not take: 2-, 4- or 8-bit codes
 // in groups of 32, 64 or 128, any N, K % 64 == 0; x, w, the scales and the biases each below 2 GiB.
 hipError_t launch_general(const uint16_t* x, const uint32_t* w, const uint16_t* s, const uint16_t* b, uint16_t* y,
-                          int M, int N, int K, int group_size, int bits, int cus, hipStream_t stream);
+                          int M, int N, int K, int group_size, int bits, int cus, hipStream_t stream,
+                          const LoraAdd* lora = nullptr);
 
 }  // namespace qmm4

@@ -36,6 +36,7 @@
 
 #include "qmm4_common.h"
 #include "qmm4_kernels.h"
+#include "qmm_lora.h"
 #include "qmm4_offsets.h"
 
 namespace qmm4 {
@@ -57,6 +58,7 @@ struct RowPhaseParams {
   int NP;         // phases along K
   int ranges;     // block ranges
   int fused;      // gate+up with the SiLU·mul epilogue (wide plans): w stacks [gate; up], y is [M, N / 2]
+  LoraAdd lora;   // LORA: added to the sums
 };
 
 template <int MB_, int V_, int BPW_, int W_, int STG_ = 3, bool OPT_ = false>
@@ -98,7 +100,7 @@ struct RpCfg {
 // Device-coherent 16-byte stores and loads (cache policy sc1: coherent across the XCDs' L2s).
 constexpr int kCoherent = 16;
 
-template <class C>
+template <class C, bool LORA>
 __global__ __launch_bounds__(C::kRpThreads) __attribute__((amdgpu_waves_per_eu(C::kRpWaves / 4)))
 void rowphase_kernel(RowPhaseParams P) {
   constexpr int MB = C::MB, MP = C::MP, V = C::V, BPW = C::BPW, RW = C::RW;
@@ -426,12 +428,15 @@ void rowphase_kernel(RowPhaseParams P) {
       if (j < nbw) {
         const int col = 16 * (wave + kRpWaves * j) + n;
 #pragma unroll
-        for (int ii = 0; ii < MB; ++ii)
+        for (int ii = 0; ii < MB; ++ii) {
+          f32x4 v = a[j][ii];
+          if constexpr (LORA) v = lora_tile16(P.lora, v, ii * 16, r0 + col, P.M, P.N);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int m = ii * 16 + 4 * g + r;
-            yt[m * RW + col] = (uint16_t)(pack_bf16x2(a[j][ii][r], 0.0f) & 0xFFFFu);
+            yt[m * RW + col] = (uint16_t)(pack_bf16x2(v[r], 0.0f) & 0xFFFFu);
           }
+        }
       }
     }
   };
@@ -472,7 +477,7 @@ void rowphase_kernel(RowPhaseParams P) {
 // one CU took 6.5-7.6 us at the end of the batched-verify down projection; spread over the GPU
 // the same bytes take a few microseconds.
 constexpr int kRedThreads = 256;
-template <class C>
+template <class C, bool LORA>
 __global__ __launch_bounds__(kRedThreads) void rowphase_reduce_kernel(RowPhaseParams P) {
   constexpr int MB = C::MB, BPW = C::BPW, kRpWaves = C::kRpWaves;
   const int ranges = P.ranges;
@@ -521,7 +526,8 @@ __global__ __launch_bounds__(kRedThreads) void rowphase_reduce_kernel(RowPhasePa
     }
     return sum;
   };
-  const f32x4 sum = add_slices(item);
+  f32x4 sum = add_slices(item);
+  if constexpr (LORA) sum = lora_tile16(P.lora, sum, ii * 16, col, P.M, P.N);
   const int ny = fused ? P.N >> 1 : P.N;  // columns of y
   const __amdgpu_buffer_rsrc_t ry = __builtin_amdgcn_make_buffer_rsrc(
       P.y, 0, rsrc_bytes((unsigned long long)P.M * ny * 2), kBufferRsrcWord3);
@@ -604,10 +610,10 @@ static bool rowphase_geometry(int id, int* mb, int* v, int* bpw, size_t* lds, in
   }
 }
 
-static const void* rowphase_func(int id) {
+static const void* rowphase_func(int id, bool lora) {
   switch (id) {
 #define QMM4_RPF(i, m, vv, b, w, stg, opt) \
-  case i: return reinterpret_cast<const void*>(&rowphase_kernel<RpCfg##i>);
+  case i: return reinterpret_cast<const void*>(lora ? (const void*)&rowphase_kernel<RpCfg##i, true> : (const void*)&rowphase_kernel<RpCfg##i, false>);
     QMM4_ROWPHASE_VARIANTS(QMM4_RPF)
 #undef QMM4_RPF
     default: return nullptr;
@@ -768,8 +774,12 @@ bool rowphase_plan(int M, int N, int K, int cus, RowPhasePlan* plan, bool fused)
 }
 
 hipError_t launch_rowphase(const RowPhasePlan& plan, const uint16_t* x, const uint32_t* w, const uint16_t* s,
-                           const uint16_t* b, uint16_t* y, float* part, int M, int N, int K, hipStream_t stream) {
+                           const uint16_t* b, uint16_t* y, float* part, int M, int N, int K, hipStream_t stream,
+                           const LoraAdd* lora) {
+  if (lora && plan.fused) return hipErrorInvalidValue;
+  const bool in_kernel = lora && plan.S == 1;  // else in the reduce kernel
   RowPhaseParams P;
+  P.lora = lora ? *lora : LoraAdd{};
   P.x = x; P.s = s; P.b = b; P.w = w; P.y = y; P.part = part;
   P.M = M; P.N = N; P.K = K;
   P.NB = N / 16; P.BW = plan.BW; P.S = plan.S; P.NP = plan.NP; P.ranges = plan.ranges;
@@ -780,24 +790,31 @@ hipError_t launch_rowphase(const RowPhasePlan& plan, const uint16_t* x, const ui
     if (!rowphase_geometry(plan.variant, &cm, &cv, &cb, &l, &items) || cm > 6 || plan.BW % 2 != 0 || N % 32 != 0)
       return hipErrorInvalidValue;
   }
-  const void* f = rowphase_func(plan.variant);
+  const void* f = rowphase_func(plan.variant, in_kernel);
   if (!f) return hipErrorInvalidValue;
   hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)plan.lds);
   if (e != hipSuccess) return e;
   // K split: the reduce kernel's grid has one thread per f32x4 item of every range's tile.
   switch (plan.variant) {
 #define QMM4_RPL(i, m, vv, bb, w, stg, opt)                                                                   \
-  case i:                                                                                                   \
-    hipLaunchKernelGGL(rowphase_kernel<RpCfg##i>, dim3(plan.blocks), dim3(RpCfg##i::kRpThreads), plan.lds,   \
-                       stream, P);                                                                          \
+  case i: {                                                                                                 \
+    const dim3 grid((unsigned)plan.blocks), block(RpCfg##i::kRpThreads);                                    \
+    if (in_kernel)                                                                                          \
+      hipLaunchKernelGGL((rowphase_kernel<RpCfg##i, true>), grid, block, plan.lds, stream, P);              \
+    else                                                                                                    \
+      hipLaunchKernelGGL((rowphase_kernel<RpCfg##i, false>), grid, block, plan.lds, stream, P);             \
     if (plan.S > 1) {                                                                                       \
       e = hipGetLastError();                                                                                \
       if (e != hipSuccess) return e;                                                                        \
       const long long items = (long long)plan.ranges * RpCfg##i::kItems;                                    \
-      hipLaunchKernelGGL(rowphase_reduce_kernel<RpCfg##i>, dim3((unsigned)((items + kRedThreads - 1) / kRedThreads)), \
-                         dim3(kRedThreads), 0, stream, P);                                                  \
+      const dim3 rgrid((unsigned)((items + kRedThreads - 1) / kRedThreads));                                \
+      if (lora)                                                                                             \
+        hipLaunchKernelGGL((rowphase_reduce_kernel<RpCfg##i, true>), rgrid, dim3(kRedThreads), 0, stream, P);  \
+      else                                                                                                  \
+        hipLaunchKernelGGL((rowphase_reduce_kernel<RpCfg##i, false>), rgrid, dim3(kRedThreads), 0, stream, P); \
     }                                                                                                       \
-    break;
+    break;                                                                                                  \
+  }
     QMM4_ROWPHASE_VARIANTS(QMM4_RPL)
 #undef QMM4_RPL
     default: return hipErrorInvalidValue;

@@ -49,6 +49,7 @@
 
 #include "qmm4_common.h"
 #include "qmm4_kernels.h"
+#include "qmm_lora.h"
 #include "qmm4_lds.h"
 
 namespace qmm4 {
@@ -107,6 +108,7 @@ struct RowSplitParams {
   uint16_t* h_out;     // h = bf16(x + r), bf16 [M, K] (written by workgroup 0)
   uint16_t* n_out;     // n = rmsnorm(h) * nw, bf16 [M, K] (written by workgroup 0)
   float eps;
+  LoraAdd lora;  // LORA: added to the sums
 };
 
 // The most K slices of a plan; the merge of a column range holds them all at once.
@@ -171,7 +173,7 @@ __host__ __device__ inline size_t rowsplit_red_offset(int Kp, int MP, int units,
 // for more waves per SIMD than the one workgroup of a CU has, each LDS read then waited for before the next:
 // so the attribute ends at the workgroup's own waves there (6 rows of the fused 2048 -> 24576 / 1536 -> 65536
 // 10.9 / 16.3 -> 10.3 / 15.8 us).
-template <int MP, int V, bool FUSED, bool KSPLIT, bool SMALL, bool NORM, int PAIR, bool OWN, int XB>
+template <int MP, int V, bool FUSED, bool KSPLIT, bool SMALL, bool NORM, int PAIR, bool OWN, int XB, bool LORA>
 __global__ __launch_bounds__(kRsThreads)
 __attribute__((amdgpu_waves_per_eu(kRsWaves / 4, MP > 4 && XB == kRsFewX && !SMALL && !OWN ? kRsWaves / 4 : 8)))
 void rowsplit_kernel(RowSplitParams P) {
@@ -527,6 +529,7 @@ void rowsplit_kernel(RowSplitParams P) {
       fetch(j, u);
       if (st == SU - 1) {
         const int col = r0 + b * 16 + n;
+        if constexpr (LORA) acc = lora_tile16(P.lora, acc, 0, col, P.M, P.N);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int m = 4 * g + r;
@@ -612,6 +615,13 @@ void rowsplit_kernel(RowSplitParams P) {
       unit(ub, std::integral_constant<int, 1>{});
     }
   }
+  // LORA: what this thread's first output column takes of the adapters, while other waves still stream.
+  bool first_item = true;
+  f32x4 first_add = {0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (LORA) {
+    const int gg = G == 1 ? 0 : tid / P.R, col = r0 + tid - gg * P.R;
+    if (tid < P.R * G && col < r1 && 4 * gg < P.M) first_add = lora_rows4(P.lora, first_add, 4 * gg, col, P.M, P.N);
+  }
   __syncthreads();
 
   // y[m, col] = sum over the block's steps, in step order, of its unit slots; element r of a slot's
@@ -628,7 +638,15 @@ void rowsplit_kernel(RowSplitParams P) {
     }
     return sum;
   };
-  auto write = [&](int col, int gg, const f32x4& sum, const f32x4& sup) __attribute__((always_inline)) {
+  auto write = [&](int col, int gg, f32x4 sum, const f32x4& sup) __attribute__((always_inline)) {
+    if constexpr (LORA) {
+      if (first_item) {
+        sum[0] += first_add[0]; sum[1] += first_add[1]; sum[2] += first_add[2]; sum[3] += first_add[3];
+        first_item = false;
+      } else {
+        sum = lora_rows4(P.lora, sum, 4 * gg, col, P.M, P.N);
+      }
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int m = 4 * gg + r;
@@ -736,6 +754,7 @@ constexpr size_t kXrSc = kXrMaxRB * 2 * 16 * 16;  // LDS bytes of a chunk's scal
 // Dynamic LDS: [chunk][block][4 groups][16 lanes] f32x4 sums, then per wave its half chunk of x and
 // its scales and biases.
 __host__ __device__ inline size_t xreg_part_bytes(int SU) { return (size_t)SU * kXrMaxRB * 4 * 16 * 16; }
+template <bool LORA>
 __global__ __launch_bounds__(64 * kXrMaxWaves) __attribute__((amdgpu_waves_per_eu(3)))
 void rowsplit_xreg_kernel(RowSplitParams P) {
   constexpr int V = kXrV;
@@ -851,6 +870,12 @@ void rowsplit_xreg_kernel(RowSplitParams P) {
 #pragma unroll
   for (int b = 0; b < kXrMaxRB; ++b)
     if (b < RB) part[((st * kXrMaxRB + b) * 4 + g) * 16 + n] = acc[b];
+  // LORA: what this thread's first output column takes of the adapters, while other waves are at their chunks.
+  f32x4 first_add = {0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (LORA) {
+    if (tid < P.R * 4 && r0 + (tid >> 2) < r1 && 4 * (tid & 3) < P.M)
+      first_add = lora_rows4(P.lora, first_add, 4 * (tid & 3), r0 + (tid >> 2), P.M, P.N);
+  }
   __syncthreads();
 
   // y[m, col]: the chunk sums of the column's block in chunk order; output row m = 4 g + r.
@@ -865,6 +890,13 @@ void rowsplit_xreg_kernel(RowSplitParams P) {
     for (int st = 0; st < SU; ++st) {
       const f32x4 v = part[((st * kXrMaxRB + b) * 4 + gg) * 16 + nn];
       sum[0] += v[0]; sum[1] += v[1]; sum[2] += v[2]; sum[3] += v[3];
+    }
+    if constexpr (LORA) {
+      if (it == tid) {
+        sum[0] += first_add[0]; sum[1] += first_add[1]; sum[2] += first_add[2]; sum[3] += first_add[3];
+      } else {
+        sum = lora_rows4(P.lora, sum, 4 * gg, col, P.M, P.N);
+      }
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -1041,15 +1073,24 @@ size_t rowsplit_smem(const RowSplitPlan& plan, bool norm) {
                                  sizeof(float) * plan.MP * (kRsNormThreads / 64));
 }
 
-template <int MP, int V, bool FUSED, bool KSPLIT, bool SMALL, bool NORM, int PAIR, bool OWN, int XB>
-hipError_t launch_rowsplit_xb(const RowSplitPlan& plan, const RowSplitParams& P, hipStream_t stream) {
+template <int MP, int V, bool FUSED, bool KSPLIT, bool SMALL, bool NORM, int PAIR, bool OWN, int XB, bool LORA>
+hipError_t launch_rowsplit_xl(const RowSplitPlan& plan, const RowSplitParams& P, hipStream_t stream) {
   static LdsAllowance lds;
   const hipError_t e = lds.allow(
-      reinterpret_cast<const void*>(&rowsplit_kernel<MP, V, FUSED, KSPLIT, SMALL, NORM, PAIR, OWN, XB>), kRsLds);
+      reinterpret_cast<const void*>(&rowsplit_kernel<MP, V, FUSED, KSPLIT, SMALL, NORM, PAIR, OWN, XB, LORA>), kRsLds);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((rowsplit_kernel<MP, V, FUSED, KSPLIT, SMALL, NORM, PAIR, OWN, XB>), dim3(plan.blocks),
+  hipLaunchKernelGGL((rowsplit_kernel<MP, V, FUSED, KSPLIT, SMALL, NORM, PAIR, OWN, XB, LORA>), dim3(plan.blocks),
                      dim3(kRsThreads), rowsplit_smem(plan, NORM), stream, P);
   return hipGetLastError();
+}
+
+template <int MP, int V, bool FUSED, bool KSPLIT, bool SMALL, bool NORM, int PAIR, bool OWN, int XB>
+hipError_t launch_rowsplit_xb(const RowSplitPlan& plan, const RowSplitParams& P, hipStream_t stream) {
+  if (P.lora.t) {
+    if constexpr (FUSED || NORM) return hipErrorInvalidValue;
+    else return launch_rowsplit_xl<MP, V, FUSED, KSPLIT, SMALL, NORM, PAIR, OWN, XB, true>(plan, P, stream);
+  }
+  return launch_rowsplit_xl<MP, V, FUSED, KSPLIT, SMALL, NORM, PAIR, OWN, XB, false>(plan, P, stream);
 }
 
 template <int MP, int V, bool FUSED, bool KSPLIT, bool SMALL, bool NORM, int PAIR = 0, bool OWN = false>
@@ -1088,11 +1129,12 @@ hipError_t launch_rowsplit_m(const RowSplitPlan& plan, const RowSplitParams& P, 
                      : launch_rowsplit_k<MP, 4, false, NORM>(plan, P, stream);
 }
 
+template <bool LORA>
 hipError_t launch_rowsplit_xreg(const RowSplitPlan& plan, const RowSplitParams& P, hipStream_t stream) {
   static LdsAllowance lds;
-  const hipError_t e = lds.allow(reinterpret_cast<const void*>(&rowsplit_xreg_kernel), kRsLds);
+  const hipError_t e = lds.allow(reinterpret_cast<const void*>(&rowsplit_xreg_kernel<LORA>), kRsLds);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(rowsplit_xreg_kernel, dim3(plan.blocks), dim3(64 * plan.SU),
+  hipLaunchKernelGGL(rowsplit_xreg_kernel<LORA>, dim3(plan.blocks), dim3(64 * plan.SU),
                      plan.smem + (size_t)plan.SU * (kXrHalf + kXrSc), stream, P);
   return hipGetLastError();
 }
@@ -1104,7 +1146,7 @@ bool rowsplit_norm_ok(const RowSplitPlan& plan, int M, int K) {
 
 hipError_t launch_rowsplit(const RowSplitPlan& plan, const uint16_t* x, const uint32_t* w, const uint16_t* s,
                            const uint16_t* b, uint16_t* y, float* part, uint32_t* cnt, int M, int N, int K,
-                           hipStream_t stream, const RowSplitNorm* norm) {
+                           hipStream_t stream, const RowSplitNorm* norm, const LoraAdd* lora) {
   if (M > plan.MP || plan.KS > rs_max_ks(plan.MP)) return hipErrorInvalidValue;
   if (norm && !rowsplit_norm_ok(plan, M, K)) return hipErrorInvalidValue;
   RowSplitParams P;
@@ -1118,7 +1160,8 @@ hipError_t launch_rowsplit(const RowSplitPlan& plan, const uint16_t* x, const ui
   P.h_out = norm ? norm->h : nullptr;
   P.n_out = norm ? norm->n : nullptr;
   P.eps = norm ? norm->eps : 0.0f;
-  if (plan.xreg) return launch_rowsplit_xreg(plan, P, stream);
+  P.lora = lora ? *lora : LoraAdd{};
+  if (plan.xreg) return lora ? launch_rowsplit_xreg<true>(plan, P, stream) : launch_rowsplit_xreg<false>(plan, P, stream);
   if (norm) return launch_rowsplit_m<4, true>(plan, P, stream);
   switch (plan.MP) {
     case 4: return launch_rowsplit_m<4, false>(plan, P, stream);

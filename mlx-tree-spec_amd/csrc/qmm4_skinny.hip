@@ -37,6 +37,7 @@
 
 #include "qmm4_common.h"
 #include "qmm4_kernels.h"
+#include "qmm_lora.h"
 
 namespace qmm4 {
 
@@ -52,6 +53,7 @@ struct SkinnyParams {
   int NS;         // steps per tile = K / (128 * V)
   int G;          // workgroups
   long long U;    // units = T * NS
+  LoraAdd lora;   // LORA: added to the sums
 };
 
 template <int MP_, int V_, int CT_, int PF_, int WPE_, int XS_, int WAVES_ = 4>
@@ -171,7 +173,7 @@ __device__ __forceinline__ void store_x(u32x4* xs, const u32x4 (&xr)[C::kXR], in
 // Last arrival of a shared tile: y[:, tile] = bf16(sum of the contributors' fp32 partials), summed
 // in contributor order (deterministic). Loads go out in batches of kE elements x kQ contributors
 // per thread, all independent, so a batch costs one memory round trip.
-template <class C>
+template <class C, bool LORA>
 __device__ __forceinline__ void reduce_tile(const SkinnyParams& P, int t, int plo, int phi, int lo_slot) {
   constexpr int kE = 4, kQ = 4;
   const int total = P.M * C::CW;
@@ -204,6 +206,9 @@ __device__ __forceinline__ void reduce_tile(const SkinnyParams& P, int t, int pl
       if (idx < total) {
         const int m = idx / C::CW;
         const int n = t * C::CW + (idx - m * C::CW);
+        if constexpr (LORA) {
+          if (n < P.N) sum[i] = lora_value(P.lora, sum[i], m, n, P.M, P.N);
+        }
         if (n < P.N) store_y(ry, (uint32_t)(m * P.N + n), sum[i]);
       }
     }
@@ -279,7 +284,7 @@ __device__ __forceinline__ void redo_segment(const SkinnyParams& P, const LaneCt
 
 // Workgroup p owns units [u0, u1) (unit = (tile, step)) and streams them in order as one
 // pipeline across tile boundaries.
-template <class C>
+template <class C, bool LORA>
 __global__ __launch_bounds__(C::kThreads) __attribute__((amdgpu_waves_per_eu(C::kWavesPerSimd)))
 void skinny_kernel(SkinnyParams P) {
   constexpr int MB = C::MB, CT = C::CT, CW = C::CW, PF = C::PF, V = C::V;
@@ -328,10 +333,12 @@ void skinny_kernel(SkinnyParams P) {
         for (int ct = 0; ct < CT; ++ct) {
           const int col = t * CW + (L.wave * CT + ct) * 16 + L.n;
           const uint32_t e0 = (uint32_t)((rb * 16 + 4 * L.g) * P.N + col);
+          f32x4 v = acc[rb][ct];
+          if constexpr (LORA) v = lora_tile16(P.lora, v, rb * 16, col, P.M, P.N);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int m = rb * 16 + 4 * L.g + r;
-            if (m < P.M && col < P.N) store_y(ry, e0 + (uint32_t)(r * P.N), acc[rb][ct][r]);
+            if (m < P.M && col < P.N) store_y(ry, e0 + (uint32_t)(r * P.N), v[r]);
           }
         }
     } else {
@@ -550,7 +557,7 @@ void skinny_kernel(SkinnyParams P) {
     // Contributor plo holds this tile in its slot 1 iff its range began in an earlier tile
     // (the tile is its last); every later contributor's range begins inside it (slot 0).
     const int lo_slot = (range_start(plo, P.U, P.G) < tile0) ? 1 : 0;
-    reduce_tile<C>(P, tt, plo, phi, lo_slot);
+    reduce_tile<C, LORA>(P, tt, plo, phi, lo_slot);
     if (tid == 0) __hip_atomic_store(&P.cnt[tt], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 }
@@ -642,7 +649,7 @@ static int skinny_threads(int variant) {
 static const void* skinny_func(int variant) {
   switch (variant) {
 #define QMM4_FUNC(id, mp, v, ct, pf, wpe, xs, wv) \
-  case id: return reinterpret_cast<const void*>(&skinny_kernel<SkCfg##id>);
+  case id: return reinterpret_cast<const void*>(&skinny_kernel<SkCfg##id, false>);
     QMM4_SKINNY_VARIANTS(QMM4_FUNC)
 #undef QMM4_FUNC
     default: return nullptr;
@@ -658,14 +665,18 @@ int skinny_occupancy(int variant) {
 
 hipError_t launch_skinny(const SkinnyPlan& plan, const uint16_t* x, const uint32_t* w,
                          const uint16_t* s, const uint16_t* b, uint16_t* y, float* part,
-                         uint32_t* cnt, int M, int N, int K, hipStream_t stream) {
+                         uint32_t* cnt, int M, int N, int K, hipStream_t stream, const LoraAdd* lora) {
   SkinnyParams P;
+  P.lora = lora ? *lora : LoraAdd{};
   P.x = x; P.w = w; P.s = s; P.b = b; P.y = y; P.part = part; P.cnt = cnt;
   P.M = M; P.N = N; P.K = K; P.NS = K / (128 * plan.steps_v); P.G = plan.blocks; P.U = plan.units;
   const dim3 grid((unsigned)plan.blocks), block((unsigned)skinny_threads(plan.variant));
   switch (plan.variant) {
 #define QMM4_LAUNCH(id, mp, v, ct, pf, wpe, xs, wv) \
-  case id: hipLaunchKernelGGL(skinny_kernel<SkCfg##id>, grid, block, 0, stream, P); break;
+  case id:                                                                                 \
+    if (lora) hipLaunchKernelGGL((skinny_kernel<SkCfg##id, true>), grid, block, 0, stream, P); \
+    else hipLaunchKernelGGL((skinny_kernel<SkCfg##id, false>), grid, block, 0, stream, P);  \
+    break;
     QMM4_SKINNY_VARIANTS(QMM4_LAUNCH)
 #undef QMM4_LAUNCH
     default: return hipErrorInvalidValue;

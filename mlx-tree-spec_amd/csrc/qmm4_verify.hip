@@ -30,6 +30,7 @@
 
 #include "qmm4_common.h"
 #include "qmm4_kernels.h"
+#include "qmm_lora.h"
 
 namespace qmm4 {
 
@@ -47,6 +48,7 @@ struct VerifyParams {
   int NS;         // steps per tile = K / (128 V)
   int G;          // workgroups
   long long U;    // units = T * NS
+  LoraAdd lora;   // LORA: added to the sums
 };
 
 template <int MB_, int C_, int V_, int PF_, int W_>
@@ -114,7 +116,7 @@ struct Slot {
   u32x4 a[C::MB][C::V][4];         // x fragments, per row block, super-step and word
 };
 
-template <class C>
+template <class C, bool LORA>
 __global__ __launch_bounds__(C::kThreads) void verify_kernel(VerifyParams P) {
   constexpr int MB = C::MB, NC = C::C, V = C::V, PF = C::PF, W = C::W, CW = C::CW;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -215,11 +217,12 @@ __global__ __launch_bounds__(C::kThreads) void verify_kernel(VerifyParams P) {
 
   // Item it = (row block i, column block j, lane l) of a tile holds rows 16 i + 4 (l / 16) + r,
   // r = 0..3, of column 16 j + l % 16 (the MFMA accumulator layout).
-  auto store_item = [&](int t, int it, const f32x4& v) __attribute__((always_inline)) {
+  auto store_item = [&](int t, int it, f32x4 v) __attribute__((always_inline)) {
     const int blk = it >> 6, ln = it & 63;
     const int i = blk / NC, j = blk - i * NC;
     const int col = t * CW + j * 16 + (ln & 15);
     const int mrow = i * 16 + 4 * (ln >> 4);
+    if constexpr (LORA) v = lora_tile16(P.lora, v, i * 16, col, P.M, P.N);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (mrow + r < P.M && col < P.N) store_y(ry, (uint32_t)((mrow + r) * P.N + col), v[r]);
@@ -412,7 +415,7 @@ QMM4_VERIFY_VARIANTS(QMM4_VCFG)
 static const void* verify_func(int variant) {
   switch (variant) {
 #define QMM4_VF(id, mb, c, v, pf, w) \
-  case id: return reinterpret_cast<const void*>(&verify_kernel<VCfg##id>);
+  case id: return reinterpret_cast<const void*>(&verify_kernel<VCfg##id, false>);
     QMM4_VERIFY_VARIANTS(QMM4_VF)
 #undef QMM4_VF
     default: return nullptr;
@@ -483,8 +486,9 @@ bool verify_plan(int M, int N, int K, int vmax, int cus, int occ, VerifyPlan* pl
 
 hipError_t launch_verify(const VerifyPlan& plan, const uint16_t* x, const uint32_t* w, const uint16_t* s,
                          const uint16_t* b, uint16_t* y, float* part, uint32_t* cnt, int M, int N, int K,
-                         hipStream_t stream) {
+                         hipStream_t stream, const LoraAdd* lora) {
   VerifyParams P;
+  P.lora = lora ? *lora : LoraAdd{};
   P.x = x; P.w = w; P.s = s; P.b = b; P.y = y; P.part = part; P.cnt = cnt;
   P.M = M; P.N = N; P.K = K;
   P.NS = K / (128 * plan.steps_v);
@@ -493,7 +497,16 @@ hipError_t launch_verify(const VerifyPlan& plan, const uint16_t* x, const uint32
   const dim3 grid((unsigned)plan.blocks), block((unsigned)plan.threads);
   switch (plan.variant) {
 #define QMM4_VL(id, mb, c, v, pf, w) \
-  case id: hipLaunchKernelGGL(verify_kernel<VCfg##id>, grid, block, plan.lds, stream, P); break;
+  case id:                                                                                       \
+    if (lora) {                                                                                  \
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&verify_kernel<VCfg##id, true>), \
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)plan.lds);    \
+      if (e != hipSuccess) return e;                                                             \
+      hipLaunchKernelGGL((verify_kernel<VCfg##id, true>), grid, block, plan.lds, stream, P);     \
+    } else {                                                                                     \
+      hipLaunchKernelGGL((verify_kernel<VCfg##id, false>), grid, block, plan.lds, stream, P);    \
+    }                                                                                            \
+    break;
     QMM4_VERIFY_VARIANTS(QMM4_VL)
 #undef QMM4_VL
     default: return hipErrorInvalidValue;

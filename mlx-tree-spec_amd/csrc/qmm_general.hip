@@ -23,6 +23,7 @@
 // 8-bit 65.8 -> 16.8, 64 x 8192 -> 8191 8-bit 80.8 -> 28.5, 256 x 8192 -> 8191 8-bit 136.9 -> 90.4.
 #include "qmm4_common.h"
 #include "qmm4_kernels.h"
+#include "qmm_lora.h"
 #include "qmm4_offsets.h"
 
 namespace qmm4 {
@@ -42,6 +43,7 @@ struct GeneralParams {
   uint16_t* y;
   int M, N, K;
   int gshift;  // log2 of the group size
+  LoraAdd lora;   // LORA: added to the sums
 };
 
 template <int BITS>
@@ -89,7 +91,7 @@ struct GnCfg {
   static_assert(kScBytes % 16 == 0, "aligned");
 };
 
-template <int BITS, int MB, int CB>
+template <int BITS, int MB, int CB, bool LORA>
 __global__ __launch_bounds__(64 * kGnWaves) __attribute__((amdgpu_waves_per_eu(2)))
 void general_kernel(GeneralParams P) {
   using C = GnCfg<MB, CB>;
@@ -222,6 +224,11 @@ void general_kernel(GeneralParams P) {
     if (u < se) compute(0, u, g0);  // an odd count ends the wave's slice (segments are of even length)
   }
 
+  // LORA: what this wave's tile takes of the adapters, while other waves are at their share of K.
+  f32x4 add = {0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (LORA) {
+    if (wave < MB * CB) add = lora_tile16(P.lora, add, m0 + 16 * (wave / CB), c0 + 16 * (wave % CB) + n, P.M, P.N);
+  }
   __syncthreads();  // the sums take the place of x
   f32x4* const red = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
@@ -238,6 +245,9 @@ void general_kernel(GeneralParams P) {
   }
   const int c = wave % CB, i = wave / CB;
   const int col = c0 + 16 * c + n;
+  if constexpr (LORA) {
+    sum[0] += add[0]; sum[1] += add[1]; sum[2] += add[2]; sum[3] += add[3];
+  }
   if (col >= P.N) return;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -246,15 +256,20 @@ void general_kernel(GeneralParams P) {
   }
 }
 
-template <int BITS, int MB, int CB>
-hipError_t launch_general_t(const GeneralParams& P, hipStream_t stream) {
+template <int BITS, int MB, int CB, bool LORA>
+hipError_t launch_general_l(const GeneralParams& P, hipStream_t stream) {
   using C = GnCfg<MB, CB>;
-  hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&general_kernel<BITS, MB, CB>),
+  hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&general_kernel<BITS, MB, CB, LORA>),
                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)C::kLds);
   if (e != hipSuccess) return e;
   const dim3 grid((unsigned)((P.N + 16 * CB - 1) / (16 * CB)), (unsigned)((P.M + 16 * MB - 1) / (16 * MB)));
-  hipLaunchKernelGGL((general_kernel<BITS, MB, CB>), grid, dim3(64 * kGnWaves), C::kLds, stream, P);
+  hipLaunchKernelGGL((general_kernel<BITS, MB, CB, LORA>), grid, dim3(64 * kGnWaves), C::kLds, stream, P);
   return hipGetLastError();
+}
+
+template <int BITS, int MB, int CB>
+hipError_t launch_general_t(const GeneralParams& P, hipStream_t stream) {
+  return P.lora.t ? launch_general_l<BITS, MB, CB, true>(P, stream) : launch_general_l<BITS, MB, CB, false>(P, stream);
 }
 
 // Two column blocks per wave (x read half as often, and each A fragment feeds two MFMAs) when the grid
@@ -274,8 +289,10 @@ hipError_t launch_general_b(const GeneralParams& P, int cus, hipStream_t stream)
 }  // namespace
 
 hipError_t launch_general(const uint16_t* x, const uint32_t* w, const uint16_t* s, const uint16_t* b, uint16_t* y,
-                          int M, int N, int K, int group_size, int bits, int cus, hipStream_t stream) {
+                          int M, int N, int K, int group_size, int bits, int cus, hipStream_t stream,
+                          const LoraAdd* lora) {
   GeneralParams P;
+  P.lora = lora ? *lora : LoraAdd{};
   P.x = x; P.w = w; P.s = s; P.b = b; P.y = y;
   P.M = M; P.N = N; P.K = K;
   P.gshift = group_size == 32 ? 5 : group_size == 64 ? 6 : group_size == 128 ? 7 : -1;

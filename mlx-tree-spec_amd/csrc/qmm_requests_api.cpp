@@ -8,6 +8,7 @@
 
 #include "qmm4.h"
 #include "qmm4_dispatch.h"
+#include "qmm4_kernels.h"
 #include "qmm_requests.h"
 #include "qmm_requests_kernels.h"
 
@@ -53,17 +54,28 @@ int check_lora(const void* x, const void* a, const void* b, const float* scale, 
   return QMM4_OK;
 }
 
-qmm4::LoraTables tables(const void* a, const void* b, const float* scale, const void* adapters, int adapter_bits,
-                        int64_t L, int64_t R) {
-  return {static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(b), scale, {adapters, adapter_bits == 64}, L, (int)R};
-}
+struct Lora {
+  qmm4::LoraTables tables;
+  qmm4::LoraAdd add;
+  Lora(const void* a, const void* b, const float* scale, const void* adapters, int adapter_bits, void* workspace,
+       int64_t L, int64_t R) {
+    const qmm4::Index ids{adapters, adapter_bits == 64};
+    tables = {static_cast<const uint16_t*>(a), scale, ids, L, (int)R};
+    add = {static_cast<const uint32_t*>(workspace), static_cast<const uint16_t*>(b), ids, L, (int)R};
+  }
+};
 
-int run_lora(const qmm4::LoraTables& lora, const void* x, void* y, void* workspace, int64_t M, int64_t N, int64_t K,
-             hipStream_t stream) {
-  hipError_t e = qmm4::launch_lora_shrink(lora, static_cast<const uint16_t*>(x), static_cast<float*>(workspace), M, K, stream);
+// x A^T into the caller's workspace (api_mutex held).
+int run_shrink(qmm4::DeviceInfo* di, qmm4::WorkspaceSource& ws, const Lora& lora, const void* x, void* workspace,
+               int64_t M, int64_t K, hipStream_t stream) {
+  const qmm4::LoraShrinkPlan plan = qmm4::lora_shrink_plan(lora.tables, (int)M, (int)K, qmm4::device_cus(di));
+  uint32_t* cnt = nullptr;
+  float* part = nullptr;
+  if (plan.part_bytes > 0)
+    if (int rc = ws.get(plan.counter_bytes, plan.part_bytes, &cnt, &part)) return rc;
+  const hipError_t e = qmm4::launch_lora_shrink(plan, lora.tables, static_cast<const uint16_t*>(x),
+                                                static_cast<uint32_t*>(workspace), part, cnt, (int)M, (int)K, stream);
   if (e != hipSuccess) return hip_error(e, "adapter shrink kernel launch");
-  e = qmm4::launch_lora_expand(lora, static_cast<const float*>(workspace), static_cast<uint16_t*>(y), M, N, stream);
-  if (e != hipSuccess) return hip_error(e, "adapter expand kernel launch");
   return QMM4_OK;
 }
 
@@ -89,7 +101,7 @@ int current_cus(int* cus) {
 
 extern "C" {
 
-int64_t qmm4_lora_workspace(int64_t M, int64_t R) { return M > 0 && R > 0 ? M * R * (int64_t)sizeof(float) : 0; }
+int64_t qmm4_lora_workspace(int64_t M, int64_t R) { return M > 0 && R > 0 ? M * R * (int64_t)sizeof(uint32_t) : 0; }
 
 int qmm4_lora_add_bf16(const void* x, const void* lora_a, const void* lora_b, const float* lora_scale,
                        const void* adapters, int adapter_bits, void* y, void* workspace, int64_t M, int64_t N,
@@ -97,8 +109,14 @@ int qmm4_lora_add_bf16(const void* x, const void* lora_a, const void* lora_b, co
   return guarded([&] {
     int rc = check_lora(x, lora_a, lora_b, lora_scale, adapters, adapter_bits, y, workspace, M, N, K, L, R);
     if (rc || M == 0 || N == 0 || L == 0) return rc;
-    return run_lora(tables(lora_a, lora_b, lora_scale, adapters, adapter_bits, L, R), x, y, workspace, M, N, K,
-                    static_cast<hipStream_t>(hip_stream));
+    const Lora lora(lora_a, lora_b, lora_scale, adapters, adapter_bits, workspace, L, R);
+    const hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+    return qmm4::with_stream_workspace(stream, [&](qmm4::DeviceInfo* di, qmm4::WorkspaceSource& ws) {
+      if (int rc2 = run_shrink(di, ws, lora, x, workspace, M, K, stream)) return rc2;
+      const hipError_t e = qmm4::launch_lora_expand(lora.add, static_cast<uint16_t*>(y), (int)M, (int)N, stream);
+      if (e != hipSuccess) return hip_error(e, "adapter expand kernel launch");
+      return (int)QMM4_OK;
+    });
   });
 }
 
@@ -107,12 +125,26 @@ int qmm4_affine_lora_bf16(const void* x, const uint32_t* w, const void* scales, 
                           int adapter_bits, void* y, void* workspace, int64_t M, int64_t N, int64_t K, int64_t L,
                           int64_t R, int group_size, int bits, int transpose, void* hip_stream) {
   return guarded([&] {
-    int rc = check_lora(x, lora_a, lora_b, lora_scale, adapters, adapter_bits, y, workspace, M, N, K, L, R);
+    if (transpose != 1) return set_error(QMM4_ERR_UNSUPPORTED, "transpose=%d: only transpose=True is supported", transpose);
+    const bool packed = bits == 4 && group_size == 64 && K % 128 == 0 && N % 16 == 0;
+    int rc = packed ? qmm4::check_qmm_args(x, w, scales, biases, y, M, N, K, group_size, bits, transpose)
+                    : qmm4::check_general_args(x, w, scales, biases, y, M, N, K, group_size, bits);
     if (rc) return rc;
-    rc = qmm4_affine_bf16(x, w, scales, biases, y, M, N, K, group_size, bits, transpose, hip_stream);
-    if (rc || M == 0 || N == 0 || L == 0) return rc;
-    return run_lora(tables(lora_a, lora_b, lora_scale, adapters, adapter_bits, L, R), x, y, workspace, M, N, K,
-                    static_cast<hipStream_t>(hip_stream));
+    rc = check_lora(x, lora_a, lora_b, lora_scale, adapters, adapter_bits, y, workspace, M, N, K, L, R);
+    if (rc || M == 0 || N == 0) return rc;
+    const Lora lora(lora_a, lora_b, lora_scale, adapters, adapter_bits, workspace, L, R);
+    const hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+    return qmm4::with_stream_workspace(stream, [&](qmm4::DeviceInfo* di, qmm4::WorkspaceSource& ws) {
+      const qmm4::LoraAdd* add = L > 0 ? &lora.add : nullptr;
+      if (add)
+        if (int rc2 = run_shrink(di, ws, lora, x, workspace, M, K, stream)) return rc2;
+      if (packed) return qmm4::dispatch_qmm(di, x, w, scales, biases, y, M, N, K, stream, ws, add);
+      const hipError_t e = qmm4::launch_general(static_cast<const uint16_t*>(x), w, static_cast<const uint16_t*>(scales),
+                                                static_cast<const uint16_t*>(biases), static_cast<uint16_t*>(y), (int)M,
+                                                (int)N, (int)K, group_size, bits, qmm4::device_cus(di), stream, add);
+      if (e != hipSuccess) return hip_error(e, "general quantized matmul kernel launch");
+      return (int)QMM4_OK;
+    });
   });
 }
 

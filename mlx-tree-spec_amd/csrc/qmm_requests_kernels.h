@@ -15,21 +15,35 @@ struct Index {
   }
 };
 
-// Adapters a: A [L, R, K], B [L, N, R], scale [L]; row m uses adapters[m] if that lies in 0 .. L - 1.
+// The first factor of the adapters: A [L, R, K], scale [L]; row m uses adapters[m] if that lies in 0 .. L - 1.
 struct LoraTables {
   const uint16_t* a;
-  const uint16_t* b;
   const float* scale;
   Index adapters;
   int64_t L;
   int R;
 };
-// t[m, j] = scale * sum_k x[m, k] A[a, j, k] (0 for rows without an adapter), fp32 [M, R].
-hipError_t launch_lora_shrink(const LoraTables& lora, const uint16_t* x, float* t, int64_t M, int64_t K,
-                              hipStream_t stream);
-// y[m, n] = bf16(y[m, n] + sum_j t[m, j] B[a, n, j]) for rows with an adapter.
-hipError_t launch_lora_expand(const LoraTables& lora, const float* t, uint16_t* y, int64_t M, int64_t N,
-                              hipStream_t stream);
+// The shrink's grid, and what it needs of the split-K workspace (counters at zero, fp32 tiles).
+struct LoraShrinkPlan {
+  int rows, across, depth, slices, width;
+  size_t counter_bytes, part_bytes;
+};
+LoraShrinkPlan lora_shrink_plan(const LoraTables& lora, int M, int K, int cus);
+// t [M, R]: t[m, j] = scale * sum_k x[m, k] A[a, j, k] as two bf16 numbers in a word (rows without an adapter are not
+// written).
+hipError_t launch_lora_shrink(const LoraShrinkPlan& plan, const LoraTables& lora, const uint16_t* x, uint32_t* t,
+                              float* part, uint32_t* cnt, int M, int K, hipStream_t stream);
+
+// What a projection's kernel adds to its sums: sum_j t[m, j] B[a, n, j] for the rows with an adapter.
+struct LoraAdd {
+  const uint32_t* t;
+  const uint16_t* b;
+  Index adapters;
+  int64_t L;
+  int R;
+};
+// The same to a finished y: y[m, n] = bf16(y[m, n] + ..).
+hipError_t launch_lora_expand(const LoraAdd& lora, uint16_t* y, int M, int N, hipStream_t stream);
 
 struct RopeHeads {
   const uint16_t* x;

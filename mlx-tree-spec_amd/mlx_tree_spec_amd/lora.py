@@ -18,7 +18,8 @@ import torch
 
 from . import _lib
 from .packed_linear import STATS, QuantizedLinear
-from .qmm import _check_device, _check_format, _check_weights, aligned_contiguous, quantized_matmul
+from .qmm import (_check_device, _check_format, _check_weights, _general_kernel_ok, aligned_contiguous,
+                  quantized_matmul)
 
 MAX_RANK = 256
 _INDEX_DTYPES = (torch.int32, torch.int64)
@@ -71,8 +72,9 @@ def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor
 
     x bf16 (..., K); w, scales, biases as in quantized_matmul, in any format that takes; lora_a bf16 [L, R, K],
     lora_b bf16 [L, N, R], lora_scale fp32 [L] (R a multiple of 8, up to 256); adapters int32 or int64 of x's
-    leading shape. A row whose adapter lies outside 0 .. L - 1 (-1, say) has the projection alone. x @ lora_a.T
-    and all sums are fp32.
+    leading shape. A row whose adapter lies outside 0 .. L - 1 (-1, say) has the projection alone, with its bits.
+    Both products are summed in fp32 and rounded once (twice at the sizes and formats for which quantized_matmul
+    dequantizes and multiplies); x @ lora_a.T is kept to 2^-18 of its value in between.
     """
     what = "quantized_matmul_lora"
     _check_format(group_size, bits, transpose, mode, general=True)
@@ -92,18 +94,19 @@ def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor
     lora_a, lora_b, lora_scale = aligned_contiguous(lora_a), aligned_contiguous(lora_b), lora_scale.contiguous()
     m, (count, rank) = x2.shape[0], lora_a.shape[:2]
     lib = _lib.load()
-    workspace = torch.empty((m, rank), dtype=torch.float32, device=dev)
+    workspace = torch.empty((m, rank), dtype=torch.int32, device=dev)
     packed = bits == 4 and group_size == 64 and k % 128 == 0 and n % 16 == 0
-    if packed:
-        w, scales, biases = aligned_contiguous(w), aligned_contiguous(scales), aligned_contiguous(biases)
+    fused = packed or _general_kernel_ok(x, m, n, k, bits)
+    w, scales, biases = aligned_contiguous(w), aligned_contiguous(scales), aligned_contiguous(biases)
+    if fused:
         y = torch.empty((*x.shape[:-1], n), dtype=torch.bfloat16, device=dev)
-    else:
-        y = quantized_matmul(x, w, scales, biases, transpose, group_size, bits, mode)
+    else:  # the sizes at which quantized_matmul dequantizes and multiplies
+        y = quantized_matmul(x2, w, scales, biases, transpose, group_size, bits, mode).reshape(*x.shape[:-1], n)
     with torch.cuda.device(dev):
         stream = torch.cuda.current_stream(dev).cuda_stream
         lora = (lora_a.data_ptr(), lora_b.data_ptr(), lora_scale.data_ptr(), adapters.data_ptr(),
                 adapters.element_size() * 8, y.data_ptr(), workspace.data_ptr(), m, n, k, count, rank)
-        if packed:
+        if fused:
             rc = lib.qmm4_affine_lora_bf16(x2.data_ptr(), w.data_ptr(), scales.data_ptr(), biases.data_ptr(), *lora,
                                            group_size, bits, 1, stream)
         else:

@@ -1,8 +1,9 @@
 """Low-rank adapters beside a quantized projection, on the GPU (needs an MI355X), against 64 bits.
 
-Bound per value: the results rounded to bf16 (half a step each: the projection's own, and the sum's), and fp32
-sums of n terms, whose error is at most n half steps of fp32 of the sum of the terms' magnitudes, whatever their
-order (n = K + R + 4 covers the K products, the R products of the second factor and the scale).
+Bound per value: the result rounded to bf16 (half a step; the projection's own rounding as well where a library product
+computes it), x A^T kept to 2^-18 of its value, and fp32 sums of n terms, whose error is at most n half steps of fp32
+of the sum of the terms' magnitudes, whatever their order (n = K + R + 4 covers the K products, the R products of the
+second factor and the scale).
 """
 
 import numpy as np
@@ -31,12 +32,13 @@ def inputs(m, k, n, rank, count, seed, bits=4, group=64, ids=None):
     return [t.to(DEV) for t in (x, w, s, b, la, lb, scale, torch.as_tensor(ids, dtype=torch.int32))]
 
 
-def check(args, y, group=64, bits=4):
+def check(args, y, group=64, bits=4, twice=False):
     x, w, s, b, la, lb, scale, ids = args
     m = x.reshape(-1, x.shape[-1]).shape[0]
     ref, base, mag = R.lora(x.reshape(m, -1), R.dequantize(w, s, b, group, bits), la, lb, scale, ids.reshape(-1))
     k, rank = x.shape[-1], la.shape[1]
-    bound = R.HALF_STEP_BF16 * (np.abs(ref) + np.abs(base)) * 1.01 + (k + rank + 4) * R.HALF_STEP_F32 * mag
+    rounded = np.abs(ref) + (np.abs(base) if twice else 0)
+    bound = R.HALF_STEP_BF16 * rounded * 1.01 + ((k + rank + 4) * R.HALF_STEP_F32 + 2.0 ** -18) * mag
     err = np.abs(R.f64(y).reshape(m, -1) - ref)
     assert (err <= bound).all(), (float((err - bound).max()), np.unravel_index((err - bound).argmax(), err.shape))
 
@@ -66,6 +68,21 @@ def test_ranks(m, rank):
 def test_general_formats(m, k, n, bits, group):
     args = inputs(m, k, n, 16, 4, m + n, bits, group)
     check(args, quantized_matmul_lora(*args, group_size=group, bits=bits), group, bits)
+
+
+# K that the general kernel does not take: the projection by dequantization and a library product.
+@pytest.mark.parametrize("m,k,n", [(1, 96, 5), (7, 96, 40), (70, 160, 300)])
+def test_added_to_a_library_product(m, k, n):
+    args = inputs(m, k, n, 24, 4, m + n, 4, 32)
+    check(args, quantized_matmul_lora(*args, group_size=32), 32, 4, twice=True)
+
+
+# Many rows of one adapter next to others (a prompt's tiles), long K in slices, and adapters far apart in the tables.
+@pytest.mark.parametrize("m,k,n,rank", [(300, 2048, 1040, 32), (64, 17408, 512, 32), (1030, 512, 2064, 64), (30, 8192, 4096, 8)])
+def test_runs_of_requests(m, k, n, rank):
+    ids = torch.tensor([2] * (m // 2) + [-1] * (m // 8) + [0] * (m // 4 + 1) + [1] * m)[:m]
+    args = inputs(m, k, n, rank, 3, m + k, ids=ids)
+    check(args, quantized_matmul_lora(*args))
 
 
 @pytest.mark.parametrize("m,k,n,bits,group", [(6, 512, 272, 4, 64), (70, 512, 512, 4, 64), (6, 192, 35, 4, 64)])
