@@ -166,10 +166,57 @@ struct TileAdapters {
   }
 };
 
+// Makes what is not finite of 8 bf16 values zero; whether there was any.
+__device__ __forceinline__ bool lora_zero_bad(u32x4* v) {
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bool lo = ((*v)[e] & 0x7F80u) == 0x7F80u, hi = ((*v)[e] & 0x7F800000u) == 0x7F800000u;
+    (*v)[e] = (lo ? 0u : (*v)[e] & 0xFFFFu) | (hi ? 0u : (*v)[e] & 0xFFFF0000u);
+    any |= lo || hi;
+  }
+  return any;
+}
+// A row of t and of B (16 k) whose product is the sum of both infinities where `own` and `bad`, else zero.
+__device__ __forceinline__ void lora_put_bad(uint16_t* t, uint16_t* b, bool own, bool bad) {
+  constexpr uint32_t kBig = 0x7F7Fu;  // the largest bf16
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  *reinterpret_cast<u32x4*>(t) = u32x4{own ? (kBig | 0x8000u) << 16 | kBig : 0u, 0u, 0u, 0u};
+  *reinterpret_cast<u32x4*>(t + 8) = zero;
+  *reinterpret_cast<u32x4*>(b) = u32x4{bad ? kBig << 16 | kBig : 0u, 0u, 0u, 0u};
+  *reinterpret_cast<u32x4*>(b + 8) = zero;
+}
+
+// The steps of gemm_ws_kernel's tile.
+template <int BM>
+struct LoraSteps {
+  int adapter[BM];  // of the tile's rows: -1 none, -2 past M
+  int list[BM];     // those that occur: 2 * adapter + (whether other rows have another one or none)
+  int count, steps, any, pad;
+  // By one wave, for the tile's rows from m0.
+  __device__ __forceinline__ void init(const LoraAdd& E, int lane, int m0, int M) {
+#pragma unroll
+    for (int q = 0; q < BM / 64; ++q)
+      adapter[q * 64 + lane] = m0 + q * 64 + lane < M ? lora_adapter(E, m0 + q * 64 + lane, M) : -2;
+    TileAdapters<BM> walk(adapter);
+    int d, n = 0;
+    bool mixed;
+    for (; walk.next(&d, &mixed); ++n)
+      if (lane == 0) list[n] = 2 * d + mixed;
+    if (lane == 0) {
+      count = n;
+      steps = (n * ((E.R + 31) / 32) + 1) & ~1;  // a last one of zeros makes them even
+      any = 0;
+    }
+  }
+};
+
 // Threads 0 .. NT - 1 stage j0 .. j0 + 63 of adapter d into LDS (to the next 16 past R with zeros); `stage` counts.
 template <int BM, int BN, int NT, int AHEAD>
 __device__ __forceinline__ void lora_stage(const LoraAdd& E, LoraLds<BM, BN>& S, uint16_t* As, uint16_t* Bs, int tid, int d,
                                            bool mixed, int j0, int stage, int m0, int n0, int M, int N) {
+  m0 = __builtin_amdgcn_readfirstlane(m0);
+  n0 = __builtin_amdgcn_readfirstlane(n0);
   constexpr uint32_t kOut = 0x80000000u;  // past the end of a tile's rows or columns: reads zero
   // (A quarter of a 256 x 256 tile may begin past M or N: no rows or columns then.)
   const int rows = max(0, min(BM, M - m0)), cols = max(0, min(BN, N - n0));
@@ -216,16 +263,9 @@ __device__ __forceinline__ void lora_stage(const LoraAdd& E, LoraLds<BM, BN>& S,
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int c = (i0 + i) * (NT / 8) + r0;
-      if (mixed) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool lo = (b[i][e] & 0x7F80u) == 0x7F80u, hi = (b[i][e] & 0x7F800000u) == 0x7F800000u;
-          if (lo || hi) {
-            S.bad[c] = 1;
-            S.any[stage & 1] = 1;
-            b[i][e] = (lo ? 0u : b[i][e] & 0xFFFFu) | (hi ? 0u : b[i][e] & 0xFFFF0000u);
-          }
-        }
+      if (mixed && lora_zero_bad(&b[i])) {
+        S.bad[c] = 1;
+        S.any[stage & 1] = 1;
       }
       if (pc < pieces) *reinterpret_cast<u32x4*>(Bs + c * LDK + pc * 8) = b[i];
     }
@@ -233,20 +273,17 @@ __device__ __forceinline__ void lora_stage(const LoraAdd& E, LoraLds<BM, BN>& S,
   }
 }
 
-// The last step of an adapter with columns noted.
+// The last step of an adapter with columns noted: only the first BM rows of t's (the low parts' place holds zeros).
 template <int BM, int BN, int NT>
 __device__ __forceinline__ void lora_stage_bad(LoraLds<BM, BN>& S, uint16_t* As, uint16_t* Bs, int tid, int d) {
-  constexpr uint32_t kBig = 0x7F7Fu;  // the largest bf16
-  for (int i = tid; i < 2 * BM; i += NT) {
-    const u32x4 v = {i < BM && S.adapter[i] == d ? (kBig | 0x8000u) << 16 | kBig : 0u, 0u, 0u, 0u};
-    *reinterpret_cast<u32x4*>(As + i * LDK) = v;
-    *reinterpret_cast<u32x4*>(As + i * LDK + 8) = u32x4{0u, 0u, 0u, 0u};
-  }
-  for (int i = tid; i < BN; i += NT) {
-    const u32x4 v = {S.bad[i] ? kBig << 16 | kBig : 0u, 0u, 0u, 0u};
-    S.bad[i] = 0;
-    *reinterpret_cast<u32x4*>(Bs + i * LDK) = v;
-    *reinterpret_cast<u32x4*>(Bs + i * LDK + 8) = u32x4{0u, 0u, 0u, 0u};
+  for (int i = tid; i < (BM > BN ? BM : BN); i += NT) {
+    uint16_t* t = As + i * LDK;
+    lora_put_bad(t, Bs + i * LDK, i < BM && S.adapter[i] == d, i < BN && S.bad[i] != 0);
+    if (i < BM) {
+      *reinterpret_cast<u32x4*>(t + BM * LDK) = u32x4{0u, 0u, 0u, 0u};
+      *reinterpret_cast<u32x4*>(t + BM * LDK + 8) = u32x4{0u, 0u, 0u, 0u};
+    }
+    if (i < BN) S.bad[i] = 0;
   }
 }
 
@@ -276,7 +313,7 @@ __device__ __forceinline__ void lora_walk(const LoraLds<BM, BN>& S, int R, Stage
 }
 
 // A wave's part of the tile (I x J blocks of 32 from its row wr and column wc) takes the staged products.
-template <int BM, int I, int J>
+template <int BM, int I, int J, int HALVES = 2>
 __device__ __forceinline__ void lora_take(const uint16_t* As, const uint16_t* Bs, f32x16 (&acc)[I][J], int steps, int wr,
                                           int wc) {
   const int lane = threadIdx.x & 63, lrow = lane & 31, lk = (lane >> 5) * 8;
@@ -286,7 +323,7 @@ __device__ __forceinline__ void lora_take(const uint16_t* As, const uint16_t* Bs
 #pragma unroll
     for (int j = 0; j < J; ++j) Bf[j] = as_bf16x8(*reinterpret_cast<const u32x4*>(Bs + (wc + j * 32 + lrow) * LDK + ks * 16 + lk));
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int half = 0; half < HALVES; ++half)
 #pragma unroll
       for (int i = 0; i < I; ++i) {
         const bf16x8 Af =
@@ -758,6 +795,10 @@ hipError_t launch_tiles(const GemmParams& P, int blocks, hipStream_t stream) {
 // better than MFMAs and VALU interleaved inside one wave: a dequantization wave beside an MFMA wave
 // ran in the time of the dequantization alone, where waves mixing both ran in ~0.8 of the sum of
 // the two. 12 waves share the SIMDs' 512 registers per lane: at most 168 per wave (154 used).
+// LORA: the adapters' products are K steps behind a whole tile's last one, each loaded and put beside the MFMAs of the
+// one before: 32 j of one adapter, t's high parts and its low parts side by side over B twice (a step of 64 k).
+// Their registers live outside the producers' loop (loaded two steps ahead there, like the weights, they made it
+// spill, and its waits for the spills end the weights' prefetch: 2000 x 5120 -> 17408 322 -> 380 us).
 // Producer thread pt (0-255): activation chunk pt % 8 of rows pt / 8 + 32 j (j < 8) and the 8 code
 // words (one group, 64 k) of column pt per K step, two steps ahead in registers; the column's scale
 // and bias come 8 groups per 16-byte load.
@@ -769,9 +810,9 @@ __global__ __launch_bounds__(kWsThreads) __attribute__((amdgpu_waves_per_eu(3)))
 void gemm_ws_kernel(GemmParams P) {
   using C = GemmCfg<256, 256>;
   constexpr int BM = 256, BN = 256, I = C::I, J = C::J, LDC = C::LDC;
-  __shared__ int s_lora[LORA ? sizeof(LoraLds<BM, BN>) / sizeof(int) : 1];
-  [[maybe_unused]] LoraLds<BM, BN>& S = *reinterpret_cast<LoraLds<BM, BN>*>(s_lora);
-  static_assert(64 * kWsProd == BM, "a producer thread per row of the tile");
+  __shared__ int s_lora[LORA ? sizeof(LoraSteps<BM>) / sizeof(int) : 1];
+  [[maybe_unused]] LoraSteps<BM>& S = *reinterpret_cast<LoraSteps<BM>*>(s_lora);
+  static_assert(64 * kWsProd == BM && BM == BN, "a producer thread per row and column of the tile");
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   uint16_t* As = smem;
   uint16_t* Bs = smem + 2 * BM * LDK;
@@ -843,7 +884,7 @@ void gemm_ws_kernel(GemmParams P) {
     }
   };
   // Every segment passes the same barriers in both roles: one after the producers' prologue, one
-  // per K step, (LORA: one and those of lora_walk,) one between the bf16 tile's LDS writes and its stores (whole tiles), one at the end
+  // per K step, (LORA: one per step of the adapters, two per adapter where one is not finite,) one between the bf16 tile's LDS writes and its stores (whole tiles), one at the end
   // (the next segment's prologue reuses the LDS stages and the output tile).
 
   if (mma) {
@@ -881,7 +922,9 @@ void gemm_ws_kernel(GemmParams P) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
       __syncthreads();  // step kb is in stage 0
-      for (int kt = kb; kt < ke; kt += 2) {
+      int end = ke;
+      if constexpr (LORA) end += kb == 0 && ke == nk ? __builtin_amdgcn_readfirstlane(S.steps) : 0;
+      for (int kt = kb; kt < end; kt += 2) {
         step(0);
         step(1);
       }
@@ -889,12 +932,13 @@ void gemm_ws_kernel(GemmParams P) {
         // The tile as bf16 into LDS (every wave is past the last step's reads).
         uint16_t* Cs = smem;
         if constexpr (LORA) {
-          __syncthreads();  // the producers have noted the rows' adapters
-          lora_walk<BM, BN>(
-              S, P.lora.R, [](int, bool, int, int) {},
-              [&](int steps) __attribute__((always_inline)) {
-                lora_take<BM, I, J>(As, Bs, acc, steps, wm * C::WM, wn * C::WN);
-              });
+          if (__builtin_amdgcn_readfirstlane(S.any)) {
+            for (int i = 0; i < S.count; ++i) {
+              __syncthreads();  // staged
+              lora_take<BM, I, J, 1>(As, Bs, acc, 1, wm * C::WM, wn * C::WN);
+              __syncthreads();
+            }
+          }
         }
 #pragma unroll
         for (int i = 0; i < I; ++i)
@@ -961,6 +1005,49 @@ void gemm_ws_kernel(GemmParams P) {
 #pragma unroll
       for (int v = 0; v < 2; ++v) R.w[v] = __builtin_amdgcn_raw_buffer_load_b128(rw, woff + v * 16, k * 32, 0);
     };
+    // LORA: step l of the adapters' products into stage st. A thread's t: row pt / 8 + 32 i, 4 j from 4 (pt % 8); its B:
+    // column pt / 4 + 64 i, 8 j from 8 (pt % 4). What lies past the rows, the columns or R, and t of rows with another
+    // adapter, reads zero.
+    [[maybe_unused]] auto put_lora = [&](int l, int st) __attribute__((always_inline)) {
+      constexpr uint32_t kOut = 0x80000000u;
+      const LoraAdd& E = P.lora;
+      const int tm = __builtin_amdgcn_readfirstlane(m0), tn = __builtin_amdgcn_readfirstlane(n0);
+      const int per = (E.R + 31) / 32, at = l / per, j0 = (l - at * per) * 32;
+      const bool live = at < S.count;
+      const int entry = live ? __builtin_amdgcn_readfirstlane(S.list[at]) : 0, d = entry >> 1;
+      const __amdgpu_buffer_rsrc_t rt = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint32_t*>(E.t + (int64_t)tm * E.R), 0, max(0, min(BM, P.M - tm)) * E.R * 4, kBufferRsrcWord3);
+      const __amdgpu_buffer_rsrc_t rl = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint16_t*>(E.b + ((int64_t)d * P.N + tn) * E.R), 0, max(0, min(BN, P.N - tn)) * E.R * 2, kBufferRsrcWord3);
+      const int jt = j0 + (pt & 7) * 4, jb = j0 + (pt & 3) * 8;
+      u32x4 t[kAJ], v[4];
+#pragma unroll
+      for (int i = 0; i < kAJ; ++i) {
+        const int r = (pt >> 3) + 32 * i;
+        const bool in = live && jt < E.R && S.adapter[r] == d;
+        t[i] = __builtin_amdgcn_raw_buffer_load_b128(rt, in ? (uint32_t)(r * E.R + jt) * 4u : kOut, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = live && jb < E.R;
+        v[i] = __builtin_amdgcn_raw_buffer_load_b128(rl, in ? (uint32_t)(((pt >> 2) + 64 * i) * E.R + jb) * 2u : kOut, 0, 0);
+      }
+      uint16_t* as = As + st * BM * LDK + (pt >> 3) * LDK + (pt & 7) * 4;
+#pragma unroll
+      for (int i = 0; i < kAJ; ++i) {
+        *reinterpret_cast<u32x2*>(as + 32 * i * LDK) =
+            u32x2{__builtin_amdgcn_perm(t[i][1], t[i][0], 0x07060302u), __builtin_amdgcn_perm(t[i][3], t[i][2], 0x07060302u)};
+        *reinterpret_cast<u32x2*>(as + 32 * i * LDK + 32) =
+            u32x2{__builtin_amdgcn_perm(t[i][1], t[i][0], 0x05040100u), __builtin_amdgcn_perm(t[i][3], t[i][2], 0x05040100u)};
+      }
+      uint16_t* bs = Bs + st * BN * LDK + (pt >> 2) * LDK + (pt & 3) * 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if ((entry & 1) && lora_zero_bad(&v[i])) S.any = 1;
+        *reinterpret_cast<u32x4*>(bs + 64 * i * LDK) = v[i];
+        *reinterpret_cast<u32x4*>(bs + 64 * i * LDK + 32) = v[i];
+      }
+    };
     u32x4 scur, bcur, snext = {0u, 0u, 0u, 0u}, bnext = snext;
     auto load_sb8 = [&](int kt, u32x4& s8, u32x4& b8) __attribute__((always_inline)) {
       const int k = kt < ke ? kt : kb;
@@ -986,9 +1073,14 @@ void gemm_ws_kernel(GemmParams P) {
 #pragma unroll
     for (int i = 0; i < kWsD; ++i) load(kb + i, raw[i]);
     load_sb8(kb, scur, bcur);
+    if constexpr (LORA) {
+      if (kb == 0 && ke == nk && pt < 64) S.init(P.lora, pt, m0, P.M);
+    }
     put(raw[0], 0, pick_c(scur, std::integral_constant<int, 0>{}), pick_c(bcur, std::integral_constant<int, 0>{}));
     load(kb + kWsD, raw[0]);
     __syncthreads();
+    [[maybe_unused]] int nl = 0;
+    if constexpr (LORA) nl = kb == 0 && ke == nk ? __builtin_amdgcn_readfirstlane(S.steps) : 0;
     // Iteration kt (the MFMA waves on stage (kt - kb) % 2): step kt + 1 into the other stage, then
     // step kt + 1 + D loaded into its registers. Unrolled by 8, so each step's group is static.
     auto it = [&](int kt, auto uc) __attribute__((always_inline)) {
@@ -1013,22 +1105,35 @@ void gemm_ws_kernel(GemmParams P) {
       it(kt + 4, std::integral_constant<int, 4>{});
       it(kt + 5, std::integral_constant<int, 5>{});
       it(kt + 6, std::integral_constant<int, 6>{});
+      if constexpr (LORA) {
+        if (nl > 0 && kt + 8 >= ke) break;  // the adapters' first step is put beside the last one
+      }
       it(kt + 7, std::integral_constant<int, 7>{});
       scur = snext;
       bcur = bnext;
     }
-    if (kb == 0 && ke == nk) {
-      if constexpr (LORA) {
-        S.init(P.lora, pt, m0, P.M);
+    if constexpr (LORA) {
+#pragma unroll 1
+      for (int l = 0; l <= nl && nl > 0; ++l) {  // step l beside the MFMA waves' step l - 1
+        if (l < nl) put_lora(l, l & 1);
         __syncthreads();
-        lora_walk<BM, BN>(
-            S, P.lora.R,
-            [&](int d, bool mixed, int j0, int n) __attribute__((always_inline)) {
-              if (j0 < 0) lora_stage_bad<BM, BN, 64 * kWsProd>(S, As, Bs, pt, d);
-              else lora_stage<BM, BN, 64 * kWsProd, 8>(P.lora, S, As, Bs, pt, d, mixed, j0, n, m0, n0, P.M, P.N);
-            },
-            [](int) {});
       }
+      if (nl > 0 && __builtin_amdgcn_readfirstlane(S.any)) {
+        // For each adapter, the columns where its B is not finite (thread pt: column pt).
+        for (int i = 0; i < S.count; ++i) {
+          const int d = S.list[i] >> 1;
+          bool bad = false;
+          if (n0 + pt < P.N) {
+            const uint16_t* b = P.lora.b + ((int64_t)d * P.N + n0 + pt) * P.lora.R;
+            for (int j = 0; j < P.lora.R; ++j) bad |= (b[j] & 0x7F80u) == 0x7F80u;
+          }
+          lora_put_bad(As + pt * LDK, Bs + pt * LDK, S.adapter[pt] == d, bad);
+          __syncthreads();
+          __syncthreads();  // taken
+        }
+      }
+    }
+    if (kb == 0 && ke == nk) {
       __syncthreads();  // the MFMA waves' bf16 tile is in LDS
       store_chunks(m0, n0);
     }

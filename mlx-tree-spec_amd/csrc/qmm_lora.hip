@@ -4,10 +4,10 @@
 // Sums are fp32; t is kept to 2^-18 of its value (qmm_lora.h). The expand is the last step of the projection's own
 // kernels; the one here serves projections that run elsewhere.
 //
-// Shrink: a workgroup takes 16 rows and 16 (or 4) values of j for one of the adapters that its rows have (the z-th of them:
-// a tree's nodes or a prompt's rows share one, so most z end at once) and a slice of K, its 16 waves a part of it each,
+// Shrink: a workgroup takes 16 rows and 16 values of j for one of the adapters that its rows have (the z-th of them:
+// a tree's nodes or a prompt's rows share one, so most z end at once) and a slice of K, its 8 waves a part of it each,
 // as 16 x 16 x 32 matrix products. Rows are loaded with 16 neighbouring lanes each and put in matrix order through LDS
-// of the wave's own (loads in matrix order, a row to each neighbouring lane, reach less than half the rate). The 16
+// of the wave's own (loads in matrix order, a row to each neighbouring lane, reach less than half the rate). The 8
 // sums meet in LDS; slices, where there are several, are added by the last workgroup to arrive, in their order.
 #include "qmm4_common.h"
 #include "qmm4_lds.h"
@@ -18,7 +18,7 @@ namespace qmm4 {
 
 namespace {
 
-constexpr int kWaves = 16;
+constexpr int kWaves = 8;
 constexpr int kMaxSlices = 8;
 constexpr int kThreads = 64 * kWaves;
 
@@ -40,14 +40,13 @@ struct Shrink {
   float* part;    // slices > 1: fp32 tiles [tile][slice][lane][4]
   uint32_t* cnt;  // arrivals per tile (0 between launches)
   int M, K, slices, units;  // units of kUnit k, the last one possibly short
-  int width;                // values of j of a workgroup: 16, or 4
 };
 
 __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(Shrink P) {
   extern __shared__ __attribute__((aligned(16))) u32x4 lds[];
   const LoraTables& T = P.T;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int slice = blockIdx.x % P.slices, m0 = blockIdx.x / P.slices * 16, j0 = blockIdx.y * P.width;
+  const int slice = blockIdx.x % P.slices, m0 = blockIdx.x / P.slices * 16, j0 = blockIdx.y * 16;
   const int64_t id = T.adapters[min(m0 + (lane & 15), P.M - 1)];
   const int a = m0 + (lane & 15) < P.M && id >= 0 && id < T.L ? (int)id : -1;
   // The z-th adapter of the rows.
@@ -80,7 +79,7 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(Shrink P) {
       for (int i = 0; i < 4; ++i) {
         xv[b][i] = av[b][i] = u32x4{0u, 0u, 0u, 0u};
         if (in && (rows >> (4 * i + r4) & 1)) xv[b][i] = *reinterpret_cast<const u32x4*>(xr + (int64_t)(4 * i) * P.K + u * kUnit);
-        if (in && 4 * i < P.width && j0 + 4 * i + r4 < T.R) av[b][i] = *reinterpret_cast<const u32x4*>(ar + (int64_t)(4 * i) * P.K + u * kUnit);
+        if (in && j0 + 4 * i + r4 < T.R) av[b][i] = *reinterpret_cast<const u32x4*>(ar + (int64_t)(4 * i) * P.K + u * kUnit);
       }
     }
 #pragma unroll
@@ -91,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(Shrink P) {
       for (int i = 0; i < 4; ++i) {
         const int row = 4 * i + r4;
         lx[row * 16 + (piece ^ row)] = xv[b][i];
-        if (4 * i < P.width) la[row * 16 + (piece ^ row)] = av[b][i];  // (rows that are not there: sums not stored)
+        la[row * 16 + (piece ^ row)] = av[b][i];
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -139,7 +138,7 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(Shrink P) {
     if (lane == 0) __hip_atomic_store(&P.cnt[tile], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   const int jj = j0 + (lane & 15);
-  if (jj >= T.R || (lane & 15) >= P.width) return;
+  if (jj >= T.R) return;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (rows >> (4 * r4 + r) & 1) P.t[(int64_t)(m0 + 4 * r4 + r) * T.R + jj] = split_bf16(scale * acc[r]);
@@ -168,18 +167,19 @@ LdsAllowance g_shrink;
 
 }  // namespace
 
-// A workgroup's time is its loads: 16 values of j where that gives every CU a workgroup (x read least often), 4 for fewer.
-// K in slices of 4096 or more where CUs are left all the same (the merge costs a round trip more than it saves below).
+// Few tiles: K in up to 8 slices of at least 512, while that gives a CU no second workgroup (counted for one adapter per
+// 16 rows). One / 4 / 8 slices: 4 x 5120 rank 16 of 4 adapters 6.7 / 5.3 / 5.1 us, 16 rows of one 6.6 / 5.2 / 4.8, 64 x
+// 17408 rank 32 of 4 adapters 15.0 / 8.0 / 7.2; many tiles, 2000 x 5120 rank 64, 21 / 30 / 48. (4 or 16 waves instead of 8: 4 x
+// 5120 5.3 / 5.6, 64 x 17408 7.9 / 6.8, 2000 x 5120 20.7 / 26.6; tiles of 4 values of j: no better in slices.)
 LoraShrinkPlan lora_shrink_plan(const LoraTables& lora, int M, int K, int cus) {
   LoraShrinkPlan p;
   const int most = M < 16 ? M : 16;  // adapters of 16 rows
   p.rows = (M + 15) / 16;
-  p.width = (int64_t)p.rows * ((lora.R + 15) / 16) >= cus ? 16 : 4;
-  p.across = (lora.R + p.width - 1) / p.width;
+  p.across = (lora.R + 15) / 16;
   p.depth = (int)(lora.L < most ? lora.L : most);
   const int64_t tiles = (int64_t)p.rows * p.across;
   int64_t s = cus / tiles;
-  if (s > K / 4096) s = K / 4096;
+  if (s > K / 512) s = K / 512;
   p.slices = s < 1 ? 1 : s > kMaxSlices ? kMaxSlices : (int)s;
   p.counter_bytes = p.slices > 1 ? (size_t)(tiles * p.depth) * sizeof(uint32_t) : 0;
   p.part_bytes = p.slices > 1 ? (size_t)(tiles * p.depth * p.slices) * 1024 : 0;
@@ -191,7 +191,7 @@ hipError_t launch_lora_shrink(const LoraShrinkPlan& plan, const LoraTables& lora
   constexpr size_t kLds = (size_t)kWaves * kWaveLds;
   const hipError_t e = g_shrink.allow(reinterpret_cast<const void*>(&lora_shrink_kernel), kLds);
   if (e != hipSuccess) return e;
-  const Shrink P{lora, x, t, part, cnt, M, K, plan.slices, (K + kUnit - 1) / kUnit, plan.width};
+  const Shrink P{lora, x, t, part, cnt, M, K, plan.slices, (K + kUnit - 1) / kUnit};
   const dim3 grid((unsigned)(plan.rows * plan.slices), (unsigned)plan.across, (unsigned)plan.depth);
   hipLaunchKernelGGL(lora_shrink_kernel, grid, dim3(kThreads), kLds, stream, P);
   return hipGetLastError();

@@ -25,7 +25,7 @@ struct LoraTables {
 };
 // The shrink's grid, and what it needs of the split-K workspace (counters at zero, fp32 tiles).
 struct LoraShrinkPlan {
-  int rows, across, depth, slices, width;
+  int rows, across, depth, slices;
   size_t counter_bytes, part_bytes;
 };
 LoraShrinkPlan lora_shrink_plan(const LoraTables& lora, int M, int K, int cus);
