@@ -27,6 +27,7 @@
 
 #include "qmm4.h"
 #include "qmm_general.h"
+#include "qmm_requests.h"
 
 namespace {
 
@@ -35,10 +36,14 @@ decltype(&qmm4_gate_up_silu_bf16) p_gate_up = nullptr;
 decltype(&qmm_affine_general_bf16) p_general = nullptr;
 decltype(&qmm4_add_rms_norm_bf16) p_norm = nullptr;
 decltype(&qmm4_add_rms_norm_qmm_bf16) p_norm_qmm = nullptr;
+decltype(&qmm4_affine_lora_bf16) p_lora = nullptr;
+decltype(&qmm4_qk_norm_rope_bf16) p_rope = nullptr;
+decltype(&qmm4_sample_bf16) p_sample = nullptr;
+decltype(&qmm4_sample_workspace) p_sample_workspace = nullptr;
 
-// A plain tensor on a HIP device, contiguous with data on an `align`-byte boundary, or null: no
-// subclass, no wrapper of a transform or a mode, nothing whose storage is not its own.
-const at::Tensor* plain(PyObject* o, size_t align) {
+// A plain tensor on a HIP device with data on an `align`-byte boundary, or null: no subclass, no wrapper of a
+// transform or a mode, nothing whose storage is not its own.
+const at::Tensor* strided(PyObject* o, size_t align) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided) return nullptr;
@@ -47,10 +52,31 @@ const at::Tensor* plain(PyObject* o, size_t align) {
       ks.has(c10::DispatchKey::FuncTorchGradWrapper) || ks.has(c10::DispatchKey::Functionalize) ||
       ks.has(c10::DispatchKey::Conjugate) || ks.has(c10::DispatchKey::Negative) || ks.has(c10::DispatchKey::Batched))
     return nullptr;
-  if (!t.has_storage() || !t.is_contiguous() || t.numel() == 0) return nullptr;
+  if (!t.has_storage() || t.numel() == 0) return nullptr;
   if (reinterpret_cast<uintptr_t>(t.const_data_ptr()) % align != 0) return nullptr;
   return &t;
 }
+
+// The same, contiguous.
+const at::Tensor* plain(PyObject* o, size_t align) {
+  const at::Tensor* t = strided(o, align);
+  return t && t->is_contiguous() ? t : nullptr;
+}
+
+// Whether a gradient of one of the inputs is asked for (the Python form raises).
+bool wants_gradient(std::initializer_list<const at::Tensor*> ts) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->requires_grad()) return true;
+  return false;
+}
+
+// An index of one value per row: int32 or int64 of `lead` (a tensor's shape without its last `drop` dimensions).
+bool is_index(const at::Tensor& t, const at::Tensor& x, int64_t drop) {
+  return (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) &&
+         t.sizes() == x.sizes().slice(0, x.dim() - drop);
+}
+int index_bits(const at::Tensor& t) { return t.scalar_type() == at::kLong ? 64 : 32; }
 
 bool same_current_device(const at::Tensor& x, std::initializer_list<const at::Tensor*> others) {
   const auto d = x.device();
@@ -228,14 +254,159 @@ PyObject* norm_qmm(PyObject*, PyObject* const* a, Py_ssize_t na) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(affine, gate_up, general, norm, norm_qmm): the addresses of the loaded library's functions.
+PyObject* pair(at::Tensor&& a, at::Tensor&& b) {
+  PyObject* out = PyTuple_New(2);
+  if (!out) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(a)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(b)));
+  return out;
+}
+
+// lora(x, w, scales, biases, lora_a, lora_b, lora_scale, adapters, group_size, bits, general): quantized_matmul_lora
+// where one call of the library does it: 4-bit groups of 64 on the packed kernels, or any format on the general
+// kernel when `general` is true (the caller's rule).
+PyObject* lora(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  if (na != 11) return none();
+  const at::Tensor *x = plain(a[0], 16), *w = plain(a[1], 16), *s = plain(a[2], 16), *b = plain(a[3], 16),
+                   *la = plain(a[4], 16), *lb = plain(a[5], 16), *sc = plain(a[6], 4), *ids = plain(a[7], 4);
+  if (!x || !w || !s || !b || !la || !lb || !sc || !ids || !is_bf16(*x) || x->dim() < 1 ||
+      !same_current_device(*x, {w, s, b, la, lb, sc, ids}) || wants_gradient({x, la, lb, sc}))
+    return none();
+  const int64_t group = PyLong_AsLongLong(a[8]), bits = PyLong_AsLongLong(a[9]);
+  if (PyErr_Occurred()) return nullptr;
+  const bool general = a[10] == Py_True;
+  const int64_t k = x->sizes().back(), m = x->numel() / k, n = w->size(0);
+  if (group <= 0 || bits <= 0 || !weights_match(*w, *s, *b, k, group, bits) || (general && observed())) return none();
+  if (!is_bf16(*la) || !is_bf16(*lb) || la->dim() != 3 || lb->dim() != 3 || la->size(2) != k || lb->size(1) != n ||
+      lb->size(0) != la->size(0) || lb->size(2) != la->size(1) || sc->scalar_type() != at::kFloat || sc->dim() != 1 ||
+      sc->size(0) != la->size(0) || !is_index(*ids, *x, 1))
+    return none();
+  const int64_t count = la->size(0), rank = la->size(1);
+  at::Tensor y = empty_like_rows(*x, n), ws = at::empty({m, rank}, x->options().dtype(at::kInt));
+  const Weights q(*w, *s, *b);
+  void *st = stream_of(*x), *xp = ptr(*x), *lap = ptr(*la), *lbp = ptr(*lb), *ip = ptr(*ids), *yp = out_ptr(y),
+       *wp = out_ptr(ws);
+  const float* sp = static_cast<const float*>(ptr(*sc));
+  const int ib = index_bits(*ids);
+  if (!yp || !wp) return none();
+  int rc;
+  CALL(rc, p_lora(xp, q.w, q.s, q.b, lap, lbp, sp, ip, ib, yp, wp, m, n, k, count, rank, (int)group, (int)bits, 1, st))
+  return rc == 0 ? THPVariable_Wrap(std::move(y)) : PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// Heads (..., H, D) as rows of heads: the row and head strides, where the leading dimensions are one run of rows and a
+// head's values lie together, 16-byte aligned; the rows in *m.
+bool heads(const at::Tensor& t, int64_t* m, int64_t* row, int64_t* head) {
+  const int64_t n = t.dim(), d = t.size(n - 1);
+  if (d > 1 && t.stride(n - 1) != 1) return false;
+  *m = 1;
+  *row = 0;
+  for (int64_t i = n - 3; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (*m == 1) *row = t.stride(i);
+    else if (t.stride(i) != *row * *m) return false;
+    *m *= t.size(i);
+  }
+  *head = t.size(n - 2) > 1 ? t.stride(n - 2) : 0;
+  return *row % 8 == 0 && *head % 8 == 0 && *row >= 0 && *head >= 0;
+}
+
+// rope(q, k, q_weight, k_weight, eps, positions, inv_freq, interleaved): (q', k') of qk_norm_rope.
+PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  if (na != 8 || !PyFloat_Check(a[4])) return none();
+  const at::Tensor *q = strided(a[0], 16), *k = strided(a[1], 16), *wq = plain(a[2], 16), *wk = plain(a[3], 16),
+                   *pos = plain(a[5], 4), *inv = plain(a[6], 4);
+  if (!q || !k || !wq || !wk || !pos || !inv || !is_bf16(*q) || !is_bf16(*k) || !is_bf16(*wq) || !is_bf16(*wk) ||
+      q->dim() < 2 || k->dim() != q->dim() || !same_current_device(*q, {k, wq, wk, pos, inv}) || wants_gradient({q, k}))
+    return none();
+  const int64_t n = q->dim(), d = q->size(n - 1), p = inv->numel();
+  if (q->sizes().slice(0, n - 2) != k->sizes().slice(0, n - 2) || k->size(n - 1) != d || wq->dim() != 1 || wk->dim() != 1 ||
+      wq->size(0) != d || wk->size(0) != d || inv->dim() != 1 || 2 * p > d || !is_index(*pos, *q, 2) ||
+      (inv->scalar_type() != at::kFloat && inv->scalar_type() != at::kDouble))
+    return none();
+  int64_t m, mk, qr, qh, kr, kh;
+  if (!heads(*q, &m, &qr, &qh) || !heads(*k, &mk, &kr, &kh)) return none();
+  const at::TensorOptions o = q->options();
+  at::Tensor qo = at::empty(q->sizes(), o), ko = at::empty(k->sizes(), o);
+  void *st = stream_of(*q), *qp = ptr(*q), *kp = ptr(*k), *wqp = ptr(*wq), *wkp = ptr(*wk), *pp = ptr(*pos), *ip = ptr(*inv);
+  void *qop = out_ptr(qo), *kop = out_ptr(ko);
+  if (!qop || !kop) return none();
+  const float eps = (float)PyFloat_AS_DOUBLE(a[4]);
+  const int pb = index_bits(*pos), fb = inv->scalar_type() == at::kDouble ? 64 : 32, il = a[7] == Py_True;
+  const int64_t hq = q->size(n - 2), hk = k->size(n - 2);
+  int rc;
+  CALL(rc, p_rope(qp, qr, qh, kp, kr, kh, wqp, wkp, eps, pp, pb, ip, fb, qop, kop, m, hq, hk, d, p, il, st))
+  return rc == 0 ? pair(std::move(qo), std::move(ko)) : PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// A setting of sample: a number (checked by the caller) or a tensor of one value per row. False: neither.
+bool setting(PyObject* o, at::ScalarType type, const at::Tensor& logits, const at::Tensor** t, double* value) {
+  *t = nullptr;
+  if (THPVariable_Check(o)) {
+    *t = plain(o, 4);
+    return *t && (*t)->scalar_type() == type && (*t)->sizes() == logits.sizes().slice(0, logits.dim() - 1);
+  }
+  if (PyFloat_CheckExact(o)) *value = PyFloat_AS_DOUBLE(o);
+  else if (PyLong_CheckExact(o)) *value = PyLong_AsDouble(o);
+  else return false;
+  return !PyErr_Occurred();
+}
+
+// sample(logits, uniform, temperature, top_k, top_p, min_p): (tokens, logprobs) of sample.
+PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  if (na != 6) return none();
+  const at::Tensor *l = strided(a[0], 2), *u = plain(a[1], 4);
+  if (!l || !u || !is_bf16(*l) || l->dim() < 1 || u->scalar_type() != at::kFloat ||
+      u->sizes() != l->sizes().slice(0, l->dim() - 1) || wants_gradient({l}))
+    return none();
+  const int64_t n = l->dim(), v = l->size(n - 1), m = l->numel() / v;
+  const int64_t stride = n == 1 ? v : l->stride(n - 2);
+  if (n > 2 ? !l->is_contiguous() : (v > 1 && l->stride(n - 1) != 1) || (m > 1 && stride < v)) return none();
+  const at::Tensor *t, *k, *p, *mp;
+  double tv = 0, kv = 0, pv = 0, mv = 0;
+  if (!setting(a[2], at::kFloat, *l, &t, &tv) || !setting(a[3], at::kInt, *l, &k, &kv) ||
+      !setting(a[4], at::kFloat, *l, &p, &pv) || !setting(a[5], at::kFloat, *l, &mp, &mv)) {
+    PyErr_Clear();
+    return none();
+  }
+  if ((!t && !(tv >= 0 && tv <= 1e30)) || (!k && !(kv >= 0 && kv < 2147483648.0)) || (!p && !(pv > 0 && pv <= 1)) ||
+      (!mp && !(mv >= 0 && mv <= 1)))
+    return none();  // (out of range: the Python form raises)
+  for (const at::Tensor* x : {u, t, k, p, mp})
+    if (x && x->device() != l->device()) return none();
+  if (!same_current_device(*l, {u})) return none();
+  const int64_t bytes = p_sample_workspace(m, v);
+  if (bytes < 0) return PyLong_FromLong((long)bytes);
+  const auto lead = l->sizes().slice(0, n - 1);
+  at::Tensor tokens = at::empty(lead, l->options().dtype(at::kLong)), logprobs = at::empty(lead, l->options().dtype(at::kFloat));
+  at::Tensor ws = at::empty({bytes}, l->options().dtype(at::kByte));
+  void *tp = out_ptr(tokens), *pp = out_ptr(logprobs), *wp = out_ptr(ws), *st = stream_of(*l), *lp = ptr(*l);
+  if (!tp || !pp || !wp) return none();
+  auto f = [](const at::Tensor* x) { return x ? static_cast<const float*>(ptr(*x)) : nullptr; };
+  const float *up = f(u), *t_p = f(t), *p_p = f(p), *m_p = f(mp);
+  const int32_t* k_p = k ? static_cast<const int32_t*>(ptr(*k)) : nullptr;
+  int rc;
+  CALL(rc, p_sample(lp, m, v, stride, up, t_p, (float)tv, k_p, (int32_t)kv, p_p, (float)pv, m_p, (float)mv,
+                    static_cast<int64_t*>(tp), static_cast<float*>(pp), wp, st))
+  return rc == 0 ? pair(std::move(tokens), std::move(logprobs)) : PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(affine, gate_up, general, norm, norm_qmm, lora, rope, sample, sample_workspace): the addresses of the loaded
+// library's functions.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t na) {
-  if (na != 5) {
-    PyErr_SetString(PyExc_TypeError, "bind takes 5 addresses");
+  constexpr int kFunctions = 9;
+  if (na != kFunctions) {
+    PyErr_Format(PyExc_TypeError, "bind takes %d addresses", kFunctions);
     return nullptr;
   }
-  void* p[5];
-  for (int i = 0; i < 5; ++i) {
+  void* p[kFunctions];
+  for (int i = 0; i < kFunctions; ++i) {
     p[i] = PyLong_AsVoidPtr(a[i]);
     if (!p[i]) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null function address");
@@ -247,6 +418,10 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t na) {
   p_general = reinterpret_cast<decltype(p_general)>(p[2]);
   p_norm = reinterpret_cast<decltype(p_norm)>(p[3]);
   p_norm_qmm = reinterpret_cast<decltype(p_norm_qmm)>(p[4]);
+  p_lora = reinterpret_cast<decltype(p_lora)>(p[5]);
+  p_rope = reinterpret_cast<decltype(p_rope)>(p[6]);
+  p_sample = reinterpret_cast<decltype(p_sample)>(p[7]);
+  p_sample_workspace = reinterpret_cast<decltype(p_sample_workspace)>(p[8]);
   Py_RETURN_NONE;
 }
 
@@ -257,6 +432,9 @@ PyMethodDef methods[] = {
     {"gate_up", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&gate_up)), METH_FASTCALL, nullptr},
     {"norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&norm)), METH_FASTCALL, nullptr},
     {"norm_qmm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&norm_qmm)), METH_FASTCALL, nullptr},
+    {"lora", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&lora)), METH_FASTCALL, nullptr},
+    {"rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&rope)), METH_FASTCALL, nullptr},
+    {"sample", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&sample)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -134,11 +134,12 @@ __device__ __forceinline__ f32x4 lora_tile16(const LoraAdd& E, f32x4 acc, int m0
 __device__ __forceinline__ f32x4 lora_part32(const LoraAdd& E, int m0, int rq, int col, int M, int N) {
   const int lane = threadIdx.x & 63, row = m0 + (lane & 31), chunk = (lane >> 5) * 8;
   const int a = lora_adapter(E, row, M);
+  const bool ours = (lane & 31) >> 3 == rq;  // (t of other rows need not be read)
   uint32_t todo = (uint32_t)__ballot(a >= 0) & 0xFFu << 8 * rq;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   while (todo != 0) {
     const int d = __builtin_amdgcn_readlane(a, __ffs((int)todo) - 1);
-    const bool mine = a == d;
+    const bool mine = a == d && ours;
     const uint32_t rows = (uint32_t)__ballot(mine);
     todo &= ~rows;
     f32x16 part;

@@ -85,7 +85,7 @@ class _NoNative:
     """Stands in for the native module where it is not built or not for this torch and Python: every
     function declines, so the Python form of each call runs."""
 
-    qmm = linear = gate_up = norm = norm_qmm = staticmethod(lambda *args: None)
+    qmm = linear = gate_up = norm = norm_qmm = lora = rope = sample = staticmethod(lambda *args: None)
 
 
 def native():
@@ -106,7 +106,8 @@ def native():
                 raise ImportError(f"built for torch {built_for}, this is {torch.__version__}")
             mod.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
                 "qmm4_affine_bf16", "qmm4_gate_up_silu_bf16", "qmm_affine_general_bf16", "qmm4_add_rms_norm_bf16",
-                "qmm4_add_rms_norm_qmm_bf16")))
+                "qmm4_add_rms_norm_qmm_bf16", "qmm4_affine_lora_bf16", "qmm4_qk_norm_rope_bf16", "qmm4_sample_bf16",
+                "qmm4_sample_workspace")))
         except ImportError as e:
             warnings.warn(f"mlx_tree_spec_amd: the native call path cannot be loaded ({e}); calls take their Python "
                           "form, 6-13 us more host time each. Build it with `python -m mlx_tree_spec_amd.build`.",

@@ -47,6 +47,12 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     angles reduced in fp64, so far positions turn by what inv_freq says, and the result is rounded once.
     """
     what = "qk_norm_rope"
+    if q.is_cuda:
+        out = _lib.native().rope(q, k, q_weight, k_weight, float(eps), positions, inv_freq, bool(interleaved))
+        if type(out) is int:
+            _lib.check(out, what)
+        if out is not None:
+            return out
     no_gradient(what, q=q, k=k)
     for name, t in (("q", q), ("k", k), ("q_weight", q_weight), ("k_weight", k_weight)):
         if t.dtype != torch.bfloat16:

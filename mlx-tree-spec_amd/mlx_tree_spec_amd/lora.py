@@ -18,8 +18,8 @@ import torch
 
 from . import _lib
 from .packed_linear import STATS, QuantizedLinear
-from .qmm import (_check_device, _check_format, _check_weights, _general_kernel_ok, aligned_contiguous,
-                  quantized_matmul)
+from .qmm import (GENERAL_BITS, GENERAL_GROUP_SIZES, _check_device, _check_format, _check_weights,
+                  _general_kernel_ok, _general_shape_ok, aligned_contiguous, quantized_matmul)
 
 MAX_RANK = 256
 _INDEX_DTYPES = (torch.int32, torch.int64)
@@ -62,6 +62,21 @@ def _check_adapters(what: str, lora_a: torch.Tensor, lora_b: torch.Tensor, lora_
                          f"{tuple(lora_scale.shape)}")
 
 
+def _native_lora(x, w, scales, biases, lora_a, lora_b, lora_scale, adapters, transpose, group_size, bits, mode):
+    """The usual call in native code (the output), or None for the general form below."""
+    if transpose is not True or mode != "affine" or not x.is_cuda or x.dim() < 1 or w.dim() != 2:
+        return None
+    k, n = x.shape[-1], w.shape[0]
+    general = bits != 4 or group_size != 64 or k % 128 != 0 or n % 16 != 0
+    if general and (bits not in GENERAL_BITS or group_size not in GENERAL_GROUP_SIZES or k == 0
+                    or not _general_shape_ok(x, x.numel() // k, n, k, bits)):
+        return None
+    y = _lib.native().lora(x, w, scales, biases, lora_a, lora_b, lora_scale, adapters, group_size, bits, general)
+    if type(y) is int:
+        _lib.check(y, "quantized_matmul_lora")
+    return y
+
+
 def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
                           lora_a: torch.Tensor, lora_b: torch.Tensor, lora_scale: torch.Tensor,
                           adapters: torch.Tensor, transpose: bool = True, group_size: int = 64, bits: int = 4,
@@ -77,6 +92,9 @@ def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor
     dequantizes and multiplies); x @ lora_a.T is kept to 2^-18 of its value in between.
     """
     what = "quantized_matmul_lora"
+    y = _native_lora(x, w, scales, biases, lora_a, lora_b, lora_scale, adapters, transpose, group_size, bits, mode)
+    if y is not None:
+        return y
     _check_format(group_size, bits, transpose, mode, general=True)
     no_gradient(what, x=x, lora_a=lora_a, lora_b=lora_b, lora_scale=lora_scale)
     if x.dtype != torch.bfloat16:

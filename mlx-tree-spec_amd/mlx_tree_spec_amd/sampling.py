@@ -47,6 +47,12 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0
     -infinity. Masses are summed in fp64.
     """
     what = "sample"
+    if logits.is_cuda:
+        out = _lib.native().sample(logits, uniform, temperature, top_k, top_p, min_p)
+        if type(out) is int:
+            _lib.check(out, what)
+        if out is not None:
+            return out
     no_gradient(what, logits=logits)
     if logits.dtype != torch.bfloat16:
         raise ValueError(f"[{what}] logits must be bfloat16, got {logits.dtype}")
