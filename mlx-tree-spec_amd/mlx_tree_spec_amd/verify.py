@@ -8,7 +8,13 @@ once over all rows, and each residual add is fused with the RMS norm that follow
     nxt  = next layer's input_layernorm, or the model's final norm # 445
     h, x = add_rms_norm(h, layer.mlp(x), nxt)                      # 446
 
-`r` is the attention (or GatedDeltaNet) output of the layer, which this package does not compute.
+`r` is the attention (or GatedDeltaNet) output of the layer, which this package does not compute. What lies before
+it, and behind the last layer, is here as well:
+
+    q, k, v, gate = attention_inputs(x, layer, positions, adapters)  # tree_verify.py:311-328: projections (with each
+                                                                     # row's adapter), head norms, rotation
+    tokens, logprobs = next_tokens(x, lm_head, uniform, ...)         # tree_verify.py:447: vocabulary head, sampling
+
 When the MLP is a QuantizedMLP, the first norm is folded into its gate+up projection
 (add_rms_norm_gate_up: the same bits, one launch fewer for up to 4 rows).
 The row count M = the sum of the requests' tree nodes decides the kernel inside libqmm4 (row-split
@@ -25,8 +31,11 @@ from __future__ import annotations
 
 import torch
 
-from .fused_ops import add_rms_norm, add_rms_norm_gate_up
+from .fused_ops import _norm_eps, add_rms_norm, add_rms_norm_gate_up
+from .heads import qk_norm_rope
+from .lora import LoRALinear
 from .packed_linear import STATS, QuantizedMLP
+from .sampling import sample
 
 
 class MLPLayer(torch.nn.Module):
@@ -58,6 +67,47 @@ def stack_tail(h: torch.Tensor, rs: list[torch.Tensor], layers: list[MLPLayer], 
         nxt = layers[i + 1].post_attention_layernorm if i + 1 < len(layers) else final_norm
         h, x = layer_tail(h, rs[i], layer, nxt)
     return h, x
+
+
+class AttentionInputs(torch.nn.Module):
+    """The parts of one decoder layer in front of its attention: q_proj, k_proj, v_proj (QuantizedLinear or LoRALinear),
+    q_norm and k_norm (RMSNorm modules over a head), the head counts and width, and inv_freq [P]. gated: q_proj gives
+    each query head followed by a gate of its width (tree_verify.py:318-321); interleaved as in qk_norm_rope."""
+
+    def __init__(self, q_proj: torch.nn.Module, k_proj: torch.nn.Module, v_proj: torch.nn.Module, q_norm: torch.nn.Module,
+                 k_norm: torch.nn.Module, heads: int, kv_heads: int, head_dim: int, inv_freq: torch.Tensor,
+                 gated: bool = False, interleaved: bool = False):
+        super().__init__()
+        self.q_proj, self.k_proj, self.v_proj, self.q_norm, self.k_norm = q_proj, k_proj, v_proj, q_norm, k_norm
+        self.heads, self.kv_heads, self.head_dim, self.gated, self.interleaved = heads, kv_heads, head_dim, gated, interleaved
+        if _norm_eps(q_norm) != _norm_eps(k_norm):
+            raise ValueError(f"[AttentionInputs] q_norm and k_norm differ in eps: {_norm_eps(q_norm)}, {_norm_eps(k_norm)}")
+        self.register_buffer("inv_freq", inv_freq)
+
+
+def _project(proj: torch.nn.Module, x: torch.Tensor, adapters: torch.Tensor | None) -> torch.Tensor:
+    return proj(x, adapters) if isinstance(proj, LoRALinear) else proj(x)
+
+
+def attention_inputs(x: torch.Tensor, layer: AttentionInputs, positions: torch.Tensor, adapters: torch.Tensor | None = None):
+    """(q, k, v, gate) of rows x (..., K): q (..., heads, D) and k (..., kv_heads, D) normed and rotated at each row's
+    position, v (..., kv_heads, D), gate (..., heads, D) or None. `adapters` (one per row) goes to the projections that
+    are LoRALinear."""
+    lead, d = x.shape[:-1], layer.head_dim
+    q = _project(layer.q_proj, x, adapters).reshape(*lead, layer.heads, -1)
+    k = _project(layer.k_proj, x, adapters).reshape(*lead, layer.kv_heads, d)
+    v = _project(layer.v_proj, x, adapters).reshape(*lead, layer.kv_heads, d)
+    gate = q[..., d:] if layer.gated else None
+    q, k = qk_norm_rope(q[..., :d] if layer.gated else q, k, layer.q_norm.weight, layer.k_norm.weight,
+                        _norm_eps(layer.q_norm), positions, layer.inv_freq, interleaved=layer.interleaved)
+    return q, k, v, gate
+
+
+def next_tokens(x: torch.Tensor, head: torch.nn.Module, uniform: torch.Tensor, adapters: torch.Tensor | None = None,
+                **settings):
+    """(tokens, logprobs) drawn from the vocabulary head's logits of rows x (tree_verify.py:447), with `sample`'s
+    settings."""
+    return sample(_project(head, x, adapters), uniform, **settings)
 
 
 class GraphedTail:
