@@ -15,14 +15,19 @@
 //           again, and only that slice is read.
 // Up to 65535 logits one pick kernel counts its row itself.
 //
-// The sums run over the values that occur, up to 4096 of them (a page) listed in LDS, 4 neighbours to a thread: a
-// prefix over the workgroup gives the count before each thread, its counts within top-k, their masses; another the
-// mass before it, what top-p and min-p keep of it; a third the kept mass before it, and with it the value that
-// passes the target. More values (152k logits of a model have about 3500; past 4096 they lie many octaves apart)
-// take their pages in turn, once per sum.
+// The sums run over the values that occur, up to 4096 of them (a page) listed in LDS, 4 neighbours to a thread: one
+// prefix over the workgroup, of counts and masses. What top-k, top-p and min-p keep is a beginning of the order, so
+// each of them is a place in that prefix, and so is the target: the thread that holds it works it out and writes it
+// down for the others. More values (152k logits of a model have about 3500; past 4096 they lie many octaves apart) take
+// their pages in turn, once per place to be found.
 //
-// What bounds it: a row's steps follow each other in one workgroup, and its 16 waves get through about 150
-// instructions each a microsecond; the steps are kept to few instructions per value and wave.
+// What bounds it: a row's steps follow each other in one workgroup, each a few hundred ns of LDS round trips and
+// barriers, and a CU gets through 2400 vector instructions of its waves each a microsecond; both kernels are kept to
+// few instructions per value. On the GPU: 1 x 151936 19.9 us, 32 x 151936 (all settings) 23.0 us, 200 x 32001 14.8 us,
+// of which the counting takes 6, 7 and 9. The prefix after prefix of counts, masses and what is kept that was here
+// first, with 64 words to a look, took 27, 30 and 18 us.
+#include <type_traits>
+
 #include "qmm4_common.h"
 #include "qmm4_lds.h"
 #include "qmm_requests_kernels.h"
@@ -179,318 +184,424 @@ __device__ __forceinline__ void zero_lds(uint32_t* p) {
   for (int i = threadIdx.x; i < BYTES / 16; i += kThreads) reinterpret_cast<u32x4*>(p)[i] = u32x4{0u, 0u, 0u, 0u};
 }
 
-// Where a batch's lists lie: n [rows][slices], entries [rows][slices][slice], an entry rank << 16 | count (a slice's
-// list padded to a multiple of 4 with count 0).
+// Where a batch's lists lie: heads [rows][slices], entries [rows][slices][slice], an entry rank << 16 | count (a
+// slice's list padded to a multiple of 4 with count 0).
+struct Head {
+  uint32_t n, lowest;  // entries, and the smallest rank (kValues where there is none)
+};
 struct Lists {
-  uint32_t* n;
+  Head* heads;
   uint32_t* entries;
   int slice, slices;
   __device__ uint32_t* list(int64_t m, int s) const { return entries + (m * slices + s) * (int64_t)slice; }
 };
 
+// How many of four counts, or of eight of 16 bits, are not zero.
+template <bool PAIRS>
+__device__ __forceinline__ uint32_t occurring(u32x4 v) {
+  uint32_t n = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (PAIRS) n += __popc((((v[e] & 0x7FFF7FFFu) + 0x7FFF7FFFu) | v[e]) & 0x80008000u);
+    else n += min(v[e], 1u);
+  }
+  return n;
+}
+
+// before(total) with the number of values that occur in a histogram, then emit(o, r, n) for each, r its number, n its
+// count and o its place among them in rising r. PAIRS: 16-bit counts, two to a word.
+// A wave looks at 256 neighbouring words at a time (16 bytes a lane), the next wave at the next: occurring values crowd
+// in a few octaves. A lane's place is a prefix over the wave, and over the looks before (look [WORDS / 256] in LDS,
+// summed by each wave itself). HELD: the words stay in registers between the two, else they are read again.
+template <bool PAIRS, int WORDS, bool HELD, class T, class F>
+__device__ __forceinline__ void list_values(const uint32_t* hist, uint32_t* look, T&& before, F&& emit) {
+  constexpr int kLooks = WORDS / 256 / kWaves, kHalf = PAIRS ? 2 : 1;
+  constexpr int kSums = (kLooks * kWaves + 63) / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto words = [&](int t) { return reinterpret_cast<const u32x4*>(hist)[(t * kWaves + wave) * 64 + lane]; };
+  auto none = [](u32x4 v) { return __ballot((v.x | v.y | v.z | v.w) != 0) == 0; };
+  u32x4 v[HELD ? kLooks : 1];
+  uint32_t own[HELD ? kLooks : 1], mine = 0;  // (own: the lane's prefix within the look, without itself)
+  auto sum = [&](int t, u32x4 v, uint32_t& own) {
+    own = 0;
+    if (none(v)) return;
+    const uint32_t n = occurring<PAIRS>(v), inc = wave_prefix(n), all = lane_value(inc, 63);  // (in every lane)
+    own = inc - n;
+    mine = lane == t ? all : mine;
+  };
+  if constexpr (HELD) {
+#pragma unroll
+    for (int t = 0; t < kLooks; ++t) v[t] = words(t);
+#pragma unroll
+    for (int t = 0; t < kLooks; ++t) sum(t, v[t], own[t]);
+  } else {
+#pragma clang loop unroll(disable)
+    for (int t = 0; t < kLooks; ++t) sum(t, words(t), own[0]);
+  }
+  if (lane < kLooks) look[lane * kWaves + wave] = mine;
+  __syncthreads();
+  uint32_t ahead[kSums], total = 0;
+#pragma unroll
+  for (int i = 0; i < kSums; ++i) {
+    const uint32_t n = i * 64 + lane < kLooks * kWaves ? look[i * 64 + lane] : 0, inc = wave_prefix(n);
+    ahead[i] = total + inc - n;
+    total += lane_value(inc, 63);
+  }
+  before(total);
+  auto list = [&](int t, u32x4 v, uint32_t o) {
+    if (none(v)) return;
+#pragma unroll
+    for (int e = 0; e < 4 * kHalf; ++e) {
+      const uint32_t n = !PAIRS ? v[e] : e & 1 ? v[e / 2] >> 16 : v[e / 2] & 0xFFFFu;
+      if (n != 0) emit(o++, (uint32_t)((t * kWaves + wave) * 256 + lane * 4) * kHalf + e, n);
+    }
+  };
+  if constexpr (HELD) {
+#pragma unroll
+    for (int t = 0; t < kLooks; ++t) list(t, v[t], own[t] + lane_value(ahead[t * kWaves / 64], t * kWaves % 64 + wave));
+  } else {
+#pragma clang loop unroll(disable)
+    for (int t = 0; t < kLooks; ++t) {
+      uint32_t at = ahead[0];
+#pragma unroll
+      for (int i = 1; i < kSums; ++i) at = t * kWaves / 64 == i ? ahead[i] : at;
+      sum(t, words(t), own[0]);
+      list(t, words(t), own[0] + lane_value(at, t * kWaves % 64 + wave));
+    }
+  }
+}
+
 constexpr int kBytes16 = 65536 * 2;
 
 __global__ __launch_bounds__(kThreads) void sample_count_kernel(SampleParams S, Lists L) {
   extern __shared__ __attribute__((aligned(16))) uint32_t hist[];
-  __shared__ uint32_t s_n[kWaves];
+  __shared__ uint32_t s_look[128];
+  __shared__ int s_lo[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t m = blockIdx.y;
   const int begin = blockIdx.x * L.slice, end = min(S.V, begin + L.slice);
   u32x4 held[kBatch];
-  count_lines(Lines(S.logits + m * S.row_stride, begin, end), hist, held, [&] {
+  const int lo = wave_min(count_lines(Lines(S.logits + m * S.row_stride, begin, end), hist, held, [&] {
     zero_lds<kBytes16>(hist);
     __syncthreads();
-  });
+  }));
+  if (lane == 0) s_lo[wave] = lo;
   __syncthreads();
-  // Each wave lists 4096 neighbouring values, 64 words of two at a time: a comparison is a mask of the lanes, and a
-  // lane's place in the list the number of values below it.
-  constexpr int kLooks = 32;
-  const uint32_t* h = hist + wave * (kLooks * 64) + lane;
-  uint32_t mine = 0, looks = 0;
-#pragma unroll
-  for (int t = 0; t < kLooks; ++t) {
-    const uint32_t v = h[t * 64];
-    const int seen = __popcll(__ballot((v & 0xFFFFu) != 0)) + __popcll(__ballot(v > 0xFFFFu));
-    mine += seen;
-    looks |= seen != 0 ? 1u << t : 0;
-  }
-  if (lane == 0) s_n[wave] = mine;
-  __syncthreads();
-  const uint32_t waves = row_prefix(s_n[lane & 15]), total = lane_value(waves, 15);
-  uint32_t at = wave ? lane_value(waves, wave - 1) : 0u;
   uint32_t* list = L.list(m, blockIdx.x);
-  for (; looks != 0; looks &= looks - 1) {
-    const int t = __ffs((int)looks) - 1;
-    const uint32_t v = h[t * 64];
-    const unsigned long long lo = __ballot((v & 0xFFFFu) != 0), hi = __ballot(v > 0xFFFFu);
-    uint32_t o = __builtin_amdgcn_mbcnt_hi((uint32_t)(lo >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lo, at));
-    o = __builtin_amdgcn_mbcnt_hi((uint32_t)(hi >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hi, o));
-    const uint32_t r = (uint32_t)((wave * kLooks + t) * 64 + lane) * 2;
-    if ((v & 0xFFFFu) != 0) list[o++] = r << 16 | (v & 0xFFFFu);
-    if (v > 0xFFFFu) list[o] = (r + 1) << 16 | v >> 16;
-    at += __popcll(lo) + __popcll(hi);
-  }
-  if (tid == 0) L.n[m * L.slices + blockIdx.x] = total;
-  if (tid < 4 && (total & 3) != 0 && tid >= (int)(total & 3)) list[(total & ~3u) + tid] = 0;
+  list_values<true, 32768, true>(
+      hist, s_look,
+      [&](uint32_t n) {
+        const int lowest = row_min(s_lo[lane & 15]);
+        if (tid == 0) L.heads[m * L.slices + blockIdx.x] = {n, (uint32_t)min(lowest, kValues)};
+        if (tid < 4 && (n & 3) != 0 && tid >= (int)(n & 3)) list[(n & ~3u) + tid] = 0;
+      },
+      [&](uint32_t o, uint32_t r, uint32_t n) { list[o] = r << 16 | n; });
 }
+
+// (The loop over pages would keep the constants of an inlined exp in 50 registers and the rest in memory: 0.8 us, in
+// rows that never come to it.)
+__device__ __attribute__((noinline)) double exp_called(double x) { return exp(x); }
 
 // One row. MERGE: from the slices' lists, else from the row itself.
 template <bool MERGE>
 __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams S, Lists L) {
-  constexpr int kSpan = MERGE ? 36 * kThreads : 65536;  // values of one histogram: +-512 with all between, or all
-  constexpr int kPer = 4;                         // listed values of a page to a thread
-  constexpr int kPage = kPer * kThreads;
+  constexpr int kSpan = MERGE ? 36864 : 65536;  // values of one histogram: +-512 with all between, or all
+  constexpr int kPage = 4096, kPer = kPage / kThreads;  // listed values at a time, of them to a thread
   extern __shared__ __attribute__((aligned(16))) uint32_t hist[];
   __shared__ uint16_t s_page[kPage];
-  __shared__ int s_lo[kWaves], s_hi[kWaves];
-  __shared__ double s_d[2][kWaves];
-  __shared__ uint32_t s_u[kBatch][kWaves], s_n[MERGE ? kMaxSlices : 1], s_occ[MERGE ? kMaxSlices : 1];
+  __shared__ int s_lo[kWaves];
+  __shared__ double s_mass[kWaves];
+  __shared__ uint32_t s_u[kBatch][kWaves], s_look[kSpan / 256], s_n[MERGE ? kMaxSlices : 1], s_occ[MERGE ? kMaxSlices : 1];
+  __shared__ uint32_t s_count[kWaves], s_above[kWaves], s_far;
+  struct Cut {  // an end of what is kept: the mass before it, the last value kept (its number in the order), how often
+    double mass;
+    uint32_t index, n;
+  };
+  __shared__ Cut s_cut[3];
   __shared__ uint32_t s_hit[2];
   __shared__ double s_weight;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t m = blockIdx.x;
   const uint16_t* row = S.logits + m * S.row_stride;
 
-  float temp = S.temperature[m], top_p = S.top_p[m], min_p = S.min_p[m];
+  // (Each with a load, one value for all or not: loads behind a branch wait for each other.)
+  const uint32_t* const any = reinterpret_cast<const uint32_t*>(S.uniform);
+  auto setting = [&](auto s) {
+    const uint32_t v = (s.p ? reinterpret_cast<const uint32_t*>(s.p) : any)[m];
+    return s.p ? __builtin_bit_cast(decltype(s.value), v) : s.value;
+  };
+  float temp = setting(S.temperature), top_p = setting(S.top_p), min_p = setting(S.min_p);
   const float u = S.uniform[m];
-  const int32_t top_k = S.top_k[m];
-  // Settings that leave the first of the order only: as top-k 1.
-  const bool first_only = !(temp > 0.0f) || top_p <= 0.0f || min_p > 1.0f;
-  const uint32_t limit = first_only ? 1u : top_k > 0 ? (uint32_t)top_k : 0xFFFFFFFFu;
-  if (first_only) {
-    temp = top_p = 1.0f;
-    min_p = 0.0f;
-  }
+  const int32_t top_k = setting(S.top_k);
+  // Settings that leave the first of the order only.
+  const bool first_only = !(temp > 0.0f) || top_p <= 0.0f || min_p > 1.0f || top_k == 1;
+  const uint32_t limit = top_k > 0 ? (uint32_t)top_k : 0xFFFFFFFFu;
 
   // `lowest`: the first value that occurs. The histogram holds values from `base`; a second one (part 1) those past
   // its end, where there are any.
-  int lowest = kValues, base = 0, parts = 1;
+  int lowest, base = 0;
   u32x4 held[kBatch];
-  if constexpr (MERGE) {
-    int lo = kValues, hi = -1;
-    for (int s = tid; s < L.slices; s += kThreads) {
-      const uint32_t n = L.n[m * L.slices + s];
-      s_n[s] = n;
-      if (n == 0) continue;
-      const uint32_t* list = L.list(m, s);
-      lo = min(lo, (int)(list[0] >> 16));
-      hi = max(hi, (int)(list[n - 1] >> 16));
+  {
+    int lo = kValues;
+    if constexpr (MERGE) {
+      for (int s = tid; s < L.slices; s += kThreads) {
+        const Head head = L.heads[m * L.slices + s];
+        s_n[s] = head.n;
+        lo = min(lo, (int)head.lowest);
+      }
+      if (tid == 0) s_far = 0;
+      zero_lds<kSpan * 4>(hist);
+    } else {
+      lo = count_lines(Lines(row, 0, S.V), hist, held, [&] {
+        zero_lds<kBytes16>(hist);
+        __syncthreads();
+      });
     }
     lo = wave_min(lo);
-    hi = wave_max(hi);
-    if (lane == 0) {
-      s_lo[wave] = lo;
-      s_hi[wave] = hi;
-    }
-    __syncthreads();
-    lowest = row_min(s_lo[lane & 15]);
-    base = lowest & ~3;
-    parts = row_max(s_hi[lane & 15]) - base >= kSpan ? 2 : 1;
-  } else {
-    const int lo = wave_min(count_lines(Lines(row, 0, S.V), hist, held, [&] {
-      zero_lds<kBytes16>(hist);
-      __syncthreads();
-    }));
     if (lane == 0) s_lo[wave] = lo;
     __syncthreads();
-    lowest = row_min(s_lo[lane & 15]);
+    lowest = row_min(s_lo[lane & (kWaves - 1)]);
+    if (MERGE) base = lowest & ~3;
   }
-  if (lowest == kValues) {
+  if (lowest >= kValues) {
     if (tid == 0) {
       S.tokens[m] = -1;
       S.logprobs[m] = -__builtin_inff();
     }
     return;
   }
-  const double largest = value_of(lowest), per_temp = 1.0 / (double)temp;
 
-  // Prefix of v over the workgroup's threads, and its total. `slot` alternates between calls.
-  auto block_prefix = [&](auto v, auto* slot, auto* total) __attribute__((always_inline)) {
-    const auto inc = wave_prefix(v);
-    if (lane == 63) slot[wave] = inc;
-    __syncthreads();
-    const auto waves = row_prefix(slot[lane & 15]);
-    *total = lane_value(waves, 15);
-    return (wave ? lane_value(waves, wave - 1) : decltype(v)(0)) + (inc - v);
-  };
-
-  // Three sums over the pages: the mass within top-k, the part of it that is kept, and up to the target. With one page
-  // the threads keep their values from sum to sum.
-  double total = 0.0, kept_total = 0.0, target = 0.0;
-  int built = MERGE ? -1 : 0;
-  bool one_page = true;
-  uint32_t c[kPer], n[kPer];
-  double w[kPer], mass = 0.0, mass_before = 0.0, kept = 0.0, kept_before = 0.0;
-  int rank[kPer], per = 0;
-  for (int sum = 0; sum < 3; ++sum) {
-    uint32_t count_sum = 0;
-    double mass_sum = 0.0, kept_sum = 0.0;
-    for (int part = 0; part < parts; ++part) {
-      const int from = base + part * kSpan;
-      if (MERGE && built != part) {
-        __syncthreads();
-        zero_lds<kSpan * 4>(hist);
-        __syncthreads();
-        built = part;
-        for (int s = wave; s < L.slices; s += kWaves) {
-          const int n4 = ((int)s_n[s] + 3) / 4;
-          const u32x4* list = reinterpret_cast<const u32x4*>(L.list(m, s));
-          constexpr int kAhead = 8;
-          for (int i0 = lane; i0 < n4; i0 += kAhead * 64) {
-            u32x4 v[kAhead];
+  uint32_t hit = lowest, left = 0;
+  double hit_weight = 1.0, kept_total = 1.0;
+  if (!first_only) {
+    const double largest = value_of(lowest), per_temp = 1.0 / (double)temp;
+    const bool some = limit < (uint32_t)S.V;  // (top-k may end the order)
+    // Four walks through the pages: the masses and counts; the end that top-k sets; those of top-p and min-p; the value
+    // that passes the target. The order's masses before each thread's values are the same in each: an end is a place in
+    // them, and the thread that holds it writes it down. One page is walked where it stands, in registers; more are
+    // listed again for each walk.
+    double target = 0.0;
+    Cut cut = {0.0, 0xFFFFFFFFu, 0};
+    uint32_t c[kPer], count = 0, count_before = 0, entries = 0;
+    double w[kPer], mass = 0.0, mass_before = 0.0;
+    double lane_waves = 0.0;  // of lane i: the mass before wave i's values; lane_has: whether those have any
+    bool lane_has = false;
+    int rank[kPer], per = 0;
+    // Sums over the values so far.
+    uint32_t count_sum = 0, above_sum = 0, above_total = 0, index0 = 0;
+    double mass_sum = 0.0;
+    // The lists' values from `from` on into the histogram (cleared before).
+    auto merge = [&](int from) __attribute__((always_inline)) {
+      bool far = false;
+      for (int s = wave; s < L.slices; s += kWaves) {
+        const int n4 = ((int)s_n[s] + 3) / 4;
+        const u32x4* list = reinterpret_cast<const u32x4*>(L.list(m, s));
+        constexpr int kAhead = 8;
+        for (int i0 = lane; i0 < n4; i0 += kAhead * 64) {
+          u32x4 v[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) v[i] = list[min(i0 + i * 64, n4 - 1)];
-            __builtin_amdgcn_sched_barrier(0);
+          for (int i = 0; i < kAhead; ++i) v[i] = list[min(i0 + i * 64, n4 - 1)];
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
+          for (int i = 0; i < kAhead; ++i) {
+            if (i0 + i * 64 >= n4) break;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {  // (what is not for this histogram goes behind it, one word for each lane)
-                const int r = (int)(v[i][e] >> 16) - from;
-                const bool in = i0 + i * 64 < n4 && (uint32_t)r < (uint32_t)kSpan;
-                atomicAdd(&hist[in ? r : kSpan + lane], v[i][e] & 0xFFFFu);
-              }
+            for (int e = 0; e < 4; ++e) {  // (what is not for this histogram goes behind it, one word for each lane)
+              const int r = (int)(v[i][e] >> 16) - from;
+              atomicAdd(&hist[min((uint32_t)r, (uint32_t)(kSpan + lane))], v[i][e] & 0xFFFFu);
+              far |= r >= kSpan;
             }
           }
         }
-        __syncthreads();
       }
-      uint32_t entries = 0;
-      for (uint32_t first = 0; first == 0 || first < entries; first += kPage) {
-        if (sum == 0 || !one_page) {
-          // The page's values: those that occur, the first-th and on. A wave lists kLooks * 64 neighbouring words of the
-          // histogram, 64 at a time: a comparison is a mask of the lanes, and a lane's place in the list the number of
-          // them below it. (Neighbouring groups of 64 to different waves took two more barriers and 0.4 us.)
-          constexpr int kLooks = kSpan / (MERGE ? 1 : 2) / kThreads;
-          const uint32_t* h = hist + wave * (kLooks * 64) + lane;
-          uint32_t here = 0;
-#pragma unroll 9
-          for (int t = 0; t < kLooks; ++t) {
-            const uint32_t v = h[t * 64];
-            if constexpr (MERGE) here += __popcll(__ballot(v != 0));
-            else here += __popcll(__ballot((v & 0xFFFFu) != 0)) + __popcll(__ballot(v > 0xFFFFu));
-          }
-          __syncthreads();  // (the page before is read)
-          uint32_t at = block_prefix(lane == 0 ? here : 0u, s_u[0], &entries);
-          at = lane_value(at, 0) - first;
-          if (sum == 0 && part == 0 && first == 0) one_page = parts == 1 && entries <= kPage;
-#pragma unroll 9
-          for (int t = 0; t < kLooks; ++t) {
-            const uint32_t v = h[t * 64];
-            const unsigned long long lo = __ballot(MERGE ? v != 0 : (v & 0xFFFFu) != 0), hi = MERGE ? 0 : __ballot(v > 0xFFFFu);
-            if ((lo | hi) == 0) continue;
-            uint32_t o = __builtin_amdgcn_mbcnt_hi((uint32_t)(lo >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lo, at));
-            const uint32_t r = (uint32_t)((wave * kLooks + t) * 64 + lane) * (MERGE ? 1 : 2);
-            if constexpr (!MERGE)
-              o = __builtin_amdgcn_mbcnt_hi((uint32_t)(hi >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hi, o));
-            if ((MERGE ? v != 0 : (v & 0xFFFFu) != 0) && o < (uint32_t)kPage) s_page[o] = (uint16_t)r;
-            if constexpr (!MERGE) {
-              o += (v & 0xFFFFu) != 0;
-              if (v > 0xFFFFu && o < (uint32_t)kPage) s_page[o] = (uint16_t)(r + 1);
-            }
-            at += __popcll(lo) + __popcll(hi);
-          }
-          __syncthreads();
-          // Counts within top-k and their masses. (Equal weights of neighbours: none of the values is taken twice.)
-          const uint32_t in_page = min(entries - first, (uint32_t)kPage);
-          per = (int)((in_page + kThreads - 1) / kThreads);
-          uint32_t own = 0, page_count, all[kPer];
+      if (far) s_far = 1;
+      __syncthreads();
+    };
+    // A page of a histogram: the values that occur, the first-th and on, with their weights and masses.
+    auto list_page = [&](auto held, int from, uint32_t first) __attribute__((always_inline)) {
+      list_values<!MERGE, kSpan / (MERGE ? 1 : 2), decltype(held)::value>(
+          hist, s_look, [&](uint32_t n) { entries = n; },
+          [&](uint32_t o, uint32_t r, uint32_t) {
+            o -= first;
+            if (o < (uint32_t)kPage) s_page[o] = (uint16_t)r;
+          });
+      __syncthreads();
+      const uint32_t in_page = min(entries - first, (uint32_t)kPage);
+      per = (int)((in_page + kThreads - 1) / kThreads);
+      uint32_t above = 0;
+      count = 0;
+      mass = 0.0;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        c[e] = 0;
+        w[e] = 0.0;
+        if (e >= per) continue;
+        const uint32_t i = tid * per + e;
+        const bool is = i < in_page;
+        const uint32_t r = is ? s_page[i] : 0u;
+        rank[e] = from + (int)r;
+        c[e] = !is ? 0u : MERGE ? hist[r] : r & 1 ? hist[r >> 1] >> 16 : hist[r >> 1] & 0xFFFFu;
+      }
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        if (e >= per) break;
+        // (The largest value itself has 1, also where it is infinite.)
+        const double d = value_of(rank[e]) - largest;
+        w[e] = rank[e] == lowest ? 1.0 : largest == __builtin_inf() ? 0.0 : (decltype(held)::value ? exp(d * per_temp) : exp_called(d * per_temp));
+        if (c[e] == 0) w[e] = 0.0;
+        if (min_p > 0.0f) above += __popcll(__ballot(w[e] >= (double)min_p));
+        count += c[e];
+        mass += c[e] * w[e];
+      }
+      const double mass_inc = wave_prefix(mass);
+      uint32_t count_inc = 0;
+      if (some) count_inc = wave_prefix(count);
+      if (lane == 63) {
+        s_mass[wave] = mass_inc;
+        s_count[wave] = count_inc;
+        s_above[wave] = above;
+      }
+      __syncthreads();
+      const double of_wave = s_mass[lane & (kWaves - 1)], waves = mass_sum + row_prefix(of_wave);
+      lane_waves = dpp<0x111, 0xF>(waves);
+      if (lane == 0) lane_waves = mass_sum;
+      lane_has = lane < kWaves && of_wave > 0.0;
+      mass_before = lane_value(lane_waves, wave) + (mass_inc - mass);
+      mass_sum = lane_value(waves, kWaves - 1);
+      if (some) {
+        const uint32_t counts = count_sum + row_prefix(s_count[lane & (kWaves - 1)]);
+        count_before = (wave ? lane_value(counts, wave - 1) : count_sum) + (count_inc - count);
+        count_sum = lane_value(counts, kWaves - 1);
+      }
+      if (min_p > 0.0f) above_sum += lane_value(row_prefix(s_above[lane & (kWaves - 1)]), kWaves - 1);
+    };
+    auto decide = [&](int walk) __attribute__((always_inline)) {
+      const uint32_t page0 = index0, own0 = page0 + tid * per;  // numbers in the order: the page's first, the thread's
+      // Whether this thread is the page's last with some mass that starts before x (or at x), up to value number `last`.
+      auto holds = [&](double x, bool at, uint32_t last) __attribute__((always_inline)) {
+        const unsigned long long in = __ballot(lane_has && (lane_waves < x || (at && lane_waves == x)) && page0 + lane * 64 * per <= last);
+        if (in == 0 || wave != 63 - __builtin_clzll(in)) return false;
+        const unsigned long long threads = __ballot(mass > 0.0 && (mass_before < x || (at && mass_before == x)) && own0 <= last);
+        return threads != 0 && lane == 63 - __builtin_clzll(threads);
+      };
+      if (walk == 1 && count_before < limit && limit - count_before <= count) {
+        uint32_t cb = count_before;
+        double mb = mass_before;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          if (cb < limit && limit - cb <= c[e]) s_cut[0] = {mb + (limit - cb) * w[e], own0 + e, limit - cb};
+          cb += c[e];
+          mb += c[e] * w[e];
+        }
+      }
+      if (walk == 2) {
+        const double bound = (double)top_p * cut.mass;
+        if (top_p < 1.0f && holds(bound, false, 0xFFFFFFFFu)) {  // kept: with less mass than the bound before them
+          Cut end = cut;
+          double mb = mass_before;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
-            all[e] = c[e] = n[e] = 0;
-            w[e] = 0.0;
-            if (e >= per) continue;
-            const uint32_t i = tid * per + e;
-            const bool is = i < in_page;
-            const uint32_t r = is ? s_page[i] : 0u;
-            rank[e] = from + (int)r;
-            all[e] = !is ? 0u : MERGE ? hist[r] : r & 1 ? hist[r >> 1] >> 16 : hist[r >> 1] & 0xFFFFu;
-            own += all[e];
+            const double after = mb + c[e] * w[e];
+            if (w[e] > 0.0 && mb < bound) {
+              const uint32_t n = after > bound ? min(c[e], (uint32_t)ceil((bound - mb) / w[e])) : c[e];
+              end = {mb + n * w[e], own0 + e, n};
+            }
+            mb = after;
           }
-          uint32_t before = count_sum + block_prefix(own, s_u[1], &page_count);
-          count_sum += page_count;
-          double page_mass;
-          mass = 0.0;
+          s_cut[1] = end;
+        }
+        if (min_p > 0.0f && above_total - 1 - own0 < (uint32_t)per) {
+          double mb = mass_before;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
-            if (e >= per) break;
-            c[e] = before >= limit ? 0u : min(all[e], limit - before);
-            before += all[e];
-            // (The largest value itself has 1, also where it is infinite.)
-            const double d = value_of(rank[e]) - largest;
-            w[e] = rank[e] == lowest ? 1.0 : largest == __builtin_inf() ? 0.0 : exp(d * per_temp);
-            if (c[e] == 0) w[e] = 0.0;
-            mass += c[e] * w[e];
-          }
-          mass_before = mass_sum + block_prefix(mass, s_d[0], &page_mass);
-          mass_sum += page_mass;
-        }
-        if (sum == 1 || (sum == 2 && !one_page)) {
-          // Kept of a value: those with less mass before them than the bound, and a weight of at least min_p.
-          if (top_p < 1.0f || min_p > 0.0f) {
-            const double bound = (double)top_p * total;
-            double mb = mass_before, page_kept;
-            kept = 0.0;
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-              if (e >= per) break;
-              const double end = mb + c[e] * w[e];
-              n[e] = c[e];
-              if (top_p < 1.0f && end > bound) {  // (the division is for one value of all: 4 in each thread took 0.7 us)
-                n[e] = 0;
-                if (mb < bound) n[e] = min(c[e], (uint32_t)ceil((bound - mb) / w[e]));
-              }
-              if (w[e] < (double)min_p) n[e] = 0;
-              mb = end;
-              kept += n[e] * w[e];
-            }
-            kept_before = kept_sum + block_prefix(kept, s_d[1], &page_kept);
-            kept_sum += page_kept;
-          } else {
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) n[e] = c[e];
-            kept = mass;
-            kept_before = mass_before;
-            kept_sum = one_page ? total : mass_sum;
+            mb += c[e] * w[e];
+            if (own0 + e == above_total - 1) s_cut[2] = {mb, own0 + e, c[e]};
           }
         }
-        if (sum == 2) {
-          // The last thread with some kept mass that starts at or before the target holds the value that passes it (up
-          // to rounding: then its last one).
-          const int thread = wave_max(kept > 0.0 && kept_before <= target ? tid : -1);
-          if (lane == 0) s_hi[wave] = thread;
-          __syncthreads();
-          if (tid == row_max(s_hi[lane & 15])) {
-            uint32_t hit_n = 1, hit_rank = 0;
-            double kb = kept_before, hit_before = 0.0, hit_weight = 1.0;
+      }
+      if (walk == 3 && holds(target, true, cut.index)) {  // (up to rounding: then the last value kept)
+        uint32_t hit_n = 1, hit_rank = 0;
+        double mb = mass_before, hit_before = 0.0, weight = 1.0;
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-              if (n[e] != 0 && w[e] > 0.0 && kb <= target) {
-                hit_n = n[e];
-                hit_rank = (uint32_t)rank[e];
-                hit_before = kb;
-                hit_weight = w[e];
-              }
-              kb += n[e] * w[e];
-            }
-            const double j = floor((target - hit_before) / hit_weight);
-            s_hit[0] = hit_rank;
-            s_hit[1] = j < (double)(hit_n - 1) ? (uint32_t)j : hit_n - 1;
-            s_weight = hit_weight;
+        for (int e = 0; e < kPer; ++e) {
+          if (own0 + e <= cut.index && w[e] > 0.0 && mb <= target) {
+            hit_n = own0 + e == cut.index ? cut.n : c[e];
+            hit_rank = (uint32_t)rank[e];
+            hit_before = mb;
+            weight = w[e];
           }
-          __syncthreads();
+          mb += c[e] * w[e];
         }
-        if (one_page) break;
+        const double j = floor((target - hit_before) / weight);
+        s_hit[0] = hit_rank;
+        s_hit[1] = j < (double)(hit_n - 1) ? (uint32_t)j : hit_n - 1;
+        s_weight = weight;
+      }
+    };
+    // Behind a walk: what it found.
+    auto walked = [&](int walk) __attribute__((always_inline)) {
+      __syncthreads();
+      if (walk == 1) cut = s_cut[0];
+      if (walk == 2 && top_p < 1.0f && s_cut[1].mass < cut.mass) cut = s_cut[1];
+      if (walk == 2 && min_p > 0.0f && s_cut[2].mass < cut.mass) cut = s_cut[2];
+    };
+    const bool by_mass = top_p < 1.0f || min_p > 0.0f;
+    if constexpr (MERGE) merge(base);
+    const int parts = MERGE && s_far != 0 ? 2 : 1;
+    list_page(std::true_type(), base, 0);
+    if (parts == 1 && entries <= kPage) {
+      const uint32_t count_total = count_sum;
+      above_total = above_sum;
+      cut.mass = mass_sum;
+      if (some && limit < count_total) {
+        decide(1);
+        walked(1);
+      }
+      if (by_mass) {
+        decide(2);
+        walked(2);
+      }
+      target = (double)(u > 0.0f ? u : 0.0f) * cut.mass;
+      decide(3);
+      walked(3);
+    } else {
+      uint32_t count_total = 0;
+      int built = 0;
+#pragma clang loop unroll(disable)
+      for (int walk = 0; walk < 4; ++walk) {
+        if (walk == 1 && !(some && limit < count_total)) continue;
+        if (walk == 2 && !by_mass) continue;
+        count_sum = above_sum = index0 = 0;
+        mass_sum = 0.0;
+        for (int part = 0; part < parts; ++part) {
+          if (MERGE && built != part) {
+            __syncthreads();
+            zero_lds<kSpan * 4>(hist);
+            __syncthreads();
+            built = part;
+            merge(base + part * kSpan);
+          }
+          for (uint32_t first = 0; first == 0 || first < entries; first += kPage) {
+            list_page(std::false_type(), base + part * kSpan, first);
+            decide(walk);
+            index0 += min(entries - first, (uint32_t)kPage);
+          }
+        }
+        walked(walk);
+        if (walk == 0) {
+          count_total = count_sum;
+          above_total = above_sum;
+          cut.mass = mass_sum;
+        }
+        target = (double)(u > 0.0f ? u : 0.0f) * cut.mass;
       }
     }
-    if (sum == 0) total = mass_sum;
-    if (sum == 1) {
-      kept_total = kept_sum;
-      target = (double)(u > 0.0f ? u : 0.0f) * kept_total;
-    }
+    hit = s_hit[0];
+    left = s_hit[1];
+    hit_weight = s_weight;
+    kept_total = cut.mass;
   }
-  const int hit = (int)s_hit[0];
-  uint32_t left = s_hit[1];
-  const double hit_weight = s_weight;
+
 
   // The slice with the occurrence: the value's count in each list, found by two looks of a wave.
   int begin = 0, end = S.V;
@@ -499,13 +610,13 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams S, L
       const int n = (int)s_n[s];
       const uint32_t* list = L.list(m, s);
       const int step = (n + 63) / 64;
-      const unsigned long long le = __ballot(lane * step < n && (int)(list[min(lane * step, max(n - 1, 0))] >> 16) <= hit);
+      const unsigned long long le = __ballot(lane * step < n && list[min(lane * step, max(n - 1, 0))] >> 16 <= hit);
       uint32_t occ = 0;
       if (le != 0) {
         const int from = (63 - __builtin_clzll(le)) * step;
         for (int i = lane; i < step; i += 64) {
-          const uint32_t v = from + i < n ? list[from + i] : 0xFFFFFFFFu;
-          if ((int)(v >> 16) == hit) occ = v & 0xFFFFu;
+          const uint32_t v = from + i < n ? list[from + i] : 0xFFFFFFFFu;  // (no rank)
+          if (v >> 16 == hit) occ = v & 0xFFFFu;
         }
       }
       occ = wave_sum(occ);
@@ -531,9 +642,15 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams S, L
     S.tokens[m] = index;
     S.logprobs[m] = (float)log(hit_weight / kept_total);
   };
-  // The value's bits; zero has two forms.
-  const uint32_t bits = hit <= 0x7F80 ? 0x7F80 - hit : 0x8000 | (hit - 0x7F80), other = bits == 0 ? 0x8000u : bits;
-  auto matches = [&](uint32_t b) { return b == bits || b == other; };
+  // The value's bits; of zero without the sign.
+  const uint32_t bits = hit <= 0x7F80 ? 0x7F80 - hit : 0x8000 | (hit - 0x7F80), mask = bits == 0 ? 0x7FFFu : 0xFFFFu;
+  auto matches = [&](uint32_t b) { return (b & mask) == bits; };
+  auto line_misses = [&](u32x4 v) {  // how many of a line's 8 do not match
+    u32x4 d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d[e] = (v[e] ^ bits * 0x10001u) & mask * 0x10001u;
+    return occurring<true>(d);
+  };
   // Occurrences in index order: the logits before the lines, the lines, the logits behind them.
   const Lines G(row, begin, end);
   const unsigned long long edges = __ballot(matches(G.edge(lane)));  // (of lanes 0 .. 15, in every wave)
@@ -547,7 +664,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams S, L
   left -= head;
   const bool in_registers = !MERGE && G.count <= kBatch * kThreads;
   for (int g0 = 0; g0 < G.count; g0 += kBatch * kThreads) {
-    uint32_t hits[kBatch], inc[kBatch];
+    uint32_t n[kBatch], inc[kBatch];
     if (!in_registers) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) held[i] = G.load(g0 + i * kThreads + tid);
@@ -555,23 +672,23 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams S, L
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      hits[i] = 0;
       if (g0 + i * kThreads >= G.count) break;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) hits[i] |= (matches(place(held[i], e)) ? 1u : 0u) << e;
-      inc[i] = wave_prefix((uint32_t)__popc(hits[i]));
+      n[i] = 8 - line_misses(held[i]);
+      inc[i] = wave_prefix(n[i]);
       if (lane == 63) s_u[i][wave] = inc[i];
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       if (g0 + i * kThreads >= G.count) break;
-      const uint32_t waves = row_prefix(s_u[i][lane & 15]);
-      const uint32_t n = __popc(hits[i]);
-      const uint32_t ahead = (wave ? lane_value(waves, wave - 1) : 0u) + inc[i] - n, all = lane_value(waves, 15);
-      if (left >= ahead && left < ahead + n) {
-        for (uint32_t skip = left - ahead; skip > 0; --skip) hits[i] &= hits[i] - 1;
-        found(G.first(g0 + i * kThreads + tid) + __ffs((int)hits[i]) - 1);
+      const uint32_t waves = row_prefix(s_u[i][lane & (kWaves - 1)]), all = lane_value(waves, kWaves - 1);
+      const uint32_t ahead = (wave ? lane_value(waves, wave - 1) : 0u) + inc[i] - n[i];
+      if (left >= ahead && left < ahead + n[i]) {
+        uint32_t hits = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) hits |= (matches(place(held[i], e)) ? 1u : 0u) << e;
+        for (uint32_t skip = left - ahead; skip > 0; --skip) hits &= hits - 1;
+        found(G.first(g0 + i * kThreads + tid) + __ffs((int)hits) - 1);
       }
       if (left < all) return;
       left -= all;
@@ -609,7 +726,7 @@ constexpr int kOneKernelV = 65535;  // counts fit 16 bits
 int64_t sample_workspace(int64_t M, int64_t V, int cus) {
   if (M <= 0 || V <= kOneKernelV) return 16;
   const Plan p = plan_of(M, (int)V, cus);
-  return ((p.batch * p.slices + 3) / 4 * 4 + p.batch * p.slices * (int64_t)p.slice) * (int64_t)sizeof(uint32_t);
+  return (p.batch * p.slices + 1) / 2 * 16 + p.batch * p.slices * (int64_t)p.slice * (int64_t)sizeof(uint32_t);
 }
 
 hipError_t launch_sample(const SampleParams& p, int64_t M, void* workspace, int cus, hipStream_t stream) {
@@ -639,8 +756,9 @@ hipError_t launch_sample(const SampleParams& p, int64_t M, void* workspace, int 
   if (e == hipSuccess) e = g_merge.allow(reinterpret_cast<const void*>(&sample_pick_kernel<true>), kMergeBytes);
   if (e != hipSuccess) return e;
   const Plan plan = plan_of(M, p.V, cus);
-  uint32_t* ws = static_cast<uint32_t*>(workspace);
-  const Lists lists{ws, ws + (plan.batch * plan.slices + 3) / 4 * 4, plan.slice, plan.slices};
+  char* ws = static_cast<char*>(workspace);
+  const Lists lists{reinterpret_cast<Head*>(ws), reinterpret_cast<uint32_t*>(ws + (plan.batch * plan.slices + 1) / 2 * 16),
+                    plan.slice, plan.slices};
   for (int64_t m0 = 0; m0 < M; m0 += plan.batch) {
     const int64_t rows = M - m0 < plan.batch ? M - m0 : plan.batch;
     const SampleParams q = rows_from(m0);
