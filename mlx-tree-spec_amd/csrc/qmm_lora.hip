@@ -144,20 +144,22 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(Shrink P) {
     if (rows >> (4 * r4 + r) & 1) P.t[(int64_t)(m0 + 4 * r4 + r) * T.R + jj] = split_bf16(scale * acc[r]);
 }
 
-// One wave per 16 x 64 values of y.
+// One wave per 16 x 64 values of y (of every so many rows, where there are more than a grid's).
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraAdd E, uint16_t* __restrict__ y, int M, int N) {
-  const int lane = threadIdx.x & 63, across = (N + 255) / 256;
-  const int m0 = blockIdx.x / across * 16, n0 = (blockIdx.x % across * 4 + (threadIdx.x >> 6)) * 64;
+  const int lane = threadIdx.x & 63, across = (N + 255) / 256, rows = gridDim.x / across * 16;
+  const int n0 = (blockIdx.x % across * 4 + (threadIdx.x >> 6)) * 64;
+  for (int m0 = blockIdx.x / across * 16; m0 < M; m0 += rows) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int col = n0 + c * 16 + (lane & 15);
-    const f32x4 d = lora_tile16(E, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, m0, col, M, N);
+    for (int c = 0; c < 4; ++c) {
+      const int col = n0 + c * 16 + (lane & 15);
+      const f32x4 d = lora_tile16(E, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, m0, col, M, N);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int m = m0 + 4 * (lane >> 4) + r;
-      if (col < N && lora_adapter(E, m, M) >= 0) {
-        uint16_t* p = y + (int64_t)m * N + col;
-        *p = (uint16_t)bf16_rne(bf16_to_f32(*p) + d[r]);
+      for (int r = 0; r < 4; ++r) {
+        const int m = m0 + 4 * (lane >> 4) + r;
+        if (col < N && lora_adapter(E, m, M) >= 0) {
+          uint16_t* p = y + (int64_t)m * N + col;
+          *p = (uint16_t)bf16_rne(bf16_to_f32(*p) + d[r]);
+        }
       }
     }
   }
@@ -199,9 +201,9 @@ hipError_t launch_lora_shrink(const LoraShrinkPlan& plan, const LoraTables& lora
 
 hipError_t launch_lora_expand(const LoraAdd& lora, uint16_t* y, int M, int N, hipStream_t stream) {
   if (M <= 0 || N <= 0) return hipSuccess;
-  const int64_t blocks = (int64_t)((M + 15) / 16) * ((N + 255) / 256);
-  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(lora_expand_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, lora, y, M, N);
+  const int64_t across = (N + 255) / 256, most = (1 << 23) / across;  // (a grid may have 2^32 threads along x)
+  const int64_t rows = (M + 15) / 16 < most ? (M + 15) / 16 : most;
+  hipLaunchKernelGGL(lora_expand_kernel, dim3((unsigned)(rows * across)), dim3(256), 0, stream, lora, y, M, N);
   return hipGetLastError();
 }
 

@@ -18,6 +18,7 @@ using qmm4::hip_error;
 using qmm4::set_error;
 
 constexpr int64_t kMaxDim = 1LL << 30;
+constexpr int64_t kMaxLoraRows = 1LL << 26;  // (the shrink's grid: a workgroup of 512 threads per 16 rows)
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
@@ -40,9 +41,9 @@ int index_bits_ok(int bits, const char* what) {
 int check_lora(const void* x, const void* a, const void* b, const float* scale, const void* adapters, int adapter_bits,
                const void* y, const void* workspace, int64_t M, int64_t N, int64_t K, int64_t L, int64_t R) {
   if (int rc = index_bits_ok(adapter_bits, "adapters")) return rc;
-  if (M < 0 || N < 0 || K <= 0 || L < 0 || M > kMaxDim || N > kMaxDim || K > kMaxDim || L > kMaxDim || K % 8 != 0)
+  if (M < 0 || N < 0 || K <= 0 || L < 0 || M > kMaxLoraRows || N > kMaxDim || K > kMaxDim || L > kMaxDim || K % 8 != 0)
     return set_error(QMM4_ERR_INVALID, "invalid shape M=%lld N=%lld K=%lld L=%lld (K must be a positive multiple of 8, "
-                     "each at most 2^30)", (long long)M, (long long)N, (long long)K, (long long)L);
+                     "at most 2^26 rows, each other at most 2^30)", (long long)M, (long long)N, (long long)K, (long long)L);
   if (R < 8 || R > QMM4_LORA_MAX_RANK || R % 8 != 0)
     return set_error(QMM4_ERR_INVALID, "R=%lld must be a multiple of 8 from 8 to %d", (long long)R, QMM4_LORA_MAX_RANK);
   if (M == 0 || N == 0 || L == 0) return QMM4_OK;

@@ -44,10 +44,10 @@ __device__ __forceinline__ float value8(u32x4 v, int e) { return bf16_to_f32(e &
 
 // TURNS: heads of each group of lanes.
 template <int MODE, int TURNS>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(RopeParams S, int G, bool past_l2) {
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(RopeParams S, int64_t m0, int G, bool past_l2) {
   __shared__ __attribute__((aligned(16))) float s_cos[kMaxP], s_sin[kMaxP];
   const int tid = threadIdx.x, per = kThreads / G;
-  const int64_t m = blockIdx.x;
+  const int64_t m = m0 + blockIdx.x;
   const int c = tid & (G - 1), h0 = blockIdx.y * (TURNS * per) + tid / G;
   const int heads = S.q.heads + S.k.heads;
   const bool in_head = c < S.D / 8;
@@ -176,12 +176,15 @@ void launch_mode(const RopeParams& p, int64_t M, int G, hipStream_t stream) {
   // Results that no L2 (4 MiB each) will hold for their reader do not push the inputs out of it: 4096 x 40 heads x 128
   // 19.5 -> 16.5 us, 1024 x 28 x 256 9.0 -> 7.2, 1500 x 32 x 64 5.2 -> 4.8.
   const bool past_l2 = M * heads * p.D * 2 > 4 << 20;
-  const dim3 grid((unsigned)M, (unsigned)blocks);
-  switch (turns) {
-    case 1: hipLaunchKernelGGL((qk_norm_rope_kernel<MODE, 1>), grid, dim3(kThreads), 0, stream, p, G, past_l2); break;
-    case 2: hipLaunchKernelGGL((qk_norm_rope_kernel<MODE, 2>), grid, dim3(kThreads), 0, stream, p, G, past_l2); break;
-    case 3: hipLaunchKernelGGL((qk_norm_rope_kernel<MODE, 3>), grid, dim3(kThreads), 0, stream, p, G, past_l2); break;
-    default: hipLaunchKernelGGL((qk_norm_rope_kernel<MODE, 4>), grid, dim3(kThreads), 0, stream, p, G, past_l2); break;
+  constexpr int64_t kRows = 1 << 23;  // (a grid may have 2^32 threads along x)
+  for (int64_t m0 = 0; m0 < M; m0 += kRows) {
+    const dim3 grid((unsigned)(M - m0 < kRows ? M - m0 : kRows), (unsigned)blocks);
+    switch (turns) {
+      case 1: hipLaunchKernelGGL((qk_norm_rope_kernel<MODE, 1>), grid, dim3(kThreads), 0, stream, p, m0, G, past_l2); break;
+      case 2: hipLaunchKernelGGL((qk_norm_rope_kernel<MODE, 2>), grid, dim3(kThreads), 0, stream, p, m0, G, past_l2); break;
+      case 3: hipLaunchKernelGGL((qk_norm_rope_kernel<MODE, 3>), grid, dim3(kThreads), 0, stream, p, m0, G, past_l2); break;
+      default: hipLaunchKernelGGL((qk_norm_rope_kernel<MODE, 4>), grid, dim3(kThreads), 0, stream, p, m0, G, past_l2); break;
+    }
   }
 }
 

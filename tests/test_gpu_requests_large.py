@@ -1,0 +1,75 @@
+"""The per-request operators past 4 GiB of an input and past a grid's rows (needs an MI355X).
+
+What lies past 32 bits of offset is compared with 64 bits, by the bounds of the operators' own tests, or with the same
+call on a copy of the last rows (each row is computed by itself, so its bits may not change)."""
+
+import numpy as np
+import pytest
+import torch
+
+import request_refs as R
+from mlx_tree_spec_amd import qk_norm_rope, quantized_matmul_lora, sample
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.mark.parametrize("m", [4, 13, 40, 300])
+@pytest.mark.parametrize("k,n,count", [(512, 8192, 1050), (8192, 512, 1050)])
+def test_adapter_tables_past_4_gib(m, k, n, count):
+    rank = 256
+    g = torch.Generator().manual_seed(m + k)
+    randn = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    used = torch.tensor([0, count // 2, count - 1])
+    la = torch.zeros(count, rank, k, dtype=torch.bfloat16, device=DEV)
+    lb = torch.zeros(count, n, rank, dtype=torch.bfloat16, device=DEV)
+    assert max(la.numel(), lb.numel()) * 2 > 1 << 32
+    scale = torch.rand(count, generator=g).to(DEV)
+    for a in used.tolist():
+        la[a] = (randn(rank, k) / k ** 0.5).to(torch.bfloat16).to(DEV)
+        lb[a] = (randn(n, rank) * 0.3).to(torch.bfloat16).to(DEV)
+    x = randn(m, k).to(torch.bfloat16).to(DEV)
+    w = torch.randint(-2**31, 2**31, (n, k // 8), generator=g, dtype=torch.int64).to(torch.int32).to(DEV)
+    s = (randn(n, k // 64).abs() * 0.004 + 1e-4).to(torch.bfloat16).to(DEV)
+    b = (-8 * s.float()).to(torch.bfloat16)
+    pick = torch.randint(0, 3, (m,), generator=g)
+    y = quantized_matmul_lora(x, w, s, b, la, lb, scale, used[pick].to(torch.int32).to(DEV))
+    ref, _, mag = R.lora(x, R.dequantize(w, s, b, 64, 4), la[used.to(DEV)], lb[used.to(DEV)], scale[used.to(DEV)], pick)
+    bound = R.HALF_STEP_BF16 * np.abs(ref) * 1.01 + ((k + rank + 4) * R.HALF_STEP_F32 + 2.0 ** -18) * mag
+    assert (np.abs(R.f64(y) - ref) <= bound).all()
+
+
+@pytest.mark.parametrize("m,v", [(70000, 32001), (16000, 151936)])
+def test_logits_past_4_gib(m, v):
+    logits = torch.empty(m, v, dtype=torch.bfloat16, device=DEV)
+    assert logits.numel() * 2 > 1 << 32
+    g = torch.Generator(device=DEV).manual_seed(v)
+    logits.fill_(-1.0)
+    logits[-4:] = (torch.randn(4, v, generator=g, device=DEV) * 2).to(torch.bfloat16)
+    logits[:3] = (torch.randn(3, v, generator=g, device=DEV) * 2).to(torch.bfloat16)
+    uniform = torch.rand(m, generator=g, device=DEV)
+    tokens, logprobs = sample(logits, uniform, top_p=0.9)
+    for rows in (slice(0, 3), slice(m - 4, m)):
+        want, want_p = R.sample(logits[rows], uniform[rows], top_p=0.9)
+        assert np.array_equal(tokens[rows].cpu().numpy(), want)
+        assert (np.abs(R.f64(logprobs[rows]) - want_p) <= R.HALF_STEP_F32 * np.abs(want_p) * 1.01 + 2.0 ** -40).all()
+    assert int(tokens.min()) >= 0 and int(tokens.max()) < v
+
+
+@pytest.mark.parametrize("m,hq,hk,d", [(600000, 32, 1, 128), ((1 << 24) + 5, 1, 1, 8)])
+def test_heads_past_4_gib_and_past_a_grid(m, hq, hk, d):
+    g = torch.Generator(device=DEV).manual_seed(d)
+    q = torch.randn(m, hq, d, generator=g, device=DEV, dtype=torch.bfloat16)
+    k = torch.randn(m, hk, d, generator=g, device=DEV, dtype=torch.bfloat16)
+    wq, wk = (torch.rand(d, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    positions = torch.randint(0, 1 << 17, (m,), generator=g, device=DEV)
+    inv = 1e4 ** (-torch.arange(d // 2, dtype=torch.float64, device=DEV) / (d // 2))
+    out = qk_norm_rope(q, k, wq, wk, 1e-6, positions, inv)
+    for at in (0, (1 << 23) - 3 if m > 1 << 23 else 524285, m - 7):
+        part = slice(at, at + 7)
+        same = qk_norm_rope(q[part].clone(), k[part].clone(), wq, wk, 1e-6, positions[part].clone(), inv)
+        for a, b, x, w in ((out[0], same[0], q, wq), (out[1], same[1], k, wk)):
+            assert torch.equal(a[part], b)
+            ref, mag = R.rope(x[part], w, 1e-6, positions[part], inv, False)
+            bound = R.HALF_STEP_BF16 * np.abs(ref) * 1.001 + (d / 2 + 16) * R.HALF_STEP_F32 * mag
+            assert (np.abs(R.f64(a[part]) - ref) <= bound).all()

@@ -172,10 +172,10 @@ def test_lora_add_at_the_c_abi(kw, code, msg):
 
 
 @pytest.mark.parametrize("kw,code,msg", [
-    (dict(bits=8), _lib.QMM4_ERR_UNSUPPORTED, "bits=8"),
-    (dict(gs=32), _lib.QMM4_ERR_UNSUPPORTED, "group_size=32"),
-    (dict(K=192), _lib.QMM4_ERR_INVALID, "K=192"),
-    (dict(N=24), _lib.QMM4_ERR_INVALID, "N=24"),
+    (dict(bits=3), _lib.QMM4_ERR_UNSUPPORTED, "bits=3"),
+    (dict(gs=48), _lib.QMM4_ERR_UNSUPPORTED, "group_size=48"),
+    (dict(K=96), _lib.QMM4_ERR_INVALID, "K=96"),
+    (dict(M=(1 << 26) + 1), _lib.QMM4_ERR_INVALID, "2^26 rows"),
     (dict(R=12), _lib.QMM4_ERR_INVALID, "R=12"),
     (dict(M=0), _lib.QMM4_OK, ""),
 ])
