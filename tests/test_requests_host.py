@@ -159,6 +159,7 @@ P = 0x10000
     (dict(x=P + 2), _lib.QMM4_ERR_INVALID, "16-byte aligned"),
     (dict(ws=P + 4), _lib.QMM4_ERR_INVALID, "16-byte aligned"),
     (dict(y=P + 1), _lib.QMM4_ERR_INVALID, "aligned to their elements"),
+    (dict(M=(1 << 26) + 1), _lib.QMM4_ERR_INVALID, "2^26 rows"),
     (dict(M=0, x=0), _lib.QMM4_OK, ""),
     (dict(L=0, x=0), _lib.QMM4_OK, ""),
     (dict(N=0, x=0), _lib.QMM4_OK, ""),
@@ -175,7 +176,7 @@ def test_lora_add_at_the_c_abi(kw, code, msg):
     (dict(bits=3), _lib.QMM4_ERR_UNSUPPORTED, "bits=3"),
     (dict(gs=48), _lib.QMM4_ERR_UNSUPPORTED, "group_size=48"),
     (dict(K=96), _lib.QMM4_ERR_INVALID, "K=96"),
-    (dict(M=(1 << 26) + 1), _lib.QMM4_ERR_INVALID, "2^26 rows"),
+    (dict(M=1 << 26), _lib.QMM4_ERR_INVALID, "exceeds 4 GiB"),
     (dict(R=12), _lib.QMM4_ERR_INVALID, "R=12"),
     (dict(M=0), _lib.QMM4_OK, ""),
 ])
