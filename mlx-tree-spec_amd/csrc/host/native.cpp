@@ -18,6 +18,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/util/SmallVector.h>
 #include <torch/csrc/Exceptions.h>
@@ -102,6 +103,11 @@ struct Weights {
 
 bool is_codes(const at::Tensor& w) { return w.dim() == 2 && (w.scalar_type() == at::kInt || w.scalar_type() == at::kUInt32); }
 bool is_bf16(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16; }
+
+// A new tensor on the current device, without the dispatcher's rounds (at::empty takes 0.2 us more: 5.8 us a call of rope, 5.4 with this).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
 
 at::Tensor empty_like_rows(const at::Tensor& x, int64_t n) {
   c10::SmallVector<int64_t, 8> sizes(x.sizes().begin(), x.sizes().end());
@@ -283,7 +289,7 @@ PyObject* lora(PyObject*, PyObject* const* a, Py_ssize_t na) {
       sc->size(0) != la->size(0) || !is_index(*ids, *x, 1))
     return none();
   const int64_t count = la->size(0), rank = la->size(1);
-  at::Tensor y = empty_like_rows(*x, n), ws = at::empty({m, rank}, x->options().dtype(at::kInt));
+  at::Tensor y = empty_like_rows(*x, n), ws = fresh({m, rank}, at::kInt, *x);
   const Weights q(*w, *s, *b);
   void *st = stream_of(*x), *xp = ptr(*x), *lap = ptr(*la), *lbp = ptr(*lb), *ip = ptr(*ids), *yp = out_ptr(y),
        *wp = out_ptr(ws);
@@ -329,8 +335,7 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t na) {
     return none();
   int64_t m, mk, qr, qh, kr, kh;
   if (!heads(*q, &m, &qr, &qh) || !heads(*k, &mk, &kr, &kh)) return none();
-  const at::TensorOptions o = q->options();
-  at::Tensor qo = at::empty(q->sizes(), o), ko = at::empty(k->sizes(), o);
+  at::Tensor qo = fresh(q->sizes(), at::kBFloat16, *q), ko = fresh(k->sizes(), at::kBFloat16, *k);
   void *st = stream_of(*q), *qp = ptr(*q), *kp = ptr(*k), *wqp = ptr(*wq), *wkp = ptr(*wk), *pp = ptr(*pos), *ip = ptr(*inv);
   void *qop = out_ptr(qo), *kop = out_ptr(ko);
   if (!qop || !kop) return none();
@@ -383,8 +388,8 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t na) {
   const int64_t bytes = p_sample_workspace(m, v);
   if (bytes < 0) return PyLong_FromLong((long)bytes);
   const auto lead = l->sizes().slice(0, n - 1);
-  at::Tensor tokens = at::empty(lead, l->options().dtype(at::kLong)), logprobs = at::empty(lead, l->options().dtype(at::kFloat));
-  at::Tensor ws = at::empty({bytes}, l->options().dtype(at::kByte));
+  at::Tensor tokens = fresh(lead, at::kLong, *l), logprobs = fresh(lead, at::kFloat, *l);
+  at::Tensor ws = fresh({bytes}, at::kByte, *l);
   void *tp = out_ptr(tokens), *pp = out_ptr(logprobs), *wp = out_ptr(ws), *st = stream_of(*l), *lp = ptr(*l);
   if (!tp || !pp || !wp) return none();
   auto f = [](const at::Tensor* x) { return x ? static_cast<const float*>(ptr(*x)) : nullptr; };

@@ -83,7 +83,7 @@ def _build_native(out: str) -> None:
            "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-I", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"),
            *sorted(os.path.join(HOST_DIR, f) for f in os.listdir(HOST_DIR) if f.endswith(".cpp")),
-           "-L", lib, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-o", out_tmp]
+           "-L", lib, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-o", out_tmp]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {out} failed:\n{r.stdout}\n{r.stderr}")
