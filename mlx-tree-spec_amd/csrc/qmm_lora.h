@@ -18,6 +18,27 @@ __device__ __forceinline__ int lora_adapter(const LoraAdd& E, int m, int M) {
   return a >= 0 && a < E.L ? (int)a : -1;
 }
 
+// The adapters of rows m0 .. m0 + 3, loaded where a kernel starts and looked at where it ends (each lane for itself).
+struct LoraIds {
+  uint32_t lo[4], hi[4];
+  __device__ __forceinline__ void load(const LoraAdd& E, int m0, int M) {
+    const uint32_t* p = static_cast<const uint32_t*>(E.adapters.p);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t m = min(m0 + r, M - 1);
+      lo[r] = p[E.adapters.wide ? 2 * m : m];
+      hi[r] = p[E.adapters.wide ? 2 * m + 1 : m];
+    }
+  }
+  __device__ __forceinline__ void adapters(const LoraAdd& E, int m0, int M, int (&a)[4]) const {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t id = E.adapters.wide ? (int64_t)((uint64_t)hi[r] << 32 | lo[r]) : (int64_t)(int32_t)lo[r];
+      a[r] = m0 + r < M && id >= 0 && id < E.L ? (int)id : -1;
+    }
+  }
+};
+
 // 8 values of t (row m from j) as high and low parts.
 __device__ __forceinline__ void lora_split(u32x4 v0, u32x4 v1, bf16x8* hi, bf16x8* lo) {
   u32x4 h, l;
