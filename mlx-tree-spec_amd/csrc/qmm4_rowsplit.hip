@@ -627,7 +627,7 @@ void rowsplit_kernel(RowSplitParams P) {
     int a[4];
     lora_ids.adapters(P.lora, 4 * lora_gg, P.M, a);
     if (tid < P.R * G && lora_col < r1 && 4 * lora_gg < P.M)
-      first_add = lora_rows4(P.lora, first_add, a, 4 * lora_gg, lora_col, P.M, P.N);
+      first_add = lora_rows4<1>(P.lora, first_add, a, 4 * lora_gg, lora_col, P.M, P.N);
   }
   __syncthreads();
 
@@ -651,7 +651,7 @@ void rowsplit_kernel(RowSplitParams P) {
         sum[0] += first_add[0]; sum[1] += first_add[1]; sum[2] += first_add[2]; sum[3] += first_add[3];
         first_item = false;
       } else {
-        sum = lora_rows4(P.lora, sum, 4 * gg, col, P.M, P.N);
+        sum = lora_rows4<1>(P.lora, sum, 4 * gg, col, P.M, P.N);
       }
     }
 #pragma unroll
@@ -881,7 +881,7 @@ void rowsplit_xreg_kernel(RowSplitParams P) {
   f32x4 first_add = {0.0f, 0.0f, 0.0f, 0.0f};
   if constexpr (LORA) {
     if (tid < P.R * 4 && r0 + (tid >> 2) < r1 && 4 * (tid & 3) < P.M)
-      first_add = lora_rows4(P.lora, first_add, 4 * (tid & 3), r0 + (tid >> 2), P.M, P.N);
+      first_add = lora_rows4<2>(P.lora, first_add, 4 * (tid & 3), r0 + (tid >> 2), P.M, P.N);
   }
   __syncthreads();
 
@@ -902,7 +902,7 @@ void rowsplit_xreg_kernel(RowSplitParams P) {
       if (it == tid) {
         sum[0] += first_add[0]; sum[1] += first_add[1]; sum[2] += first_add[2]; sum[3] += first_add[3];
       } else {
-        sum = lora_rows4(P.lora, sum, 4 * gg, col, P.M, P.N);
+        sum = lora_rows4<1>(P.lora, sum, 4 * gg, col, P.M, P.N);
       }
     }
 #pragma unroll
