@@ -39,14 +39,19 @@ struct Shrink {
   uint32_t* t;
   float* part;    // slices > 1: fp32 tiles [tile][slice][lane][4]
   uint32_t* cnt;  // arrivals per tile (0 between launches)
-  int M, K, slices, units;  // units of kUnit k, the last one possibly short
+  int M, K, slices, across, units;  // units of kUnit k, the last one possibly short
+  int first;  // not in slices: the first row
 };
 
+template <bool SLICED>
 __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(Shrink P) {
   extern __shared__ __attribute__((aligned(16))) u32x4 lds[];
   const LoraTables& T = P.T;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int slice = blockIdx.x % P.slices, m0 = blockIdx.x / P.slices * 16, j0 = blockIdx.y * 16;
+  const int slices = SLICED ? P.slices : 1, slice = SLICED ? blockIdx.x % slices : 0;
+  const int m0 = SLICED ? blockIdx.x / slices * 16 : P.first + ((blockIdx.x >> 3) / P.across * 8 + (blockIdx.x & 7)) * 16;
+  const int j0 = (SLICED ? blockIdx.y : (blockIdx.x >> 3) % P.across) * 16;
+  if (!SLICED && m0 >= P.M) return;
   const int64_t id = T.adapters[min(m0 + (lane & 15), P.M - 1)];
   const int a = m0 + (lane & 15) < P.M && id >= 0 && id < T.L ? (int)id : -1;
   // The z-th adapter of the rows.
@@ -59,7 +64,7 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(Shrink P) {
     todo &= ~rows;
   }
   const float scale = T.scale[d];
-  const int part = slice * kWaves + wave, parts = P.slices * kWaves;
+  const int part = slice * kWaves + wave, parts = slices * kWaves;
   const int ub = (int)((int64_t)part * P.units / parts), ue = (int)((int64_t)(part + 1) * P.units / parts);
   // Load i: row 4 i + lane / 16 of the tile, 16-byte piece lane % 16 of the unit.
   const int r4 = lane >> 4, piece = lane & 15;
@@ -113,21 +118,21 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(Shrink P) {
     const f32x4 v = sums[w * 64 + lane];
     acc[0] += v[0]; acc[1] += v[1]; acc[2] += v[2]; acc[3] += v[3];
   }
-  if (P.slices > 1) {
-    const uint32_t tile = (blockIdx.z * gridDim.y + blockIdx.y) * (gridDim.x / P.slices) + blockIdx.x / P.slices;
+  if constexpr (SLICED) {
+    const uint32_t tile = (blockIdx.z * gridDim.y + blockIdx.y) * (gridDim.x / slices) + blockIdx.x / slices;
     const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc(
         P.part, 0, rsrc_bytes((unsigned long long)gridDim.x * gridDim.y * gridDim.z * 1024), kBufferRsrcWord3);
-    const uint32_t o = tile * (uint32_t)P.slices * 1024u + (uint32_t)lane * 16u;
+    const uint32_t o = tile * (uint32_t)slices * 1024u + (uint32_t)lane * 16u;
     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), rp, o + (uint32_t)slice * 1024u, 0, kCoherent);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     uint32_t before = 0;
     if (lane == 0) before = __hip_atomic_fetch_add(&P.cnt[tile], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (__builtin_amdgcn_readfirstlane(before) != (uint32_t)P.slices - 1) return;
+    if (__builtin_amdgcn_readfirstlane(before) != (uint32_t)slices - 1) return;
     f32x4 v[kMaxSlices];
 #pragma unroll
     for (int q = 0; q < kMaxSlices; ++q) {
       v[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (q < P.slices)
+      if (q < slices)
         v[q] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, o + (uint32_t)q * 1024u, 0, kCoherent));
     }
     acc = v[0];
@@ -165,14 +170,14 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraAdd E, uint16_t* _
   }
 }
 
-LdsAllowance g_shrink;
+LdsAllowance g_sliced, g_whole;
 
 }  // namespace
 
 // Few tiles: K in up to 8 slices of at least 512, while that gives a CU no second workgroup (counted for one adapter per
 // 16 rows). One / 4 / 8 slices: 4 x 5120 rank 16 of 4 adapters 6.7 / 5.3 / 5.1 us, 16 rows of one 6.6 / 5.2 / 4.8, 64 x
-// 17408 rank 32 of 4 adapters 15.0 / 8.0 / 7.2; many tiles, 2000 x 5120 rank 64, 21 / 30 / 48. (4 or 16 waves instead of 8: 4 x
-// 5120 5.3 / 5.6, 64 x 17408 7.9 / 6.8, 2000 x 5120 20.7 / 26.6; tiles of 4 values of j: no better in slices.)
+// 17408 rank 32 of 4 adapters 15.0 / 8.0 / 7.2; many tiles, 2000 x 5120 rank 64, 15.5 / 29 / 46. (4 or 16 waves instead of 8: 4 x
+// 5120 5.3 / 5.6, 64 x 17408 7.9 / 6.8, many tiles no better; tiles of 4 values of j: no better in slices.)
 LoraShrinkPlan lora_shrink_plan(const LoraTables& lora, int M, int K, int cus) {
   LoraShrinkPlan p;
   const int most = M < 16 ? M : 16;  // adapters of 16 rows
@@ -191,11 +196,25 @@ LoraShrinkPlan lora_shrink_plan(const LoraTables& lora, int M, int K, int cus) {
 hipError_t launch_lora_shrink(const LoraShrinkPlan& plan, const LoraTables& lora, const uint16_t* x, uint32_t* t,
                               float* part, uint32_t* cnt, int M, int K, hipStream_t stream) {
   constexpr size_t kLds = (size_t)kWaves * kWaveLds;
-  const hipError_t e = g_shrink.allow(reinterpret_cast<const void*>(&lora_shrink_kernel), kLds);
-  if (e != hipSuccess) return e;
-  const Shrink P{lora, x, t, part, cnt, M, K, plan.slices, (K + kUnit - 1) / kUnit};
-  const dim3 grid((unsigned)(plan.rows * plan.slices), (unsigned)plan.across, (unsigned)plan.depth);
-  hipLaunchKernelGGL(lora_shrink_kernel, grid, dim3(kThreads), kLds, stream, P);
+  Shrink P{lora, x, t, part, cnt, M, K, plan.slices, plan.across, (K + kUnit - 1) / kUnit, 0};
+  if (plan.slices > 1) {
+    const hipError_t e = g_sliced.allow(reinterpret_cast<const void*>(&lora_shrink_kernel<true>), kLds);
+    if (e != hipSuccess) return e;
+    const dim3 grid((unsigned)(plan.rows * plan.slices), (unsigned)plan.across, (unsigned)plan.depth);
+    hipLaunchKernelGGL(lora_shrink_kernel<true>, grid, dim3(kThreads), kLds, stream, P);
+  } else {
+    // Workgroups 8 apart (of one XCD) in turn take the tiles of j of the same rows: x comes into one L2 instead of up to 8
+    // (2000 x 5120 rank 64: 20.9 -> 15.5 us).
+    const hipError_t e = g_whole.allow(reinterpret_cast<const void*>(&lora_shrink_kernel<false>), kLds);
+    if (e != hipSuccess) return e;
+    constexpr int kMost = 1 << 18;  // tiles of rows per launch (a grid may have 2^32 threads along x)
+    for (int tile = 0; tile < plan.rows; tile += kMost) {
+      const int rows = plan.rows - tile < kMost ? plan.rows - tile : kMost;
+      P.first = tile * 16;
+      const dim3 grid((unsigned)((rows + 7) / 8 * 8 * plan.across), 1, (unsigned)plan.depth);
+      hipLaunchKernelGGL(lora_shrink_kernel<false>, grid, dim3(kThreads), kLds, stream, P);
+    }
+  }
   return hipGetLastError();
 }
 

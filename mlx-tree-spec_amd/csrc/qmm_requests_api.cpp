@@ -18,7 +18,7 @@ using qmm4::hip_error;
 using qmm4::set_error;
 
 constexpr int64_t kMaxDim = 1LL << 30;
-constexpr int64_t kMaxLoraRows = 1LL << 26;  // (the shrink's grid: a workgroup of 512 threads per 16 rows)
+constexpr int64_t kMaxLoraRows = 1LL << 26;  // (row numbers of a tile past the last stay far below 2^31)
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 

@@ -73,3 +73,23 @@ def test_heads_past_4_gib_and_past_a_grid(m, hq, hk, d):
             ref, mag = R.rope(x[part], w, 1e-6, positions[part], inv, False)
             bound = R.HALF_STEP_BF16 * np.abs(ref) * 1.001 + (d / 2 + 16) * R.HALF_STEP_F32 * mag
             assert (np.abs(R.f64(a[part]) - ref) <= bound).all()
+
+
+def test_adapter_rows_past_a_grid():
+    """More than 2^22 rows: several launches of the shrink; a library product's result with the adapters added."""
+    m, k, n = (1 << 22) + 37, 32, 8
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(m, k, generator=g, device=DEV).to(torch.bfloat16)
+    w = torch.randint(-2**31, 2**31 - 1, (n, k // 8), generator=g, device=DEV, dtype=torch.int64).to(torch.int32)
+    s = torch.full((n, 1), 2.0 ** -6, dtype=torch.bfloat16, device=DEV)
+    b = torch.full((n, 1), -0.125, dtype=torch.bfloat16, device=DEV)
+    la, lb = (torch.randn(3, *shape, generator=g, device=DEV).to(torch.bfloat16) for shape in ((8, k), (n, 8)))
+    scale = torch.tensor([0.5, 1.0, -0.25], device=DEV)
+    ids = torch.randint(-1, 3, (m,), generator=g, device=DEV)
+    y = quantized_matmul_lora(x, w, s, b, la, lb, scale, ids, group_size=32)
+    wd = R.dequantize(w, s, b, 32, 4)
+    for at in (0, (1 << 22) - 20, m - 30):
+        part = slice(at, at + 30)
+        ref, base, mag = R.lora(x[part], wd, la, lb, scale, ids[part])
+        bound = R.HALF_STEP_BF16 * (np.abs(ref) + np.abs(base)) * 1.01 + ((k + 12) * R.HALF_STEP_F32 + 2.0 ** -18) * mag
+        assert (np.abs(R.f64(y[part]) - ref) <= bound).all()
