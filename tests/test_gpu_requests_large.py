@@ -93,3 +93,54 @@ def test_adapter_rows_past_a_grid():
         ref, base, mag = R.lora(x[part], wd, la, lb, scale, ids[part])
         bound = R.HALF_STEP_BF16 * (np.abs(ref) + np.abs(base)) * 1.01 + ((k + 12) * R.HALF_STEP_F32 + 2.0 ** -18) * mag
         assert (np.abs(R.f64(y[part]) - ref) <= bound).all()
+
+
+def sampled(logits, uniform, **settings):
+    tokens, logprobs = sample(logits, uniform, **settings)
+    want, want_p = R.sample(logits, uniform, **settings)
+    assert np.array_equal(tokens.cpu().numpy(), want)
+    assert (np.abs(R.f64(logprobs) - want_p) <= R.HALF_STEP_F32 * np.abs(want_p) * 1.01 + 2.0 ** -40).all()
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=100000, top_p=0.8, min_p=1e-5)], ids=str)
+def test_largest_vocabulary(settings):
+    g = torch.Generator().manual_seed(24)
+    logits = (torch.randn(2, 1 << 24, generator=g) * 2).to(torch.bfloat16).to(DEV)
+    sampled(logits, torch.tensor([0.25, 0.875], device=DEV), **settings)
+
+
+@pytest.mark.parametrize("v", [65535, 65536, 1 << 20])
+def test_equal_logits_fill_the_counts(v):
+    """Every logit the same (16-bit counts at their most), but one above and one below in other slices."""
+    logits = torch.full((4, v), -3.0, dtype=torch.bfloat16, device=DEV)
+    logits[1, v - 1], logits[2, 0] = -2.984375, -3.015625
+    logits[3, v // 2] = -2.984375
+    sampled(logits, torch.tensor([0.5, 0.25, 0.75, 0.125], device=DEV), top_p=0.75)
+
+
+def test_calls_on_two_streams_at_once():
+    """Each call has a workspace of its own (the adapters' also their stream's): the results are those of one stream."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    logits = (torch.randn(2, 3, 151936, generator=g, device=DEV) * 2).to(torch.bfloat16)
+    uniform = torch.rand(2, 3, generator=g, device=DEV)
+    x = torch.randn(2, 7, 1024, generator=g, device=DEV).to(torch.bfloat16)
+    w = torch.randint(-2**31, 2**31 - 1, (512, 128), generator=g, device=DEV, dtype=torch.int64).to(torch.int32)
+    s = torch.full((512, 16), 2.0 ** -6, dtype=torch.bfloat16, device=DEV)
+    b = torch.full((512, 16), -0.125, dtype=torch.bfloat16, device=DEV)
+    la, lb = (torch.randn(3, *shape, generator=g, device=DEV).to(torch.bfloat16) for shape in ((16, 1024), (512, 16)))
+    scale = torch.tensor([0.5, 1.0, -0.25], device=DEV)
+    ids = torch.randint(-1, 3, (2, 7), generator=g, device=DEV)
+    both = lambda i: (*sample(logits[i], uniform[i], top_p=0.9),  # noqa: E731
+                      quantized_matmul_lora(x[i], w, s, b, la, lb, scale, ids[i]))
+    want = [both(0), both(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(both(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for result in got[i]:
+            assert all(torch.equal(a, c) for a, c in zip(result, want[i]))
