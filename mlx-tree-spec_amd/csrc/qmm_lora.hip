@@ -73,7 +73,9 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(Shrink P) {
   u32x4* const lx = lds + wave * (kWaveLds / 16);
   u32x4* const la = lx + 16 * 16;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  constexpr int kBatch = 2;
+  // Units in flight: a sliced wave has 1 or 2 (4 x 5120 4.8 us with 1 and with 2, 64 x 17408 rank 32 7.0 and 7.2), one with
+  // all of K several (2000 x 5120 rank 64 15.5, 15.0 and 14.7 us with 1, 2 and 3, 20.7 with 4).
+  constexpr int kBatch = SLICED ? 1 : 3;
   for (int u0 = ub; u0 < ue; u0 += kBatch) {
     u32x4 xv[kBatch][4], av[kBatch][4];
 #pragma unroll
