@@ -23,8 +23,8 @@
 //
 // What bounds it: a row's steps follow each other in one workgroup, each a few hundred ns of LDS round trips and
 // barriers, and a CU gets through 2400 vector instructions of its waves each a microsecond; both kernels are kept to
-// few instructions per value. On the GPU: 1 x 151936 19.9 us, 32 x 151936 (all settings) 23.0 us, 200 x 32001 14.8 us,
-// of which the counting takes 6, 7 and 9. The prefix after prefix of counts, masses and what is kept that was here
+// few instructions per value. On the GPU: 1 x 151936 19.7 us, 32 x 151936 (all settings) 22.8 us, 200 x 32001 14.2 us,
+// of which the counting takes 6, 7 and 8. The prefix after prefix of counts, masses and what is kept that was here
 // first, with 64 words to a look, took 27, 30 and 18 us.
 #include <type_traits>
 
@@ -38,20 +38,28 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
-constexpr int kValues = 0xff00;    // ranks 0 (+infinity) .. 0xfeff (the lowest finite value)
+constexpr int kFirstRank = 0x7F, kLastRank = 0xFF7E;  // +infinity, the lowest finite value
+constexpr int kNoRank = 0x10000;
 constexpr int kMaxSlice = 32768;   // logits per slice: its counts fit 16 bits
 constexpr int kMinSlice = 4096;
 constexpr int kMaxSlices = 512;
 constexpr int kMaxBatch = 256;     // rows per launch: bounds the workspace
 
-// Rank of a bf16 value in falling order (0: +infinity, -0 equal to +0); outside 0 .. kValues - 1 for -infinity and
-// NaN.
-__device__ __forceinline__ int rank_of(uint32_t b) {
-  const int mag = (int)(b & 0x7FFFu);
-  return 0x7F80 + (b & 0x8000u ? mag : -mag);
+// A rank is a bf16 value's number in falling order: 0x7FFF - b for bits b of a positive value, b - 1 of a negative one
+// (0x7FFF for both zeros). -infinity (kLastRank + 1) and NaN lie either side of kFirstRank .. kLastRank.
+__device__ __forceinline__ uint32_t bits_of(int rank) { return rank <= 0x7FFF ? 0x7FFF - rank : rank + 1; }
+__device__ __forceinline__ double value_of(int rank) { return (double)bf16_to_f32(bits_of(rank)); }
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+// The ranks of two values.
+__device__ __forceinline__ u16x2 ranks_of(uint32_t b) {
+  const uint32_t negative = __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, b) >> 15);
+  return __builtin_bit_cast(u16x2, b ^ (0x7FFF7FFFu & ~negative)) + __builtin_bit_cast(u16x2, negative);
 }
-__device__ __forceinline__ double value_of(int rank) {
-  return (double)bf16_to_f32(rank <= 0x7F80 ? 0x7F80 - rank : 0x8000 | (rank - 0x7F80));
+__device__ __forceinline__ u16x2 min2(u16x2 a, u16x2 b) {  // (a minimum with 1 would be compiled into comparisons)
+  u16x2 r;
+  asm("v_pk_min_u16 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
 }
 
 // Logits [begin, end) of a row: whole 16-byte lines of 8 (line g from index first(g)), and up to 7 logits either side
@@ -141,22 +149,28 @@ __device__ __forceinline__ int wave_max(int v) {
   v = max(v, dpp<0x143, 0xC>(v));
   return lane_value(v, 63) - 1;
 }
-// The smallest of values up to kValues.
-__device__ __forceinline__ int row_min(int v) { return kValues - row_max(kValues - v); }
-__device__ __forceinline__ int wave_min(int v) { return kValues - wave_max(kValues - v); }
+// The smallest of ranks up to kNoRank.
+__device__ __forceinline__ int row_min(int v) { return kNoRank - row_max(kNoRank - v); }
+__device__ __forceinline__ int wave_min(int v) { return kNoRank - wave_max(kNoRank - v); }
 
-// 16-bit counts of the logits, two to a word; returns the smallest rank this thread saw. `held`: the lines loaded
-// last (lines threadIdx.x + i kThreads where there are at most kBatch * kThreads of them). `between` runs while the
-// first loads are under way.
+// 16-bit counts of the logits, two to a word; returns the smallest rank this thread saw, NaN's included. `held`: the
+// lines loaded last (lines threadIdx.x + i kThreads where there are at most kBatch * kThreads of them). `between` runs
+// while the first loads are under way. Two logits at a time up to their addresses, 9 instructions each (one at a time
+// 14: 200 x 32001 14.1 us instead of 13.5).
 constexpr int kBatch = 4;
 template <class F>
 __device__ __forceinline__ int count_lines(const Lines& G, uint32_t* hist, u32x4 (&held)[kBatch], F&& between) {
-  int lowest = kValues;
-  auto count = [&](uint32_t b) {  // -infinity and NaN go to bins past the values, one for each lane
-    int r = rank_of(b);
-    r = (uint32_t)r < (uint32_t)kValues ? r : kValues + (int)(threadIdx.x & 63);
-    atomicAdd(&hist[r >> 1], r & 1 ? 0x10000u : 1u);
-    lowest = min(lowest, r);
+  const uint16_t lane = threadIdx.x & 63;
+  const u16x2 last = {kLastRank, kLastRank}, one = {1, 1}, lanes = {lane, lane};
+  u16x2 lowest = {0xFFFF, 0xFFFF};
+  auto count = [&](uint32_t b) {
+    u16x2 r = ranks_of(b);
+    lowest = min2(lowest, r);
+    // -infinity goes to a bin of each lane's own past the values (a masked row would add to one word). NaN goes to some
+    // bin past them or, around the 16 bits, in front of them.
+    r += min2(__builtin_elementwise_sub_sat(r, last), one) * lanes;
+    atomicAdd(&hist[r.x >> 1], __umul24(r.x & 1u, 0xFFFFu) + 1u);
+    atomicAdd(&hist[r.y >> 1], __umul24(r.y & 1u, 0xFFFFu) + 1u);
   };
   const uint32_t edge = G.edge(threadIdx.x);
   for (int g0 = threadIdx.x, at = 0; at < max(G.count, 1); g0 += kBatch * kThreads, at += kBatch * kThreads) {
@@ -165,18 +179,42 @@ __device__ __forceinline__ int count_lines(const Lines& G, uint32_t* hist, u32x4
     if (at == 0) {
       __builtin_amdgcn_sched_barrier(0);
       between();
-      count(edge);
+      count(kNone << 16 | edge);
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       if (at + i * kThreads >= G.count) break;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) count(place(held[i], e));
+      for (int e = 0; e < 4; ++e) count(held[i][e]);
     }
   }
   __syncthreads();
-  if (threadIdx.x < 32) hist[kValues / 2 + threadIdx.x] = 0;
-  return lowest;
+  // What lies either side of the values is cleared.
+  constexpr int kFront = kFirstRank / 2, kBack = kLastRank / 2;  // words that the first and the last value share with it
+  const int t = threadIdx.x;
+  if (t < kFront) hist[t] = 0;
+  if (t == kFront) hist[t] &= 0xFFFF0000u;
+  if (t > kFront && t <= kFront + 0x7FFF - kBack) hist[kBack + t - kFront] = 0;
+  if (t == kThreads - 1) hist[kBack] &= 0xFFFFu;
+  return min((int)lowest.x, (int)lowest.y);
+}
+
+// The smallest rank of the workgroup's logits (kNoRank: none), `mine` from count_lines. With a NaN among them
+// it is looked for in the histogram.
+__device__ __forceinline__ int lowest_rank(const uint32_t* hist, int mine, int* s_lo) {
+  for (;;) {
+    mine = wave_min(mine);
+    if ((threadIdx.x & 63) == 0) s_lo[threadIdx.x >> 6] = mine;
+    __syncthreads();
+    const int lowest = row_min(s_lo[threadIdx.x & (kWaves - 1)]);
+    if (lowest >= kFirstRank) return lowest <= kLastRank ? lowest : kNoRank;
+    __syncthreads();
+    mine = kNoRank;
+    for (int w = threadIdx.x; w < 32768; w += kThreads) {
+      const uint32_t n = hist[w];
+      if (n != 0) mine = min(mine, 2 * w + ((n & 0xFFFFu) == 0));
+    }
+  }
 }
 
 template <int BYTES>
@@ -187,7 +225,7 @@ __device__ __forceinline__ void zero_lds(uint32_t* p) {
 // Where a batch's lists lie: heads [rows][slices], entries [rows][slices][slice], an entry rank << 16 | count (a
 // slice's list padded to a multiple of 4 with count 0).
 struct Head {
-  uint32_t n, lowest;  // entries, and the smallest rank (kValues where there is none)
+  uint32_t n, lowest;  // entries, and the smallest rank (kNoRank where there is none)
 };
 struct Lists {
   Head* heads;
@@ -281,18 +319,16 @@ __global__ __launch_bounds__(kThreads) void sample_count_kernel(SampleParams S, 
   const int64_t m = blockIdx.y;
   const int begin = blockIdx.x * L.slice, end = min(S.V, begin + L.slice);
   u32x4 held[kBatch];
-  const int lo = wave_min(count_lines(Lines(S.logits + m * S.row_stride, begin, end), hist, held, [&] {
+  const int mine = count_lines(Lines(S.logits + m * S.row_stride, begin, end), hist, held, [&] {
     zero_lds<kBytes16>(hist);
     __syncthreads();
-  }));
-  if (lane == 0) s_lo[wave] = lo;
-  __syncthreads();
+  });
+  const int lowest = lowest_rank(hist, mine, s_lo);
   uint32_t* list = L.list(m, blockIdx.x);
   list_values<true, 32768, true>(
       hist, s_look,
       [&](uint32_t n) {
-        const int lowest = row_min(s_lo[lane & 15]);
-        if (tid == 0) L.heads[m * L.slices + blockIdx.x] = {n, (uint32_t)min(lowest, kValues)};
+        if (tid == 0) L.heads[m * L.slices + blockIdx.x] = {n, (uint32_t)lowest};
         if (tid < 4 && (n & 3) != 0 && tid >= (int)(n & 3)) list[(n & ~3u) + tid] = 0;
       },
       [&](uint32_t o, uint32_t r, uint32_t n) { list[o] = r << 16 | n; });
@@ -341,29 +377,25 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams S, L
   // its end, where there are any.
   int lowest, base = 0;
   u32x4 held[kBatch];
-  {
-    int lo = kValues;
-    if constexpr (MERGE) {
-      for (int s = tid; s < L.slices; s += kThreads) {
-        const Head head = L.heads[m * L.slices + s];
-        s_n[s] = head.n;
-        lo = min(lo, (int)head.lowest);
-      }
-      if (tid == 0) s_far = 0;
-      zero_lds<kSpan * 4>(hist);
-    } else {
-      lo = count_lines(Lines(row, 0, S.V), hist, held, [&] {
-        zero_lds<kBytes16>(hist);
-        __syncthreads();
-      });
+  if constexpr (MERGE) {
+    int lo = kNoRank;
+    for (int s = tid; s < L.slices; s += kThreads) {
+      const Head head = L.heads[m * L.slices + s];
+      s_n[s] = head.n;
+      lo = min(lo, (int)head.lowest);
     }
-    lo = wave_min(lo);
-    if (lane == 0) s_lo[wave] = lo;
-    __syncthreads();
-    lowest = row_min(s_lo[lane & (kWaves - 1)]);
-    if (MERGE) base = lowest & ~3;
+    if (tid == 0) s_far = 0;
+    zero_lds<kSpan * 4>(hist);
+    lowest = lowest_rank(hist, lo, s_lo);
+    base = lowest & ~3;
+  } else {
+    const int mine = count_lines(Lines(row, 0, S.V), hist, held, [&] {
+      zero_lds<kBytes16>(hist);
+      __syncthreads();
+    });
+    lowest = lowest_rank(hist, mine, s_lo);
   }
-  if (lowest >= kValues) {
+  if (lowest == kNoRank) {
     if (tid == 0) {
       S.tokens[m] = -1;
       S.logprobs[m] = -__builtin_inff();
@@ -643,7 +675,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams S, L
     S.logprobs[m] = (float)log(hit_weight / kept_total);
   };
   // The value's bits; of zero without the sign.
-  const uint32_t bits = hit <= 0x7F80 ? 0x7F80 - hit : 0x8000 | (hit - 0x7F80), mask = bits == 0 ? 0x7FFFu : 0xFFFFu;
+  const uint32_t bits = bits_of((int)hit), mask = bits == 0 ? 0x7FFFu : 0xFFFFu;
   auto matches = [&](uint32_t b) { return (b & mask) == bits; };
   auto line_misses = [&](u32x4 v) {  // how many of a line's 8 do not match
     u32x4 d;

@@ -186,3 +186,18 @@ def test_deterministic_on_a_stream_and_captured():
             g.replay()
             torch.cuda.synchronize()
             assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("count", [65535, 65536, 70000])
+@pytest.mark.parametrize("settings", [dict(), dict(temperature=3e38), dict(temperature=1e38, top_k=30000, top_p=0.9, min_p=0.1)],
+                         ids=str)
+def test_every_bit_pattern(count, settings):
+    """All bf16 words, NaN of either sign among them, in any order; rows with +infinity, without, and of NaN alone."""
+    g = torch.Generator().manual_seed(count)
+    words = torch.stack([torch.randperm(count, generator=g) % 65536 for _ in range(4)])
+    words[1:][words[1:] == 0x7F80] = 0xFF80
+    words[3] = torch.where((words[3] & 0x7F80) == 0x7F80, words[3], 0xFFFF)
+    words[2, ::2] |= 0x7F80
+    words[2][words[2] == 0x7F80] = 0x7FFF
+    logits = torch.where(words >= 32768, words - 65536, words).to(torch.int16).view(torch.bfloat16).to(DEV)
+    check(logits, torch.tensor([0.25, 0.5, 0.75, 0.125], device=DEV), **settings)
