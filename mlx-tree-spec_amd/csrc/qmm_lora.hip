@@ -177,9 +177,9 @@ LdsAllowance g_sliced, g_whole;
 }  // namespace
 
 // Few tiles: K in up to 8 slices of at least 512, while that gives a CU no second workgroup (counted for one adapter per
-// 16 rows). One / 4 / 8 slices: 4 x 5120 rank 16 of 4 adapters 6.7 / 5.3 / 5.1 us, 16 rows of one 6.6 / 5.2 / 4.8, 64 x
-// 17408 rank 32 of 4 adapters 15.0 / 8.0 / 7.2; many tiles, 2000 x 5120 rank 64, 15.5 / 29 / 46. (4 or 16 waves instead of 8: 4 x
-// 5120 5.3 / 5.6, 64 x 17408 7.9 / 6.8, many tiles no better; tiles of 4 values of j: no better in slices.)
+// 16 rows). One / 4 / 8 slices: 4 x 5120 rank 16 of 4 adapters 6.1 / 5.3 / 4.8 us, 16 rows of one 6.3 / 5.3 / 4.7, 64 x
+// 17408 rank 32 of 4 adapters 14.9 / 7.8 / 6.9; many tiles, 2000 x 5120 rank 64, 15.0 / 30 / 47. (4 or 16 waves instead of
+// 8: 4 x 5120 0.2 or 0.5 more, many tiles no better; tiles of 4 values of j: no better in slices.)
 LoraShrinkPlan lora_shrink_plan(const LoraTables& lora, int M, int K, int cus) {
   LoraShrinkPlan p;
   const int most = M < 16 ? M : 16;  // adapters of 16 rows
