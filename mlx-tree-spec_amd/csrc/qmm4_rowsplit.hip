@@ -621,7 +621,7 @@ void rowsplit_kernel(RowSplitParams P) {
   }
   // LORA: what this thread's first output column takes of the adapters, while other waves still stream. (Its adapters
   // loaded at the start: 4 x 5120 -> 34816 with rank 16 34.1 -> 32.1 us. All of it in front of the first unit: 32.8.)
-  bool first_item = true;
+  // It belongs to item number tid alone: in a last range cut short that item may be none while a later one is.
   f32x4 first_add = {0.0f, 0.0f, 0.0f, 0.0f};
   if constexpr (LORA) {
     int a[4];
@@ -645,11 +645,10 @@ void rowsplit_kernel(RowSplitParams P) {
     }
     return sum;
   };
-  auto write = [&](int col, int gg, f32x4 sum, const f32x4& sup) __attribute__((always_inline)) {
+  auto write = [&](int it, int col, int gg, f32x4 sum, const f32x4& sup) __attribute__((always_inline)) {
     if constexpr (LORA) {
-      if (first_item) {
+      if (it == tid) {
         sum[0] += first_add[0]; sum[1] += first_add[1]; sum[2] += first_add[2]; sum[3] += first_add[3];
-        first_item = false;
       } else {
         sum = lora_rows4<1>(P.lora, sum, 4 * gg, col, P.M, P.N);
       }
@@ -670,7 +669,7 @@ void rowsplit_kernel(RowSplitParams P) {
       if (col >= r1 || 4 * gg >= P.M) continue;
       const f32x4 sum = row_sum(c, gg);
       const f32x4 sup = FUSED ? row_sum(P.R + c, gg) : sum;
-      write(col, gg, sum, sup);
+      write(it, col, gg, sum, sup);
     }
     return;
   }
@@ -736,7 +735,7 @@ void rowsplit_kernel(RowSplitParams P) {
         sup[0] += vu[qq][0]; sup[1] += vu[qq][1]; sup[2] += vu[qq][2]; sup[3] += vu[qq][3];
       }
     }
-    write(col, gg, sum, sup);
+    write(it, col, gg, sum, sup);
   }
   if (tid == 0) __hip_atomic_store(&P.cnt[range], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }

@@ -1,0 +1,30 @@
+"""GPU shapes of the adapters' tests whose kernel route is their point, with the route each takes on a 256-CU MI355X
+(test_adapter_routes.py checks every label against the built planners on the CPU)."""
+
+CUS = 256
+
+# (M, K, N, K slices, super-steps per unit, form, wrapped): row-split launches. form: "slots" (a slot per unit), "groups"
+# (one per group of units), "own" (a wave's whole blocks in registers) or "small" (every unit in flight at once). wrapped: more items (column, lane group) than
+# threads, so that a thread takes several, and a last column range so narrow that some thread's first item lies past its
+# end and a later one does not.
+ROWSPLIT = [
+    (5, 512, 152064, 1, 4, "slots", True),     # a vocabulary head
+    (8, 640, 152064, 1, 5, "slots", True),
+    (5, 3584, 152064, 1, 4, "groups", True),
+    (8, 12288, 33856, 4, 4, "slots", True),
+    (13, 512, 50304, 1, 4, "slots", True),
+    (16, 640, 64000, 1, 5, "slots", True),
+    (9, 2560, 65984, 1, 4, "groups", True),    # the drafter's vocabulary, one row in the last lane group
+    (13, 1024, 21760, 2, 4, "slots", True),
+    (16, 5120, 21760, 2, 4, "slots", True),
+    (13, 4096, 32000, 2, 4, "slots", True),
+    (16, 5120, 33856, 2, 5, "slots", True),
+    (3, 1024, 4096, 1, 4, "slots", False),
+    (5, 12288, 21760, 4, 4, "slots", False),   # more items than threads, ranges all whole
+    (5, 8192, 17408, 1, 4, "groups", False),
+    (6, 1024, 5120, 2, 4, "slots", False),
+    (8, 512, 2048, 1, 4, "small", False),
+    (9, 12288, 2048, 4, 4, "slots", False),
+    (16, 5120, 50304, 4, 5, "slots", False),
+    (9, 512, 589824, 1, 4, "own", False),      # whole blocks to each wave
+]

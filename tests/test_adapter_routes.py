@@ -1,0 +1,33 @@
+"""The routes of the adapters' GPU tests, from the built planners (CPU only, no GPU call)."""
+
+import adapter_cases as C
+from test_plans import dispatch_route, planner_exe, query  # noqa: F401  (a fixture among them)
+
+THREADS = 512  # of a row-split workgroup
+
+
+def first_items(m, n, p):
+    """(items of a range, threads of the last range that write an item other than their own number first): item i of a
+    range of R columns is column i % R of lane group i / R, thread t takes t, t + 512, .., and items past the range's
+    last column or the last row are none."""
+    groups, slices = int(p["MP"]) // 4, int(p["KS"])
+    width = (-(-n // max(1, C.CUS // slices)) + 3) // 4 * 4
+    ranges = -(-n // width)
+    assert ranges * slices == int(p["blocks"])
+    last = n - (ranges - 1) * width
+    late = 0
+    for t in range(THREADS):
+        mine = [i for i in range(t, width * groups, THREADS) if i % width < last and 4 * (i // width) < m]
+        late += bool(mine) and mine[0] != t
+    return width * groups, late
+
+
+def test_rowsplit_cases_take_their_routes(planner_exe):  # noqa: F811
+    shapes = [(m, n, k) for m, k, n, *_ in C.ROWSPLIT]
+    assert dispatch_route(planner_exe, shapes) == ["row-split"] * len(shapes)
+    plans = query(planner_exe, [f"rowsplit {m} {n} {k} {C.CUS}" for m, n, k in shapes])
+    for (m, k, n, slices, steps, form, wrapped), p in zip(C.ROWSPLIT, plans):
+        takes = "small" if p["small"] == "1" else "groups" if p["pair"] == "1" else "own" if p["own"] == "1" else "slots"
+        assert (int(p["KS"]), int(p["V"]), takes) == (slices, steps, form), (m, k, n, p)
+        items, late = first_items(m, n, p)
+        assert (late > 0) == wrapped and (items > THREADS or not wrapped), (m, k, n, items, late)
