@@ -28,3 +28,21 @@ ROWSPLIT = [
     (16, 5120, 50304, 4, 5, "slots", False),
     (9, 512, 589824, 1, 4, "own", False),      # whole blocks to each wave
 ]
+
+# (M, K, N, form): GEMM launches. Whole 256 x 256 tiles with waves split by role ("whole") or not ("whole, plain": K not a
+# multiple of 512), what a last round leaves as 128 x 128 quarters or as stream-K over the quarters, and stream-K over each tile.
+GEMM = [
+    (2304, 512, 4096, "whole"),
+    (2048, 512, 4096, "quarters"),               # half the CUs' whole tiles, all cut
+    (2000, 1024, 4112, "whole"),                 # a partial last row and column of tiles
+    (2000, 640, 4112, "whole, plain"),
+    (5100, 512, 3312, "whole, tail in stream-K"),
+    (5100, 512, 4336, "whole, tail in quarters"),
+    (5100, 640, 4336, "whole, plain, tail in quarters"),
+    (600, 12288, 4112, "stream-K 256x256"),
+    (136, 5120, 10256, "stream-K 128x256"),
+    (203, 5120, 17408, "stream-K 128x256"),      # in units of 4 K steps
+    (515, 2048, 1040, "stream-K 128x128"),
+    (129, 2048, 10240, "stream-K 128x128"),      # in units of 4 K steps
+    (300, 640, 4112, "stream-K 128x128, plain"),
+]

@@ -31,3 +31,24 @@ def test_rowsplit_cases_take_their_routes(planner_exe):  # noqa: F811
         assert (int(p["KS"]), int(p["V"]), takes) == (slices, steps, form), (m, k, n, p)
         items, late = first_items(m, n, p)
         assert (late > 0) == wrapped and (items > THREADS or not wrapped), (m, k, n, items, late)
+
+
+def gemm_form(m, k, n, p):
+    plain = k % 512 != 0
+    if p["sk"] == "1":
+        tile = "256x256" if p["sk256"] == "1" else "128x256" if p["sk_wide"] == "1" else "128x128"
+        return f"stream-K {tile}" + ", plain" * plain
+    tiles = -(-m // 256) * -(-n // 256)
+    tail = tiles % C.CUS
+    if tail == 0 or 4 * tail > 2 * C.CUS:
+        return "whole" + ", plain" * plain
+    cut = "stream-K" if p["tail_sk"] == "1" else "quarters"
+    return cut + ", plain" * plain if tail == tiles else "whole" + ", plain" * plain + ", tail in " + cut
+
+
+def test_gemm_cases_take_their_routes(planner_exe):  # noqa: F811
+    shapes = [(m, n, k) for m, k, n, _ in C.GEMM]
+    assert dispatch_route(planner_exe, shapes) == ["gemm"] * len(shapes)
+    plans = query(planner_exe, [f"gemm {m} {n} {k} {C.CUS}" for m, n, k in shapes])
+    for (m, k, n, form), p in zip(C.GEMM, plans):
+        assert gemm_form(m, k, n, p) == form, (m, k, n, p)
