@@ -32,8 +32,10 @@ extern "C" {
  *   N % 16 == 0), else of qmm_affine_general_bf16; lora_a: bf16 [L, R, K]; lora_b: bf16 [L, N, R]; lora_scale: fp32
  *   [L]; adapters: int32 or int64 [M] (adapter_bits 32 or 64).
  *   The sums of both products are fp32 and rounded once; between its factors the second one is kept (in `workspace`) to
- *   2^-18 of its value. Requires R % 8 == 0, 8 <= R <= QMM4_LORA_MAX_RANK, L <= 2^30, M <= 2^26, lora_a, lora_b and
- *   workspace 16-byte aligned, lora_scale 4-byte, adapters by their own size. M == 0 or N == 0 is a no-op. Deterministic.
+ *   2^-18 of its value. What is not finite in x, lora_a, lora_b or lora_scale gives what the formula gives, in the rows
+ *   that use it and in no other. Requires R % 8 == 0, 8 <= R <= QMM4_LORA_MAX_RANK, L <= 2^30, M <= 2^26, lora_a,
+ *   lora_b and workspace 16-byte aligned, lora_scale 4-byte, adapters by their own size. M == 0 or N == 0 is a no-op.
+ *   Deterministic.
  */
 int64_t qmm4_lora_workspace(int64_t M, int64_t R);
 int qmm4_affine_lora_bf16(const void* x, const uint32_t* w, const void* scales, const void* biases,

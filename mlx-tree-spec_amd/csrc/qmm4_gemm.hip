@@ -120,20 +120,22 @@ struct Raw {
 // two activation stages in LDS and B that of the first weight stage. One round trip to memory per 64 j, where loads
 // straight into fragments took one per 16 (and 150 us of 2000 x 5120 -> 17408 in spilled registers).
 // A tile of several adapters holds rows whose t is zero beside a B that is not theirs, and a product of zero with an
-// infinity would reach them: what is not finite in B is zeroed and its column noted, and a last step of two products
-// that overflow to both infinities makes those columns of the adapter's own rows NaN. (Only matrix products touch the
-// accumulators: selections on them spilled the registers of the whole kernel.)
+// infinity would reach them: the products take what is not finite in t and B as zero, and note that there is some. The
+// terms left out are added to the finished tile (lora_nonfinite). (Only matrix products touch the accumulators:
+// selections on them spilled the registers of the whole kernel.)
 constexpr int kLoraK = BK;
-template <int BM, int BN>
+template <int BM>
 struct LoraLds {
-  int adapter[BM];  // of the tile's rows: -1 none, -2 past M
-  int bad[BN];      // columns with a B that is not finite (zero between adapters)
-  int any[2];       // whether this stage (by its parity) saw one
-  // Rows r and columns c < max(BM, BN), before the first stage.
+  int adapter[BM];   // of the tile's rows: -1 none
+  int bad_row[BM];   // rows with a t that is not finite
+  int any;           // whether t or B has something that is not
+  // Row i, before the first stage.
   __device__ __forceinline__ void init(const LoraAdd& E, int i, int m0, int M) {
-    if (i < BM) adapter[i] = m0 + i < M ? lora_adapter(E, m0 + i, M) : -2;
-    if (i < BN) bad[i] = 0;
-    if (i < 2) any[i] = 0;
+    if (i < BM) {
+      adapter[i] = lora_adapter(E, m0 + i, M);
+      bad_row[i] = 0;
+    }
+    if (i == 0) any = 0;
   }
 };
 
@@ -149,72 +151,98 @@ struct TileAdapters {
       todo[q] = __ballot(a[q] >= 0);
     }
   }
-  __device__ __forceinline__ bool next(int* d, bool* mixed) {
+  __device__ __forceinline__ bool next(int* d) {
     *d = -1;
-    *mixed = false;
 #pragma unroll
     for (int q = BM / 64 - 1; q >= 0; --q)
       if (todo[q] != 0) *d = __builtin_amdgcn_readlane(a[q], __ffsll(todo[q]) - 1);
     if (*d < 0) return false;
 #pragma unroll
-    for (int q = 0; q < BM / 64; ++q) {
-      const unsigned long long mine = __ballot(a[q] == *d);
-      todo[q] &= ~mine;
-      *mixed |= (mine | __ballot(a[q] == -2)) != ~0ull;
-    }
+    for (int q = 0; q < BM / 64; ++q) todo[q] &= ~__ballot(a[q] == *d);
     return true;
   }
 };
 
-// Makes what is not finite of 8 bf16 values zero; whether there was any.
-__device__ __forceinline__ bool lora_zero_bad(u32x4* v) {
+// Makes what is not finite zero, of 8 values of B or of 4 of t (a high part in each upper half); whether there was any.
+__device__ __forceinline__ bool lora_zero_b(u32x4* v) {
+  const bool any = lora_any_nonfinite(*v);
+  *v = lora_finite(*v);
+  return any;
+}
+__device__ __forceinline__ bool lora_zero_t(u32x4* v) {
   bool any = false;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const bool lo = ((*v)[e] & 0x7F80u) == 0x7F80u, hi = ((*v)[e] & 0x7F800000u) == 0x7F800000u;
-    (*v)[e] = (lo ? 0u : (*v)[e] & 0xFFFFu) | (hi ? 0u : (*v)[e] & 0xFFFF0000u);
-    any |= lo || hi;
+    const bool fine = __builtin_isfinite(__uint_as_float((*v)[e]));
+    (*v)[e] = fine ? (*v)[e] : 0u;
+    any |= !fine;
   }
   return any;
 }
-// A row of t and of B (16 k) whose product is the sum of both infinities where `own` and `bad`, else zero.
-__device__ __forceinline__ void lora_put_bad(uint16_t* t, uint16_t* b, bool own, bool bad) {
-  constexpr uint32_t kBig = 0x7F7Fu;  // the largest bf16
-  const u32x4 zero = {0u, 0u, 0u, 0u};
-  *reinterpret_cast<u32x4*>(t) = u32x4{own ? (kBig | 0x8000u) << 16 | kBig : 0u, 0u, 0u, 0u};
-  *reinterpret_cast<u32x4*>(t + 8) = zero;
-  *reinterpret_cast<u32x4*>(b) = u32x4{bad ? kBig << 16 | kBig : 0u, 0u, 0u, 0u};
-  *reinterpret_cast<u32x4*>(b + 8) = zero;
+
+// The terms that a tile's products left out, added to its values in LDS (rounded already: such a sum is an infinity or
+// NaN, whatever it is added to). NT threads, each a column and every so many rows; a column's B is looked at again
+// where the rows' adapter changes.
+template <int BM, int BN, int NT>
+__device__ __forceinline__ void lora_nonfinite(const LoraAdd& E, const int* adapter, const int* bad_row, uint16_t* Cs,
+                                               int ldc, int tid, int m0, int n0, int N) {
+  static_assert(NT % BN == 0, "whole rows at a time");
+  const int c = tid % BN;
+  if (n0 + c >= N) return;
+  const uint16_t* b = E.b;
+  int of = -1;
+  bool bad = false;
+#pragma unroll 1
+  for (int r = tid / BN; r < BM; r += NT / BN) {
+    const int a = adapter[r];
+    if (a < 0) continue;
+    if (a != of) {
+      of = a;
+      b = E.b + ((int64_t)a * N + n0 + c) * E.R;
+      bad = false;
+#pragma unroll 1
+      for (int j = 0; j < E.R; j += 8) bad |= lora_any_nonfinite(*reinterpret_cast<const u32x4*>(b + j));
+    }
+    if (!bad && bad_row[r] == 0) continue;
+    const uint32_t* t = E.t + (int64_t)(m0 + r) * E.R;
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int j = 0; j < E.R; ++j) {
+      const uint32_t w = t[j];
+      const float bv = bf16_to_f32(b[j]);
+      if (!__builtin_isfinite(__uint_as_float(w)) || !__builtin_isfinite(bv))
+        sum = __builtin_fmaf(__uint_as_float(w & 0xFFFF0000u) + __uint_as_float(w << 16), bv, sum);
+    }
+    uint16_t* p = Cs + r * ldc + c;
+    *p = (uint16_t)bf16_rne(bf16_to_f32(*p) + sum);
+  }
 }
 
 // The steps of gemm_ws_kernel's tile.
 template <int BM>
 struct LoraSteps {
-  int adapter[BM];  // of the tile's rows: -1 none, -2 past M
-  int list[BM];     // those that occur: 2 * adapter + (whether other rows have another one or none)
-  int count, steps, any, pad;
+  LoraLds<BM> rows;
+  int list[BM];  // the adapters that occur
+  int count, steps;
   // By one wave, for the tile's rows from m0.
   __device__ __forceinline__ void init(const LoraAdd& E, int lane, int m0, int M) {
 #pragma unroll
-    for (int q = 0; q < BM / 64; ++q)
-      adapter[q * 64 + lane] = m0 + q * 64 + lane < M ? lora_adapter(E, m0 + q * 64 + lane, M) : -2;
-    TileAdapters<BM> walk(adapter);
+    for (int q = 0; q < BM / 64; ++q) rows.init(E, q * 64 + lane, m0, M);
+    TileAdapters<BM> walk(rows.adapter);
     int d, n = 0;
-    bool mixed;
-    for (; walk.next(&d, &mixed); ++n)
-      if (lane == 0) list[n] = 2 * d + mixed;
+    for (; walk.next(&d); ++n)
+      if (lane == 0) list[n] = d;
     if (lane == 0) {
       count = n;
       steps = (n * ((E.R + 31) / 32) + 1) & ~1;  // a last one of zeros makes them even
-      any = 0;
     }
   }
 };
 
-// Threads 0 .. NT - 1 stage j0 .. j0 + 63 of adapter d into LDS (to the next 16 past R with zeros); `stage` counts.
+// Threads 0 .. NT - 1 stage j0 .. j0 + 63 of adapter d into LDS (to the next 16 past R with zeros).
 template <int BM, int BN, int NT, int AHEAD>
-__device__ __forceinline__ void lora_stage(const LoraAdd& E, LoraLds<BM, BN>& S, uint16_t* As, uint16_t* Bs, int tid, int d,
-                                           bool mixed, int j0, int stage, int m0, int n0, int M, int N) {
+__device__ __forceinline__ void lora_stage(const LoraAdd& E, LoraLds<BM>& S, uint16_t* As, uint16_t* Bs, int tid, int d,
+                                           int j0, int m0, int n0, int M, int N) {
   m0 = __builtin_amdgcn_readfirstlane(m0);
   n0 = __builtin_amdgcn_readfirstlane(n0);
   constexpr uint32_t kOut = 0x80000000u;  // past the end of a tile's rows or columns: reads zero
@@ -223,7 +251,6 @@ __device__ __forceinline__ void lora_stage(const LoraAdd& E, LoraLds<BM, BN>& S,
   const int width = min(E.R - j0, kLoraK), pieces = (width + 15) / 16 * 2;
   const int pc = tid & 7, r0 = tid >> 3;
   const bool in = pc * 8 < width;
-  if (tid == 0) S.any[~stage & 1] = 0;  // (the stage before is read)
   const __amdgpu_buffer_rsrc_t rt = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint32_t*>(E.t + (int64_t)m0 * E.R), 0, rows * E.R * 4, kBufferRsrcWord3);
   const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
@@ -243,6 +270,7 @@ __device__ __forceinline__ void lora_stage(const LoraAdd& E, LoraLds<BM, BN>& S,
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
         const int r = (i0 + i) * (NT / 8) + r0;
+        if (lora_zero_t(&t0[i]) | lora_zero_t(&t1[i])) S.bad_row[r] = S.any = 1;
         bf16x8 hi, lo;
         lora_split(t0[i], t1[i], &hi, &lo);
         *reinterpret_cast<u32x4*>(As + r * LDK + pc * 8) = __builtin_bit_cast(u32x4, hi);
@@ -263,57 +291,30 @@ __device__ __forceinline__ void lora_stage(const LoraAdd& E, LoraLds<BM, BN>& S,
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int c = (i0 + i) * (NT / 8) + r0;
-      if (mixed && lora_zero_bad(&b[i])) {
-        S.bad[c] = 1;
-        S.any[stage & 1] = 1;
-      }
+      if (lora_zero_b(&b[i])) S.any = 1;
       if (pc < pieces) *reinterpret_cast<u32x4*>(Bs + c * LDK + pc * 8) = b[i];
     }
     __builtin_amdgcn_sched_barrier(0);
   }
 }
 
-// The last step of an adapter with columns noted: only the first BM rows of t's (the low parts' place holds zeros).
-template <int BM, int BN, int NT>
-__device__ __forceinline__ void lora_stage_bad(LoraLds<BM, BN>& S, uint16_t* As, uint16_t* Bs, int tid, int d) {
-  for (int i = tid; i < (BM > BN ? BM : BN); i += NT) {
-    uint16_t* t = As + i * LDK;
-    lora_put_bad(t, Bs + i * LDK, i < BM && S.adapter[i] == d, i < BN && S.bad[i] != 0);
-    if (i < BM) {
-      *reinterpret_cast<u32x4*>(t + BM * LDK) = u32x4{0u, 0u, 0u, 0u};
-      *reinterpret_cast<u32x4*>(t + BM * LDK + 8) = u32x4{0u, 0u, 0u, 0u};
-    }
-    if (i < BN) S.bad[i] = 0;
-  }
-}
-
-// Every wave's walk over the tile's adapters: stage(d, mixed, j0, n) (j0 < 0: lora_stage_bad), a barrier, take(steps of 16), a
-// barrier. Roles that do not stage or take pass functions that do nothing.
-template <int BM, int BN, class Stage, class Take>
-__device__ __forceinline__ void lora_walk(const LoraLds<BM, BN>& S, int R, Stage&& stage, Take&& take) {
+// Every wave's walk over the tile's adapters: stage(d, j0), a barrier, take(steps of 16), a barrier.
+template <int BM, class Stage, class Take>
+__device__ __forceinline__ void lora_walk(const LoraLds<BM>& S, int R, Stage&& stage, Take&& take) {
   TileAdapters<BM> list(S.adapter);
-  int d, n = 0;
-  bool mixed;
-  while (list.next(&d, &mixed)) {
-    int bad = 0;
-    for (int j0 = 0; j0 < R; j0 += kLoraK, ++n) {
-      stage(d, mixed, j0, n);
+  int d;
+  while (list.next(&d)) {
+    for (int j0 = 0; j0 < R; j0 += kLoraK) {
+      stage(d, j0);
       __syncthreads();
-      bad |= *const_cast<const volatile int*>(&S.any[n & 1]);
       take((min(R - j0, kLoraK) + 15) / 16);
-      __syncthreads();
-    }
-    if (__builtin_amdgcn_readfirstlane(bad)) {
-      stage(d, mixed, -1, n);
-      __syncthreads();
-      take(1);
       __syncthreads();
     }
   }
 }
 
 // A wave's part of the tile (I x J blocks of 32 from its row wr and column wc) takes the staged products.
-template <int BM, int I, int J, int HALVES = 2>
+template <int BM, int I, int J>
 __device__ __forceinline__ void lora_take(const uint16_t* As, const uint16_t* Bs, f32x16 (&acc)[I][J], int steps, int wr,
                                           int wc) {
   const int lane = threadIdx.x & 63, lrow = lane & 31, lk = (lane >> 5) * 8;
@@ -323,7 +324,7 @@ __device__ __forceinline__ void lora_take(const uint16_t* As, const uint16_t* Bs
 #pragma unroll
     for (int j = 0; j < J; ++j) Bf[j] = as_bf16x8(*reinterpret_cast<const u32x4*>(Bs + (wc + j * 32 + lrow) * LDK + ks * 16 + lk));
 #pragma unroll
-    for (int half = 0; half < HALVES; ++half)
+    for (int half = 0; half < 2; ++half)
 #pragma unroll
       for (int i = 0; i < I; ++i) {
         const bf16x8 Af =
@@ -364,7 +365,7 @@ void gemm_kernel(GemmParams P) {
   static_assert(D == 2 || (SB8 && D == 4), "raw ring depth: its index must be static in the loop unrolled by 8");
   using C = GemmCfg<BM, BN>;
   constexpr int I = C::I, J = C::J, AJ = C::AJ, WPT = C::WPT, LDC = C::LDC;
-  __shared__ int s_lora[LORA ? sizeof(LoraLds<BM, BN>) / sizeof(int) : 1];
+  __shared__ int s_lora[LORA ? sizeof(LoraLds<BM>) / sizeof(int) : 1];
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   uint16_t* As = smem;                    // [2][BM * LDK]
   uint16_t* Bs = smem + 2 * BM * LDK;     // [2][BN * LDK]
@@ -621,16 +622,15 @@ void gemm_kernel(GemmParams P) {
   // so a chunk is entirely inside or outside).
   auto write_tile = [&](int m0, int n0) __attribute__((always_inline)) {
     uint16_t* Cs = smem;
+    [[maybe_unused]] LoraLds<BM>& S = *reinterpret_cast<LoraLds<BM>*>(s_lora);
     if constexpr (LORA) {
-      LoraLds<BM, BN>& S = *reinterpret_cast<LoraLds<BM, BN>*>(s_lora);
-      static_assert(kThreads >= BM && kThreads >= BN, "a thread per row and column of the tile");
+      static_assert(kThreads >= BM, "a thread per row of the tile");
       S.init(P.lora, tid, m0, P.M);
       __syncthreads();
-      lora_walk<BM, BN>(
+      lora_walk<BM>(
           S, P.lora.R,
-          [&](int d, bool mixed, int j0, int n) __attribute__((always_inline)) {
-            if (j0 < 0) lora_stage_bad<BM, BN, kThreads>(S, As, Bs, tid, d);
-            else lora_stage<BM, BN, kThreads, 2>(P.lora, S, As, Bs, tid, d, mixed, j0, n, m0, n0, P.M, P.N);
+          [&](int d, int j0) __attribute__((always_inline)) {
+            lora_stage<BM, BN, kThreads, 2>(P.lora, S, As, Bs, tid, d, j0, m0, n0, P.M, P.N);
           },
           [&](int steps) __attribute__((always_inline)) {
             lora_take<BM, I, J>(As, Bs, acc, steps, wm * C::WM, wn * C::WN);
@@ -648,6 +648,12 @@ void gemm_kernel(GemmParams P) {
         }
       }
     __syncthreads();
+    if constexpr (LORA) {
+      if (S.any) {
+        lora_nonfinite<BM, BN, kThreads>(P.lora, S.adapter, S.bad_row, Cs, LDC, tid, m0, n0, P.N);
+        __syncthreads();
+      }
+    }
     constexpr int kChunksPerRow = BN / 8;
 #pragma unroll 4
     for (int c = tid; c < BM * kChunksPerRow; c += kThreads) {
@@ -862,6 +868,15 @@ void gemm_ws_kernel(GemmParams P) {
       }
     }
   };
+  // LORA: the terms that the products left out, by all 12 waves.
+  auto add_nonfinite = [&](int m0, int n0) __attribute__((always_inline)) {
+    if constexpr (LORA) {
+      if (__builtin_amdgcn_readfirstlane(S.rows.any)) {
+        lora_nonfinite<BM, BN, kWsThreads>(P.lora, S.rows.adapter, S.rows.bad_row, smem, LDC, tid, m0, n0, P.N);
+        __syncthreads();
+      }
+    }
+  };
   // The workgroup's tile segments: the whole K of tile P.tile0 + bid, or its stream-K range of units
   // (gemm_kernel's bookkeeping: the same ranges, segments and partial slots, so
   // gemm_sk_reduce_kernel adds the same bits). f(m0, n0, kb, ke, first) per segment.
@@ -884,7 +899,8 @@ void gemm_ws_kernel(GemmParams P) {
     }
   };
   // Every segment passes the same barriers in both roles: one after the producers' prologue, one
-  // per K step, (LORA: one per step of the adapters, two per adapter where one is not finite,) one between the bf16 tile's LDS writes and its stores (whole tiles), one at the end
+  // per K step, (LORA: one per step of the adapters,) one between the bf16 tile's LDS writes and its stores (whole
+  // tiles; LORA: two where t or B is not finite), one at the end
   // (the next segment's prologue reuses the LDS stages and the output tile).
 
   if (mma) {
@@ -931,15 +947,6 @@ void gemm_ws_kernel(GemmParams P) {
       if (kb == 0 && ke == nk) {
         // The tile as bf16 into LDS (every wave is past the last step's reads).
         uint16_t* Cs = smem;
-        if constexpr (LORA) {
-          if (__builtin_amdgcn_readfirstlane(S.any)) {
-            for (int i = 0; i < S.count; ++i) {
-              __syncthreads();  // staged
-              lora_take<BM, I, J, 1>(As, Bs, acc, 1, wm * C::WM, wn * C::WN);
-              __syncthreads();
-            }
-          }
-        }
 #pragma unroll
         for (int i = 0; i < I; ++i)
 #pragma unroll
@@ -952,6 +959,7 @@ void gemm_ws_kernel(GemmParams P) {
             }
           }
         __syncthreads();
+        add_nonfinite(m0, n0);
         store_chunks(m0, n0);
       } else {
         // A part of the tile: its fp32 sums to this workgroup's slot (0: its first segment, 1: its
@@ -1014,7 +1022,7 @@ void gemm_ws_kernel(GemmParams P) {
       const int tm = __builtin_amdgcn_readfirstlane(m0), tn = __builtin_amdgcn_readfirstlane(n0);
       const int per = (E.R + 31) / 32, at = l / per, j0 = (l - at * per) * 32;
       const bool live = at < S.count;
-      const int entry = live ? __builtin_amdgcn_readfirstlane(S.list[at]) : 0, d = entry >> 1;
+      const int d = live ? __builtin_amdgcn_readfirstlane(S.list[at]) : 0;
       const __amdgpu_buffer_rsrc_t rt = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<uint32_t*>(E.t + (int64_t)tm * E.R), 0, max(0, min(BM, P.M - tm)) * E.R * 4, kBufferRsrcWord3);
       const __amdgpu_buffer_rsrc_t rl = __builtin_amdgcn_make_buffer_rsrc(
@@ -1024,7 +1032,7 @@ void gemm_ws_kernel(GemmParams P) {
 #pragma unroll
       for (int i = 0; i < kAJ; ++i) {
         const int r = (pt >> 3) + 32 * i;
-        const bool in = live && jt < E.R && S.adapter[r] == d;
+        const bool in = live && jt < E.R && S.rows.adapter[r] == d;
         t[i] = __builtin_amdgcn_raw_buffer_load_b128(rt, in ? (uint32_t)(r * E.R + jt) * 4u : kOut, 0, 0);
       }
 #pragma unroll
@@ -1035,6 +1043,7 @@ void gemm_ws_kernel(GemmParams P) {
       uint16_t* as = As + st * BM * LDK + (pt >> 3) * LDK + (pt & 7) * 4;
 #pragma unroll
       for (int i = 0; i < kAJ; ++i) {
+        if (lora_zero_t(&t[i])) S.rows.bad_row[(pt >> 3) + 32 * i] = S.rows.any = 1;
         *reinterpret_cast<u32x2*>(as + 32 * i * LDK) =
             u32x2{__builtin_amdgcn_perm(t[i][1], t[i][0], 0x07060302u), __builtin_amdgcn_perm(t[i][3], t[i][2], 0x07060302u)};
         *reinterpret_cast<u32x2*>(as + 32 * i * LDK + 32) =
@@ -1043,7 +1052,7 @@ void gemm_ws_kernel(GemmParams P) {
       uint16_t* bs = Bs + st * BN * LDK + (pt >> 2) * LDK + (pt & 3) * 8;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if ((entry & 1) && lora_zero_bad(&v[i])) S.any = 1;
+        if (lora_zero_b(&v[i])) S.rows.any = 1;
         *reinterpret_cast<u32x4*>(bs + 64 * i * LDK) = v[i];
         *reinterpret_cast<u32x4*>(bs + 64 * i * LDK + 32) = v[i];
       }
@@ -1118,23 +1127,10 @@ void gemm_ws_kernel(GemmParams P) {
         if (l < nl) put_lora(l, l & 1);
         __syncthreads();
       }
-      if (nl > 0 && __builtin_amdgcn_readfirstlane(S.any)) {
-        // For each adapter, the columns where its B is not finite (thread pt: column pt).
-        for (int i = 0; i < S.count; ++i) {
-          const int d = S.list[i] >> 1;
-          bool bad = false;
-          if (n0 + pt < P.N) {
-            const uint16_t* b = P.lora.b + ((int64_t)d * P.N + n0 + pt) * P.lora.R;
-            for (int j = 0; j < P.lora.R; ++j) bad |= (b[j] & 0x7F80u) == 0x7F80u;
-          }
-          lora_put_bad(As + pt * LDK, Bs + pt * LDK, S.adapter[pt] == d, bad);
-          __syncthreads();
-          __syncthreads();  // taken
-        }
-      }
     }
     if (kb == 0 && ke == nk) {
       __syncthreads();  // the MFMA waves' bf16 tile is in LDS
+      add_nonfinite(m0, n0);
       store_chunks(m0, n0);
     }
     __syncthreads();

@@ -89,7 +89,8 @@ def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor
     lora_b bf16 [L, N, R], lora_scale fp32 [L] (R a multiple of 8, up to 256); adapters int32 or int64 of x's
     leading shape. A row whose adapter lies outside 0 .. L - 1 (-1, say) has the projection alone, with its bits.
     Both products are summed in fp32 and rounded once (twice at the sizes and formats for which quantized_matmul
-    dequantizes and multiplies); x @ lora_a.T is kept to 2^-18 of its value in between.
+    dequantizes and multiplies); x @ lora_a.T is kept to 2^-18 of its value in between. What is not finite in an
+    adapter reaches the rows that use it, as the formula has it, and no other.
     """
     what = "quantized_matmul_lora"
     y = _native_lora(x, w, scales, biases, lora_a, lora_b, lora_scale, adapters, transpose, group_size, bits, mode)
