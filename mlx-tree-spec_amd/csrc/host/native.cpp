@@ -268,12 +268,11 @@ PyObject* pair(at::Tensor&& a, at::Tensor&& b) {
   return out;
 }
 
-// lora(x, w, scales, biases, lora_a, lora_b, lora_scale, adapters, group_size, bits, general): quantized_matmul_lora
-// where one call of the library does it: 4-bit groups of 64 on the packed kernels, or any format on the general
-// kernel when `general` is true (the caller's rule).
+// lora(x, w, scales, biases, lora_a, lora_b, lora_scale, adapters, group_size, bits): quantized_matmul_lora where one
+// call of the library does it (the caller's rule).
 PyObject* lora(PyObject*, PyObject* const* a, Py_ssize_t na) {
   HANDLE_TH_ERRORS
-  if (na != 11) return none();
+  if (na != 10) return none();
   const at::Tensor *x = plain(a[0], 16), *w = plain(a[1], 16), *s = plain(a[2], 16), *b = plain(a[3], 16),
                    *la = plain(a[4], 16), *lb = plain(a[5], 16), *sc = plain(a[6], 4), *ids = plain(a[7], 4);
   if (!x || !w || !s || !b || !la || !lb || !sc || !ids || !is_bf16(*x) || x->dim() < 1 ||
@@ -281,9 +280,8 @@ PyObject* lora(PyObject*, PyObject* const* a, Py_ssize_t na) {
     return none();
   const int64_t group = PyLong_AsLongLong(a[8]), bits = PyLong_AsLongLong(a[9]);
   if (PyErr_Occurred()) return nullptr;
-  const bool general = a[10] == Py_True;
   const int64_t k = x->sizes().back(), m = x->numel() / k, n = w->size(0);
-  if (group <= 0 || bits <= 0 || !weights_match(*w, *s, *b, k, group, bits) || (general && observed())) return none();
+  if (group <= 0 || bits <= 0 || !weights_match(*w, *s, *b, k, group, bits)) return none();
   if (!is_bf16(*la) || !is_bf16(*lb) || la->dim() != 3 || lb->dim() != 3 || la->size(2) != k || lb->size(1) != n ||
       lb->size(0) != la->size(0) || lb->size(2) != la->size(1) || sc->scalar_type() != at::kFloat || sc->dim() != 1 ||
       sc->size(0) != la->size(0) || !is_index(*ids, *x, 1))

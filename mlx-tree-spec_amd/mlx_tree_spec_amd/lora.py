@@ -19,7 +19,7 @@ import torch
 from . import _lib
 from .packed_linear import STATS, QuantizedLinear
 from .qmm import (GENERAL_BITS, GENERAL_GROUP_SIZES, _check_device, _check_format, _check_weights,
-                  _general_kernel_ok, _general_shape_ok, aligned_contiguous, quantized_matmul)
+                  _general_shape_ok, aligned_contiguous, quantized_matmul)
 
 MAX_RANK = 256
 _INDEX_DTYPES = (torch.int32, torch.int64)
@@ -71,17 +71,27 @@ def _native_lora(x, w, scales, biases, lora_a, lora_b, lora_scale, adapters, tra
     if general and (bits not in GENERAL_BITS or group_size not in GENERAL_GROUP_SIZES or k == 0
                     or not _general_shape_ok(x, x.numel() // k, n, k, bits)):
         return None
-    y = _lib.native().lora(x, w, scales, biases, lora_a, lora_b, lora_scale, adapters, group_size, bits, general)
+    y = _lib.native().lora(x, w, scales, biases, lora_a, lora_b, lora_scale, adapters, group_size, bits)
     if type(y) is int:
         _lib.check(y, "quantized_matmul_lora")
     return y
+
+
+def _library_product(x2: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, group_size: int,
+                     bits: int) -> torch.Tensor:
+    """The projection at the sizes at which quantized_matmul dequantizes and multiplies, in bf16 under autocast too: the
+    adapters are added to its words."""
+    if not torch.is_autocast_enabled("cuda"):
+        return quantized_matmul(x2, w, scales, biases, group_size=group_size, bits=bits)
+    with torch.autocast("cuda", enabled=False):
+        return quantized_matmul(x2, w, scales, biases, group_size=group_size, bits=bits)
 
 
 def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
                           lora_a: torch.Tensor, lora_b: torch.Tensor, lora_scale: torch.Tensor,
                           adapters: torch.Tensor, transpose: bool = True, group_size: int = 64, bits: int = 4,
                           mode: str = "affine") -> torch.Tensor:
-    """quantized_matmul with each row's low-rank adapter: bf16 (..., N),
+    """quantized_matmul with each row's low-rank adapter: bf16 (..., N), under autocast to another type too,
 
         y[m] = x[m] @ dequant(w).T + lora_scale[a] * (x[m] @ lora_a[a].T) @ lora_b[a].T,   a = adapters[m].
 
@@ -115,12 +125,12 @@ def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor
     lib = _lib.load()
     workspace = torch.empty((m, rank), dtype=torch.int32, device=dev)
     packed = bits == 4 and group_size == 64 and k % 128 == 0 and n % 16 == 0
-    fused = packed or _general_kernel_ok(x, m, n, k, bits)
+    fused = packed or _general_shape_ok(x, m, n, k, bits)
     w, scales, biases = aligned_contiguous(w), aligned_contiguous(scales), aligned_contiguous(biases)
     if fused:
         y = torch.empty((*x.shape[:-1], n), dtype=torch.bfloat16, device=dev)
-    else:  # the sizes at which quantized_matmul dequantizes and multiplies
-        y = quantized_matmul(x2, w, scales, biases, transpose, group_size, bits, mode).reshape(*x.shape[:-1], n)
+    else:
+        y = _library_product(x2, w, scales, biases, group_size, bits).reshape(*x.shape[:-1], n)
     with torch.cuda.device(dev):
         stream = torch.cuda.current_stream(dev).cuda_stream
         lora = (lora_a.data_ptr(), lora_b.data_ptr(), lora_scale.data_ptr(), adapters.data_ptr(),
