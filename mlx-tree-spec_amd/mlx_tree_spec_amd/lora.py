@@ -19,7 +19,7 @@ import torch
 from . import _lib
 from .packed_linear import STATS, QuantizedLinear
 from .qmm import (GENERAL_BITS, GENERAL_GROUP_SIZES, _check_device, _check_format, _check_weights,
-                  _general_shape_ok, aligned_contiguous, quantized_matmul)
+                  _general_shape_ok, _watched, aligned_contiguous, quantized_matmul)
 
 MAX_RANK = 256
 _INDEX_DTYPES = (torch.int32, torch.int64)
@@ -100,7 +100,9 @@ def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor
     leading shape. A row whose adapter lies outside 0 .. L - 1 (-1, say) has the projection alone, with its bits.
     Both products are summed in fp32 and rounded once (twice at the sizes and formats for which quantized_matmul
     dequantizes and multiplies); x @ lora_a.T is kept to 2^-18 of its value in between. What is not finite in an
-    adapter reaches the rows that use it, as the formula has it, and no other.
+    adapter reaches the rows that use it, as the formula has it, and no other. Nothing sees the call as torch operations;
+    where a library product computes the projection it is refused under a function or dispatch mode or for a tensor
+    subclass, which would see that product alone.
     """
     what = "quantized_matmul_lora"
     y = _native_lora(x, w, scales, biases, lora_a, lora_b, lora_scale, adapters, transpose, group_size, bits, mode)
@@ -130,6 +132,9 @@ def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor
     if fused:
         y = torch.empty((*x.shape[:-1], n), dtype=torch.bfloat16, device=dev)
     else:
+        if _watched(x):
+            raise ValueError(f"[{what}] at this size and format a library product computes the projection: a tensor "
+                             "subclass, a function mode or a dispatch mode would see it without the adapters' part")
         y = _library_product(x2, w, scales, biases, group_size, bits).reshape(*x.shape[:-1], n)
     with torch.cuda.device(dev):
         stream = torch.cuda.current_stream(dev).cuda_stream

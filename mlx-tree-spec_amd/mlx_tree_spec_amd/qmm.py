@@ -131,16 +131,21 @@ def _general_shape_ok(x: torch.Tensor, m: int, n: int, k: int, bits: int) -> boo
     return not (x.requires_grad and torch.is_grad_enabled()) and torch.autograd.forward_ad._current_level < 0
 
 
-def _observed(x: torch.Tensor) -> bool:
-    """Whether something sees or rewrites torch's own operations on x, of which the general path's library
-    product is one: autocast to another type (its result then has that type), a tensor subclass, a function or
-    dispatch mode (the default device's own mode sees nothing of a product)."""
-    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") != torch.bfloat16:
-        return True
+def _watched(x: torch.Tensor) -> bool:
+    """Whether a tensor subclass, a function or a dispatch mode sees torch's operations on x (the default device's
+    own mode sees nothing of a product)."""
     if torch._C._len_torch_function_stack() > 0 and not all(
             isinstance(mode, DeviceContext) for mode in _get_current_function_mode_stack()):
         return True
     return type(x) not in (torch.Tensor, torch.nn.Parameter) or torch._C._len_torch_dispatch_stack() > 0
+
+
+def _observed(x: torch.Tensor) -> bool:
+    """Whether something sees or rewrites torch's own operations on x, of which the general path's library
+    product is one: autocast to another type (its result then has that type), or what _watched names."""
+    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") != torch.bfloat16:
+        return True
+    return _watched(x)
 
 
 def _general_kernel_ok(x: torch.Tensor, m: int, n: int, k: int, bits: int) -> bool:

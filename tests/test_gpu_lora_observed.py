@@ -1,8 +1,13 @@
-"""Adapters under autocast, on every form of the projection (needs an MI355X): the result is bf16 with the bits of the
-plain call."""
+"""Adapters under autocast, function and dispatch modes, on every form of the projection (needs an MI355X): the result is
+bf16 with the bits of the plain call, and where a library product computes the projection, what would see that product
+and not the adapters' is refused."""
+
+import contextlib
 
 import pytest
 import torch
+from torch.overrides import TorchFunctionMode
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from mlx_tree_spec_amd import quantized_matmul_lora
 from test_gpu_lora import check, inputs
@@ -11,6 +16,20 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 # (m, k, n, bits, group, whether a library product computes the projection)
 FORMS = [(7, 256, 96, 4, 64, False), (9, 512, 96, 8, 32, False), (7, 96, 40, 4, 32, True), (300, 128, 77, 8, 64, False)]
+
+
+class Functions(TorchFunctionMode):
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+class Operations(TorchDispatchMode):
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+class Wrapped(torch.Tensor):
+    pass
 
 
 def call(form):
@@ -30,3 +49,43 @@ def test_autocast_and_default_device(form, context):
     with context():
         got = f()
     assert got.dtype == torch.bfloat16 and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("mode", [Functions, Operations])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_modes(form, mode):
+    _, f = call(form)
+    want = f()
+    with mode(), (pytest.raises(ValueError, match="mode") if form[5] else contextlib.nullcontext()):
+        got = f()
+    assert form[5] or torch.equal(got, want)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_subclasses(form):
+    args, f = call(form)
+    want = f()
+    x = args[0].as_subclass(Wrapped)
+    if form[5]:
+        with pytest.raises(ValueError, match="subclass"):
+            f(x)
+    else:
+        assert torch.equal(f(x).as_subclass(torch.Tensor), want)
+
+
+class Counts(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.seen.append(func.overloadpacket.__name__)
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("form", [f for f in FORMS if not f[5]], ids=str)
+def test_nothing_is_seen_in_part(form):
+    _, f = call(form)
+    with Counts() as mode:
+        f()
+    assert not {"linear", "mm", "addmm", "matmul"} & set(mode.seen)
