@@ -64,11 +64,11 @@ const at::Tensor* plain(PyObject* o, size_t align) {
   return t && t->is_contiguous() ? t : nullptr;
 }
 
-// Whether a gradient of one of the inputs is asked for (the Python form raises).
+// Whether a gradient of one of the inputs (or null) is asked for (the Python form raises).
 bool wants_gradient(std::initializer_list<const at::Tensor*> ts) {
   if (!c10::GradMode::is_enabled()) return false;
   for (const at::Tensor* t : ts)
-    if (t->requires_grad()) return true;
+    if (t && t->requires_grad()) return true;
   return false;
 }
 
@@ -276,7 +276,7 @@ PyObject* lora(PyObject*, PyObject* const* a, Py_ssize_t na) {
   const at::Tensor *x = plain(a[0], 16), *w = plain(a[1], 16), *s = plain(a[2], 16), *b = plain(a[3], 16),
                    *la = plain(a[4], 16), *lb = plain(a[5], 16), *sc = plain(a[6], 4), *ids = plain(a[7], 4);
   if (!x || !w || !s || !b || !la || !lb || !sc || !ids || !is_bf16(*x) || x->dim() < 1 ||
-      !same_current_device(*x, {w, s, b, la, lb, sc, ids}) || wants_gradient({x, la, lb, sc}))
+      !same_current_device(*x, {w, s, b, la, lb, sc, ids}) || wants_gradient({x, s, b, la, lb, sc}))
     return none();
   const int64_t group = PyLong_AsLongLong(a[8]), bits = PyLong_AsLongLong(a[9]);
   if (PyErr_Occurred()) return nullptr;
@@ -324,7 +324,7 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t na) {
   const at::Tensor *q = strided(a[0], 16), *k = strided(a[1], 16), *wq = plain(a[2], 16), *wk = plain(a[3], 16),
                    *pos = plain(a[5], 4), *inv = plain(a[6], 4);
   if (!q || !k || !wq || !wk || !pos || !inv || !is_bf16(*q) || !is_bf16(*k) || !is_bf16(*wq) || !is_bf16(*wk) ||
-      q->dim() < 2 || k->dim() != q->dim() || !same_current_device(*q, {k, wq, wk, pos, inv}) || wants_gradient({q, k}))
+      q->dim() < 2 || k->dim() != q->dim() || !same_current_device(*q, {k, wq, wk, pos, inv}) || wants_gradient({q, k, inv}))
     return none();
   const int64_t n = q->dim(), d = q->size(n - 1), p = inv->numel();
   if (q->sizes().slice(0, n - 2) != k->sizes().slice(0, n - 2) || k->size(n - 1) != d || wq->dim() != 1 || wk->dim() != 1 ||
@@ -365,7 +365,7 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t na) {
   if (na != 6) return none();
   const at::Tensor *l = strided(a[0], 2), *u = plain(a[1], 4);
   if (!l || !u || !is_bf16(*l) || l->dim() < 1 || u->scalar_type() != at::kFloat ||
-      u->sizes() != l->sizes().slice(0, l->dim() - 1) || wants_gradient({l}))
+      u->sizes() != l->sizes().slice(0, l->dim() - 1))
     return none();
   const int64_t n = l->dim(), v = l->size(n - 1), m = l->numel() / v;
   const int64_t stride = n == 1 ? v : l->stride(n - 2);
@@ -380,6 +380,7 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t na) {
   if ((!t && !(tv >= 0 && tv <= 1e30)) || (!k && !(kv >= 0 && kv < 2147483648.0)) || (!p && !(pv > 0 && pv <= 1)) ||
       (!mp && !(mv >= 0 && mv <= 1)))
     return none();  // (out of range: the Python form raises)
+  if (wants_gradient({l, u, t, p, mp})) return none();
   for (const at::Tensor* x : {u, t, k, p, mp})
     if (x && x->device() != l->device()) return none();
   if (!same_current_device(*l, {u})) return none();

@@ -44,7 +44,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     heads are read in place); q_weight, k_weight bf16 [D]; positions int32 or int64 of the leading shape; inv_freq
     fp32 or fp64 [P], 2 P <= D: pair i turns by positions * inv_freq[i]. Pairs are (i, i + P), or (2 i, 2 i + 1)
     when `interleaved` (MLX's traditional=True); values past 2 P are normed only. Norm and rotation are fp32 with
-    angles reduced in fp64, so far positions turn by what inv_freq says, and the result is rounded once.
+    angles reduced in fp64, so far positions turn by what inv_freq says, and the result is rounded once. q, k and
+    inv_freq may not ask for a gradient; the weights, which a norm module holds as parameters, may and get none, as in
+    add_rms_norm.
     """
     what = "qk_norm_rope"
     if q.is_cuda:
@@ -53,7 +55,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
             _lib.check(out, what)
         if out is not None:
             return out
-    no_gradient(what, q=q, k=k)
+    no_gradient(what, q=q, k=k, inv_freq=inv_freq)
     for name, t in (("q", q), ("k", k), ("q_weight", q_weight), ("k_weight", k_weight)):
         if t.dtype != torch.bfloat16:
             raise ValueError(f"[{what}] {name} must be bfloat16, got {t.dtype}")

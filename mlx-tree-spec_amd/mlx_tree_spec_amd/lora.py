@@ -25,11 +25,12 @@ MAX_RANK = 256
 _INDEX_DTYPES = (torch.int32, torch.int64)
 
 
-def no_gradient(what: str, **tensors: torch.Tensor) -> None:
-    """Raises where a gradient of an input is asked for: the kernels have none, and would cut it unseen."""
+def no_gradient(what: str, **inputs) -> None:
+    """Raises where a gradient of an input is asked for: the kernels have none, and would cut it unseen. (What is
+    no tensor is passed over.)"""
     if torch.is_grad_enabled():
-        for name, t in tensors.items():
-            if t.requires_grad:
+        for name, t in inputs.items():
+            if isinstance(t, torch.Tensor) and t.requires_grad:
                 raise ValueError(f"[{what}] {name} requires a gradient, which this operator does not have; "
                                  "call it under torch.no_grad() or detach the tensor")
 
@@ -109,7 +110,7 @@ def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor
     if y is not None:
         return y
     _check_format(group_size, bits, transpose, mode, general=True)
-    no_gradient(what, x=x, lora_a=lora_a, lora_b=lora_b, lora_scale=lora_scale)
+    no_gradient(what, x=x, scales=scales, biases=biases, lora_a=lora_a, lora_b=lora_b, lora_scale=lora_scale)
     if x.dtype != torch.bfloat16:
         raise ValueError(f"[{what}] x must be bfloat16, got {x.dtype}")
     if x.dim() < 1:

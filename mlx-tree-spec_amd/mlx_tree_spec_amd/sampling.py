@@ -53,7 +53,7 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0
             _lib.check(out, what)
         if out is not None:
             return out
-    no_gradient(what, logits=logits)
+    no_gradient(what, logits=logits, uniform=uniform, temperature=temperature, top_p=top_p, min_p=min_p)
     if logits.dtype != torch.bfloat16:
         raise ValueError(f"[{what}] logits must be bfloat16, got {logits.dtype}")
     if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_VOCAB:
