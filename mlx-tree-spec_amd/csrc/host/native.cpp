@@ -64,8 +64,15 @@ const at::Tensor* plain(PyObject* o, size_t align) {
   return t && t->is_contiguous() ? t : nullptr;
 }
 
-// Whether a gradient of one of the inputs (or null) is asked for (the Python form raises).
+// Whether one of the inputs (or null) carries a tangent of forward mode (the Python form raises).
+bool has_tangent(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    if (t && t->_fw_grad(0).defined()) return true;
+  return false;
+}
+// Whether a gradient of one of them is asked for, in either mode (the Python form raises).
 bool wants_gradient(std::initializer_list<const at::Tensor*> ts) {
+  if (has_tangent(ts)) return true;
   if (!c10::GradMode::is_enabled()) return false;
   for (const at::Tensor* t : ts)
     if (t && t->requires_grad()) return true;
@@ -324,7 +331,8 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t na) {
   const at::Tensor *q = strided(a[0], 16), *k = strided(a[1], 16), *wq = plain(a[2], 16), *wk = plain(a[3], 16),
                    *pos = plain(a[5], 4), *inv = plain(a[6], 4);
   if (!q || !k || !wq || !wk || !pos || !inv || !is_bf16(*q) || !is_bf16(*k) || !is_bf16(*wq) || !is_bf16(*wk) ||
-      q->dim() < 2 || k->dim() != q->dim() || !same_current_device(*q, {k, wq, wk, pos, inv}) || wants_gradient({q, k, inv}))
+      q->dim() < 2 || k->dim() != q->dim() || !same_current_device(*q, {k, wq, wk, pos, inv}) || wants_gradient({q, k, inv}) ||
+      has_tangent({wq, wk}))
     return none();
   const int64_t n = q->dim(), d = q->size(n - 1), p = inv->numel();
   if (q->sizes().slice(0, n - 2) != k->sizes().slice(0, n - 2) || k->size(n - 1) != d || wq->dim() != 1 || wk->dim() != 1 ||

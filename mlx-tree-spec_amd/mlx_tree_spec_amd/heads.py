@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import _lib
-from .lora import check_index, no_gradient
+from .lora import check_index, no_gradient, no_tangent
 from .qmm import _check_device, aligned_contiguous
 
 MAX_DIM = 512
@@ -56,6 +56,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
         if out is not None:
             return out
     no_gradient(what, q=q, k=k, inv_freq=inv_freq)
+    no_tangent(what, q_weight=q_weight, k_weight=k_weight)
     for name, t in (("q", q), ("k", k), ("q_weight", q_weight), ("k_weight", k_weight)):
         if t.dtype != torch.bfloat16:
             raise ValueError(f"[{what}] {name} must be bfloat16, got {t.dtype}")

@@ -15,6 +15,7 @@ bfloat16 on a HIP device; there is no CPU path, and no gradient.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .packed_linear import STATS, QuantizedLinear
@@ -25,9 +26,18 @@ MAX_RANK = 256
 _INDEX_DTYPES = (torch.int32, torch.int64)
 
 
+def no_tangent(what: str, **inputs) -> None:
+    """Raises where an input carries a tangent of forward mode, which the kernels would drop unseen."""
+    if forward_ad._current_level >= 0:
+        for name, t in inputs.items():
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"[{what}] {name} carries a tangent, which this operator does not have; detach the tensor")
+
+
 def no_gradient(what: str, **inputs) -> None:
-    """Raises where a gradient of an input is asked for: the kernels have none, and would cut it unseen. (What is
-    no tensor is passed over.)"""
+    """Raises where a gradient of an input is asked for, in either mode: the kernels have none, and would cut it
+    unseen. (What is no tensor is passed over.)"""
+    no_tangent(what, **inputs)
     if torch.is_grad_enabled():
         for name, t in inputs.items():
             if isinstance(t, torch.Tensor) and t.requires_grad:

@@ -3,8 +3,9 @@ MI355X)."""
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from test_requests_gradients import CASES, IDS
+from test_requests_gradients import CASES, IDS, TANGENT_IDS, TANGENTS
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +25,13 @@ def test_inputs_that_require_a_gradient(op, args, name):
         got = op(**a)
     for x, y in zip(*(t if isinstance(t, tuple) else (t,) for t in (got, want))):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("op,args,name", TANGENTS, ids=TANGENT_IDS)
+def test_inputs_with_a_tangent(op, args, name):
+    a = on_gpu(args())
+    with forward_ad.dual_level():
+        op(**a)
+        dual = {**a, name: forward_ad.make_dual(a[name], torch.ones_like(a[name]))}
+        with torch.no_grad(), pytest.raises(ValueError, match=f"{name} carries a tangent"):
+            op(**dual)

@@ -3,6 +3,7 @@ norms' weights (CPU only: each call ends before any GPU work)."""
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from mlx_tree_spec_amd import qk_norm_rope, quantized_matmul_lora, sample
 from test_requests_host import lora_args, rope_args, z
@@ -30,3 +31,20 @@ def test_inputs_that_require_a_gradient(op, args, name):
     a[name] = a[name] * 2  # not a leaf
     with pytest.raises(ValueError, match=f"{name} requires a gradient"):
         op(**a)
+
+
+TANGENTS = CASES + [(qk_norm_rope, rope_args, n) for n in ("q_weight", "k_weight")]
+TANGENT_IDS = [f"{f.__name__}-{n}" for f, _, n in TANGENTS]
+
+
+@pytest.mark.parametrize("op,args,name", TANGENTS, ids=TANGENT_IDS)
+def test_inputs_with_a_tangent(op, args, name):
+    a = args()
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="no CPU path"):
+            op(**a)
+        dual = {**a, name: forward_ad.make_dual(a[name], torch.ones_like(a[name]))}
+        with torch.no_grad(), pytest.raises(ValueError, match=f"{name} carries a tangent"):
+            op(**dual)
+    with pytest.raises(ValueError, match="carries a tangent"):
+        torch.func.jvp(lambda t: op(**{**a, name: t}), (a[name],), (torch.ones_like(a[name]),))
