@@ -94,12 +94,13 @@ def attention_inputs(x: torch.Tensor, layer: AttentionInputs, positions: torch.T
     position, v (..., kv_heads, D), gate (..., heads, D) or None. `adapters` (one per row) goes to the projections that
     are LoRALinear."""
     lead, d = x.shape[:-1], layer.head_dim
-    q = _project(layer.q_proj, x, adapters).reshape(*lead, layer.heads, -1)
+    width = 2 * d if layer.gated else d
+    q = _project(layer.q_proj, x, adapters)
+    if q.shape[-1] != layer.heads * width:
+        raise ValueError(f"[attention_inputs] q_proj gives {q.shape[-1]} values, expected {layer.heads} heads of {width}")
+    q = q.reshape(*lead, layer.heads, width)
     k = _project(layer.k_proj, x, adapters).reshape(*lead, layer.kv_heads, d)
     v = _project(layer.v_proj, x, adapters).reshape(*lead, layer.kv_heads, d)
-    if q.shape[-1] != (2 * d if layer.gated else d):
-        raise ValueError(f"[attention_inputs] q_proj gives {layer.heads} heads {q.shape[-1]} values each, expected "
-                         f"{2 * d if layer.gated else d}")
     gate = q[..., d:] if layer.gated else None
     q, k = qk_norm_rope(q[..., :d] if layer.gated else q, k, layer.q_norm.weight, layer.k_norm.weight,
                         _norm_eps(layer.q_norm), positions, layer.inv_freq, interleaved=layer.interleaved)
