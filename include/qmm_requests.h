@@ -84,7 +84,8 @@ int qmm4_qk_norm_rope_bf16(const void* q, int64_t q_row, int64_t q_head, const v
  *   Requires 1 <= V <= QMM4_SAMPLE_MAX_VOCAB, M <= 2^20, row_stride >= V (M > 1), logits 2-byte, fp32 and int32
  *   arrays 4-byte, tokens 8-byte aligned. Deterministic.
  */
-int64_t qmm4_sample_workspace(int64_t M, int64_t V); /* on the current device; negative: an error code */
+/* On the current device, at most 1025 MiB (4 bytes a logit up to there); negative: an error code. */
+int64_t qmm4_sample_workspace(int64_t M, int64_t V);
 int qmm4_sample_bf16(const void* logits, int64_t M, int64_t V, int64_t row_stride, const float* uniform,
                      const float* temperature, float temperature_value, const int32_t* top_k, int32_t top_k_value,
                      const float* top_p, float top_p_value, const float* min_p, float min_p_value, int64_t* tokens,

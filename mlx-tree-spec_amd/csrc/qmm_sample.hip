@@ -43,7 +43,9 @@ constexpr int kNoRank = 0x10000;
 constexpr int kMaxSlice = 32768;   // logits per slice: its counts fit 16 bits
 constexpr int kMinSlice = 4096;
 constexpr int kMaxSlices = 512;
-constexpr int kMaxBatch = 256;     // rows per launch: bounds the workspace
+constexpr int kMaxBatch = 256;     // rows per launch, and
+constexpr int kMaxLogits = 1 << 28;  // their logits: bound the lists at 1 GiB (any row fits; past 2^20 logits a row:
+                                     // 64 x 2^24 1.27 -> 1.82 ms, with 1 instead of 4 GiB)
 
 // A rank is a bf16 value's number in falling order: 0x7FFF - b for bits b of a positive value, b - 1 of a negative one
 // (0x7FFF for both zeros). -infinity (kLastRank + 1) and NaN lie either side of kFirstRank .. kLastRank.
@@ -742,7 +744,8 @@ struct Plan {
 // Slices of a row: enough workgroups (one per CU: the histogram takes most of its LDS) for the GPU, at least 4096
 // logits each.
 Plan plan_of(int64_t M, int V, int cus) {
-  const int64_t batch = M < kMaxBatch ? M : kMaxBatch;
+  const int64_t most = kMaxLogits / V < kMaxBatch ? kMaxLogits / V : kMaxBatch;
+  const int64_t batch = M < most ? M : most;
   int64_t s = cus / batch;
   if (s > kWaves) s = kWaves;  // (a list to each wave of the merge: 37 slices of one row took it 7 us, 16 take 3)
   if (s > V / kMinSlice) s = V / kMinSlice;
