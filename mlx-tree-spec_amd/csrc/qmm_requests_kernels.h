@@ -67,7 +67,6 @@ template <class T>
 struct PerRow {
   const T* p;
   T value;
-  __device__ __forceinline__ T operator[](int64_t m) const { return p ? p[m] : value; }
 };
 struct SampleParams {
   const uint16_t* logits;
