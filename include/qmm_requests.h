@@ -32,8 +32,8 @@ extern "C" {
  *   N % 16 == 0), else of qmm_affine_general_bf16; lora_a: bf16 [L, R, K]; lora_b: bf16 [L, N, R]; lora_scale: fp32
  *   [L]; adapters: int32 or int64 [M] (adapter_bits 32 or 64).
  *   The sums of both products are fp32 and rounded once; between its factors the second one is kept (in `workspace`) to
- *   2^-18 of its value. What is not finite in x, lora_a, lora_b or lora_scale gives what the formula gives, in the rows
- *   that use it and in no other. Requires R % 8 == 0, 8 <= R <= QMM4_LORA_MAX_RANK, L <= 2^30, M <= 2^26, lora_a,
+ *   2^-18 of its value. What is not finite in x, lora_a or lora_b gives what the formula gives, in the rows that use
+ *   it and in no other (an infinite lora_scale: infinities or NaN in its rows). Requires R % 8 == 0, 8 <= R <= QMM4_LORA_MAX_RANK, L <= 2^30, M <= 2^26, lora_a,
  *   lora_b and workspace 16-byte aligned, lora_scale 4-byte, adapters by their own size. M == 0 or N == 0 is a no-op.
  *   Deterministic.
  */
@@ -56,8 +56,8 @@ int qmm4_lora_add_bf16(const void* x, const void* lora_a, const void* lora_b, co
  * between the q/k projections and attention (src/mlx_tree_spec/tree_verify.py:311-328). Per head of D values
  *   n = x / sqrt(mean(x^2) + eps) * weight,   angle_i = positions[m] * inv_freq[i], i < P,
  *   (n[i], n[i + P]) -> (n[i] cos - n[i + P] sin, n[i + P] cos + n[i] sin)       (interleaved: n[2i], n[2i + 1])
- * and n past 2 P unrotated; fp32 throughout (squares too: a mean square under 2^-126 beside eps 0 is lost; angles
- * reduced in 64 bits), one rounding to bf16.
+ * and n past 2 P unrotated; fp32 throughout (squares too: a sum of squares past 2^128 gives zeros, a mean square
+ * under 2^-126 beside eps 0 is lost; angles reduced in 64 bits), one rounding to bf16.
  *   q: bf16, element (m, h, d) at q[m * q_row + h * q_head + d], k alike (strides in elements, multiples of 8);
  *   q_weight, k_weight: bf16 [D]; positions: int32 or int64 [M]; inv_freq: fp32 or fp64 [P]; q_out: bf16
  *   [M, Hq, D], k_out: bf16 [M, Hk, D], contiguous, overlapping no input.

@@ -23,8 +23,9 @@
 //
 // What bounds it: a row's steps follow each other in one workgroup, each a few hundred ns of LDS round trips and
 // barriers, and a CU gets through 2400 vector instructions of its waves each a microsecond; both kernels are kept to
-// few instructions per value. On the GPU: 1 x 151936 19.7 us, 32 x 151936 (all settings) 22.8 us, 200 x 32001 14.2 us,
-// of which the counting takes 6, 7 and 8. The prefix after prefix of counts, masses and what is kept that was here
+// few instructions per value. On the GPU: 1 x 151936 20.1 us, 32 x 151936 (all settings) 22.8 us, 200 x 32001 14.4 us
+// (13.4 in a row of eager calls). Of these the count kernel takes 6.8 and 7.7, and the counting of the last, inside the
+// pick kernel, 4.5. The prefix after prefix of counts, masses and what is kept that was here
 // first, with 64 words to a look, took 27, 30 and 18 us.
 #include <type_traits>
 
