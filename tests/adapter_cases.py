@@ -26,6 +26,11 @@ ROWSPLIT = [
     (8, 512, 2048, 1, 4, "small", False),
     (9, 12288, 2048, 4, 4, "slots", False),
     (16, 5120, 50304, 4, 5, "slots", False),
+    (4, 640, 10240, 1, 5, "slots", False),
+    (1, 12288, 5120, 2, 4, "slots", False),
+    (1, 6400, 176160, 2, 5, "slots", False),
+    (3, 5120, 248320, 1, 4, "groups", False),
+    (6, 2560, 7168, 2, 5, "slots", False),
     (9, 512, 589824, 1, 4, "own", False),      # whole blocks to each wave
 ]
 
@@ -46,3 +51,20 @@ GEMM = [
     (129, 2048, 10240, "stream-K 128x128"),      # in units of 4 K steps
     (300, 640, 4112, "stream-K 128x128, plain"),
 ]
+
+# (M, K, N, variant of the row-phase kernel, K split): 28 variants less those that no shape takes.
+ROWPHASE = [
+    (33, 1024, 17408, 2, True), (33, 512, 99984, 2, False), (9, 20480, 8192, 3, True), (17, 4096, 17408, 4, True),
+    (48, 2048, 17408, 5, True), (12, 20480, 512, 6, True), (24, 1024, 272, 7, True), (17, 512, 256, 7, False),
+    (64, 512, 272, 8, True), (33, 512, 17408, 8, False), (9, 20480, 1024, 9, True), (24, 8192, 2064, 10, True),
+    (12, 5120, 99984, 11, False), (17, 512, 99984, 12, False), (72, 2048, 17408, 13, True), (65, 512, 272, 14, True),
+    (72, 512, 17408, 14, False), (81, 2048, 17408, 15, True), (96, 512, 272, 16, True), (90, 512, 17408, 16, False),
+    (100, 2048, 17408, 17, True), (112, 512, 272, 18, True), (97, 512, 17408, 18, False), (120, 512, 272, 19, True),
+    (24, 512, 32784, 20, False), (48, 512, 32784, 21, False), (17, 512, 65984, 22, False), (64, 512, 65984, 23, False),
+    (65, 512, 32784, 24, False), (90, 512, 32784, 25, False), (9, 5120, 65984, 26, False), (12, 8192, 32784, 27, False),
+]
+
+# (M, K, N): what no other kernel takes, up to 64 rows. From 5 rows K that is not a multiple of 512 (the verify kernel),
+# up to 4 rows too little work for the row-split kernel (the skinny kernel: K in steps of 1, 2 and 4 x 128).
+VERIFY = [(6, 128, 48), (9, 384, 272), (16, 768, 2064), (17, 1152, 528), (32, 1280, 4112), (33, 640, 528), (64, 2432, 5136)]
+SKINNY = [(1, 128, 16), (3, 2176, 5120), (4, 256, 5136), (2, 768, 272), (1, 20480, 2048), (3, 20480, 48), (4, 20480, 528)]

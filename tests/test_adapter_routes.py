@@ -52,3 +52,18 @@ def test_gemm_cases_take_their_routes(planner_exe):  # noqa: F811
     plans = query(planner_exe, [f"gemm {m} {n} {k} {C.CUS}" for m, n, k in shapes])
     for (m, k, n, form), p in zip(C.GEMM, plans):
         assert gemm_form(m, k, n, p) == form, (m, k, n, p)
+
+
+def test_rowphase_cases_take_their_variants(planner_exe):  # noqa: F811
+    shapes = [(m, n, k) for m, k, n, *_ in C.ROWPHASE]
+    assert dispatch_route(planner_exe, shapes) == ["row-phase"] * len(shapes)
+    plans = query(planner_exe, [f"rowphase {m} {n} {k} {C.CUS}" for m, n, k in shapes])
+    for (m, k, n, variant, split), p in zip(C.ROWPHASE, plans):
+        assert (int(p["variant"]), int(p["S"]) > 1) == (variant, split), (m, k, n, p)
+    assert {case[3] for case in C.ROWPHASE} == set(range(2, 28))
+
+
+def test_other_cases_take_the_remaining_kernels(planner_exe):  # noqa: F811
+    shapes = [(m, n, k) for m, k, n in C.VERIFY + C.SKINNY]
+    assert dispatch_route(planner_exe, shapes) == ["other"] * len(shapes)
+    assert all(m >= 5 for m, *_ in C.VERIFY) and all(m <= 4 for m, *_ in C.SKINNY)
