@@ -143,7 +143,7 @@ def quantized_matmul_lora(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor
     if fused:
         y = torch.empty((*x.shape[:-1], n), dtype=torch.bfloat16, device=dev)
     else:
-        if _watched(x):
+        if m * n * count > 0 and _watched(x):
             raise ValueError(f"[{what}] at this size and format a library product computes the projection: a tensor "
                              "subclass, a function mode or a dispatch mode would see it without the adapters' part")
         y = _library_product(x2, w, scales, biases, group_size, bits).reshape(*x.shape[:-1], n)

@@ -89,3 +89,13 @@ def test_nothing_is_seen_in_part(form):
     with Counts() as mode:
         f()
     assert not {"linear", "mm", "addmm", "matmul"} & set(mode.seen)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_modes_where_there_is_nothing_to_add(form):
+    m, k, n, bits, group, _ = form
+    x, w, s, b, la, lb, scale, ids = inputs(m, k, n, 16, 3, m + n, bits, group)
+    with Operations():
+        no_rows = quantized_matmul_lora(x[:0], w, s, b, la, lb, scale, ids[:0], group_size=group, bits=bits)
+        no_adapters = quantized_matmul_lora(x, w, s, b, la[:0], lb[:0], scale[:0], ids, group_size=group, bits=bits)
+    assert no_rows.shape == (0, n) and no_adapters.shape == (m, n)
