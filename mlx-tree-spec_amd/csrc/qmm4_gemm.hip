@@ -1015,7 +1015,7 @@ void gemm_ws_kernel(GemmParams P) {
     };
     // LORA: step l of the adapters' products into stage st. A thread's t: row pt / 8 + 32 i, 4 j from 4 (pt % 8); its B:
     // column pt / 4 + 64 i, 8 j from 8 (pt % 4). What lies past the rows, the columns or R, and t of rows with another
-    // adapter, reads zero.
+    // adapter, reads zero; what is not finite becomes zero and is noted.
     [[maybe_unused]] auto put_lora = [&](int l, int st) __attribute__((always_inline)) {
       constexpr uint32_t kOut = 0x80000000u;
       const LoraAdd& E = P.lora;
