@@ -27,6 +27,7 @@
 #include <cstdint>
 
 #include "qmm4.h"
+#include "qmm_cache.h"
 #include "qmm_general.h"
 #include "qmm_requests.h"
 
@@ -41,6 +42,11 @@ decltype(&qmm4_affine_lora_bf16) p_lora = nullptr;
 decltype(&qmm4_qk_norm_rope_bf16) p_rope = nullptr;
 decltype(&qmm4_sample_bf16) p_sample = nullptr;
 decltype(&qmm4_sample_workspace) p_sample_workspace = nullptr;
+decltype(&qmm4_cache_plan_words) p_plan_words = nullptr;
+decltype(&qmm4_cache_step) p_cache_step = nullptr;
+decltype(&qmm4_store_kv_bf16) p_store_kv = nullptr;
+decltype(&qmm4_paged_workspace) p_paged_workspace = nullptr;
+decltype(&qmm4_paged_attention_bf16) p_paged = nullptr;
 
 // A plain tensor on a HIP device with data on an `align`-byte boundary, or null: no subclass, no wrapper of a
 // transform or a mode, nothing whose storage is not its own.
@@ -409,10 +415,169 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t na) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(affine, gate_up, general, norm, norm_qmm, lora, rope, sample, sample_workspace): the addresses of the loaded
-// library's functions.
+// A tensor of `type` and `sizes`.
+bool is_table(const at::Tensor& t, at::ScalarType type, at::IntArrayRef sizes) {
+  return t.scalar_type() == type && t.sizes() == sizes;
+}
+
+// Integers from..from + N - 1 of a call's arguments. False: not all are integers.
+template <int N>
+bool integers(PyObject* const* a, int from, int64_t (&out)[N]) {
+  for (int i = 0; i < N; ++i) {
+    if (!PyLong_CheckExact(a[from + i])) return false;
+    out[i] = PyLong_AsLongLong(a[from + i]);
+    if (out[i] == -1 && PyErr_Occurred()) {
+      PyErr_Clear();
+      return false;
+    }
+  }
+  return true;
+}
+
+// An optional tensor: null where the argument is None. False: neither.
+bool optional(PyObject* o, size_t align, const at::Tensor** t) {
+  *t = nullptr;
+  return o == Py_None || (*t = plain(o, align));
+}
+
+// cache_step(lengths, block_table, free_pages, free_count, rows, total, page_size, heads, kv_heads, head_dim, base, keep,
+// max_rows): (slots, positions, request, plan) of step_tables_.
+PyObject* cache_step(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  if (na != 13) return none();
+  const at::Tensor *len = plain(a[0], 4), *tab = plain(a[1], 4), *fp = plain(a[2], 4), *fc = plain(a[3], 4), *rows = plain(a[4], 4);
+  const at::Tensor *base, *keep;
+  int64_t v[5], most[1];  // total, page_size, heads, kv_heads, head_dim; max_rows
+  if (!len || !tab || !fp || !fc || !rows || !integers(a, 5, v) || !optional(a[10], 4, &base) || !optional(a[11], 1, &keep) ||
+      !integers(a, 12, most) || len->dim() != 1 || tab->dim() != 2 || fp->dim() != 1)
+    return none();
+  const int64_t r = len->size(0), capacity = tab->size(1), pages = fp->size(0), total = v[0];
+  if (total <= 0 || !is_table(*len, at::kInt, {r}) || !is_table(*tab, at::kInt, {r, capacity}) || !is_table(*fp, at::kInt, {pages}) ||
+      !is_table(*fc, at::kInt, {1}) || !is_table(*rows, at::kInt, {r}) || (base && !is_table(*base, at::kInt, {r})) ||
+      (keep && !is_table(*keep, at::kBool, {total})) ||
+      (v[4] != 64 && v[4] != 96 && v[4] != 128 && v[4] != 192 && v[4] != 256))
+    return none();
+  for (const at::Tensor* t : {base, keep})
+    if (t && t->device() != len->device()) return none();
+  if (!same_current_device(*len, {tab, fp, fc, rows})) return none();
+  const int64_t words = p_plan_words(r, v[2], v[3], v[4], most[0]);
+  if (words < 0 || total > QMM4_CACHE_MAX_ROWS) return none();  // (the Python form raises)
+  at::Tensor slots = fresh({total}, at::kInt, *len), positions = fresh({total}, at::kInt, *len),
+             request = fresh({total}, at::kInt, *len), plan;
+  if (!keep) plan = fresh({words}, at::kInt, *len);
+  auto i32 = [](const at::Tensor* t) { return t ? static_cast<int32_t*>(ptr(*t)) : nullptr; };
+  auto out = [](const at::Tensor& t) { return static_cast<int32_t*>(out_ptr(t)); };
+  int32_t *sp = out(slots), *pp = out(positions), *rp = out(request), *plp = keep ? nullptr : out(plan);
+  if (!sp || !pp || !rp || (!keep && !plp)) return none();
+  int32_t *lenp = i32(len), *tabp = i32(tab), *fpp = i32(fp), *fcp = i32(fc), *rowsp = i32(rows), *basep = i32(base);
+  const uint8_t* keepp = keep ? static_cast<const uint8_t*>(ptr(*keep)) : nullptr;
+  void* st = stream_of(*len);
+  int rc;
+  CALL(rc, p_cache_step(lenp, tabp, fpp, fcp, rowsp, basep, keepp, sp, pp, rp, plp, r, capacity, pages, total, most[0], v[1],
+                        v[2], v[3], v[4], st))
+  if (rc != 0) return PyLong_FromLong(rc);
+  PyObject* o = PyTuple_New(4);
+  if (!o) return nullptr;
+  PyTuple_SET_ITEM(o, 0, THPVariable_Wrap(std::move(slots)));
+  PyTuple_SET_ITEM(o, 1, THPVariable_Wrap(std::move(positions)));
+  PyTuple_SET_ITEM(o, 2, THPVariable_Wrap(std::move(request)));
+  PyTuple_SET_ITEM(o, 3, keep ? none() : THPVariable_Wrap(std::move(plan)));
+  return o;
+  END_HANDLE_TH_ERRORS
+}
+
+// A layer's cache (keys, values, key_scales, value_scales): a KVCache of these arguments.
+struct Cache {
+  const at::Tensor *keys, *values, *ks, *vs;
+  int64_t pages, heads, dim, page;
+  int bits;
+  bool read(PyObject* const* a) {
+    keys = plain(a[0], 16);
+    values = plain(a[1], 16);
+    if (!keys || !values || !optional(a[2], 16, &ks) || !optional(a[3], 16, &vs) || keys->dim() != 5) return false;
+    const bool codes = keys->scalar_type() == at::kChar;
+    if (!codes && !is_bf16(*keys)) return false;
+    bits = codes ? 8 : 16;
+    const int64_t e = codes ? 16 : 8;
+    pages = keys->size(0);
+    heads = keys->size(1);
+    dim = keys->size(2) * e;
+    page = keys->size(3);
+    if (keys->size(4) != e || page % e != 0 || codes != (ks != nullptr) || codes != (vs != nullptr) ||
+        !is_table(*values, keys->scalar_type(), {pages, heads, page / e, dim, e}))
+      return false;
+    for (const at::Tensor* t : {ks, vs})
+      if (t && (!is_table(*t, at::kFloat, {pages, heads, page}) || t->device() != keys->device())) return false;
+    return !wants_gradient({keys, values, ks, vs});
+  }
+};
+
+// store_kv(k, v, keys, values, key_scales, value_scales, slots): store_kv_ (0).
+PyObject* store_kv(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  if (na != 7) return none();
+  const at::Tensor *k = strided(a[0], 16), *v = strided(a[1], 16), *slots = plain(a[6], 4);
+  Cache c;
+  if (!k || !v || !slots || !c.read(a + 2) || !is_bf16(*k) || !is_bf16(*v) || k->dim() != 3 || v->sizes() != k->sizes() ||
+      k->size(1) != c.heads || k->size(2) != c.dim || !is_table(*slots, at::kInt, {k->size(0)}) ||
+      !same_current_device(*k, {v, slots, c.keys, c.values}) || wants_gradient({k, v}))
+    return none();
+  int64_t m, mv, kr, kh, vr, vh;
+  if (!heads(*k, &m, &kr, &kh) || !heads(*v, &mv, &vr, &vh)) return none();
+  void *st = stream_of(*k), *kp = ptr(*k), *vp = ptr(*v), *keys = ptr(*c.keys), *values = ptr(*c.values);
+  const int32_t* sp = static_cast<const int32_t*>(ptr(*slots));
+  float *ks = c.ks ? static_cast<float*>(ptr(*c.ks)) : nullptr, *vs = c.vs ? static_cast<float*>(ptr(*c.vs)) : nullptr;
+  int rc;
+  CALL(rc, p_store_kv(kp, kr, kh, vp, vr, vh, sp, keys, values, ks, vs, m, c.heads, c.dim, c.pages, c.page, c.bits, st))
+  return PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged(q, keys, values, key_scales, value_scales, block_table, request, plan, heads, kv_heads, head_dim, max_rows, page_size,
+// scale, ancestors, gate): paged_attention's output.
+PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  if (na != 16 || !PyFloat_CheckExact(a[13])) return none();
+  const at::Tensor *q = strided(a[0], 16), *tab = plain(a[5], 4), *req = plain(a[6], 4), *plan = plain(a[7], 4), *anc;
+  const at::Tensor* gate = a[15] == Py_None ? nullptr : strided(a[15], 16);
+  Cache c;
+  int64_t v[5];  // heads, kv_heads, head_dim, max_rows, page_size
+  if (!q || !tab || !req || !plan || (a[15] != Py_None && !gate) || !c.read(a + 1) || !optional(a[14], 8, &anc) ||
+      !integers(a, 8, v) || !is_bf16(*q) || q->dim() != 3 || tab->dim() != 2)
+    return none();
+  const int64_t m = q->size(0), r = tab->size(0), capacity = tab->size(1);
+  if (q->size(1) != v[0] || q->size(2) != c.dim || v[1] != c.heads || v[2] != c.dim || v[4] != c.page ||
+      !is_table(*tab, at::kInt, {r, capacity}) || !is_table(*req, at::kInt, {m}) || plan->scalar_type() != at::kInt ||
+      (anc && !is_table(*anc, at::kLong, {m})) || (gate && (!is_bf16(*gate) || gate->sizes() != q->sizes())) ||
+      !same_current_device(*q, {tab, req, plan, c.keys, c.values}) || wants_gradient({q, gate}))
+    return none();
+  for (const at::Tensor* t : {anc, gate})
+    if (t && t->device() != q->device()) return none();
+  int64_t mq, qr, qh, gr = 0, gh = 0;
+  if (!heads(*q, &mq, &qr, &qh) || (gate && !heads(*gate, &mq, &gr, &gh))) return none();
+  const int64_t bytes = p_paged_workspace(m, r, v[0], v[1], v[2], v[3]);
+  if (bytes < 0) return PyLong_FromLong((long)bytes);
+  at::Tensor out = fresh(q->sizes(), at::kBFloat16, *q), ws = fresh({bytes}, at::kByte, *q);
+  void *op = out_ptr(out), *wp = out_ptr(ws), *st = stream_of(*q), *qp = ptr(*q), *keys = ptr(*c.keys), *values = ptr(*c.values),
+       *gp = gate ? ptr(*gate) : nullptr;
+  if (!op || !wp) return none();
+  const float *ks = c.ks ? static_cast<const float*>(ptr(*c.ks)) : nullptr,
+              *vs = c.vs ? static_cast<const float*>(ptr(*c.vs)) : nullptr;
+  const int32_t *tabp = static_cast<const int32_t*>(ptr(*tab)), *reqp = static_cast<const int32_t*>(ptr(*req)),
+                *planp = static_cast<const int32_t*>(ptr(*plan));
+  const int64_t* ancp = anc ? static_cast<const int64_t*>(ptr(*anc)) : nullptr;
+  const float scale = (float)PyFloat_AS_DOUBLE(a[13]);
+  int rc;
+  CALL(rc, p_paged(qp, qr, qh, keys, values, ks, vs, tabp, reqp, planp, ancp, gp, gr, gh, op, wp, scale, m, r, v[0], v[1], v[2],
+                   c.pages, c.page, capacity, v[3], c.bits, st))
+  return rc == 0 ? THPVariable_Wrap(std::move(out)) : PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(affine, gate_up, general, norm, norm_qmm, lora, rope, sample, sample_workspace, cache_plan_words, cache_step, store_kv,
+// paged_workspace, paged_attention): the addresses of the loaded library's functions.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t na) {
-  constexpr int kFunctions = 9;
+  constexpr int kFunctions = 14;
   if (na != kFunctions) {
     PyErr_Format(PyExc_TypeError, "bind takes %d addresses", kFunctions);
     return nullptr;
@@ -434,6 +599,11 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t na) {
   p_rope = reinterpret_cast<decltype(p_rope)>(p[6]);
   p_sample = reinterpret_cast<decltype(p_sample)>(p[7]);
   p_sample_workspace = reinterpret_cast<decltype(p_sample_workspace)>(p[8]);
+  p_plan_words = reinterpret_cast<decltype(p_plan_words)>(p[9]);
+  p_cache_step = reinterpret_cast<decltype(p_cache_step)>(p[10]);
+  p_store_kv = reinterpret_cast<decltype(p_store_kv)>(p[11]);
+  p_paged_workspace = reinterpret_cast<decltype(p_paged_workspace)>(p[12]);
+  p_paged = reinterpret_cast<decltype(p_paged)>(p[13]);
   Py_RETURN_NONE;
 }
 
@@ -447,6 +617,9 @@ PyMethodDef methods[] = {
     {"lora", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&lora)), METH_FASTCALL, nullptr},
     {"rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&rope)), METH_FASTCALL, nullptr},
     {"sample", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&sample)), METH_FASTCALL, nullptr},
+    {"cache_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&cache_step)), METH_FASTCALL, nullptr},
+    {"store_kv", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&store_kv)), METH_FASTCALL, nullptr},
+    {"paged", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&paged)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -2,11 +2,13 @@
 
     from mlx_tree_spec_amd import quantized_matmul, dequantize, QuantizedLinear, install
     from mlx_tree_spec_amd import quantized_matmul_lora, qk_norm_rope, sample    # what differs per request
+    from mlx_tree_spec_amd import CacheTables, store_kv_, paged_attention        # the paged key-value cache
 
 All compute runs in libqmm4.so (hand-written HIP kernels, C ABI in include/); importing
 this package does not load it, the first call does, and fails loudly if it is not built.
 """
 
+from .cache import CacheStep, CacheTables, KVCache, paged_attention, step_tables_, store_kv_
 from .fused_ops import add_rms_norm, add_rms_norm_, add_rms_norm_gate_up, add_rms_norm_qmm_
 from .heads import qk_norm_rope
 from .lora import LoRALinear, quantized_matmul_lora, stack_adapters
@@ -20,5 +22,6 @@ __all__ = [
     "add_rms_norm_", "add_rms_norm_qmm_", "add_rms_norm_gate_up", "QuantizedLinear", "QuantizedMLP",
     "quantized_matmul_lora", "stack_adapters", "LoRALinear", "qk_norm_rope", "sample", "eligible", "install",
     "STATS", "MLPLayer", "layer_tail", "stack_tail", "GraphedTail", "AttentionInputs", "attention_inputs", "next_tokens",
+    "KVCache", "CacheTables", "CacheStep", "step_tables_", "store_kv_", "paged_attention",
 ]
 __version__ = "0.1.0"

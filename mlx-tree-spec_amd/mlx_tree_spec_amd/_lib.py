@@ -49,6 +49,12 @@ SIGNATURES = {
     "qmm4_sample_workspace": (_i64, [_i64, _i64]),
     "qmm4_sample_bf16": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _f32, _vp, _i32, _vp, _f32, _vp, _f32, _vp, _vp, _vp,
                                 _vp]),
+    "qmm4_cache_plan_words": (_i64, [_i64] * 5),
+    "qmm4_cache_step": (_int, [_vp] * 11 + [_i64] * 9 + [_vp]),
+    "qmm4_store_kv_bf16": (_int, [_vp, _i64, _i64, _vp, _i64, _i64] + [_vp] * 5 + [_i64] * 5 + [_int, _vp]),
+    "qmm4_paged_workspace": (_i64, [_i64] * 6),
+    "qmm4_paged_attention_bf16": (_int, [_vp, _i64, _i64] + [_vp] * 9 + [_i64, _i64, _vp, _vp, _f32] + [_i64] * 9
+                                  + [_int, _vp]),
     "qmm4_last_error": (ctypes.c_char_p, []),
     "qmm4_abi_version": (_int, []),
 }
@@ -85,7 +91,7 @@ class _NoNative:
     """Stands in for the native module where it is not built or not for this torch and Python: every
     function declines, so the Python form of each call runs."""
 
-    qmm = linear = gate_up = norm = norm_qmm = lora = rope = sample = staticmethod(lambda *args: None)
+    qmm = linear = gate_up = norm = norm_qmm = lora = rope = sample = cache_step = store_kv = paged = staticmethod(lambda *args: None)
 
 
 def native():
@@ -107,7 +113,8 @@ def native():
             mod.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
                 "qmm4_affine_bf16", "qmm4_gate_up_silu_bf16", "qmm_affine_general_bf16", "qmm4_add_rms_norm_bf16",
                 "qmm4_add_rms_norm_qmm_bf16", "qmm4_affine_lora_bf16", "qmm4_qk_norm_rope_bf16", "qmm4_sample_bf16",
-                "qmm4_sample_workspace")))
+                "qmm4_sample_workspace", "qmm4_cache_plan_words", "qmm4_cache_step", "qmm4_store_kv_bf16",
+                "qmm4_paged_workspace", "qmm4_paged_attention_bf16")))
         except ImportError as e:
             warnings.warn(f"mlx_tree_spec_amd: the native call path cannot be loaded ({e}); calls take their Python "
                           "form, 6-13 us more host time each. Build it with `python -m mlx_tree_spec_amd.build`.",
