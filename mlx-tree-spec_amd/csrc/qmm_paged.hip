@@ -35,8 +35,9 @@ struct PagedTraits {
   static constexpr int kKC = D / (4 * E);    // 16-byte pieces of a key for each lane
   static constexpr int kQK = D / 32;         // matrix instructions along D
   static constexpr int kVT = D / 16;         // tiles of 16 dimensions
-  // Two tiles of query rows beside 192 dimensions or more take over 256 registers: one wave to a SIMD.
-  static constexpr int kWaves = QT == 2 && D > 128 ? 4 : 8;
+  // Registers of o, q, s, keys, values and scales; with what else there is more than 256: one wave to a SIMD.
+  static constexpr int kRegisters = 4 * (QT * (kVT + kQK + kKT) + kKT * kKC + kVT + (Q8 ? 3 * kKT : 0));
+  static constexpr int kWaves = kRegisters > 176 ? 4 : 8;
   static constexpr size_t kJoin = (size_t)(kWaves / 2) * QT * (kVT * 1024 + 128);  // LDS of a join
 };
 
@@ -53,6 +54,11 @@ __device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi) {
 __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
+
+// A query row, null where there is none.
+struct QueryAddress {
+  const uint16_t* x;
+};
 
 // What a wave knows of one of its query rows (the one of lane % 16 in tile qt).
 struct QueryRow {
@@ -75,6 +81,7 @@ struct PagedWave {
   f32x4 o[QT][T::kVT];
   u32x4 kf[T::kKT][T::kKC], vf[T::kVT];
   f32x4 ks[Q8 ? T::kKT : 1], vs[Q8 ? T::kKT : 1];
+  bool odd = false;  // a value that is not finite was left out
 
   __device__ __forceinline__ PagedWave(const PagedParams& s) : S(s) {}
 
@@ -125,62 +132,67 @@ struct PagedWave {
     return (j < 0) | ((tok < seen[qt]) & ((uint32_t)(row[qt].bits >> (j & 63)) & 1u));
   }
 
-  // What a step's values that are not finite add to o, token by token, for the rows that see them; 0 in their place in vf (as
-  // for the tokens past the last, which the cache need not hold).
-  __device__ __forceinline__ void set_apart(int t, const bf16x8 (&p)[QT][E / 8], int vpage) {
-    const int tok = t + E * g;
-    bool odd = false;
-#pragma unroll
-    for (int dt = 0; dt < T::kVT; ++dt)
+  // Zeros in a step's values in place of tokens past the last, which the cache need not hold, and of what is not finite:
+  // a probability of zero would not keep it from the rows that do not see it. `odd`: there was some of it.
+  __device__ __forceinline__ void clean_values(int t) {
+    if constexpr (!Q8) {
+      const int past = t + E * g - length;
+      bool any = false;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const int past = tok + 2 * w + 1 - length;  // (of the word's second token: 0 past the last, 1 the first too)
-        if (past >= 0) vf[dt][w] &= past >= 1 ? 0u : 0xFFFFu;
-        odd |= (vf[dt][w] & 0x7F80u) == 0x7F80u || (vf[dt][w] & 0x7F800000u) == 0x7F800000u;
+        const uint32_t keep = past + 2 * w >= 0 ? 0u : past + 2 * w + 1 >= 0 ? 0xFFFFu : 0xFFFFFFFFu;
+#pragma unroll
+        for (int dt = 0; dt < T::kVT; ++dt) {
+          uint32_t x = vf[dt][w] & keep;
+          const bool lo = (x & 0x7F80u) == 0x7F80u, hi = (x & 0x7F800000u) == 0x7F800000u;
+          any |= lo | hi;
+          x = lo ? x & 0xFFFF0000u : x;
+          vf[dt][w] = hi ? x & 0xFFFFu : x;
+        }
       }
-    if (!__any(odd)) return;
+      odd |= __any(any) != 0;
+    }
+  }
+
+  // What those values add to o for the rows that see them: the wave's steps from t on again, token by token.
+  __device__ __forceinline__ void add_odd_values(int t, int end, int stride, const QueryAddress (&at)[QT]) {
     const int shift = S.cache.page_shift;
-    const int pages = vpage;
-#pragma unroll 1
-    for (int j = 0; j < T::kStep; ++j) {
-      if (t + j >= length) break;
-      // The page and the probabilities of the token are those of the lanes of group j / E.
-      const int from = (j / E) * 16, pg = __shfl(pages, from);
-      const uint16_t* v = static_cast<const uint16_t*>(S.cache.values) +
-                          (((((int64_t)pg * S.cache.heads + h) << shift) + ((t + j) & ((1 << shift) - 1) & ~(E - 1))) / E * D) * E + j % E;
+    for (; t < end; t += stride) {
+      if (t + T::kStep <= context) continue;
+      for (int tok = t; tok < min(t + T::kStep, length); ++tok) {
+        const int64_t head = (int64_t)max(0, min(table[tok >> shift], (int)S.cache.pages - 1)) * S.cache.heads + h;
+        const int off = tok & ((1 << shift) - 1);
+        const uint16_t* v = static_cast<const uint16_t*>(S.cache.values) + ((((head << shift) + off) / 8) * D) * 8 + off % 8;
+        const uint16_t* k = static_cast<const uint16_t*>(S.cache.keys) + (((head * (D / 8)) << shift) + off) * 8;
+        bool any = false;
+        for (int d = lane; d < D; d += 64) any |= (v[d * 8] & 0x7F80u) == 0x7F80u;
+        if (!__any(any)) continue;
 #pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
-        const u32x4 words = __builtin_bit_cast(u32x4, p[qt][0]);
-        const int e = j % E;
-        uint32_t word = words[0];
-        word = e >= 2 ? words[1] : word;
-        word = e >= 4 ? words[2] : word;
-        word = e >= 6 ? words[3] : word;
-        const uint32_t mine = e & 1 ? word >> 16 : word & 0xFFFFu;
-        const float pj = bf16_to_f32((uint32_t)__shfl((int)mine, from + r16));
-        const bool see = sees(qt, t + j);
+        for (int qt = 0; qt < QT; ++qt) {
+          float x = 0.0f;
+          for (int d = g; d < D; d += 4)
+            x += at[qt].x ? bf16_to_f32(at[qt].x[d]) * bf16_to_f32(k[((int64_t)(d / 8) << shift) * 8 + d % 8]) : 0.0f;
+          x += __shfl_xor(x, 16);
+          x += __shfl_xor(x, 32);
+          const float p = __builtin_amdgcn_exp2f(x * (S.scale * kLog2e) - m[qt]);
+          const bool see = sees(qt, tok);
 #pragma unroll
-        for (int dt = 0; dt < T::kVT; ++dt)
+          for (int dt = 0; dt < T::kVT; ++dt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t x = v[(dt * 16 + 4 * g + i) * E];
-            if (see && (x & 0x7F80u) == 0x7F80u) o[qt][dt][i] += pj * bf16_to_f32(x);
-          }
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t y = v[(dt * 16 + 4 * g + i) * 8];
+              const float add = p * bf16_to_f32(y);
+              o[qt][dt][i] += (see & ((y & 0x7F80u) == 0x7F80u)) ? add : 0.0f;
+            }
+        }
       }
     }
-#pragma unroll
-    for (int dt = 0; dt < T::kVT; ++dt)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        if ((vf[dt][w] & 0x7F80u) == 0x7F80u) vf[dt][w] &= 0xFFFF0000u;
-        if ((vf[dt][w] & 0x7F800000u) == 0x7F800000u) vf[dt][w] &= 0xFFFFu;
-      }
   }
 
   // One step of kStep tokens from t, whose keys and values are loaded; MORE: those of t + stride are, meanwhile (kp, vp: their
   // pages on entry; on return those of t + 2 stride).
   template <bool MORE>
-  __device__ __forceinline__ void step(int t, int stride, int* kp, int* vp, int* vpage) {
+  __device__ __forceinline__ void step(int t, int stride, int* kp, int* vp) {
     f32x4 s[QT][T::kKT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
@@ -281,7 +293,7 @@ struct PagedWave {
       }
     }
     if constexpr (!Q8) {
-      if (masked) set_apart(t, p, *vpage);
+      if (masked) clean_values(t);
     }
 #pragma unroll
     for (int dt = 0; dt < T::kVT; ++dt) {
@@ -293,23 +305,20 @@ struct PagedWave {
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (MORE) {
-      load_values(t + stride, next_page);
-      *vpage = next_page;
-    }
+    if constexpr (MORE) load_values(t + stride, next_page);
     __builtin_amdgcn_sched_barrier(0);
   }
 
   // Steps t, t + stride, .. below end.
   __device__ __forceinline__ void run(int t, int end, int stride) {
     if (t >= end) return;
-    int vpage = page(t + E * g);
+    const int vpage = page(t + E * g);
     load_keys(t, page(t + E * (r16 >> 2)));
     load_scales(t, vpage);
     load_values(t, vpage);
     int kp = page(t + stride + E * (r16 >> 2)), vp = page(t + stride + E * g);
-    for (; t + stride < end; t += stride) step<true>(t, stride, &kp, &vp, &vpage);
-    step<false>(t, stride, &kp, &vp, &vpage);
+    for (; t + stride < end; t += stride) step<true>(t, stride, &kp, &vp);
+    step<false>(t, stride, &kp, &vp);
   }
 };
 
@@ -369,7 +378,21 @@ __global__ __launch_bounds__((PagedTraits<D, QT, Q8>::kWaves * 64)) void paged_k
     const int begin = split * per;
     int end = min(begin + per, length);
     if (!S.ancestors) end = min(end, W.context + last + 1);  // (nothing later is seen)
-    if (rw < tiles) W.run(begin + kw * T::kStep, end, KW * T::kStep);
+    if (rw < tiles) {
+      const int t = begin + kw * T::kStep, stride = KW * T::kStep;
+      W.run(t, end, stride);
+      if (!Q8 && W.odd) {
+        QueryAddress at[QT];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          const int64_t row = row0 + (rw * QT + qt) * 16 + W.r16;
+          const int i = (int)(row / S.G), hq = W.h * S.G + (int)(row - (int64_t)i * S.G);
+          at[qt].x = W.row[qt].valid ? S.q.x + (int64_t)(first + i) * S.q.row + (int64_t)hq * S.q.head : nullptr;
+        }
+        W.add_odd_values(t, end, stride, at);
+        W.odd = false;
+      }
+    }
 
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
