@@ -1,6 +1,7 @@
 // C ABI of the paged key-value cache (declared in include/qmm_cache.h): argument checks and launches.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <exception>
@@ -201,7 +202,10 @@ int qmm4_paged_attention_bf16(const void* q, int64_t q_row, int64_t q_head, cons
       return set_error(QMM4_ERR_INVALID, "keys, values, out and workspace must be 16-byte aligned, tables to their elements");
     if (pages == 0 || capacity == 0)
       return set_error(QMM4_ERR_INVALID, "a cache without pages has nothing to attend to");
-    const int64_t most = clamp_rows(max_rows);
+    const int64_t most = std::min(max_rows, M);
+    if (most * (Hq / Hk) > (1LL << 30))
+      return set_error(QMM4_ERR_INVALID, "%lld rows of %lld query heads to a key head: up to 2^30 of both are supported",
+                       (long long)most, (long long)(Hq / Hk));
     qmm4::PagedShape s;
     if (int rc = shape_of(Hq, Hk, D, most, &s)) return rc;
     float* part = static_cast<float*>(workspace);

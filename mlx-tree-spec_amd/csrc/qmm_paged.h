@@ -1,0 +1,339 @@
+// What the paged attention's two kernels share (qmm_paged.hip, qmm_paged_tile.hip): a wave's query rows, their softmax, what
+// they see, and how waves and splits are joined.
+//
+// Both products run on 16x16x32 matrix instructions with the tokens' side as the first operand:
+//   S^T = K Q^T  (16 tokens x 16 query rows),   O^T = V^T P^T  (16 dimensions x 16 query rows)
+// The cache's layout makes 16 bytes of keys (E dimensions of a token) and of values (E tokens of a dimension) operands as they
+// lie. S^T leaves each lane with probabilities of one query row (lane % 16); the order of tokens within a step of 4 E is chosen
+// (row 4 g + i of tile tt is token E g + 4 tt + i, g = lane / 16) so that they are the second operand of O^T without a move
+// between lanes.
+//
+// The running maximum moves only where a logit passes it by more than 2^8: probabilities up to 256 lose nothing in fp32, and
+// most steps need no exchange between lanes.
+#pragma once
+
+#include "qmm4_common.h"
+#include "qmm_cache_kernels.h"
+
+namespace qmm4 {
+
+constexpr float kLog2e = 1.44269504f;
+// How far (in powers of two) a logit may pass the running maximum.
+constexpr float kSlack = 8.0f;
+
+__device__ __forceinline__ f32x4 paged_mma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// 8 codes -> bf16 (exact).
+__device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi) {
+  u32x4 r;
+  r.x = pack_bf16x2((float)(int8_t)(lo & 0xFFu), (float)(int8_t)((lo >> 8) & 0xFFu));
+  r.y = pack_bf16x2((float)(int8_t)((lo >> 16) & 0xFFu), (float)(int8_t)(lo >> 24));
+  r.z = pack_bf16x2((float)(int8_t)(hi & 0xFFu), (float)(int8_t)((hi >> 8) & 0xFFu));
+  r.w = pack_bf16x2((float)(int8_t)((hi >> 16) & 0xFFu), (float)(int8_t)(hi >> 24));
+  return as_bf16x8(r);
+}
+
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
+
+// x * sigmoid(gate) of 4 neighbouring dimensions, rounded.
+__device__ __forceinline__ u32x2 gated_bf16(f32x4 x, const uint16_t* gate) {
+  if (gate) {
+    const u32x2 y = *reinterpret_cast<const u32x2*>(gate);
+    x[0] *= sigmoid(bf16_to_f32(y[0] & 0xFFFFu));
+    x[1] *= sigmoid(bf16_to_f32(y[0] >> 16));
+    x[2] *= sigmoid(bf16_to_f32(y[1] & 0xFFFFu));
+    x[3] *= sigmoid(bf16_to_f32(y[1] >> 16));
+  }
+  return u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+}
+
+// Whether a row without a context sees none of its request's n rows: its result is zero.
+__device__ __forceinline__ bool paged_empty(const int64_t* ancestors, int64_t row, int length, int n) {
+  if (!ancestors || length != n) return false;
+  return ((uint64_t)ancestors[row] & (n < 64 ? (1ull << n) - 1 : ~0ull)) == 0;
+}
+
+template <int D, int QT, bool Q8>
+struct PagedRows {
+  static constexpr int E = Q8 ? 16 : 8;  // elements of 16 bytes
+  static constexpr int kStep = 4 * E;    // tokens of a wave's step
+  static constexpr int kKT = E / 4;      // tiles of 16 tokens
+  static constexpr int kKC = D / (4 * E);  // 16-byte pieces of a key for each lane
+  static constexpr int kQK = D / 32;     // matrix instructions along D
+  static constexpr int kVT = D / 16;     // tiles of 16 dimensions
+  // LDS of a wave that hands over its results.
+  static constexpr int kHandBytes = QT * (kVT * 1024 + 128);
+
+  const PagedParams& S;
+  const int32_t* table;  // the request's row
+  int r, lane, r16, g, h, n, length, context;
+  float unit;  // of a logit, in powers of two
+  bf16x8 q[QT][kQK];
+  uint64_t bits[QT];  // the step's rows that the row sees (all ones without ancestors)
+  int seen[QT];       // no token from this on is seen
+  float m[QT], l[QT];
+  f32x4 o[QT][kVT];
+  bool odd = false;  // a value that is not finite was left out
+
+  __device__ __forceinline__ PagedRows(const PagedParams& s, int request, int head) : S(s), r(request), h(head) {
+    lane = threadIdx.x & 63;
+    r16 = lane & 15;
+    g = lane >> 4;
+    n = S.plan.count()[r];
+    length = S.plan.length()[r];
+    context = length - n;
+    table = S.table + (int64_t)r * S.capacity;
+    unit = fabsf(S.scale) * kLog2e;
+  }
+
+  // Query row `at` of the request's n G: its row of the step and its head.
+  __device__ __forceinline__ void place(int at, int* i, int* hq) const {
+    *i = (int)((uint32_t)at / (uint32_t)S.G);
+    *hq = h * S.G + at - *i * S.G;
+  }
+  __device__ __forceinline__ const uint16_t* query(int at) const {
+    int i, hq;
+    place(at, &i, &hq);
+    return at < n * S.G ? S.q.x + (int64_t)(S.plan.first()[r] + i) * S.q.row + (int64_t)hq * S.q.head : nullptr;
+  }
+
+  // The wave's query rows from `row0` on, with their sign turned where scale is negative (what the maximum is taken of rises
+  // with the logit then). Returns one past the last token that any of them sees.
+  __device__ __forceinline__ int load_rows(int row0) {
+    const uint32_t sign = S.scale < 0.0f ? 0x80008000u : 0u;
+    int end = 0;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int at = row0 + qt * 16 + r16;
+      int i, hq;
+      place(at, &i, &hq);
+      const uint16_t* x = query(at);
+      bits[qt] = ~0ull;
+      seen[qt] = min(length, context + min(i, n) + 1);
+      if (S.ancestors) {
+        bits[qt] = x ? (uint64_t)S.ancestors[S.plan.first()[r] + i] : 0;
+        seen[qt] = min(length, context + 64);
+      }
+#pragma unroll
+      for (int c = 0; c < kQK; ++c) {
+        const int d = Q8 ? (c / 2) * 64 + g * 16 + (c & 1) * 8 : c * 32 + g * 8;
+        u32x4 v = {0u, 0u, 0u, 0u};
+        if (x) v = *reinterpret_cast<const u32x4*>(x + d);
+        v ^= sign;
+        q[qt][c] = as_bf16x8(v);
+      }
+      m[qt] = -__builtin_inff();
+      l[qt] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < kVT; ++dt) o[qt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      end = max(end, min((row0 + qt * 16 + 15) / S.G, n - 1));
+    }
+    return S.ancestors ? length : context + end + 1;
+  }
+
+  // The first token of a group of E, within the request's.
+  __device__ __forceinline__ int group(int token) const { return min(token, (length - 1) & ~(E - 1)); }
+  // A page of the cache, whatever the table holds.
+  __device__ __forceinline__ int valid_page(int page) const { return max(0, min(page, (int)S.cache.pages - 1)); }
+
+  // Whether the row sees a token: all of the context, and of what follows up to `seen` what its bits say. (Without branches:
+  // hipcc 7.2 has lost the selected value of nested divergent ones here.)
+  __device__ __forceinline__ bool sees(int qt, int tok) const {
+    const int j = tok - context;
+    return (j < 0) | ((tok < seen[qt]) & ((uint32_t)(bits[qt] >> (j & 63)) & 1u));
+  }
+
+  // The probabilities of a step's tokens from t, whose products are s, as the second operand of the values' product; m, l and
+  // o move with them. 8 bits: kscale multiplies the products, vscale the probabilities.
+  __device__ __forceinline__ void softmax(int t, int qt, f32x4 (&s)[kKT], const f32x4* kscale, const f32x4* vscale,
+                                          bf16x8 (&p)[E / 8]) {
+    const bool masked = t + kStep > context;
+    if constexpr (Q8) {
+#pragma unroll
+      for (int tt = 0; tt < kKT; ++tt) s[tt] *= kscale[tt];
+    }
+    if (masked) {
+#pragma unroll
+      for (int tt = 0; tt < kKT; ++tt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[tt][i] = sees(qt, t + E * g + 4 * tt + i) ? s[tt][i] : -__builtin_inff();
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int tt = 0; tt < kKT; ++tt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tt][i]);
+    // (A unit of 0 leaves masked tokens at -infinity too.)
+    top = top == -__builtin_inff() ? top : top * unit;
+    if (__any(top > m[qt] + kSlack)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m[qt]);
+      // (Nothing seen yet: l and o are zero.)
+      const float f = m[qt] == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[qt] - top);
+      l[qt] *= f;
+#pragma unroll
+      for (int dt = 0; dt < kVT; ++dt) o[qt][dt] *= f;
+      m[qt] = top;
+    }
+    const float ref = m[qt] == -__builtin_inff() ? 0.0f : m[qt];
+    float e[E];
+#pragma unroll
+    for (int tt = 0; tt < kKT; ++tt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[tt * 4 + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], unit, -ref));
+    if (masked) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) e[j] = sees(qt, t + E * g + j) ? e[j] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) l[qt] += e[j];
+    if constexpr (Q8) {
+#pragma unroll
+      for (int tt = 0; tt < kKT; ++tt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = e[tt * 4 + i] * vscale[tt][i];
+          e[tt * 4 + i] = masked && !sees(qt, t + E * g + 4 * tt + i) ? 0.0f : x;
+        }
+    }
+#pragma unroll
+    for (int half = 0; half < E / 8; ++half) {
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(e[half * 8 + 2 * i], e[half * 8 + 2 * i + 1]);
+      p[half] = as_bf16x8(w);
+    }
+  }
+
+  // Zeros in 8 tokens' values (of one dimension, from t + E g on) in place of those past the last, which the cache need not
+  // hold, and of what is not finite: a probability of zero would not keep it from the rows that do not see it.
+  __device__ __forceinline__ u32x4 clean(u32x4 v, int t) {
+    const int past = t + E * g - length;
+    bool any = false;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t keep = past + 2 * w >= 0 ? 0u : past + 2 * w + 1 >= 0 ? 0xFFFFu : 0xFFFFFFFFu;
+      uint32_t x = v[w] & keep;
+      const bool lo = (x & 0x7F80u) == 0x7F80u, hi = (x & 0x7F800000u) == 0x7F800000u;
+      any |= lo | hi;
+      x = lo ? x & 0xFFFF0000u : x;
+      v[w] = hi ? x & 0xFFFFu : x;
+    }
+    odd |= any;
+    return v;
+  }
+
+  // What those values add to o for the rows that see them: the wave's steps t, t + stride, .. again, token by token.
+  __device__ __forceinline__ void add_odd_values(int t, int end, int stride, int row0) {
+    if (Q8 || !__any(odd)) return;
+    odd = false;
+    const int shift = S.cache.page_shift;
+    for (; t < end; t += stride) {
+      if (t + kStep <= context) continue;
+      for (int tok = t; tok < min(t + kStep, length); ++tok) {
+        const int64_t head = (int64_t)valid_page(table[tok >> shift]) * S.cache.heads + h;
+        const int off = tok & ((1 << shift) - 1);
+        const uint16_t* v = static_cast<const uint16_t*>(S.cache.values) + ((((head << shift) + off) / 8) * D) * 8 + off % 8;
+        const uint16_t* k = static_cast<const uint16_t*>(S.cache.keys) + (((head * (D / 8)) << shift) + off) * 8;
+        bool any = false;
+        for (int d = lane; d < D; d += 64) any |= (v[d * 8] & 0x7F80u) == 0x7F80u;
+        if (!__any(any)) continue;
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          const uint16_t* y = query(row0 + qt * 16 + r16);
+          float x = 0.0f;
+          for (int d = g; d < D; d += 4)
+            x += y ? bf16_to_f32(y[d]) * bf16_to_f32(k[((int64_t)(d / 8) << shift) * 8 + d % 8]) : 0.0f;
+          x += __shfl_xor(x, 16);
+          x += __shfl_xor(x, 32);
+          const float p = __builtin_amdgcn_exp2f(x * (S.scale * kLog2e) - m[qt]);
+          const bool see = sees(qt, tok);
+#pragma unroll
+          for (int dt = 0; dt < kVT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t z = v[(dt * 16 + 4 * g + i) * 8];
+              const float add = p * bf16_to_f32(z);
+              o[qt][dt][i] += (see & ((z & 0x7F80u) == 0x7F80u)) ? add : 0.0f;
+            }
+        }
+      }
+    }
+  }
+
+  // l of a row in all of its lanes.
+  __device__ __forceinline__ void sum_lanes() {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      l[qt] += __shfl_xor(l[qt], 16);
+      l[qt] += __shfl_xor(l[qt], 32);
+    }
+  }
+
+  // The wave's results to LDS (kHandBytes), and another wave's, of the same rows, joined to its own.
+  __device__ __forceinline__ void hand_over(char* lds) const {
+    f32x4* s_o = reinterpret_cast<f32x4*>(lds);
+    float* s_ml = reinterpret_cast<float*>(lds + QT * kVT * 1024);
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+#pragma unroll
+      for (int dt = 0; dt < kVT; ++dt) s_o[(qt * kVT + dt) * 64 + lane] = o[qt][dt];
+      if (g == 0) {
+        s_ml[qt * 32 + r16] = m[qt];
+        s_ml[qt * 32 + 16 + r16] = l[qt];
+      }
+    }
+  }
+  __device__ __forceinline__ void take_over(const char* lds) {
+    const f32x4* s_o = reinterpret_cast<const f32x4*>(lds);
+    const float* s_ml = reinterpret_cast<const float*>(lds + QT * kVT * 1024);
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const float m2 = s_ml[qt * 32 + r16], l2 = s_ml[qt * 32 + 16 + r16], top = fmaxf(m[qt], m2);
+      const float f1 = m[qt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[qt] - top);
+      const float f2 = m2 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m2 - top);
+      m[qt] = top;
+      l[qt] = l[qt] * f1 + l2 * f2;
+#pragma unroll
+      for (int dt = 0; dt < kVT; ++dt) o[qt][dt] = o[qt][dt] * f1 + s_o[(qt * kVT + dt) * 64 + lane] * f2;
+    }
+  }
+
+  // The rows' results, or where the request has several splits the part of this one.
+  __device__ __forceinline__ void write(int row0, int split) const {
+    const int64_t heads = (int64_t)S.cache.heads * S.G;
+    const int first = S.plan.first()[r];
+    const bool whole = S.plan.per()[r] >= length;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int at = row0 + qt * 16 + r16;
+      if (at >= n * S.G) continue;
+      int i, hq;
+      place(at, &i, &hq);
+      if (whole) {
+        const float inv = paged_empty(S.ancestors, first + i, length, n) ? 0.0f : 1.0f / l[qt];
+        uint16_t* out = S.out + ((int64_t)(first + i) * heads + hq) * D + 4 * g;
+        const uint16_t* gate = S.gate.x ? S.gate.x + (int64_t)(first + i) * S.gate.row + (int64_t)hq * S.gate.head + 4 * g : nullptr;
+#pragma unroll
+        for (int dt = 0; dt < kVT; ++dt)
+          *reinterpret_cast<u32x2*>(out + dt * 16) = gated_bf16(o[qt][dt] * inv, gate ? gate + dt * 16 : nullptr);
+      } else {
+        const int64_t part = ((int64_t)S.plan.part()[r] + (int64_t)split * n + i) * heads + hq;
+#pragma unroll
+        for (int dt = 0; dt < kVT; ++dt) *reinterpret_cast<f32x4*>(S.part + part * D + dt * 16 + g * 4) = o[qt][dt];
+        if (g == 0) {
+          S.part_ml[part * 2] = m[qt];
+          S.part_ml[part * 2 + 1] = l[qt];
+        }
+      }
+    }
+  }
+};
+
+// The kernel of up to 16 query rows to a key head, and that of more.
+hipError_t launch_paged_rows(const PagedParams& p, int64_t items, int D, bool q8, hipStream_t stream);
+hipError_t launch_paged_tile(const PagedParams& p, int64_t items, int D, bool q8, hipStream_t stream);
+
+}  // namespace qmm4

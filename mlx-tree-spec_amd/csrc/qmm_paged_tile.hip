@@ -1,0 +1,264 @@
+// Paged attention of more than 16 query rows to a key head: tree verify and prompt rows (qmm_paged.h has the products and the
+// softmax). Each byte of the cache serves up to 128 query rows of a workgroup: bound by HBM up to about that many, past it by the
+// matrix instructions and what feeds them.
+//
+// A workgroup takes up to kPagedRows query rows of one key head over one split: 8 waves with 16 QT rows each, or with two SIDES
+// 4 of them on the even steps and the others with the same rows on the odd ones. The steps' keys and values go from memory to a ring of stages in
+// LDS without registers (1 KB an instruction), kStages - 1 stages ahead, in the order in which the waves read them: a
+// fragment is then 256 neighbouring bytes for 16 lanes, without bank conflicts. One barrier a stage, behind an exact count of the
+// loads that may still be on their way.
+#include <algorithm>
+#include <type_traits>
+
+#include "qmm4_lds.h"
+#include "qmm_paged.h"
+
+namespace qmm4 {
+
+namespace {
+
+constexpr int kWaves = 8;
+constexpr int kThreads = kWaves * 64;
+constexpr int kIds = 1024;  // page numbers held in LDS at once
+
+template <int D, int QT, int SIDES, bool Q8>
+struct TileTraits {
+  using R = PagedRows<D, QT, Q8>;
+  static constexpr int kAcross = kWaves / SIDES;          // waves side by side along the rows
+  static constexpr int kRows = kAcross * 16 * QT;
+  static constexpr int kStage = 2 * R::kStep;             // tokens
+  static constexpr int kPieces = D * 16;                  // 16-byte pieces of a stage: keys, then values
+  static constexpr int kScaleBytes = Q8 ? kStage * 8 : 0;
+  static constexpr int kStageBytes = kPieces * 16 + kScaleBytes;
+  static constexpr int kLoads = D / 32 + (Q8 ? 1 : 0);    // a wave's loads of a stage
+  static constexpr int kRoom = 160 * 1024 - kIds * 4 - 512;
+  static constexpr int kStages = kRoom / kStageBytes < 4 ? kRoom / kStageBytes : 4;
+  static constexpr size_t kRing = (size_t)kStages * kStageBytes;
+  static constexpr size_t kJoin = SIDES > 1 ? (size_t)kAcross * R::kHandBytes : 0;
+  static constexpr size_t kLds = (kRing > kJoin ? kRing : kJoin) + kIds * 4;
+  static_assert(kStages >= 2 && kPieces / 64 == kWaves * (D / 32) && kLds <= 160 * 1024, "whole loads, LDS");
+};
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void bare_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+template <int D, int QT, int SIDES, bool Q8>
+__global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int block0, int blocks) {
+  using T = TileTraits<D, QT, SIDES, Q8>;
+  using R = PagedRows<D, QT, Q8>;
+  constexpr int E = R::E;
+  typedef __attribute__((address_space(1))) const void* global_ptr;
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  extern __shared__ __attribute__((aligned(16))) char s_ring[];
+  int* s_ids = reinterpret_cast<int*>(s_ring + T::kLds - kIds * 4);
+  // The row blocks of one split and key head follow each other on one XCD (workgroups go round the 8 of them): the later
+  // ones find the cache's bytes in its L2.
+  const int unit = blockIdx.x / (8 * blocks) * 8 + (blockIdx.x & 7), block = block0 + blockIdx.x / 8 % blocks;
+  const int item = unit / S.cache.heads;
+  if (item >= S.plan.words[0]) return;
+  const int split = S.plan.items()[2 * item + 1];
+  R W(S, S.plan.items()[2 * item], unit - item * S.cache.heads);
+  const int row0 = block * T::kRows, rows = W.n * S.G;
+  if (row0 >= rows) return;
+  const int wave = threadIdx.x >> 6, side = wave / T::kAcross, rw = wave % T::kAcross;
+  const int mine = row0 + rw * 16 * QT;
+  const bool active = mine < rows;
+  W.load_rows(mine);
+
+  const int per = S.plan.per()[W.r], begin = split * per;
+  int end = min(begin + per, W.length);
+  // (Without ancestors nothing past the block's last row is seen.)
+  if (!S.ancestors) end = min(end, W.context + min((row0 + T::kRows - 1) / S.G, W.n - 1) + 1);
+  const int shift = S.cache.page_shift, page_mask = (1 << shift) - 1, lane = W.lane;
+  const char* keys = static_cast<const char*>(S.cache.keys);
+  const char* values = static_cast<const char*>(S.cache.values);
+
+  // One step, from a stage in LDS.
+  auto step = [&](const u32x4* ring, int sd, int t) __attribute__((always_inline)) {
+    const u32x4* kr = ring + W.g * T::kStage + sd * R::kStep + W.r16;
+    const u32x4* vr = ring + T::kPieces / 2 + (sd * 4 + W.g) * D + W.r16;
+    f32x4 s[QT][R::kKT], ks[Q8 ? R::kKT : 1], vs[Q8 ? R::kKT : 1];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+      for (int tt = 0; tt < R::kKT; ++tt) s[qt][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < R::kKC; ++c) {
+#pragma unroll
+      for (int tt = 0; tt < R::kKT; ++tt) {
+        const u32x4 k = kr[c * 4 * T::kStage + tt * 16];
+        if constexpr (Q8) {
+          const bf16x8 lo = codes8(k[0], k[1]), hi = codes8(k[2], k[3]);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            s[qt][tt] = paged_mma(lo, W.q[qt][2 * c], s[qt][tt]);
+            s[qt][tt] = paged_mma(hi, W.q[qt][2 * c + 1], s[qt][tt]);
+          }
+        } else {
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) s[qt][tt] = paged_mma(as_bf16x8(k), W.q[qt][c], s[qt][tt]);
+        }
+      }
+      if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);  // (few codes at a time in registers)
+    }
+    if constexpr (Q8) {
+      const f32x4* scales = reinterpret_cast<const f32x4*>(ring + T::kPieces) + sd * 16 + W.g * 4;
+#pragma unroll
+      for (int tt = 0; tt < R::kKT; ++tt) {
+        ks[tt] = scales[tt];
+        vs[tt] = scales[32 + tt];
+      }
+    }
+    bf16x8 p[QT][E / 8];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) W.softmax(t, qt, s[qt], ks, vs, p[qt]);
+    const auto values = [&](auto masked) __attribute__((always_inline)) {
+#pragma unroll
+      for (int dt = 0; dt < R::kVT; ++dt) {
+        u32x4 v = vr[dt * 16];
+        if constexpr (Q8) {
+          const bf16x8 lo = codes8(v[0], v[1]), hi = codes8(v[2], v[3]);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            W.o[qt][dt] = paged_mma(lo, p[qt][0], W.o[qt][dt]);
+            W.o[qt][dt] = paged_mma(hi, p[qt][E / 8 - 1], W.o[qt][dt]);
+          }
+          if (dt % 2) __builtin_amdgcn_sched_barrier(0);
+        } else {
+          if constexpr (decltype(masked)::value) v = W.clean(v, t);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) W.o[qt][dt] = paged_mma(as_bf16x8(v), p[qt][0], W.o[qt][dt]);
+        }
+      }
+    };
+    if (!Q8 && t + R::kStep > W.context) values(std::true_type{});
+    else values(std::false_type{});
+  };
+
+  const int segment = kIds << shift;  // tokens whose pages are held at once
+  for (int base = begin & ~page_mask; base < end; base += segment) {
+    const int from = max(begin, base), to = min(end, base + segment), stages = (to - from + T::kStage - 1) / T::kStage;
+    __syncthreads();
+    for (int i = threadIdx.x; i < kIds; i += kThreads) {
+      const int tok = base + (i << shift);
+      s_ids[i] = tok < W.length ? W.valid_page(W.table[tok >> shift]) : 0;
+    }
+    __syncthreads();
+
+    // Stage `st` of the segment into its place of the ring. (Tokens past the last are those of the last group again.)
+    auto load = [&](int st) __attribute__((always_inline)) {
+      const int t = from + st * T::kStage;
+      char* ring = s_ring + (st % T::kStages) * T::kStageBytes;
+      const auto head_of = [&](int tok) { return (int64_t)s_ids[(tok - base) >> shift] * S.cache.heads + W.h; };
+      // A key's lane: its token in the order of the tiles' rows, the same in every piece (8 bits: in both halves of a stage).
+      const char* kp[E / 8];
+#pragma unroll
+      for (int half = 0; half < E / 8; ++half) {
+        const int slot = half * 64 + lane, row = slot & 15, tt = slot / 16 % R::kKT, sd = slot / R::kStep;
+        const int grp = min(W.group(t + sd * R::kStep + E * (row >> 2)), base + segment - E);
+        kp[half] = keys + ((head_of(grp) * (D / E) << shift) + (grp & page_mask) + 4 * tt + (row & 3)) * 16;
+      }
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const int chunk = wave + kWaves * j;
+        const char* src;
+        if (chunk < D / 8) {
+          const int piece = chunk / (E / 8), half = chunk % (E / 8);
+          src = kp[0] + ((int64_t)piece << (shift + 4));
+          if constexpr (Q8) src = (half ? kp[1] : kp[0]) + ((int64_t)piece << (shift + 4));
+        } else {
+          const int f = (chunk - D / 8) * 64 + lane, grp = f / D, d = f - grp * D;
+          const int tok = min(W.group(t + grp * E), base + segment - E);
+          src = values + (((head_of(tok) << shift) + (tok & page_mask)) / E * D + d) * 16;
+        }
+        __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(ring + chunk * 1024), 16, 0, 0);
+      }
+      if constexpr (Q8) {
+        // (One wave's load would do: every wave's loads are counted alike.)
+        const int tok = min(W.group(t + (lane & 28) * 4), base + segment - E) + (lane & 3) * 4;
+        const float* src = (lane < 32 ? S.cache.key_scales : S.cache.value_scales) + (head_of(tok) << shift) + (tok & page_mask);
+        __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(ring + T::kPieces * 16), 16, 0, 0);
+      }
+    };
+
+    for (int st = 0; st < T::kStages - 1 && st < stages; ++st) load(st);
+    for (int st = 0; st < stages; ++st) {
+      if (st + T::kStages - 2 < stages) wait_loads<(T::kStages - 2) * T::kLoads>();
+      else wait_loads<0>();
+      bare_barrier();
+      if (st + T::kStages - 1 < stages) load(st + T::kStages - 1);
+      if (!active) continue;
+      const u32x4* ring = reinterpret_cast<const u32x4*>(s_ring + (st % T::kStages) * T::kStageBytes);
+#pragma unroll 1
+      for (int sd = side; sd < 2; sd += SIDES) {
+        const int t = from + st * T::kStage + sd * R::kStep;
+        if (t < to) step(ring, sd, t);
+      }
+    }
+    // (Every load has been waited for: the ring is free behind the next barrier.)
+    if (active) W.add_odd_values(from + side * R::kStep, to, SIDES * R::kStep, mine);
+  }
+
+  W.sum_lanes();
+  if constexpr (SIDES > 1) {
+    __syncthreads();
+    if (side == 1) W.hand_over(s_ring + rw * R::kHandBytes);
+    __syncthreads();
+    if (side == 0) W.take_over(s_ring + rw * R::kHandBytes);
+  }
+  if (side == 0 && active) W.write(mine, split);
+}
+
+template <int D, int QT, int SIDES, bool Q8>
+hipError_t launch_tile(const PagedParams& p, int64_t items, hipStream_t stream) {
+  using T = TileTraits<D, QT, SIDES, Q8>;
+  static LdsAllowance allowance;
+  if (hipError_t e = allowance.allow(reinterpret_cast<const void*>(&paged_tile_kernel<D, QT, SIDES, Q8>), T::kLds)) return e;
+  const int64_t units = (items * p.cache.heads + 7) / 8 * 8, blocks = ((int64_t)p.max_rows * p.G + T::kRows - 1) / T::kRows;
+  const int64_t most = std::max<int64_t>(1, (int64_t{1} << 22) / units);  // (a grid may have 2^32 threads)
+  for (int64_t b0 = 0; b0 < blocks; b0 += most) {
+    const int64_t count = std::min(most, blocks - b0);
+    hipLaunchKernelGGL((paged_tile_kernel<D, QT, SIDES, Q8>), dim3((unsigned)(units * count)), dim3(kThreads), T::kLds, stream, p,
+                       (int)b0, (int)count);
+  }
+  return hipGetLastError();
+}
+
+template <int D, bool Q8>
+hipError_t launch_rows(const PagedParams& p, int64_t items, hipStream_t stream) {
+  // Two sides where 4 waves of 16 rows hold a request's; past that 32 rows to a wave, or where their sums and queries would not
+  // leave room in 256 registers 16 rows to each of 8.
+  if ((int64_t)p.max_rows * p.G <= 64) return launch_tile<D, 1, 2, Q8>(p, items, stream);
+  if constexpr (D <= 128) return launch_tile<D, 2, 2, Q8>(p, items, stream);
+  else return launch_tile<D, 1, 1, Q8>(p, items, stream);
+}
+
+template <int D>
+hipError_t launch_dim(const PagedParams& p, int64_t items, bool q8, hipStream_t stream) {
+  if constexpr (D % 64 == 0) {
+    if (q8) return launch_rows<D, true>(p, items, stream);
+  }
+  return launch_rows<D, false>(p, items, stream);
+}
+
+}  // namespace
+
+hipError_t launch_paged_tile(const PagedParams& p, int64_t items, int D, bool q8, hipStream_t stream) {
+  switch (D) {
+    case 64: return launch_dim<64>(p, items, q8, stream);
+    case 96: return launch_dim<96>(p, items, q8, stream);
+    case 128: return launch_dim<128>(p, items, q8, stream);
+    case 192: return launch_dim<192>(p, items, q8, stream);
+    default: return launch_dim<256>(p, items, q8, stream);
+  }
+}
+
+}  // namespace qmm4
