@@ -38,7 +38,7 @@ extern "C" {
  *   (not kept, refused, behind the last request) get -1 in all three.
  *   lengths, rows, base: int32 [R]; block_table: int32 [R, capacity]; free_pages: int32 [pages], whose first free_count[0]
  *   are free; keep: one byte per row [total], or null; slots, positions, request: int32 [total].
- *   plan: int32 [qmm4_cache_plan_words(..)] for qmm4_paged_attention_bf16 on this step, 4-byte aligned, or null where there
+ *   plan: int32 [qmm4_cache_plan_words(..)] for qmm4_paged_attention_bf16 on this step, 16-byte aligned, or null where there
  *   is none (with keep: none is made).
  *   Requires R <= QMM4_CACHE_MAX_REQUESTS, total <= QMM4_CACHE_MAX_ROWS, max_rows >= 0, pages * page_size and capacity *
  *   page_size <= 2^30, heads % kv_heads == 0, heads <= 1024. Numbers in the tables that cannot be (lengths past the table,

@@ -110,7 +110,7 @@ int64_t qmm4_cache_plan_words(int64_t R, int64_t heads, int64_t kv_heads, int64_
     if (int bad = check_requests(R, 0, max_rows)) return bad;
     qmm4::PagedShape s;
     if (int bad = shape_of(heads, kv_heads, head_dim, clamp_rows(max_rows), &s)) return bad;
-    words = 8 + 5 * R + 2 * (s.splits + R);
+    words = qmm4::CachePlan::kHead + qmm4::CachePlan::kRecord * (2 * R + s.splits);
     return (int)QMM4_OK;
   });
   return rc ? rc : words;
@@ -128,9 +128,10 @@ int qmm4_cache_step(int32_t* lengths, int32_t* block_table, int32_t* free_pages,
     if ((R > 0 && (!lengths || !rows || (capacity > 0 && !block_table))) || !free_count || (pages > 0 && !free_pages) ||
         (total > 0 && (!slots || !positions || !request)))
       return set_error(QMM4_ERR_INVALID, "null pointer argument");
+    if (!aligned(plan, 16)) return set_error(QMM4_ERR_INVALID, "plan must be 16-byte aligned");
     for (const void* p : {(const void*)lengths, (const void*)block_table, (const void*)free_pages, (const void*)free_count,
                           (const void*)rows, (const void*)base, (const void*)slots, (const void*)positions,
-                          (const void*)request, (const void*)plan})
+                          (const void*)request})
       if (!aligned(p, 4)) return set_error(QMM4_ERR_INVALID, "tables must be aligned to their elements");
     qmm4::PagedShape s;
     const int64_t most = clamp_rows(max_rows);
@@ -198,7 +199,7 @@ int qmm4_paged_attention_bf16(const void* q, int64_t q_row, int64_t q_head, cons
     if (int rc = rows_ok(q, q_row, q_head, "q")) return rc;
     if (int rc = rows_ok(gate, gate_row, gate_head, "gate")) return rc;
     if (!aligned(keys, 16) || !aligned(values, 16) || !aligned(out, 16) || !aligned(workspace, 16) || !aligned(block_table, 4) ||
-        !aligned(request, 4) || !aligned(plan, 4) || !aligned(ancestors, 8))
+        !aligned(request, 4) || !aligned(plan, 16) || !aligned(ancestors, 8))
       return set_error(QMM4_ERR_INVALID, "keys, values, out and workspace must be 16-byte aligned, tables to their elements");
     if (pages == 0 || capacity == 0)
       return set_error(QMM4_ERR_INVALID, "a cache without pages has nothing to attend to");
@@ -214,8 +215,8 @@ int qmm4_paged_attention_bf16(const void* q, int64_t q_row, int64_t q_head, cons
                               {const_cast<void*>(keys), const_cast<void*>(values), const_cast<float*>(key_scales),
                                const_cast<float*>(value_scales), pages, log2_of(page_size), (int)Hk},
                               block_table, request, {const_cast<int32_t*>(plan), (int)R}, ancestors,
-                              static_cast<uint16_t*>(out), part, part + rows * D, capacity, scale, s.G, (int)most};
-    const hipError_t e = qmm4::launch_paged_attention(p, M, s, (int)D, bits == 8, static_cast<hipStream_t>(hip_stream));
+                              static_cast<uint16_t*>(out), part, part + rows * D, capacity, scale, s.G, (int)most, (int)(s.splits + R)};
+    const hipError_t e = qmm4::launch_paged_attention(p, M, (int)D, bits == 8, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return hip_error(e, "paged attention kernel launch");
     return (int)QMM4_OK;
   });

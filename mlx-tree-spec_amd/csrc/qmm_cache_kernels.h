@@ -11,18 +11,29 @@ constexpr int kPagedRows = 128;
 // Tokens at which a request's cache may be cut into splits.
 constexpr int kPagedUnit = 64;
 
-// The plan of a step's attention: 8 words (the first: how many items there are), then arrays of R, then the items. Item: one
-// split of one request's tokens, for every key head.
+// The plan of a step's attention, in words: how many items there are (a block of 8), a record of each request, one of each
+// item. An item is one split of one request's tokens, for every key head.
+struct PagedRequest {
+  int32_t first, rows;   // its rows of the step
+  int32_t length;        // its tokens, the rows among them
+  int32_t per, splits;   // tokens of a split; splits
+  int32_t part;          // first partial row (of more than one split)
+  int32_t unused[2];
+};
+struct PagedItem {
+  int32_t request, first, rows, length;
+  int32_t begin, end;  // its tokens
+  int32_t part;        // its first partial row, or -1: it is the request's only one
+  int32_t unused;
+};
 struct CachePlan {
   int32_t* words;
   int R;
-  __host__ __device__ int32_t* first() const { return words + 8; }                 // first row
-  __host__ __device__ int32_t* count() const { return words + 8 + (int64_t)R; }    // rows
-  __host__ __device__ int32_t* length() const { return words + 8 + 2 * (int64_t)R; }  // tokens, the rows among them
-  __host__ __device__ int32_t* per() const { return words + 8 + 3 * (int64_t)R; }     // tokens of a split
-  __host__ __device__ int32_t* part() const { return words + 8 + 4 * (int64_t)R; }    // first partial row
-  __host__ __device__ int32_t* items() const { return words + 8 + 5 * (int64_t)R; }   // (request, split)
+  static constexpr int kHead = 8, kRecord = 8;
+  __host__ __device__ PagedRequest* requests() const { return reinterpret_cast<PagedRequest*>(words + kHead); }
+  __host__ __device__ PagedItem* items() const { return reinterpret_cast<PagedItem*>(words + kHead + (int64_t)kRecord * R); }
 };
+static_assert(sizeof(PagedRequest) == CachePlan::kRecord * 4 && sizeof(PagedItem) == CachePlan::kRecord * 4, "records");
 
 // How a step's attention is cut: at most `splits` + R items.
 struct PagedShape {
@@ -70,7 +81,8 @@ struct PagedParams {
   int64_t capacity;
   float scale;
   int G, max_rows;
+  int items;  // records of items in the plan
 };
-hipError_t launch_paged_attention(const PagedParams& p, int64_t M, const PagedShape& shape, int D, bool q8, hipStream_t stream);
+hipError_t launch_paged_attention(const PagedParams& p, int64_t M, int D, bool q8, hipStream_t stream);
 
 }  // namespace qmm4

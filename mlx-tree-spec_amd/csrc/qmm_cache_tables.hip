@@ -160,7 +160,7 @@ __global__ __launch_bounds__(kThreads) void cache_step_kernel(CacheStepParams S)
     }
   }
   int64_t at_need = block_scan(sum_need, s_scan, &total);
-  int64_t cost = 0, taken = 0;
+  int64_t cost = 0, blocks = 0, taken = 0;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     const int r = tid * kPer + e;
@@ -177,6 +177,7 @@ __global__ __launch_bounds__(kThreads) void cache_step_kernel(CacheStepParams S)
       S.lengths[r] = base[e] + a[e];
       if (S.plan.words) {
         const int64_t rows = s_rows[r] > 0 ? (int64_t)s_rows[r] * S.G : 0;
+        blocks += (rows + kPagedRows - 1) / kPagedRows;
         cost += (int64_t)(base[e] + a[e]) * ((rows + kPagedRows - 1) / kPagedRows);
       }
     }
@@ -206,30 +207,31 @@ __global__ __launch_bounds__(kThreads) void cache_step_kernel(CacheStepParams S)
   }
   if (!S.plan.words) return;
 
-  // The attention's splits: as many tokens each as leave S.splits in all (a request of several row blocks counts as often).
+  // The attention's splits: as many tokens each as leave S.splits in all (a request of several row blocks counts as often). Every
+  // request ends in a split that is not full; where those are few, their number is taken off, so that the splits do not pass
+  // S.splits by them (one workgroup more than the GPU holds at once takes as long again).
   block_scan(cost, s_scan, &total);
-  int64_t chunk = (total + S.splits - 1) / S.splits;
-  chunk = max((int64_t)kPagedUnit, (chunk + kPagedUnit - 1) / kPagedUnit * kPagedUnit);
-  int splits[kPer];
+  int64_t all_blocks;
+  block_scan(blocks, s_scan, &all_blocks);
+  const int64_t aim = S.splits > 2 * all_blocks ? S.splits - all_blocks : S.splits;
+  const int64_t chunk = max((int64_t)kPagedUnit, ((total + aim - 1) / aim + kPagedUnit - 1) / kPagedUnit * kPagedUnit);
+  PagedRequest q[kPer];
   int64_t sum_splits = 0, sum_part = 0;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     const int r = tid * kPer + e;
-    splits[e] = 0;
+    q[e] = {0, 0, 0, kPagedUnit, 0, 0, {0, 0}};
     if (r < R) {
-      const int rows = max(0, s_rows[r]), length = base[e] + a[e];
-      int per = kPagedUnit;
-      if (rows > 0) {
-        const int64_t pieces = (length + chunk - 1) / chunk;
-        per = (int)(((length + pieces - 1) / pieces + kPagedUnit - 1) / kPagedUnit * kPagedUnit);
-        splits[e] = (length + per - 1) / per;
+      q[e].first = s_first[r];
+      q[e].rows = max(0, s_rows[r]);
+      q[e].length = base[e] + a[e];
+      if (q[e].rows > 0) {
+        const int64_t pieces = (q[e].length + chunk - 1) / chunk;
+        q[e].per = (int)(((q[e].length + pieces - 1) / pieces + kPagedUnit - 1) / kPagedUnit * kPagedUnit);
+        q[e].splits = (q[e].length + q[e].per - 1) / q[e].per;
       }
-      S.plan.first()[r] = s_first[r];
-      S.plan.count()[r] = rows;
-      S.plan.length()[r] = length;
-      S.plan.per()[r] = per;
-      sum_splits += splits[e];
-      sum_part += splits[e] > 1 ? (int64_t)splits[e] * rows : 0;
+      sum_splits += q[e].splits;
+      sum_part += q[e].splits > 1 ? (int64_t)q[e].splits * q[e].rows : 0;
     }
   }
   int64_t at_part = block_scan(sum_part, s_scan, &total);
@@ -238,34 +240,36 @@ __global__ __launch_bounds__(kThreads) void cache_step_kernel(CacheStepParams S)
   for (int e = 0; e < kPer; ++e) {
     const int r = tid * kPer + e;
     if (r < R) {
-      S.plan.part()[r] = (int)at_part;
-      at_part += splits[e] > 1 ? (int64_t)splits[e] * max(0, s_rows[r]) : 0;
+      q[e].part = (int)at_part;
+      S.plan.requests()[r] = q[e];
+      at_part += q[e].splits > 1 ? (int64_t)q[e].splits * q[e].rows : 0;
       s_off[r] = (int)at_splits;
-      at_splits += splits[e];
+      at_splits += q[e].splits;
     }
   }
   if (tid == 0) S.plan.words[0] = (int)total;
   __syncthreads();
   for (int i = tid; i < (int)total; i += kThreads) {
-    const int r = last_at_most(s_off, R, i);
-    S.plan.items()[2 * i] = r;
-    S.plan.items()[2 * i + 1] = i - s_off[r];
+    const int r = last_at_most(s_off, R, i), split = i - s_off[r];
+    const PagedRequest& t = S.plan.requests()[r];
+    S.plan.items()[i] = {r, t.first, t.rows, t.length, split * t.per, min(t.length, (split + 1) * t.per),
+                         t.splits > 1 ? t.part + split * t.rows : -1, 0};
   }
 }
 
 // The places of many rows, from the plan.
 __global__ __launch_bounds__(kThreads) void cache_rows_kernel(CacheStepParams S) {
   __shared__ int s_first[kMaxRequests];
-  for (int r = threadIdx.x; r < S.R; r += kThreads) s_first[r] = S.plan.first()[r];
+  for (int r = threadIdx.x; r < S.R; r += kThreads) s_first[r] = S.plan.requests()[r].first;
   __syncthreads();
   const int m = blockIdx.x * kThreads + threadIdx.x;
   if (m >= S.total) return;
   int slot = -1, position = -1, request = -1;
   if (S.R > 0) {
-    const int r = last_at_most(s_first, S.R, m), n = S.plan.count()[r];
+    const int r = last_at_most(s_first, S.R, m), n = S.plan.requests()[r].rows;
     if (m - s_first[r] < n) {
       request = r;
-      position = S.plan.length()[r] - n + (m - s_first[r]);
+      position = S.plan.requests()[r].length - n + (m - s_first[r]);
       slot = slot_of(S, r, position);
     }
   }

@@ -3,10 +3,10 @@
 //
 // Both products run on 16x16x32 matrix instructions with the tokens' side as the first operand:
 //   S^T = K Q^T  (16 tokens x 16 query rows),   O^T = V^T P^T  (16 dimensions x 16 query rows)
-// The cache's layout makes 16 bytes of keys (E dimensions of a token) and of values (E tokens of a dimension) operands as they
-// lie. S^T leaves each lane with probabilities of one query row (lane % 16); the order of tokens within a step of 4 E is chosen
-// (row 4 g + i of tile tt is token E g + 4 tt + i, g = lane / 16) so that they are the second operand of O^T without a move
-// between lanes.
+// The cache's layout makes pieces of keys (8 dimensions of a token) and of values (8 tokens of a dimension) operands as they
+// lie, or behind a conversion from 8 bits. S^T leaves each lane with probabilities of one query row (lane % 16); the order of
+// tokens within a step of 32 is chosen (row 4 g + i of tile tt is token 8 g + 4 tt + i, g = lane / 16) so that they are the
+// second operand of O^T without a move between lanes.
 //
 // The running maximum moves only where a logit passes it by more than 2^8: probabilities up to 256 lose nothing in fp32, and
 // most steps need no exchange between lanes.
@@ -25,14 +25,21 @@ __device__ __forceinline__ f32x4 paged_mma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+// Byte BYTE of w, signed, as a float: one instruction. (Written out: from C++ hipcc 7.2 takes two, and keeps a loaded word's bytes
+// in registers of their own from the load on.)
+template <int BYTE>
+__device__ __forceinline__ float code(uint32_t w) {
+  float f;
+  if constexpr (BYTE == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(w));
+  if constexpr (BYTE == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(w));
+  if constexpr (BYTE == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(w));
+  if constexpr (BYTE == 3) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(w));
+  return f;
+}
 // 8 codes -> bf16 (exact).
 __device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi) {
-  u32x4 r;
-  r.x = pack_bf16x2((float)(int8_t)(lo & 0xFFu), (float)(int8_t)((lo >> 8) & 0xFFu));
-  r.y = pack_bf16x2((float)(int8_t)((lo >> 16) & 0xFFu), (float)(int8_t)(lo >> 24));
-  r.z = pack_bf16x2((float)(int8_t)(hi & 0xFFu), (float)(int8_t)((hi >> 8) & 0xFFu));
-  r.w = pack_bf16x2((float)(int8_t)((hi >> 16) & 0xFFu), (float)(int8_t)(hi >> 24));
-  return as_bf16x8(r);
+  return as_bf16x8(u32x4{pack_bf16x2(code<0>(lo), code<1>(lo)), pack_bf16x2(code<2>(lo), code<3>(lo)),
+                         pack_bf16x2(code<0>(hi), code<1>(hi)), pack_bf16x2(code<2>(hi), code<3>(hi))});
 }
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
@@ -58,8 +65,8 @@ __device__ __forceinline__ bool paged_empty(const int64_t* ancestors, int64_t ro
 template <int D, int QT, bool Q8>
 struct PagedRows {
   static constexpr int E = Q8 ? 16 : 8;  // elements of 16 bytes
-  static constexpr int kStep = 4 * E;    // tokens of a wave's step
-  static constexpr int kKT = E / 4;      // tiles of 16 tokens
+  static constexpr int kStep = 32;       // tokens of a wave's step
+  static constexpr int kKT = 2;          // tiles of 16 tokens
   static constexpr int kKC = D / (4 * E);  // 16-byte pieces of a key for each lane
   static constexpr int kQK = D / 32;     // matrix instructions along D
   static constexpr int kVT = D / 16;     // tiles of 16 dimensions
@@ -67,8 +74,9 @@ struct PagedRows {
   static constexpr int kHandBytes = QT * (kVT * 1024 + 128);
 
   const PagedParams& S;
+  const PagedItem& I;
   const int32_t* table;  // the request's row
-  int r, lane, r16, g, h, n, length, context;
+  int lane, r16, g, h, length, context;
   float unit;  // of a logit, in powers of two
   bf16x8 q[QT][kQK];
   uint64_t bits[QT];  // the step's rows that the row sees (all ones without ancestors)
@@ -77,14 +85,13 @@ struct PagedRows {
   f32x4 o[QT][kVT];
   bool odd = false;  // a value that is not finite was left out
 
-  __device__ __forceinline__ PagedRows(const PagedParams& s, int request, int head) : S(s), r(request), h(head) {
+  __device__ __forceinline__ PagedRows(const PagedParams& s, const PagedItem& item, int head) : S(s), I(item), h(head) {
     lane = threadIdx.x & 63;
     r16 = lane & 15;
     g = lane >> 4;
-    n = S.plan.count()[r];
-    length = S.plan.length()[r];
-    context = length - n;
-    table = S.table + (int64_t)r * S.capacity;
+    length = I.length;
+    context = length - I.rows;
+    table = S.table + (int64_t)I.request * S.capacity;
     unit = fabsf(S.scale) * kLog2e;
   }
 
@@ -96,7 +103,7 @@ struct PagedRows {
   __device__ __forceinline__ const uint16_t* query(int at) const {
     int i, hq;
     place(at, &i, &hq);
-    return at < n * S.G ? S.q.x + (int64_t)(S.plan.first()[r] + i) * S.q.row + (int64_t)hq * S.q.head : nullptr;
+    return at < I.rows * S.G ? S.q.x + (int64_t)(I.first + i) * S.q.row + (int64_t)hq * S.q.head : nullptr;
   }
 
   // The wave's query rows from `row0` on, with their sign turned where scale is negative (what the maximum is taken of rises
@@ -111,9 +118,9 @@ struct PagedRows {
       place(at, &i, &hq);
       const uint16_t* x = query(at);
       bits[qt] = ~0ull;
-      seen[qt] = min(length, context + min(i, n) + 1);
+      seen[qt] = min(length, context + min(i, I.rows) + 1);
       if (S.ancestors) {
-        bits[qt] = x ? (uint64_t)S.ancestors[S.plan.first()[r] + i] : 0;
+        bits[qt] = x ? (uint64_t)S.ancestors[I.first + i] : 0;
         seen[qt] = min(length, context + 64);
       }
 #pragma unroll
@@ -128,13 +135,13 @@ struct PagedRows {
       l[qt] = 0.0f;
 #pragma unroll
       for (int dt = 0; dt < kVT; ++dt) o[qt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      end = max(end, min((row0 + qt * 16 + 15) / S.G, n - 1));
+      end = max(end, min((row0 + qt * 16 + 15) / S.G, I.rows - 1));
     }
     return S.ancestors ? length : context + end + 1;
   }
 
-  // The first token of a group of E, within the request's.
-  __device__ __forceinline__ int group(int token) const { return min(token, (length - 1) & ~(E - 1)); }
+  // The first token of a group of 8, within the request's.
+  __device__ __forceinline__ int group(int token) const { return min(token, (length - 1) & ~7); }
   // A page of the cache, whatever the table holds.
   __device__ __forceinline__ int valid_page(int page) const { return max(0, min(page, (int)S.cache.pages - 1)); }
 
@@ -148,7 +155,7 @@ struct PagedRows {
   // The probabilities of a step's tokens from t, whose products are s, as the second operand of the values' product; m, l and
   // o move with them. 8 bits: kscale multiplies the products, vscale the probabilities.
   __device__ __forceinline__ void softmax(int t, int qt, f32x4 (&s)[kKT], const f32x4* kscale, const f32x4* vscale,
-                                          bf16x8 (&p)[E / 8]) {
+                                          bf16x8* p) {
     const bool masked = t + kStep > context;
     if constexpr (Q8) {
 #pragma unroll
@@ -158,7 +165,7 @@ struct PagedRows {
 #pragma unroll
       for (int tt = 0; tt < kKT; ++tt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[tt][i] = sees(qt, t + E * g + 4 * tt + i) ? s[tt][i] : -__builtin_inff();
+        for (int i = 0; i < 4; ++i) s[tt][i] = sees(qt, t + 8 * g + 4 * tt + i) ? s[tt][i] : -__builtin_inff();
     }
     float top = s[0][0];
 #pragma unroll
@@ -178,39 +185,36 @@ struct PagedRows {
       m[qt] = top;
     }
     const float ref = m[qt] == -__builtin_inff() ? 0.0f : m[qt];
-    float e[E];
+    float e[8];
 #pragma unroll
     for (int tt = 0; tt < kKT; ++tt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) e[tt * 4 + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], unit, -ref));
     if (masked) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) e[j] = sees(qt, t + E * g + j) ? e[j] : 0.0f;
+      for (int j = 0; j < 8; ++j) e[j] = sees(qt, t + 8 * g + j) ? e[j] : 0.0f;
     }
 #pragma unroll
-    for (int j = 0; j < E; ++j) l[qt] += e[j];
+    for (int j = 0; j < 8; ++j) l[qt] += e[j];
     if constexpr (Q8) {
 #pragma unroll
       for (int tt = 0; tt < kKT; ++tt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float x = e[tt * 4 + i] * vscale[tt][i];
-          e[tt * 4 + i] = masked && !sees(qt, t + E * g + 4 * tt + i) ? 0.0f : x;
+          e[tt * 4 + i] = masked && !sees(qt, t + 8 * g + 4 * tt + i) ? 0.0f : x;
         }
     }
+    u32x4 w;
 #pragma unroll
-    for (int half = 0; half < E / 8; ++half) {
-      u32x4 w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(e[half * 8 + 2 * i], e[half * 8 + 2 * i + 1]);
-      p[half] = as_bf16x8(w);
-    }
+    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+    *p = as_bf16x8(w);
   }
 
-  // Zeros in 8 tokens' values (of one dimension, from t + E g on) in place of those past the last, which the cache need not
+  // Zeros in 8 tokens' values (of one dimension, from t + 8 g on) in place of those past the last, which the cache need not
   // hold, and of what is not finite: a probability of zero would not keep it from the rows that do not see it.
   __device__ __forceinline__ u32x4 clean(u32x4 v, int t) {
-    const int past = t + E * g - length;
+    const int past = t + 8 * g - length;
     bool any = false;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -302,25 +306,23 @@ struct PagedRows {
   }
 
   // The rows' results, or where the request has several splits the part of this one.
-  __device__ __forceinline__ void write(int row0, int split) const {
+  __device__ __forceinline__ void write(int row0) const {
     const int64_t heads = (int64_t)S.cache.heads * S.G;
-    const int first = S.plan.first()[r];
-    const bool whole = S.plan.per()[r] >= length;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const int at = row0 + qt * 16 + r16;
-      if (at >= n * S.G) continue;
+      if (at >= I.rows * S.G) continue;
       int i, hq;
       place(at, &i, &hq);
-      if (whole) {
-        const float inv = paged_empty(S.ancestors, first + i, length, n) ? 0.0f : 1.0f / l[qt];
-        uint16_t* out = S.out + ((int64_t)(first + i) * heads + hq) * D + 4 * g;
-        const uint16_t* gate = S.gate.x ? S.gate.x + (int64_t)(first + i) * S.gate.row + (int64_t)hq * S.gate.head + 4 * g : nullptr;
+      if (I.part < 0) {
+        const float inv = paged_empty(S.ancestors, I.first + i, length, I.rows) ? 0.0f : 1.0f / l[qt];
+        uint16_t* out = S.out + ((int64_t)(I.first + i) * heads + hq) * D + 4 * g;
+        const uint16_t* gate = S.gate.x ? S.gate.x + (int64_t)(I.first + i) * S.gate.row + (int64_t)hq * S.gate.head + 4 * g : nullptr;
 #pragma unroll
         for (int dt = 0; dt < kVT; ++dt)
           *reinterpret_cast<u32x2*>(out + dt * 16) = gated_bf16(o[qt][dt] * inv, gate ? gate + dt * 16 : nullptr);
       } else {
-        const int64_t part = ((int64_t)S.plan.part()[r] + (int64_t)split * n + i) * heads + hq;
+        const int64_t part = ((int64_t)I.part + i) * heads + hq;
 #pragma unroll
         for (int dt = 0; dt < kVT; ++dt) *reinterpret_cast<f32x4*>(S.part + part * D + dt * 16 + g * 4) = o[qt][dt];
         if (g == 0) {
@@ -332,8 +334,7 @@ struct PagedRows {
   }
 };
 
-// The kernel of up to 16 query rows to a key head, and that of more.
-hipError_t launch_paged_rows(const PagedParams& p, int64_t items, int D, bool q8, hipStream_t stream);
-hipError_t launch_paged_tile(const PagedParams& p, int64_t items, int D, bool q8, hipStream_t stream);
+// The kernel of more than 16 query rows to a key head.
+hipError_t launch_paged_tile(const PagedParams& p, int D, bool q8, hipStream_t stream);
 
 }  // namespace qmm4

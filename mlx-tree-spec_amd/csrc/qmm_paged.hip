@@ -7,6 +7,9 @@
 // runs of 64 bytes and more, without LDS, and takes every KW-th step of its workgroup's split; while a step's probabilities
 // are made the next step's keys are on their way, and its values while the products with the present ones run. Waves join
 // through LDS, splits through memory (fp32) and a second kernel.
+#include <type_traits>
+
+#include "qmm4_lds.h"
 #include "qmm_paged.h"
 
 namespace qmm4 {
@@ -17,16 +20,17 @@ template <int D, bool Q8>
 struct RowsTraits {
   using R = PagedRows<D, 1, Q8>;
   // Registers of o, q, s, keys, values and scales; with what else there is more than 256: one wave to a SIMD.
-  static constexpr int kRegisters = 4 * (R::kVT + R::kQK + R::kKT + R::kKT * R::kKC + R::kVT + (Q8 ? 3 * R::kKT : 0));
-  static constexpr int kWaves = kRegisters > 176 ? 4 : 8;
-  static constexpr size_t kJoin = (size_t)(kWaves / 2) * R::kHandBytes;
+  static constexpr int kRegisters = 4 * (R::kVT + R::kQK + R::kKT + R::kKT * R::kKC + (Q8 ? R::kVT / 2 + 3 * R::kKT : R::kVT));
+  static constexpr int kWaves = kRegisters > 200 ? 4 : 8;
+  static constexpr size_t kLds = (size_t)(kWaves / 2) * R::kHandBytes;
 };
 
 template <int D, bool Q8>
 struct PagedWave : PagedRows<D, 1, Q8> {
   using R = PagedRows<D, 1, Q8>;
-  static constexpr int E = R::E;
-  u32x4 kf[R::kKT][R::kKC], vf[R::kVT];
+  using Piece = std::conditional_t<Q8, u32x2, u32x4>;  // 8 tokens of a dimension
+  u32x4 kf[R::kKT][R::kKC];
+  Piece vf[R::kVT];
   f32x4 ks[Q8 ? R::kKT : 1], vs[Q8 ? R::kKT : 1];
 
   using R::R;
@@ -37,9 +41,9 @@ struct PagedWave : PagedRows<D, 1, Q8> {
 
   __device__ __forceinline__ void load_keys(int t, int page) {
     const CacheArrays& C = this->S.cache;
-    const int shift = C.page_shift, tok = this->group(t + E * (this->r16 >> 2)) & ((1 << shift) - 1);
+    const int shift = C.page_shift, tok = this->group(t + 8 * (this->r16 >> 2)) & ((1 << shift) - 1);
     const char* p = static_cast<const char*>(C.keys) +
-                    (((((int64_t)page * C.heads + this->h) * (D / E) + this->g) << shift) + tok + (this->r16 & 3)) * 16;
+                    (((((int64_t)page * C.heads + this->h) * (D / R::E) + this->g) << shift) + tok + (this->r16 & 3)) * 16;
 #pragma unroll
     for (int c = 0; c < R::kKC; ++c)
 #pragma unroll
@@ -48,17 +52,17 @@ struct PagedWave : PagedRows<D, 1, Q8> {
 
   __device__ __forceinline__ void load_values(int t, int page) {
     const CacheArrays& C = this->S.cache;
-    const int shift = C.page_shift, tok = this->group(t + E * this->g) & ((1 << shift) - 1);
+    const int shift = C.page_shift, tok = this->group(t + 8 * this->g) & ((1 << shift) - 1);
     const char* p = static_cast<const char*>(C.values) +
-                    ((((((int64_t)page * C.heads + this->h) << shift) + tok) / E) * D + this->r16) * 16;
+                    ((((((int64_t)page * C.heads + this->h) << shift) + tok) / R::E) * D + this->r16) * 16 + (Q8 ? tok & 8 : 0);
 #pragma unroll
-    for (int dt = 0; dt < R::kVT; ++dt) vf[dt] = *reinterpret_cast<const u32x4*>(p + dt * 256);
+    for (int dt = 0; dt < R::kVT; ++dt) vf[dt] = *reinterpret_cast<const Piece*>(p + dt * 256);
   }
 
   __device__ __forceinline__ void load_scales(int t, int page) {
     if constexpr (Q8) {
       const CacheArrays& C = this->S.cache;
-      const int shift = C.page_shift, tok = this->group(t + E * this->g) & ((1 << shift) - 1);
+      const int shift = C.page_shift, tok = this->group(t + 8 * this->g) & ((1 << shift) - 1);
       const int64_t at = (((int64_t)page * C.heads + this->h) << shift) + tok;
 #pragma unroll
       for (int tt = 0; tt < R::kKT; ++tt) {
@@ -76,7 +80,7 @@ struct PagedWave : PagedRows<D, 1, Q8> {
 #pragma unroll
     for (int tt = 0; tt < R::kKT; ++tt) s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int c = 0; c < R::kKC; ++c)
+    for (int c = 0; c < R::kKC; ++c) {
 #pragma unroll
       for (int tt = 0; tt < R::kKT; ++tt) {
         if constexpr (Q8) {
@@ -86,6 +90,8 @@ struct PagedWave : PagedRows<D, 1, Q8> {
           s[tt] = paged_mma(as_bf16x8(kf[tt][c]), this->q[0][c], s[tt]);
         }
       }
+      if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);  // (few codes at a time in registers)
+    }
     if constexpr (Q8) {
 #pragma unroll
       for (int tt = 0; tt < R::kKT; ++tt) {
@@ -99,38 +105,41 @@ struct PagedWave : PagedRows<D, 1, Q8> {
       next_page = *vp;
       load_keys(t + stride, *kp);
       load_scales(t + stride, next_page);
-      *kp = page(t + 2 * stride + E * (this->r16 >> 2));
-      *vp = page(t + 2 * stride + E * this->g);
+      *kp = page(t + 2 * stride + 8 * (this->r16 >> 2));
+      *vp = page(t + 2 * stride + 8 * this->g);
     }
     __builtin_amdgcn_sched_barrier(0);
-    bf16x8 p[E / 8];
-    this->softmax(t, 0, s, kscale, vscale, p);
-    if (!Q8 && t + R::kStep > this->context) {
+    bf16x8 p;
+    this->softmax(t, 0, s, kscale, vscale, &p);
+    if constexpr (!Q8) {
+      if (t + R::kStep > this->context) {
 #pragma unroll
-      for (int dt = 0; dt < R::kVT; ++dt) vf[dt] = this->clean(vf[dt], t);
+        for (int dt = 0; dt < R::kVT; ++dt) vf[dt] = this->clean(vf[dt], t);
+      }
     }
 #pragma unroll
     for (int dt = 0; dt < R::kVT; ++dt) {
-      if constexpr (Q8) {
-        this->o[0][dt] = paged_mma(codes8(vf[dt][0], vf[dt][1]), p[0], this->o[0][dt]);
-        this->o[0][dt] = paged_mma(codes8(vf[dt][2], vf[dt][3]), p[E / 8 - 1], this->o[0][dt]);
-      } else {
-        this->o[0][dt] = paged_mma(as_bf16x8(vf[dt]), p[0], this->o[0][dt]);
-      }
+      if constexpr (Q8) this->o[0][dt] = paged_mma(codes8(vf[dt][0], vf[dt][1]), p, this->o[0][dt]);
+      else this->o[0][dt] = paged_mma(as_bf16x8(vf[dt]), p, this->o[0][dt]);
+      if (Q8 && dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (MORE) load_values(t + stride, next_page);
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  // Steps t, t + stride, .. below end.
+  // Steps t, t + stride, .. below end; the query rows are loaded behind the first keys and values.
   __device__ __forceinline__ void run(int t, int end, int stride) {
-    if (t >= end) return;
-    const int vpage = page(t + E * this->g);
-    load_keys(t, page(t + E * (this->r16 >> 2)));
-    load_scales(t, vpage);
-    load_values(t, vpage);
-    int kp = page(t + stride + E * (this->r16 >> 2)), vp = page(t + stride + E * this->g);
+    const bool any = t < end;
+    if (any) {
+      const int vpage = page(t + 8 * this->g);
+      load_keys(t, page(t + 8 * (this->r16 >> 2)));
+      load_scales(t, vpage);
+      load_values(t, vpage);
+    }
+    this->load_rows(0);
+    if (!any) return;
+    int kp = page(t + stride + 8 * (this->r16 >> 2)), vp = page(t + stride + 8 * this->g);
     for (; t + stride < end; t += stride) step<true>(t, stride, &kp, &vp);
     step<false>(t, stride, &kp, &vp);
   }
@@ -140,16 +149,14 @@ template <int D, bool Q8>
 __global__ __launch_bounds__((RowsTraits<D, Q8>::kWaves * 64)) void paged_rows_kernel(PagedParams S) {
   using T = RowsTraits<D, Q8>;
   using R = PagedRows<D, 1, Q8>;
-  __shared__ __attribute__((aligned(16))) char s_join[T::kJoin];
+  extern __shared__ __attribute__((aligned(16))) char s_join[];
   const int item = blockIdx.x / S.cache.heads;
+  const PagedItem I = S.plan.items()[item];
   if (item >= S.plan.words[0]) return;
-  const int split = S.plan.items()[2 * item + 1];
-  PagedWave<D, Q8> W(S, S.plan.items()[2 * item], blockIdx.x - item * S.cache.heads);
-  const int wave = threadIdx.x >> 6, per = S.plan.per()[W.r];
-  const int sees = W.load_rows(0), begin = split * per, end = min(min(begin + per, W.length), sees);
-  const int t = begin + wave * R::kStep, stride = T::kWaves * R::kStep;
-  W.run(t, end, stride);
-  W.add_odd_values(t, end, stride, 0);
+  PagedWave<D, Q8> W(S, I, blockIdx.x - item * S.cache.heads);
+  const int wave = threadIdx.x >> 6, t = I.begin + wave * R::kStep, stride = T::kWaves * R::kStep;
+  W.run(t, I.end, stride);
+  W.add_odd_values(t, I.end, stride, 0);
   W.sum_lanes();
   // The upper half of the waves hands over to the lower.
 #pragma unroll
@@ -159,15 +166,16 @@ __global__ __launch_bounds__((RowsTraits<D, Q8>::kWaves * 64)) void paged_rows_k
     __syncthreads();
     if (wave < half) W.take_over(s_join + wave * R::kHandBytes);
   }
-  if (wave == 0) W.write(0, split);
+  if (wave == 0) W.write(0);
 }
 
 constexpr int kJoinThreads = 256;
 
-// The splits of each row and head joined; zeros for rows without a request. kLanes lanes of 4 dimensions to a split.
+// The splits of each row and head joined; zeros for rows without a request. kLanes lanes of 4 dimensions to a split, kAhead
+// splits of each loaded together.
 template <int D>
 __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedParams S, int64_t m0) {
-  constexpr int kLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, kSlices = kJoinThreads / kLanes;
+  constexpr int kLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, kSlices = kJoinThreads / kLanes, kAhead = 8;
   __shared__ f32x4 s_o[kSlices][kLanes];
   __shared__ float s_m[kSlices], s_l[kSlices];
   const int64_t row = m0 + blockIdx.y, heads_q = gridDim.x;
@@ -178,22 +186,38 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedParams S,
     if (slice == 0 && c * 4 < D) *reinterpret_cast<u32x2*>(out) = u32x2{0u, 0u};
     return;
   }
-  const int n = S.plan.count()[r], length = S.plan.length()[r], per = S.plan.per()[r];
-  if (per >= length) return;
-  const int i = (int)row - S.plan.first()[r], splits = (length + per - 1) / per;
-  const int64_t part = ((int64_t)S.plan.part()[r] + i) * heads_q + hq, stride = (int64_t)n * heads_q;
+  const PagedRequest Q = S.plan.requests()[r];
+  if (Q.splits <= 1) return;
+  const int64_t part = ((int64_t)Q.part + (row - Q.first)) * heads_q + hq, stride = (int64_t)Q.rows * heads_q;
   float m = -__builtin_inff(), l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = slice; s < splits; s += kSlices) {
-    const int64_t at = part + s * stride;
-    const float m2 = S.part_ml[at * 2], l2 = S.part_ml[at * 2 + 1];
-    const f32x4 o2 = c * 4 < D ? *reinterpret_cast<const f32x4*>(S.part + at * D + c * 4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const float top = fmaxf(m, m2);
-    const float f1 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-    const float f2 = m2 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m2 - top);
+  for (int s0 = slice; s0 < Q.splits; s0 += kSlices * kAhead) {
+    float m2[kAhead], l2[kAhead];
+    f32x4 o2[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      // (Past the last: the first again, with nothing in it.)
+      const bool here = s0 + j * kSlices < Q.splits;
+      const int64_t at = part + (here ? s0 + j * kSlices : s0) * stride;
+      m2[j] = here ? S.part_ml[at * 2] : -__builtin_inff();
+      l2[j] = S.part_ml[at * 2 + 1];
+      o2[j] = *reinterpret_cast<const f32x4*>(S.part + at * D + (c * 4 < D ? c * 4 : 0));
+    }
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) top = fmaxf(top, m2[j]);
+    const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
     m = top;
-    l = l * f1 + l2 * f2;
-    o = o * f1 + o2 * f2;
+    l *= f;
+    o *= f;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      // (What a split without a visible token holds is zeros, not to be multiplied by more than one.)
+      if (m2[j] == -__builtin_inff()) continue;
+      const float f2 = __builtin_amdgcn_exp2f(m2[j] - top);
+      l += l2[j] * f2;
+      o += o2[j] * f2;
+    }
   }
   s_o[slice][c] = o;
   if (c == 0) {
@@ -213,18 +237,27 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedParams S,
     l += s_l[s] * f;
     o += s_o[s][c] * f;
   }
-  o *= paged_empty(S.ancestors, row, length, n) ? 0.0f : 1.0f / l;
+  o *= paged_empty(S.ancestors, row, Q.length, Q.rows) ? 0.0f : 1.0f / l;
   *reinterpret_cast<u32x2*>(out) =
       gated_bf16(o, S.gate.x ? S.gate.x + row * S.gate.row + (int64_t)hq * S.gate.head + c * 4 : nullptr);
 }
 
+template <int D, bool Q8>
+hipError_t launch_rows(const PagedParams& p, hipStream_t stream) {
+  using T = RowsTraits<D, Q8>;
+  static LdsAllowance allowance;
+  if (T::kLds > 64 * 1024)
+    if (hipError_t e = allowance.allow(reinterpret_cast<const void*>(&paged_rows_kernel<D, Q8>), T::kLds)) return e;
+  hipLaunchKernelGGL((paged_rows_kernel<D, Q8>), dim3((unsigned)p.items * p.cache.heads), dim3(T::kWaves * 64), T::kLds, stream, p);
+  return hipGetLastError();
+}
+
 template <int D>
-void launch_rows(const PagedParams& p, int64_t items, bool q8, hipStream_t stream) {
-  const dim3 grid((unsigned)(items * p.cache.heads));
+hipError_t launch_dim(const PagedParams& p, bool q8, hipStream_t stream) {
   if constexpr (D % 64 == 0) {
-    if (q8) hipLaunchKernelGGL((paged_rows_kernel<D, true>), grid, dim3(RowsTraits<D, true>::kWaves * 64), 0, stream, p);
+    if (q8) return launch_rows<D, true>(p, stream);
   }
-  if (!q8) hipLaunchKernelGGL((paged_rows_kernel<D, false>), grid, dim3(RowsTraits<D, false>::kWaves * 64), 0, stream, p);
+  return launch_rows<D, false>(p, stream);
 }
 
 template <int D>
@@ -248,22 +281,20 @@ int64_t paged_partial_rows(const PagedShape& s, int64_t M, int64_t R, int64_t ma
   return by_block < by_rows ? by_block : by_rows;
 }
 
-hipError_t launch_paged_rows(const PagedParams& p, int64_t items, int D, bool q8, hipStream_t stream) {
+static hipError_t launch_paged_rows(const PagedParams& p, int D, bool q8, hipStream_t stream) {
   switch (D) {
-    case 64: launch_rows<64>(p, items, q8, stream); break;
-    case 96: launch_rows<96>(p, items, q8, stream); break;
-    case 128: launch_rows<128>(p, items, q8, stream); break;
-    case 192: launch_rows<192>(p, items, q8, stream); break;
-    default: launch_rows<256>(p, items, q8, stream);
+    case 64: return launch_dim<64>(p, q8, stream);
+    case 96: return launch_dim<96>(p, q8, stream);
+    case 128: return launch_dim<128>(p, q8, stream);
+    case 192: return launch_dim<192>(p, q8, stream);
+    default: return launch_dim<256>(p, q8, stream);
   }
-  return hipGetLastError();
 }
 
-hipError_t launch_paged_attention(const PagedParams& p, int64_t M, const PagedShape& shape, int D, bool q8, hipStream_t stream) {
-  const int64_t items = shape.splits + p.plan.R, rows = (int64_t)p.max_rows * p.G;
+hipError_t launch_paged_attention(const PagedParams& p, int64_t M, int D, bool q8, hipStream_t stream) {
+  const int64_t rows = (int64_t)p.max_rows * p.G;
   if (p.plan.R > 0 && rows > 0) {
-    const hipError_t e = rows <= 16 ? launch_paged_rows(p, items, D, q8, stream)
-                                    : launch_paged_tile(p, items, D, q8, stream);
+    const hipError_t e = rows <= 16 ? launch_paged_rows(p, D, q8, stream) : launch_paged_tile(p, D, q8, stream);
     if (e != hipSuccess) return e;
   }
   switch (D) {

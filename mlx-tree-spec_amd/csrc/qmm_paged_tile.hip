@@ -27,16 +27,17 @@ struct TileTraits {
   static constexpr int kAcross = kWaves / SIDES;          // waves side by side along the rows
   static constexpr int kRows = kAcross * 16 * QT;
   static constexpr int kStage = 2 * R::kStep;             // tokens
-  static constexpr int kPieces = D * 16;                  // 16-byte pieces of a stage: keys, then values
-  static constexpr int kScaleBytes = Q8 ? kStage * 8 : 0;
-  static constexpr int kStageBytes = kPieces * 16 + kScaleBytes;
-  static constexpr int kLoads = D / 32 + (Q8 ? 1 : 0);    // a wave's loads of a stage
+  static constexpr int kPieces = D * 128 / R::E;          // 16-byte pieces of a stage: keys, then values
+  static constexpr int kChunks = kPieces / 64;            // loads of them
+  static constexpr int kStageBytes = kPieces * 16 + (Q8 ? 1024 : 0);  // (scales: 512 bytes, twice)
+  static constexpr int kChunkLoads = (kChunks + kWaves - 1) / kWaves;
+  static constexpr int kLoads = kChunkLoads + (Q8 ? 1 : 0);  // a wave's loads of a stage
   static constexpr int kRoom = 160 * 1024 - kIds * 4 - 512;
   static constexpr int kStages = kRoom / kStageBytes < 4 ? kRoom / kStageBytes : 4;
   static constexpr size_t kRing = (size_t)kStages * kStageBytes;
   static constexpr size_t kJoin = SIDES > 1 ? (size_t)kAcross * R::kHandBytes : 0;
   static constexpr size_t kLds = (kRing > kJoin ? kRing : kJoin) + kIds * 4;
-  static_assert(kStages >= 2 && kPieces / 64 == kWaves * (D / 32) && kLds <= 160 * 1024, "whole loads, LDS");
+  static_assert(kStages >= 2 && kChunks % kWaves == 0 && kLds <= 160 * 1024, "whole loads, LDS");
 };
 
 template <int N>
@@ -63,20 +64,20 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   // ones find the cache's bytes in its L2.
   const int unit = blockIdx.x / (8 * blocks) * 8 + (blockIdx.x & 7), block = block0 + blockIdx.x / 8 % blocks;
   const int item = unit / S.cache.heads;
+  const PagedItem I = S.plan.items()[item < S.items ? item : 0];
   if (item >= S.plan.words[0]) return;
-  const int split = S.plan.items()[2 * item + 1];
-  R W(S, S.plan.items()[2 * item], unit - item * S.cache.heads);
-  const int row0 = block * T::kRows, rows = W.n * S.G;
+  R W(S, I, unit - item * S.cache.heads);
+  const int row0 = block * T::kRows, rows = I.rows * S.G;
   if (row0 >= rows) return;
   const int wave = threadIdx.x >> 6, side = wave / T::kAcross, rw = wave % T::kAcross;
   const int mine = row0 + rw * 16 * QT;
   const bool active = mine < rows;
   W.load_rows(mine);
 
-  const int per = S.plan.per()[W.r], begin = split * per;
-  int end = min(begin + per, W.length);
+  const int begin = I.begin;
+  int end = I.end;
   // (Without ancestors nothing past the block's last row is seen.)
-  if (!S.ancestors) end = min(end, W.context + min((row0 + T::kRows - 1) / S.G, W.n - 1) + 1);
+  if (!S.ancestors) end = min(end, W.context + min((row0 + T::kRows - 1) / S.G, I.rows - 1) + 1);
   const int shift = S.cache.page_shift, page_mask = (1 << shift) - 1, lane = W.lane;
   const char* keys = static_cast<const char*>(S.cache.keys);
   const char* values = static_cast<const char*>(S.cache.values);
@@ -84,7 +85,8 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   // One step, from a stage in LDS.
   auto step = [&](const u32x4* ring, int sd, int t) __attribute__((always_inline)) {
     const u32x4* kr = ring + W.g * T::kStage + sd * R::kStep + W.r16;
-    const u32x4* vr = ring + T::kPieces / 2 + (sd * 4 + W.g) * D + W.r16;
+    // (8 bits: two groups of 8 tokens share a piece.)
+    const u32x4* vr = ring + T::kPieces / 2 + (Q8 ? sd * 2 + (W.g >> 1) : sd * 4 + W.g) * D + W.r16;
     f32x4 s[QT][R::kKT], ks[Q8 ? R::kKT : 1], vs[Q8 ? R::kKT : 1];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
@@ -110,33 +112,29 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
       if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);  // (few codes at a time in registers)
     }
     if constexpr (Q8) {
-      const f32x4* scales = reinterpret_cast<const f32x4*>(ring + T::kPieces) + sd * 16 + W.g * 4;
+      const f32x4* scales = reinterpret_cast<const f32x4*>(ring + T::kPieces) + sd * 8 + W.g * 2;
 #pragma unroll
       for (int tt = 0; tt < R::kKT; ++tt) {
         ks[tt] = scales[tt];
-        vs[tt] = scales[32 + tt];
+        vs[tt] = scales[16 + tt];
       }
     }
-    bf16x8 p[QT][E / 8];
+    bf16x8 p[QT];
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) W.softmax(t, qt, s[qt], ks, vs, p[qt]);
+    for (int qt = 0; qt < QT; ++qt) W.softmax(t, qt, s[qt], ks, vs, &p[qt]);
     const auto values = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
       for (int dt = 0; dt < R::kVT; ++dt) {
-        u32x4 v = vr[dt * 16];
+        bf16x8 v;
         if constexpr (Q8) {
-          const bf16x8 lo = codes8(v[0], v[1]), hi = codes8(v[2], v[3]);
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) {
-            W.o[qt][dt] = paged_mma(lo, p[qt][0], W.o[qt][dt]);
-            W.o[qt][dt] = paged_mma(hi, p[qt][E / 8 - 1], W.o[qt][dt]);
-          }
-          if (dt % 2) __builtin_amdgcn_sched_barrier(0);
+          const u32x2 codes = reinterpret_cast<const u32x2*>(vr + dt * 16)[W.g & 1];
+          v = codes8(codes[0], codes[1]);
         } else {
-          if constexpr (decltype(masked)::value) v = W.clean(v, t);
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) W.o[qt][dt] = paged_mma(as_bf16x8(v), p[qt][0], W.o[qt][dt]);
+          v = as_bf16x8(decltype(masked)::value ? W.clean(vr[dt * 16], t) : vr[dt * 16]);
         }
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) W.o[qt][dt] = paged_mma(v, p[qt], W.o[qt][dt]);
+        if (Q8 && dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
     };
     if (!Q8 && t + R::kStep > W.context) values(std::true_type{});
@@ -158,33 +156,27 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
       const int t = from + st * T::kStage;
       char* ring = s_ring + (st % T::kStages) * T::kStageBytes;
       const auto head_of = [&](int tok) { return (int64_t)s_ids[(tok - base) >> shift] * S.cache.heads + W.h; };
-      // A key's lane: its token in the order of the tiles' rows, the same in every piece (8 bits: in both halves of a stage).
-      const char* kp[E / 8];
+      // A key's lane: its token in the order of the tiles' rows, the same in every piece.
+      const int sd = lane / R::kStep, row = lane & 15;
+      const int grp = min(W.group(t + sd * R::kStep + 8 * (row >> 2)), base + segment - 8);
+      const char* kp = keys + ((head_of(grp) * (D / E) << shift) + (grp & page_mask) + 4 * (lane / 16 % R::kKT) + (row & 3)) * 16;
 #pragma unroll
-      for (int half = 0; half < E / 8; ++half) {
-        const int slot = half * 64 + lane, row = slot & 15, tt = slot / 16 % R::kKT, sd = slot / R::kStep;
-        const int grp = min(W.group(t + sd * R::kStep + E * (row >> 2)), base + segment - E);
-        kp[half] = keys + ((head_of(grp) * (D / E) << shift) + (grp & page_mask) + 4 * tt + (row & 3)) * 16;
-      }
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
+      for (int j = 0; j < T::kChunkLoads; ++j) {
         const int chunk = wave + kWaves * j;
         const char* src;
-        if (chunk < D / 8) {
-          const int piece = chunk / (E / 8), half = chunk % (E / 8);
-          src = kp[0] + ((int64_t)piece << (shift + 4));
-          if constexpr (Q8) src = (half ? kp[1] : kp[0]) + ((int64_t)piece << (shift + 4));
+        if (chunk < T::kChunks / 2) {
+          src = kp + ((int64_t)chunk << (shift + 4));
         } else {
-          const int f = (chunk - D / 8) * 64 + lane, grp = f / D, d = f - grp * D;
-          const int tok = min(W.group(t + grp * E), base + segment - E);
+          const int f = (chunk - T::kChunks / 2) * 64 + lane, at = f / D, d = f - at * D;
+          const int tok = min(W.group(t + at * E), base + segment - E) & ~(E - 1);
           src = values + (((head_of(tok) << shift) + (tok & page_mask)) / E * D + d) * 16;
         }
         __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(ring + chunk * 1024), 16, 0, 0);
       }
       if constexpr (Q8) {
-        // (One wave's load would do: every wave's loads are counted alike.)
-        const int tok = min(W.group(t + (lane & 28) * 4), base + segment - E) + (lane & 3) * 4;
-        const float* src = (lane < 32 ? S.cache.key_scales : S.cache.value_scales) + (head_of(tok) << shift) + (tok & page_mask);
+        // 4 tokens a lane: key scales, value scales, and both again (every lane of a load writes).
+        const int tok = min(W.group(t + (lane & 14) * 4), base + segment - 8) + (lane & 1) * 4;
+        const float* src = (lane & 16 ? S.cache.value_scales : S.cache.key_scales) + (head_of(tok) << shift) + (tok & page_mask);
         __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(ring + T::kPieces * 16), 16, 0, 0);
       }
     };
@@ -214,15 +206,15 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
     __syncthreads();
     if (side == 0) W.take_over(s_ring + rw * R::kHandBytes);
   }
-  if (side == 0 && active) W.write(mine, split);
+  if (side == 0 && active) W.write(mine);
 }
 
 template <int D, int QT, int SIDES, bool Q8>
-hipError_t launch_tile(const PagedParams& p, int64_t items, hipStream_t stream) {
+hipError_t launch_tile(const PagedParams& p, hipStream_t stream) {
   using T = TileTraits<D, QT, SIDES, Q8>;
   static LdsAllowance allowance;
   if (hipError_t e = allowance.allow(reinterpret_cast<const void*>(&paged_tile_kernel<D, QT, SIDES, Q8>), T::kLds)) return e;
-  const int64_t units = (items * p.cache.heads + 7) / 8 * 8, blocks = ((int64_t)p.max_rows * p.G + T::kRows - 1) / T::kRows;
+  const int64_t units = ((int64_t)p.items * p.cache.heads + 7) / 8 * 8, blocks = ((int64_t)p.max_rows * p.G + T::kRows - 1) / T::kRows;
   const int64_t most = std::max<int64_t>(1, (int64_t{1} << 22) / units);  // (a grid may have 2^32 threads)
   for (int64_t b0 = 0; b0 < blocks; b0 += most) {
     const int64_t count = std::min(most, blocks - b0);
@@ -233,31 +225,31 @@ hipError_t launch_tile(const PagedParams& p, int64_t items, hipStream_t stream) 
 }
 
 template <int D, bool Q8>
-hipError_t launch_rows(const PagedParams& p, int64_t items, hipStream_t stream) {
+hipError_t launch_rows(const PagedParams& p, hipStream_t stream) {
   // Two sides where 4 waves of 16 rows hold a request's; past that 32 rows to a wave, or where their sums and queries would not
   // leave room in 256 registers 16 rows to each of 8.
-  if ((int64_t)p.max_rows * p.G <= 64) return launch_tile<D, 1, 2, Q8>(p, items, stream);
-  if constexpr (D <= 128) return launch_tile<D, 2, 2, Q8>(p, items, stream);
-  else return launch_tile<D, 1, 1, Q8>(p, items, stream);
+  if ((int64_t)p.max_rows * p.G <= 64) return launch_tile<D, 1, 2, Q8>(p, stream);
+  if constexpr (D <= 128) return launch_tile<D, 2, 2, Q8>(p, stream);
+  else return launch_tile<D, 1, 1, Q8>(p, stream);
 }
 
 template <int D>
-hipError_t launch_dim(const PagedParams& p, int64_t items, bool q8, hipStream_t stream) {
+hipError_t launch_dim(const PagedParams& p, bool q8, hipStream_t stream) {
   if constexpr (D % 64 == 0) {
-    if (q8) return launch_rows<D, true>(p, items, stream);
+    if (q8) return launch_rows<D, true>(p, stream);
   }
-  return launch_rows<D, false>(p, items, stream);
+  return launch_rows<D, false>(p, stream);
 }
 
 }  // namespace
 
-hipError_t launch_paged_tile(const PagedParams& p, int64_t items, int D, bool q8, hipStream_t stream) {
+hipError_t launch_paged_tile(const PagedParams& p, int D, bool q8, hipStream_t stream) {
   switch (D) {
-    case 64: return launch_dim<64>(p, items, q8, stream);
-    case 96: return launch_dim<96>(p, items, q8, stream);
-    case 128: return launch_dim<128>(p, items, q8, stream);
-    case 192: return launch_dim<192>(p, items, q8, stream);
-    default: return launch_dim<256>(p, items, q8, stream);
+    case 64: return launch_dim<64>(p, q8, stream);
+    case 96: return launch_dim<96>(p, q8, stream);
+    case 128: return launch_dim<128>(p, q8, stream);
+    case 192: return launch_dim<192>(p, q8, stream);
+    default: return launch_dim<256>(p, q8, stream);
   }
 }
 
