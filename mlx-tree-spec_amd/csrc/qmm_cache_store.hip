@@ -1,9 +1,10 @@
 // New keys and values into the paged cache (include/qmm_cache.h).
 //
-// A key's 16-byte pieces lie in the cache as in the row: they are stored whole. A value's do not: 16 bytes of the cache hold
-// one dimension of E neighbouring tokens. Rows whose tokens share such a piece are stored together by the first of them,
-// whole pieces where all E are there (prompts), single elements where not (decode). Bound by latency up to some hundred rows,
-// by HBM past that.
+// A key's 16-byte pieces lie in the cache as in the row, those of neighbouring tokens side by side. A value's do not: 16 bytes of
+// the cache hold one dimension of E neighbouring tokens. Rows whose tokens share such a piece are a run, and a run is stored by
+// one workgroup: in whole pieces where all E tokens are there (prompts), in single elements where not (decode); lines of the
+// cache are not written in parts by several XCDs. A workgroup takes the runs that begin in its block of rows, up to 16 rows at a
+// time, for some 256 values of each, of keys or of values. Bound by latency up to some hundred rows, by HBM past that.
 #include "qmm4_common.h"
 #include "qmm_cache_kernels.h"
 
@@ -12,65 +13,14 @@ namespace qmm4 {
 namespace {
 
 constexpr int kThreads = 256;
-// Values of a row whose codes the 8-bit form holds in LDS at once.
-constexpr int kTile = 1024;
-
-// How many of the rows from m on the workgroup of row m stores: those whose tokens follow its own within the aligned E, if no
-// earlier row has the token before it there. 0: an earlier row's workgroup stores it.
-template <int E>
-__device__ __forceinline__ int run_of(const int32_t* slots, int64_t m, int64_t M, int slot) {
-  if ((slot & (E - 1)) != 0 && m > 0 && slots[m - 1] == slot - 1) return 0;
-  const int lane = threadIdx.x & 63;
-  const bool follows = lane < E - (slot & (E - 1)) && m + lane < M && slots[m + lane] == slot + lane;
-  return __builtin_ctzll(~__ballot(follows));
-}
-
-__global__ __launch_bounds__(kThreads) void store_kv_kernel(CacheRows K, CacheRows V, const int32_t* slots, CacheArrays C, int64_t M,
-                                                            int D) {
-  const int64_t m = blockIdx.x;
-  const int tid = threadIdx.x, slot = slots[m], page_size = 1 << C.page_shift;
-  if ((uint32_t)slot >= (uint64_t)C.pages << C.page_shift) return;
-  const int64_t head0 = (int64_t)(slot >> C.page_shift) * C.heads;
-  const int off = slot & (page_size - 1), chunks = D / 8;
-  for (int i = tid; i < C.heads * chunks; i += kThreads) {
-    const int h = i / chunks, c = i - h * chunks;
-    const u32x4 x = *reinterpret_cast<const u32x4*>(K.x + m * K.row + h * K.head + c * 8);
-    static_cast<u32x4*>(C.keys)[((head0 + h) * chunks + c) * page_size + off] = x;
-  }
-  const int run = run_of<8>(slots, m, M, slot);
-  if (run == 0) return;
-  // A pair of dimensions each thread.
-  for (int i = tid; i < C.heads * D / 2; i += kThreads) {
-    const int h = i / (D / 2), d = (i - h * (D / 2)) * 2;
-    const uint16_t* x = V.x + m * V.row + h * V.head + d;
-    uint32_t v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < run ? *reinterpret_cast<const uint32_t*>(x + j * V.row) : 0u;
-    uint16_t* y = static_cast<uint16_t*>(C.values) + (((head0 + h) * (page_size / 8) + off / 8) * D + d) * 8;
-    if (run == 8) {
-      u32x4 lo, hi;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        lo[j] = (v[2 * j] & 0xFFFFu) | v[2 * j + 1] << 16;
-        hi[j] = v[2 * j] >> 16 | (v[2 * j + 1] & 0xFFFF0000u);
-      }
-      reinterpret_cast<u32x4*>(y)[0] = lo;
-      reinterpret_cast<u32x4*>(y)[1] = hi;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j < run) {
-          y[(off & 7) + j] = (uint16_t)v[j];
-          y[(off & 7) + j + 8] = (uint16_t)(v[j] >> 16);
-        }
-      }
-    }
-  }
-}
+constexpr int kWindow = 16;  // rows at a time
+constexpr int kWidth = 256;  // values of a row's part
 
 // 16 values of a head, at most 16 lanes a head: their codes, four to a word, and the head's scale (in all its lanes).
-// |x| is compared as bits, where NaN is above infinity above what is finite. The division by the scale is a correctly rounded
-// one, so that a code is off from x / scale by half and 2^-17 at most.
+// |x| is compared as bits, where NaN is above infinity above what is finite. x / scale is a product with the scale's inverse,
+// corrected by its remainder (a division's own steps for every value take four times as many instructions): off by little more
+// than its rounding, so that a code is off from x / scale by half and 2^-17 at most. Both are raised where the inverse would not be
+// finite.
 __device__ __forceinline__ u32x4 codes16(u32x4 a, u32x4 b, float* scale) {
   uint32_t top = 0;
 #pragma unroll
@@ -83,6 +33,7 @@ __device__ __forceinline__ u32x4 codes16(u32x4 a, u32x4 b, float* scale) {
   const bool finite = top < 0x7F80u;
   const float s = finite ? __fdiv_rn(bf16_to_f32(top), 127.0f) : __uint_as_float(0x7FC00000u);
   *scale = s;
+  const float up = s < 0x1p-100f ? 0x1p100f : 1.0f, divisor = s * up, inverse = __fdiv_rn(1.0f, divisor);
   u32x4 out;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -91,8 +42,8 @@ __device__ __forceinline__ u32x4 codes16(u32x4 a, u32x4 b, float* scale) {
     for (int e = 0; e < 4; ++e) {
       const int i = w * 4 + e;
       const uint32_t word = i < 8 ? a[i / 2] : b[i / 2 - 4];
-      const float x = bf16_to_f32(i & 1 ? word >> 16 : word & 0xFFFFu);
-      const float c = finite && s > 0.0f ? rintf(__fdiv_rn(x, s)) : 0.0f;
+      const float x = bf16_to_f32(i & 1 ? word >> 16 : word & 0xFFFFu) * up, y = x * inverse;
+      const float c = finite && s > 0.0f ? rintf(__builtin_fmaf(__builtin_fmaf(-y, divisor, x), inverse, y)) : 0.0f;
       packed |= ((uint32_t)(int)fminf(fmaxf(c, -127.0f), 127.0f) & 0xFFu) << (8 * e);
     }
     out[w] = packed;
@@ -100,69 +51,149 @@ __device__ __forceinline__ u32x4 codes16(u32x4 a, u32x4 b, float* scale) {
   return out;
 }
 
-// The same into codes of 8 bits.
-__global__ __launch_bounds__(kThreads) void store_kv8_kernel(CacheRows K, CacheRows V, const int32_t* slots, CacheArrays C, int64_t M,
-                                                             int D) {
-  __shared__ __attribute__((aligned(16))) uint8_t s_codes[16][kTile + 16];
-  const int64_t m = blockIdx.x;
-  const int tid = threadIdx.x, slot = slots[m], page_size = 1 << C.page_shift;
-  if ((uint32_t)slot >= (uint64_t)C.pages << C.page_shift) return;
-  const int64_t head0 = (int64_t)(slot >> C.page_shift) * C.heads;
-  const int off = slot & (page_size - 1), chunks = D / 16;
-  const int c = tid & 15, group = tid >> 4;
-  const u32x4 none = {0u, 0u, 0u, 0u};
-  for (int h0 = 0; h0 < C.heads; h0 += 16) {
-    const int h = h0 + group;
-    const bool here = h < C.heads && c < chunks;
-    const u32x4* x = reinterpret_cast<const u32x4*>(K.x + m * K.row + h * K.head + c * 16);
-    u32x4 a = none, b = none;
-    if (here) {
-      a = x[0];
-      b = x[1];
+struct StoreParams {
+  CacheRows k, v;
+  const int32_t* slots;
+  CacheArrays cache;
+  int64_t M;
+  int D, block, heads;  // rows of a block; heads of a part
+};
+
+template <bool Q8>
+__global__ __launch_bounds__(kThreads) void store_kv_kernel(StoreParams S) {
+  constexpr int E = Q8 ? 16 : 8;
+  __shared__ __attribute__((aligned(16))) uint8_t s_codes[Q8 ? kWindow : 1][kWidth + 16];
+  __shared__ int s_slot[kWindow], s_run[kWindow + 1];
+  const CacheArrays& C = S.cache;
+  const int tid = threadIdx.x, lane = tid & 63, D = S.D, page_size = 1 << C.page_shift;
+  const int64_t m0 = (int64_t)blockIdx.x * S.block;
+  const bool keys = (blockIdx.y & 1) == 0;
+  const int h0 = (blockIdx.y >> 1) * S.heads, heads = min(S.heads, C.heads - h0);
+  const CacheRows& X = keys ? S.k : S.v;
+  // Where runs begin among the block's rows and those behind it (a run has at most 16; past the last row: one more).
+  const int64_t m = m0 + lane;
+  const int slot = m < S.M ? S.slots[m] : -1, before = m > 0 && m < S.M ? S.slots[m - 1] : -1;
+  const uint64_t begins = __ballot(m == 0 || m >= S.M || (slot & (E - 1)) == 0 || before != slot - 1 || lane >= 48);
+  const int last = S.block + __builtin_ctzll(begins >> S.block);
+  for (int a = __builtin_ctzll(begins); a < last;) {
+    // Whole runs of up to 16 rows.
+    const int most = min(a + kWindow, last);
+    const int e = most == last ? last : 63 - __builtin_clzll(begins & ((2ull << most) - 1)), rows = e - a;
+    const uint64_t mine = (begins >> a) & ((1ull << rows) - 1);
+    const int runs = __builtin_popcountll(mine);
+    if (tid < 64 && lane >= a && lane < e) {
+      s_slot[lane - a] = (uint32_t)slot < (uint64_t)C.pages << C.page_shift ? slot : -1;
+      if (begins >> lane & 1) s_run[__builtin_popcountll(mine & ((1ull << (lane - a)) - 1))] = lane - a;
     }
-    float scale;
-    const u32x4 codes = codes16(a, b, &scale);
-    if (here) {
-      static_cast<u32x4*>(C.keys)[((head0 + h) * chunks + c) * page_size + off] = codes;
-      if (c == 0) C.key_scales[((head0 + h) << C.page_shift) + off] = scale;
-    }
-  }
-  const int run = run_of<16>(slots, m, M, slot);
-  if (run == 0) return;
-  const int per = kTile / D;  // heads of a tile
-  for (int h0 = 0; h0 < C.heads; h0 += per) {
-    const int heads = min(per, C.heads - h0);
+    if (tid == 0) s_run[runs] = rows;
     __syncthreads();
-    for (int i0 = 0; i0 < run * heads; i0 += 16) {
-      const int i = i0 + group, j = i / heads, h = h0 + i - j * heads;
-      const bool here = i < run * heads && c < chunks;
-      const u32x4* x = reinterpret_cast<const u32x4*>(V.x + (m + j) * V.row + h * V.head + c * 16);
-      u32x4 a = none, b = none;
-      if (here) {
-        a = x[0];
-        b = x[1];
-      }
-      float scale;
-      const u32x4 codes = codes16(a, b, &scale);
-      if (here) {
-        *reinterpret_cast<u32x4*>(&s_codes[j][(h - h0) * D + c * 16]) = codes;
-        if (c == 0) C.value_scales[((head0 + h) << C.page_shift) + off + j] = scale;
-      }
-    }
-    __syncthreads();
-    for (int i = tid; i < heads * D; i += kThreads) {
-      const int h = i / D, d = i - h * D;
-      uint8_t* y = static_cast<uint8_t*>(C.values) + (((head0 + h0 + h) * (page_size / 16) + off / 16) * D + d) * 16;
-      if (run == 16) {
-        u32x4 v;
+
+    if (Q8) {
+      // 16 lanes to a head of a row; neighbouring ones: the rows, whose keys' pieces lie side by side.
+      const int c = lane & 15, chunks = D / 16, pairs = rows * heads;
+      constexpr int kAhead = 2, kGroups = kThreads / 16;
+      for (int i0 = 0; i0 < pairs; i0 += kGroups * kAhead) {
+        u32x4 x[kAhead][2];
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-          v[w] = s_codes[4 * w][i] | s_codes[4 * w + 1][i] << 8 | s_codes[4 * w + 2][i] << 16 | (uint32_t)s_codes[4 * w + 3][i] << 24;
-        *reinterpret_cast<u32x4*>(y) = v;
-      } else {
-        for (int j = 0; j < run; ++j) y[(off & 15) + j] = s_codes[j][i];
+        for (int n = 0; n < kAhead; ++n) {
+          const int i = i0 + kGroups * n + tid / 16, h = i / rows, j = i - h * rows;
+          x[n][0] = x[n][1] = u32x4{0u, 0u, 0u, 0u};
+          if (i < pairs && c < chunks && s_slot[j] >= 0) {
+            const u32x4* p = reinterpret_cast<const u32x4*>(X.x + (m0 + a + j) * X.row + (h0 + h) * X.head + c * 16);
+            x[n][0] = p[0];
+            x[n][1] = p[1];
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+          const int i = i0 + kGroups * n + tid / 16, h = i / rows, j = i - h * rows;
+          if (i0 + kGroups * n >= pairs) break;  // (the same for all: their lanes exchange)
+          float scale;
+          const u32x4 codes = codes16(x[n][0], x[n][1], &scale);
+          if (i >= pairs || c >= chunks || s_slot[j] < 0) continue;
+          const int off = s_slot[j] & (page_size - 1);
+          const int64_t head = (int64_t)(s_slot[j] >> C.page_shift) * C.heads + h0 + h;
+          if (c == 0) (keys ? C.key_scales : C.value_scales)[(head << C.page_shift) + off] = scale;
+          if (keys) static_cast<u32x4*>(C.keys)[(head * chunks + c) * page_size + off] = codes;
+          else *reinterpret_cast<u32x4*>(&s_codes[j][h * D + c * 16]) = codes;
+        }
+      }
+      if (!keys) {
+        __syncthreads();
+        for (int i = tid; i < runs * heads * D; i += kThreads) {
+          const int k = i / (heads * D), d = i - k * (heads * D), j0 = s_run[k], run = s_run[k + 1] - j0, at = s_slot[j0];
+          if (at < 0) continue;
+          const int off = at & (page_size - 1), h = d / D;
+          const int64_t head = (int64_t)(at >> C.page_shift) * C.heads + h0 + h;
+          uint8_t* y = static_cast<uint8_t*>(C.values) + ((head * (page_size / 16) + off / 16) * D + (d - h * D)) * 16;
+          if (run == 16) {
+            u32x4 v;
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              v[w] = s_codes[4 * w][d] | s_codes[4 * w + 1][d] << 8 | s_codes[4 * w + 2][d] << 16 | (uint32_t)s_codes[4 * w + 3][d] << 24;
+            *reinterpret_cast<u32x4*>(y) = v;
+          } else {
+            for (int j = 0; j < run; ++j) y[(off & 15) + j] = s_codes[j0 + j][d];
+          }
+        }
+      }
+    } else if (keys) {
+      // Neighbouring lanes: the rows, then the next piece.
+      constexpr int kAhead = 2;
+      const int width = rows > 8 ? 16 : rows > 4 ? 8 : rows > 2 ? 4 : rows;  // (a power of two)
+      const int j = tid & (width - 1), step = kThreads / width, chunks = D / 8, pieces = heads * chunks;
+      const int at = j < rows ? s_slot[j] : -1, off = at & (page_size - 1);
+      const int64_t head0 = (int64_t)(at >> C.page_shift) * C.heads + h0;
+      const uint16_t* row = X.x + (m0 + a + j) * X.row + h0 * X.head;
+      for (int i0 = tid / width; i0 < pieces; i0 += step * kAhead) {
+        u32x4 x[kAhead];
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+          const int i = i0 + n * step, h = i / chunks;
+          if (at >= 0 && i < pieces) x[n] = *reinterpret_cast<const u32x4*>(row + h * X.head + (i - h * chunks) * 8);
+        }
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+          const int i = i0 + n * step;
+          if (at >= 0 && i < pieces) static_cast<u32x4*>(C.keys)[(head0 * chunks + i) * page_size + off] = x[n];
+        }
+      }
+    } else {
+      // A pair of dimensions of a run each thread.
+      const int pairs = heads * (D / 2);
+      for (int i = tid; i < runs * pairs; i += kThreads) {
+        const int k = i / pairs, d2 = (i - k * pairs) * 2, h = d2 / D, d = d2 - h * D, j0 = s_run[k], run = s_run[k + 1] - j0;
+        const int at = s_slot[j0];
+        if (at < 0) continue;
+        const int off = at & (page_size - 1);
+        const uint16_t* x = X.x + (m0 + a + j0) * X.row + (h0 + h) * X.head + d;
+        uint32_t v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < run ? *reinterpret_cast<const uint32_t*>(x + j * X.row) : 0u;
+        const int64_t head = (int64_t)(at >> C.page_shift) * C.heads + h0 + h;
+        uint16_t* y = static_cast<uint16_t*>(C.values) + ((head * (page_size / 8) + off / 8) * D + d) * 8;
+        if (run == 8) {
+          u32x4 lo, hi;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            lo[j] = (v[2 * j] & 0xFFFFu) | v[2 * j + 1] << 16;
+            hi[j] = v[2 * j] >> 16 | (v[2 * j + 1] & 0xFFFF0000u);
+          }
+          reinterpret_cast<u32x4*>(y)[0] = lo;
+          reinterpret_cast<u32x4*>(y)[1] = hi;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (j < run) {
+              y[(off & 7) + j] = (uint16_t)v[j];
+              y[(off & 7) + j + 8] = (uint16_t)(v[j] >> 16);
+            }
+          }
+        }
       }
     }
+    a = e;
+    __syncthreads();
   }
 }
 
@@ -170,8 +201,12 @@ __global__ __launch_bounds__(kThreads) void store_kv8_kernel(CacheRows K, CacheR
 
 hipError_t launch_store_kv(const CacheRows& k, const CacheRows& v, const int32_t* slots, const CacheArrays& cache, int64_t M,
                            int D, bool q8, hipStream_t stream) {
-  if (q8) hipLaunchKernelGGL(store_kv8_kernel, dim3((unsigned)M), dim3(kThreads), 0, stream, k, v, slots, cache, M, D);
-  else hipLaunchKernelGGL(store_kv_kernel, dim3((unsigned)M), dim3(kThreads), 0, stream, k, v, slots, cache, M, D);
+  // A row to a block where there are few.
+  const int block = M <= 256 ? 1 : 16, heads = kWidth / D;
+  const StoreParams p{k, v, slots, cache, M, D, block, heads};
+  const dim3 grid((unsigned)((M + block - 1) / block), (unsigned)((cache.heads + heads - 1) / heads * 2));
+  if (q8) hipLaunchKernelGGL(store_kv_kernel<true>, grid, dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL(store_kv_kernel<false>, grid, dim3(kThreads), 0, stream, p);
   return hipGetLastError();
 }
 
