@@ -203,7 +203,7 @@ int qmm4_paged_attention_bf16(const void* q, int64_t q_row, int64_t q_head, cons
       return set_error(QMM4_ERR_INVALID, "keys, values, out and workspace must be 16-byte aligned, tables to their elements");
     if (pages == 0 || capacity == 0)
       return set_error(QMM4_ERR_INVALID, "a cache without pages has nothing to attend to");
-    const int64_t most = std::min(max_rows, M);
+    const int64_t most = clamp_rows(max_rows);
     if (most * (Hq / Hk) > (1LL << 30))
       return set_error(QMM4_ERR_INVALID, "%lld rows of %lld query heads to a key head: up to 2^30 of both are supported",
                        (long long)most, (long long)(Hq / Hk));

@@ -20,6 +20,16 @@ namespace qmm4 {
 constexpr float kLog2e = 1.44269504f;
 // How far (in powers of two) a logit may pass the running maximum.
 constexpr float kSlack = 8.0f;
+// The running maximum before any token is seen: below every finite logit (in powers of two), finite itself, so that no difference
+// of two is NaN.
+constexpr float kNone = -0x1p127f;
+
+// The largest of three. (v_max3_f32 by itself: fmaxf has every operand made quiet first.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 
 __device__ __forceinline__ f32x4 paged_mma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -109,7 +119,6 @@ struct PagedRows {
   // The wave's query rows from `row0` on, with their sign turned where scale is negative (what the maximum is taken of rises
   // with the logit then). Returns one past the last token that any of them sees.
   __device__ __forceinline__ int load_rows(int row0) {
-    const uint32_t sign = S.scale < 0.0f ? 0x80008000u : 0u;
     int end = 0;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -128,14 +137,19 @@ struct PagedRows {
         const int d = Q8 ? (c / 2) * 64 + g * 16 + (c & 1) * 8 : c * 32 + g * 8;
         u32x4 v = {0u, 0u, 0u, 0u};
         if (x) v = *reinterpret_cast<const u32x4*>(x + d);
-        v ^= sign;
         q[qt][c] = as_bf16x8(v);
       }
-      m[qt] = -__builtin_inff();
+      m[qt] = kNone;
       l[qt] = 0.0f;
 #pragma unroll
       for (int dt = 0; dt < kVT; ++dt) o[qt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       end = max(end, min((row0 + qt * 16 + 15) / S.G, I.rows - 1));
+    }
+    if (S.scale < 0.0f) {  // (behind a branch: nothing else waits for the rows here)
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+        for (int c = 0; c < kQK; ++c) q[qt][c] = as_bf16x8(__builtin_bit_cast(u32x4, q[qt][c]) ^ 0x80008000u);
     }
     return S.ancestors ? length : context + end + 1;
   }
@@ -167,29 +181,34 @@ struct PagedRows {
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[tt][i] = sees(qt, t + 8 * g + 4 * tt + i) ? s[tt][i] : -__builtin_inff();
     }
-    float top = s[0][0];
+    // Arguments of the exponentials beside the present maximum, which stays where none passes it by more than kSlack.
+    float e[8];
+    const auto arguments = [&](float ref) __attribute__((always_inline)) {
 #pragma unroll
-    for (int tt = 0; tt < kKT; ++tt)
+      for (int tt = 0; tt < kKT; ++tt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tt][i]);
-    // (A unit of 0 leaves masked tokens at -infinity too.)
-    top = top == -__builtin_inff() ? top : top * unit;
-    if (__any(top > m[qt] + kSlack)) {
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m[qt]);
-      // (Nothing seen yet: l and o are zero.)
-      const float f = m[qt] == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[qt] - top);
+        for (int i = 0; i < 4; ++i) e[tt * 4 + i] = __builtin_fmaf(s[tt][i], unit, -ref);
+    };
+    arguments(m[qt]);
+    const float top = max3(max3(e[0], e[1], e[2]), max3(e[3], e[4], e[5]), max3(e[6], e[7], e[7]));
+    if (__any(top > kSlack)) {
+      float now = s[0][0];
+#pragma unroll
+      for (int tt = 0; tt < kKT; ++tt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) now = fmaxf(now, s[tt][i]);
+      now = now == -__builtin_inff() ? kNone : now * unit;  // (a unit of 0 as well)
+      now = fmaxf(now, __shfl_xor(now, 16));
+      now = fmaxf(fmaxf(now, __shfl_xor(now, 32)), m[qt]);
+      const float f = __builtin_amdgcn_exp2f(m[qt] - now);
       l[qt] *= f;
 #pragma unroll
       for (int dt = 0; dt < kVT; ++dt) o[qt][dt] *= f;
-      m[qt] = top;
+      m[qt] = now;
+      arguments(now);
     }
-    const float ref = m[qt] == -__builtin_inff() ? 0.0f : m[qt];
-    float e[8];
 #pragma unroll
-    for (int tt = 0; tt < kKT; ++tt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) e[tt * 4 + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], unit, -ref));
+    for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(e[j]);
     if (masked) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) e[j] = sees(qt, t + 8 * g + j) ? e[j] : 0.0f;
@@ -296,8 +315,7 @@ struct PagedRows {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const float m2 = s_ml[qt * 32 + r16], l2 = s_ml[qt * 32 + 16 + r16], top = fmaxf(m[qt], m2);
-      const float f1 = m[qt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[qt] - top);
-      const float f2 = m2 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m2 - top);
+      const float f1 = __builtin_amdgcn_exp2f(m[qt] - top), f2 = __builtin_amdgcn_exp2f(m2 - top);
       m[qt] = top;
       l[qt] = l[qt] * f1 + l2 * f2;
 #pragma unroll

@@ -212,7 +212,6 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedParams S,
     o *= f;
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      // (What a split without a visible token holds is zeros, not to be multiplied by more than one.)
       if (m2[j] == -__builtin_inff()) continue;
       const float f2 = __builtin_amdgcn_exp2f(m2[j] - top);
       l += l2[j] * f2;
@@ -273,7 +272,9 @@ void launch_join(const PagedParams& p, int64_t M, hipStream_t stream) {
 
 PagedShape paged_shape(int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_rows, int cus) {
   const int G = (int)(heads / kv_heads);
-  return {G, (2 * cus + kv_heads - 1) / kv_heads};
+  // A workgroup of the tile kernel fills a CU: splits for one round of them. The rows kernel's run in two.
+  const int64_t rounds = max_rows * G > 16 ? 1 : 2;
+  return {G, (rounds * cus + kv_heads - 1) / kv_heads};
 }
 
 int64_t paged_partial_rows(const PagedShape& s, int64_t M, int64_t R, int64_t max_rows) {

@@ -79,6 +79,8 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   // (Without ancestors nothing past the block's last row is seen.)
   if (!S.ancestors) end = min(end, W.context + min((row0 + T::kRows - 1) / S.G, I.rows - 1) + 1);
   const int shift = S.cache.page_shift, page_mask = (1 << shift) - 1, lane = W.lane;
+  typedef __attribute__((address_space(4))) const int32_t* constant_ptr;
+  const constant_ptr constant_table = (constant_ptr)W.table;  // (nothing in this kernel writes it: scalar loads)
   const char* keys = static_cast<const char*>(S.cache.keys);
   const char* values = static_cast<const char*>(S.cache.values);
 
@@ -141,25 +143,55 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
     else values(std::false_type{});
   };
 
-  const int segment = kIds << shift;  // tokens whose pages are held at once
+  // Pages of a stage's tokens and more: one page for a stage, addresses that only the scalar unit makes.
+  static_assert(T::kStage == 64, "a stage begins at a multiple of its tokens");
+  const bool wide = shift >= 6;
+  const int segment = wide ? 1 << 30 : kIds << shift;  // tokens whose pages are known at once
+  // A lane's token of a key's piece, in the order of the tiles' rows.
+  const int key_token = lane / R::kStep * R::kStep + 8 * ((lane & 15) >> 2) + 4 * (lane / 16 % R::kKT) + (lane & 3);
+  const auto page_at = [&](int tok) { return W.valid_page(constant_table[min(tok, W.length - 1) >> shift]); };
   for (int base = begin & ~page_mask; base < end; base += segment) {
-    const int from = max(begin, base), to = min(end, base + segment), stages = (to - from + T::kStage - 1) / T::kStage;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kIds; i += kThreads) {
-      const int tok = base + (i << shift);
-      s_ids[i] = tok < W.length ? W.valid_page(W.table[tok >> shift]) : 0;
+    const int from = max(begin, base), to = min(end, base > (1 << 30) - segment ? end : base + segment);
+    const int stages = (to - from + T::kStage - 1) / T::kStage;
+    int next_page = 0;
+    if (wide) {
+      next_page = page_at(from);
+    } else {
+      __syncthreads();
+      for (int i = threadIdx.x; i < kIds; i += kThreads) {
+        const int tok = base + (i << shift);
+        s_ids[i] = tok < W.length ? W.valid_page(W.table[tok >> shift]) : 0;
+      }
+      __syncthreads();
     }
-    __syncthreads();
 
-    // Stage `st` of the segment into its place of the ring. (Tokens past the last are those of the last group again.)
+    // Stage `st` of the segment into its place of the ring. (Tokens past the last: others of the page, or the last group again.)
     auto load = [&](int st) __attribute__((always_inline)) {
       const int t = from + st * T::kStage;
       char* ring = s_ring + (st % T::kStages) * T::kStageBytes;
+      if (wide) {
+        const int64_t head = (int64_t)next_page * S.cache.heads + W.h;
+        const int off = t & page_mask;
+        next_page = page_at(t + T::kStage);
+        const char* kp = keys + ((head * (D / E) << shift) + off) * 16;
+        const char* vp = values + ((head << shift) + off) / E * (D * 16);
+#pragma unroll
+        for (int j = 0; j < T::kChunkLoads; ++j) {
+          const int chunk = wave + kWaves * j;
+          const char* src = chunk < T::kChunks / 2 ? kp + ((int64_t)chunk << (shift + 4)) : vp + (chunk - T::kChunks / 2) * 1024;
+          const uint32_t mine = chunk < T::kChunks / 2 ? key_token * 16 : lane * 16;
+          __builtin_amdgcn_global_load_lds((global_ptr)(src + mine), (lds_ptr)(ring + chunk * 1024), 16, 0, 0);
+        }
+        if constexpr (Q8) {
+          // 4 tokens a lane: key scales, value scales, and both again (every lane of a load writes).
+          const float* src = (lane & 16 ? S.cache.value_scales : S.cache.key_scales) + (head << shift) + off;
+          __builtin_amdgcn_global_load_lds((global_ptr)(src + (lane & 15) * 4), (lds_ptr)(ring + T::kPieces * 16), 16, 0, 0);
+        }
+        return;
+      }
       const auto head_of = [&](int tok) { return (int64_t)s_ids[(tok - base) >> shift] * S.cache.heads + W.h; };
-      // A key's lane: its token in the order of the tiles' rows, the same in every piece.
-      const int sd = lane / R::kStep, row = lane & 15;
-      const int grp = min(W.group(t + sd * R::kStep + 8 * (row >> 2)), base + segment - 8);
-      const char* kp = keys + ((head_of(grp) * (D / E) << shift) + (grp & page_mask) + 4 * (lane / 16 % R::kKT) + (row & 3)) * 16;
+      const int grp = min(W.group(t + (key_token & ~7)), base + segment - 8);
+      const char* kp = keys + ((head_of(grp) * (D / E) << shift) + (grp & page_mask) + (key_token & 7)) * 16;
 #pragma unroll
       for (int j = 0; j < T::kChunkLoads; ++j) {
         const int chunk = wave + kWaves * j;
@@ -174,7 +206,6 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
         __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(ring + chunk * 1024), 16, 0, 0);
       }
       if constexpr (Q8) {
-        // 4 tokens a lane: key scales, value scales, and both again (every lane of a load writes).
         const int tok = min(W.group(t + (lane & 14) * 4), base + segment - 8) + (lane & 1) * 4;
         const float* src = (lane & 16 ? S.cache.value_scales : S.cache.key_scales) + (head_of(tok) << shift) + (tok & page_mask);
         __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(ring + T::kPieces * 16), 16, 0, 0);
