@@ -66,6 +66,22 @@ __device__ __forceinline__ u32x2 gated_bf16(f32x4 x, const uint16_t* gate) {
   return u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
 }
 
+// 8 tokens' values of one dimension, the first of them `past` behind the request's tokens (below 0: before their end), with zeros in
+// place of the tokens past the last, which the cache need not hold, and of what is not finite (*odd: there was some): a
+// probability of zero would not keep it from the rows that do not see it.
+__device__ __forceinline__ u32x4 clean_values(u32x4 v, int past, bool* odd) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const uint32_t keep = past + 2 * w >= 0 ? 0u : past + 2 * w + 1 >= 0 ? 0xFFFFu : 0xFFFFFFFFu;
+    uint32_t x = v[w] & keep;
+    const bool lo = (x & 0x7F80u) == 0x7F80u, hi = (x & 0x7F800000u) == 0x7F800000u;
+    *odd |= lo | hi;
+    x = lo ? x & 0xFFFF0000u : x;
+    v[w] = hi ? x & 0xFFFFu : x;
+  }
+  return v;
+}
+
 // Whether a row without a context sees none of its request's n rows: its result is zero.
 __device__ __forceinline__ bool paged_empty(const int64_t* ancestors, int64_t row, int length, int n) {
   if (!ancestors || length != n) return false;
@@ -102,7 +118,8 @@ struct PagedRows {
     length = I.length;
     context = length - I.rows;
     table = S.table + (int64_t)I.request * S.capacity;
-    unit = fabsf(S.scale) * kLog2e;
+    // (Never 0: what is masked has to stay at -infinity.)
+    unit = S.scale == 0.0f ? 0x1p-149f : fabsf(S.scale) * kLog2e;
   }
 
   // Query row `at` of the request's n G: its row of the step and its head.
@@ -197,7 +214,7 @@ struct PagedRows {
       for (int tt = 0; tt < kKT; ++tt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) now = fmaxf(now, s[tt][i]);
-      now = now == -__builtin_inff() ? kNone : now * unit;  // (a unit of 0 as well)
+      now *= unit;
       now = fmaxf(now, __shfl_xor(now, 16));
       now = fmaxf(fmaxf(now, __shfl_xor(now, 32)), m[qt]);
       const float f = __builtin_amdgcn_exp2f(m[qt] - now);
@@ -209,10 +226,6 @@ struct PagedRows {
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(e[j]);
-    if (masked) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = sees(qt, t + 8 * g + j) ? e[j] : 0.0f;
-    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) l[qt] += e[j];
     if constexpr (Q8) {
@@ -228,24 +241,6 @@ struct PagedRows {
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
     *p = as_bf16x8(w);
-  }
-
-  // Zeros in 8 tokens' values (of one dimension, from t + 8 g on) in place of those past the last, which the cache need not
-  // hold, and of what is not finite: a probability of zero would not keep it from the rows that do not see it.
-  __device__ __forceinline__ u32x4 clean(u32x4 v, int t) {
-    const int past = t + 8 * g - length;
-    bool any = false;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const uint32_t keep = past + 2 * w >= 0 ? 0u : past + 2 * w + 1 >= 0 ? 0xFFFFu : 0xFFFFFFFFu;
-      uint32_t x = v[w] & keep;
-      const bool lo = (x & 0x7F80u) == 0x7F80u, hi = (x & 0x7F800000u) == 0x7F800000u;
-      any |= lo | hi;
-      x = lo ? x & 0xFFFF0000u : x;
-      v[w] = hi ? x & 0xFFFFu : x;
-    }
-    odd |= any;
-    return v;
   }
 
   // What those values add to o for the rows that see them: the wave's steps t, t + stride, .. again, token by token.

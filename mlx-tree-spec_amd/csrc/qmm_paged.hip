@@ -114,7 +114,7 @@ struct PagedWave : PagedRows<D, 1, Q8> {
     if constexpr (!Q8) {
       if (t + R::kStep > this->context) {
 #pragma unroll
-        for (int dt = 0; dt < R::kVT; ++dt) vf[dt] = this->clean(vf[dt], t);
+        for (int dt = 0; dt < R::kVT; ++dt) vf[dt] = clean_values(vf[dt], t + 8 * this->g - this->length, &this->odd);
       }
     }
 #pragma unroll
@@ -154,7 +154,7 @@ __global__ __launch_bounds__((RowsTraits<D, Q8>::kWaves * 64)) void paged_rows_k
   const PagedItem I = S.plan.items()[item];
   if (item >= S.plan.words[0]) return;
   PagedWave<D, Q8> W(S, I, blockIdx.x - item * S.cache.heads);
-  const int wave = threadIdx.x >> 6, t = I.begin + wave * R::kStep, stride = T::kWaves * R::kStep;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = I.begin + wave * R::kStep, stride = T::kWaves * R::kStep;
   W.run(t, I.end, stride);
   W.add_odd_values(t, I.end, stride, 0);
   W.sum_lanes();

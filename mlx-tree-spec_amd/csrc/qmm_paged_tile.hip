@@ -3,12 +3,14 @@
 // matrix instructions and what feeds them.
 //
 // A workgroup takes up to kPagedRows query rows of one key head over one split: 8 waves with 16 QT rows each, or with two SIDES
-// 4 of them on the even steps and the others with the same rows on the odd ones. The steps' keys and values go from memory to a ring of stages in
-// LDS without registers (1 KB an instruction), kStages - 1 stages ahead, in the order in which the waves read them: a
-// fragment is then 256 neighbouring bytes for 16 lanes, without bank conflicts. One barrier a stage, behind an exact count of the
-// loads that may still be on their way.
+// 4 of them on the even steps and the others with the same rows on the odd ones. The steps' keys and values go from memory to
+// a ring of stages in LDS without registers (1 KB an instruction), kAhead stages ahead, in the order in which the waves read
+// them: a fragment is then 256 neighbouring bytes for 16 lanes, without bank conflicts. One barrier a stage, behind an exact
+// count of the loads that may still be on their way.
+//
+// The barrier would have all waves multiply and exponentiate at the same time. Waves 4 to 7, which share the SIMDs with 0 to 3,
+// are half a stage late: they end the stage before (exponentials, values' product) while the others begin with this one's keys.
 #include <algorithm>
-#include <type_traits>
 
 #include "qmm4_lds.h"
 #include "qmm_paged.h"
@@ -26,18 +28,19 @@ struct TileTraits {
   using R = PagedRows<D, QT, Q8>;
   static constexpr int kAcross = kWaves / SIDES;          // waves side by side along the rows
   static constexpr int kRows = kAcross * 16 * QT;
-  static constexpr int kStage = 2 * R::kStep;             // tokens
-  static constexpr int kPieces = D * 128 / R::E;          // 16-byte pieces of a stage: keys, then values
+  static constexpr int kStage = SIDES * R::kStep;         // tokens
+  static constexpr int kPieces = D * kStage * 2 / R::E;   // 16-byte pieces of a stage: keys, then values
   static constexpr int kChunks = kPieces / 64;            // loads of them
-  static constexpr int kStageBytes = kPieces * 16 + (Q8 ? 1024 : 0);  // (scales: 512 bytes, twice)
+  static constexpr int kStageBytes = kPieces * 16 + (Q8 ? 1024 : 0);  // (scales, over and over)
   static constexpr int kChunkLoads = (kChunks + kWaves - 1) / kWaves;
   static constexpr int kLoads = kChunkLoads + (Q8 ? 1 : 0);  // a wave's loads of a stage
   static constexpr int kRoom = 160 * 1024 - kIds * 4 - 512;
   static constexpr int kStages = kRoom / kStageBytes < 4 ? kRoom / kStageBytes : 4;
+  static constexpr int kAhead = kStages - 2;              // (the stage before this one is still read)
   static constexpr size_t kRing = (size_t)kStages * kStageBytes;
   static constexpr size_t kJoin = SIDES > 1 ? (size_t)kAcross * R::kHandBytes : 0;
-  static constexpr size_t kLds = (kRing > kJoin ? kRing : kJoin) + kIds * 4;
-  static_assert(kStages >= 2 && kChunks % kWaves == 0 && kLds <= 160 * 1024, "whole loads, LDS");
+  static constexpr size_t kLds = (kRing > kJoin ? kRing : kJoin) + kIds * 4 + 16;
+  static_assert(kAhead >= 1 && kLds <= 160 * 1024, "LDS");
 };
 
 template <int N>
@@ -59,7 +62,8 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   typedef __attribute__((address_space(1))) const void* global_ptr;
   typedef __attribute__((address_space(3))) void* lds_ptr;
   extern __shared__ __attribute__((aligned(16))) char s_ring[];
-  int* s_ids = reinterpret_cast<int*>(s_ring + T::kLds - kIds * 4);
+  int* s_ids = reinterpret_cast<int*>(s_ring + T::kLds - kIds * 4 - 16);
+  int* s_odd = s_ids + kIds;  // a value that is not finite was left out
   // The row blocks of one split and key head follow each other on one XCD (workgroups go round the 8 of them): the later
   // ones find the cache's bytes in its L2.
   const int unit = blockIdx.x / (8 * blocks) * 8 + (blockIdx.x & 7), block = block0 + blockIdx.x / 8 % blocks;
@@ -69,11 +73,12 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   R W(S, I, unit - item * S.cache.heads);
   const int row0 = block * T::kRows, rows = I.rows * S.G;
   if (row0 >= rows) return;
-  const int wave = threadIdx.x >> 6, side = wave / T::kAcross, rw = wave % T::kAcross;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), side = wave / T::kAcross, rw = wave % T::kAcross;
   const int mine = row0 + rw * 16 * QT;
   const bool active = mine < rows;
   W.load_rows(mine);
 
+  if (threadIdx.x == 0) *s_odd = 0;  // (read and written behind the barrier of a stage at least)
   const int begin = I.begin;
   int end = I.end;
   // (Without ancestors nothing past the block's last row is seen.)
@@ -84,12 +89,10 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   const char* keys = static_cast<const char*>(S.cache.keys);
   const char* values = static_cast<const char*>(S.cache.values);
 
-  // One step, from a stage in LDS.
-  auto step = [&](const u32x4* ring, int sd, int t) __attribute__((always_inline)) {
+  // A step from a stage in LDS: its products with the queries ..
+  f32x4 s[QT][R::kKT];
+  const auto multiply = [&](const u32x4* ring, int sd) __attribute__((always_inline)) {
     const u32x4* kr = ring + W.g * T::kStage + sd * R::kStep + W.r16;
-    // (8 bits: two groups of 8 tokens share a piece.)
-    const u32x4* vr = ring + T::kPieces / 2 + (Q8 ? sd * 2 + (W.g >> 1) : sd * 4 + W.g) * D + W.r16;
-    f32x4 s[QT][R::kKT], ks[Q8 ? R::kKT : 1], vs[Q8 ? R::kKT : 1];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
@@ -113,42 +116,47 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
       }
       if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);  // (few codes at a time in registers)
     }
+  };
+  // .. and what they add to the rows.
+  const auto finish = [&](const u32x4* ring, int sd, int t) __attribute__((always_inline)) {
+    // (8 bits: two groups of 8 tokens share a piece.)
+    const u32x4* vr = ring + T::kPieces / 2 + (Q8 ? sd * 2 + (W.g >> 1) : sd * 4 + W.g) * D + W.r16;
+    f32x4 ks[Q8 ? R::kKT : 1], vs[Q8 ? R::kKT : 1];
     if constexpr (Q8) {
       const f32x4* scales = reinterpret_cast<const f32x4*>(ring + T::kPieces) + sd * 8 + W.g * 2;
 #pragma unroll
       for (int tt = 0; tt < R::kKT; ++tt) {
         ks[tt] = scales[tt];
-        vs[tt] = scales[16 + tt];
+        vs[tt] = scales[T::kStage / 4 + tt];
       }
     }
     bf16x8 p[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) W.softmax(t, qt, s[qt], ks, vs, &p[qt]);
-    const auto values = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
-      for (int dt = 0; dt < R::kVT; ++dt) {
-        bf16x8 v;
-        if constexpr (Q8) {
-          const u32x2 codes = reinterpret_cast<const u32x2*>(vr + dt * 16)[W.g & 1];
-          v = codes8(codes[0], codes[1]);
-        } else {
-          v = as_bf16x8(decltype(masked)::value ? W.clean(vr[dt * 16], t) : vr[dt * 16]);
-        }
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) W.o[qt][dt] = paged_mma(v, p[qt], W.o[qt][dt]);
-        if (Q8 && dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    for (int dt = 0; dt < R::kVT; ++dt) {
+      bf16x8 v;
+      if constexpr (Q8) {
+        const u32x2 codes = reinterpret_cast<const u32x2*>(vr + dt * 16)[W.g & 1];
+        v = codes8(codes[0], codes[1]);
+      } else {
+        v = as_bf16x8(vr[dt * 16]);
       }
-    };
-    if (!Q8 && t + R::kStep > W.context) values(std::true_type{});
-    else values(std::false_type{});
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) W.o[qt][dt] = paged_mma(v, p[qt], W.o[qt][dt]);
+      if (Q8 && dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
   // Pages of a stage's tokens and more: one page for a stage, addresses that only the scalar unit makes.
-  static_assert(T::kStage == 64, "a stage begins at a multiple of its tokens");
-  const bool wide = shift >= 6;
+  static_assert(kPagedUnit % T::kStage == 0, "a stage begins at a multiple of its tokens");
+  const bool wide = page_mask + 1 >= T::kStage;
   const int segment = wide ? 1 << 30 : kIds << shift;  // tokens whose pages are known at once
   // A lane's token of a key's piece, in the order of the tiles' rows.
-  const int key_token = lane / R::kStep * R::kStep + 8 * ((lane & 15) >> 2) + 4 * (lane / 16 % R::kKT) + (lane & 3);
+  const int key_token = lane % T::kStage / R::kStep * R::kStep + 8 * ((lane & 15) >> 2) + 4 * (lane / 16 % R::kKT) + (lane & 3);
+  constexpr int kScaleLanes = T::kStage / 4;
+  constexpr int kKeyPieces = 64 / T::kStage;  // pieces of keys in one load
+  const uint32_t key_offset = ((uint32_t)(lane / T::kStage) << (shift + 4)) + key_token * 16;
   const auto page_at = [&](int tok) { return W.valid_page(constant_table[min(tok, W.length - 1) >> shift]); };
   for (int base = begin & ~page_mask; base < end; base += segment) {
     const int from = max(begin, base), to = min(end, base > (1 << 30) - segment ? end : base + segment);
@@ -177,15 +185,15 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
         const char* vp = values + ((head << shift) + off) / E * (D * 16);
 #pragma unroll
         for (int j = 0; j < T::kChunkLoads; ++j) {
-          const int chunk = wave + kWaves * j;
-          const char* src = chunk < T::kChunks / 2 ? kp + ((int64_t)chunk << (shift + 4)) : vp + (chunk - T::kChunks / 2) * 1024;
-          const uint32_t mine = chunk < T::kChunks / 2 ? key_token * 16 : lane * 16;
+          const int chunk = min(wave + kWaves * j, T::kChunks - 1);  // (the last one again where they do not divide)
+          const char* src = chunk < T::kChunks / 2 ? kp + ((int64_t)chunk * kKeyPieces << (shift + 4)) : vp + (chunk - T::kChunks / 2) * 1024;
+          const uint32_t mine = chunk < T::kChunks / 2 ? key_offset : lane * 16;
           __builtin_amdgcn_global_load_lds((global_ptr)(src + mine), (lds_ptr)(ring + chunk * 1024), 16, 0, 0);
         }
         if constexpr (Q8) {
           // 4 tokens a lane: key scales, value scales, and both again (every lane of a load writes).
-          const float* src = (lane & 16 ? S.cache.value_scales : S.cache.key_scales) + (head << shift) + off;
-          __builtin_amdgcn_global_load_lds((global_ptr)(src + (lane & 15) * 4), (lds_ptr)(ring + T::kPieces * 16), 16, 0, 0);
+          const float* src = (lane & kScaleLanes ? S.cache.value_scales : S.cache.key_scales) + (head << shift) + off;
+          __builtin_amdgcn_global_load_lds((global_ptr)(src + (lane & (kScaleLanes - 1)) * 4), (lds_ptr)(ring + T::kPieces * 16), 16, 0, 0);
         }
         return;
       }
@@ -194,10 +202,10 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
       const char* kp = keys + ((head_of(grp) * (D / E) << shift) + (grp & page_mask) + (key_token & 7)) * 16;
 #pragma unroll
       for (int j = 0; j < T::kChunkLoads; ++j) {
-        const int chunk = wave + kWaves * j;
+        const int chunk = min(wave + kWaves * j, T::kChunks - 1);  // (the last one again where they do not divide)
         const char* src;
         if (chunk < T::kChunks / 2) {
-          src = kp + ((int64_t)chunk << (shift + 4));
+          src = kp + ((int64_t)(chunk * kKeyPieces + lane / T::kStage) << (shift + 4));
         } else {
           const int f = (chunk - T::kChunks / 2) * 64 + lane, at = f / D, d = f - at * D;
           const int tok = min(W.group(t + at * E), base + segment - E) & ~(E - 1);
@@ -206,27 +214,46 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
         __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(ring + chunk * 1024), 16, 0, 0);
       }
       if constexpr (Q8) {
-        const int tok = min(W.group(t + (lane & 14) * 4), base + segment - 8) + (lane & 1) * 4;
-        const float* src = (lane & 16 ? S.cache.value_scales : S.cache.key_scales) + (head_of(tok) << shift) + (tok & page_mask);
+        const int tok = min(W.group(t + (lane & (kScaleLanes - 2)) * 4), base + segment - 8) + (lane & 1) * 4;
+        const float* src = (lane & kScaleLanes ? S.cache.value_scales : S.cache.key_scales) + (head_of(tok) << shift) + (tok & page_mask);
         __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(ring + T::kPieces * 16), 16, 0, 0);
       }
     };
 
-    for (int st = 0; st < T::kStages - 1 && st < stages; ++st) load(st);
-    for (int st = 0; st < stages; ++st) {
-      if (st + T::kStages - 2 < stages) wait_loads<(T::kStages - 2) * T::kLoads>();
+    const auto ring_of = [&](int st) { return reinterpret_cast<const u32x4*>(s_ring + (st % T::kStages) * T::kStageBytes); };
+    const auto token_of = [&](int st) { return from + st * T::kStage + side * R::kStep; };
+    const bool late = wave >= kWaves / 2;
+    // The values of a stage past the context made clean in place, by all waves (once: a branch around products of clean and other
+    // values would have every sum in registers twice).
+    const auto clean = [&](int st) {
+      u32x4* values = reinterpret_cast<u32x4*>(s_ring + (st % T::kStages) * T::kStageBytes) + T::kPieces / 2;
+      for (int f = threadIdx.x; f < T::kPieces / 2; f += kThreads) {
+        bool odd = false;
+        values[f] = clean_values(values[f], from + st * T::kStage + f / D * 8 - W.length, &odd);
+        if (odd) *s_odd = 1;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      bare_barrier();
+    };
+    const auto arrive = [&](int st) __attribute__((always_inline)) {
+      if (st + T::kAhead - 1 < stages) wait_loads<(T::kAhead - 1) * T::kLoads>();
       else wait_loads<0>();
       bare_barrier();
-      if (st + T::kStages - 1 < stages) load(st + T::kStages - 1);
-      if (!active) continue;
-      const u32x4* ring = reinterpret_cast<const u32x4*>(s_ring + (st % T::kStages) * T::kStageBytes);
+      if (!Q8 && from + (st + 1) * T::kStage > W.context) clean(st);
+    };
+    for (int st = 0; st < T::kAhead && st < stages; ++st) load(st);
+    // Late waves meet the others at a stage's barrier before they end the stage before it.
 #pragma unroll 1
-      for (int sd = side; sd < 2; sd += SIDES) {
-        const int t = from + st * T::kStage + sd * R::kStep;
-        if (t < to) step(ring, sd, t);
-      }
+    for (int st = 0; st <= stages; ++st) {
+      if (late && st < stages) arrive(st);
+      if (active && st > 0 && token_of(st - 1) < to) finish(ring_of(st - 1), side, token_of(st - 1));
+      if (!late && st < stages) arrive(st);
+      if (st + T::kAhead < stages) load(st + T::kAhead);
+      if (active && st < stages) multiply(ring_of(st), side);
     }
     // (Every load has been waited for: the ring is free behind the next barrier.)
+    __syncthreads();
+    W.odd = *s_odd != 0;
     if (active) W.add_odd_values(from + side * R::kStep, to, SIDES * R::kStep, mine);
   }
 
@@ -257,11 +284,11 @@ hipError_t launch_tile(const PagedParams& p, hipStream_t stream) {
 
 template <int D, bool Q8>
 hipError_t launch_rows(const PagedParams& p, hipStream_t stream) {
-  // Two sides where 4 waves of 16 rows hold a request's; past that 32 rows to a wave, or where their sums and queries would not
-  // leave room in 256 registers 16 rows to each of 8.
-  if ((int64_t)p.max_rows * p.G <= 64) return launch_tile<D, 1, 2, Q8>(p, stream);
-  if constexpr (D <= 128) return launch_tile<D, 2, 2, Q8>(p, stream);
-  else return launch_tile<D, 1, 1, Q8>(p, stream);
+  // Two sides of 4 waves; 16 rows to a wave where those hold a request's, else 32. Heads of 192 and more, whose sums and queries
+  // would not leave room for 32 rows in 256 registers (nor their stages of 64 tokens for 3 of them in LDS): 16 rows to each of 8.
+  if constexpr (D > 128) return launch_tile<D, 1, 1, Q8>(p, stream);
+  else if ((int64_t)p.max_rows * p.G <= 64) return launch_tile<D, 1, 2, Q8>(p, stream);
+  else return launch_tile<D, 2, 2, Q8>(p, stream);
 }
 
 template <int D>
