@@ -226,8 +226,10 @@ struct PagedRows {
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(e[j]);
+    float sum[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) l[qt] += e[j];
+    for (int j = 0; j < 4; ++j) sum[j] = e[j] + e[j + 4];
+    l[qt] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     if constexpr (Q8) {
 #pragma unroll
       for (int tt = 0; tt < kKT; ++tt)

@@ -11,6 +11,7 @@
 // The barrier would have all waves multiply and exponentiate at the same time. Waves 4 to 7, which share the SIMDs with 0 to 3,
 // are half a stage late: they end the stage before (exponentials, values' product) while the others begin with this one's keys.
 #include <algorithm>
+#include <type_traits>
 
 #include "qmm4_lds.h"
 #include "qmm_paged.h"
@@ -32,20 +33,22 @@ struct TileTraits {
   static constexpr int kPieces = D * kStage * 2 / R::E;   // 16-byte pieces of a stage: keys, then values
   static constexpr int kChunks = kPieces / 64;            // loads of them
   static constexpr int kStageBytes = kPieces * 16 + (Q8 ? 1024 : 0);  // (scales, over and over)
-  static constexpr int kChunkLoads = (kChunks + kWaves - 1) / kWaves;
+  static constexpr int kChunkLoads = (kChunks / 2 + kWaves / 2 - 1) / (kWaves / 2);
   static constexpr int kLoads = kChunkLoads + (Q8 ? 1 : 0);  // a wave's loads of a stage
   static constexpr int kRoom = 160 * 1024 - kIds * 4 - 512;
   static constexpr int kStages = kRoom / kStageBytes < 4 ? kRoom / kStageBytes : 4;
-  static constexpr int kAhead = kStages - 2;              // (the stage before this one is still read)
+  static constexpr int kAhead = kStages - 1;              // (a stage is read between its barrier and the next)
   static constexpr size_t kRing = (size_t)kStages * kStageBytes;
   static constexpr size_t kJoin = SIDES > 1 ? (size_t)kAcross * R::kHandBytes : 0;
   static constexpr size_t kLds = (kRing > kJoin ? kRing : kJoin) + kIds * 4 + 16;
   static_assert(kAhead >= 1 && kLds <= 160 * 1024, "LDS");
 };
 
+// Waits until at most N of the wave's loads into LDS are on their way, and none of its reads out of LDS (what it has read may be
+// written over behind the next barrier).
 template <int N>
 __device__ __forceinline__ void wait_loads() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void bare_barrier() {
@@ -90,9 +93,11 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   const char* values = static_cast<const char*>(S.cache.values);
 
   // A step from a stage in LDS: its products with the queries ..
+  using Piece = std::conditional_t<Q8, u32x2, u32x4>;  // 8 tokens of a dimension
   f32x4 s[QT][R::kKT];
-  const auto multiply = [&](const u32x4* ring, int sd) __attribute__((always_inline)) {
-    const u32x4* kr = ring + W.g * T::kStage + sd * R::kStep + W.r16;
+  Piece vf[R::kVT];
+  f32x4 ks[Q8 ? R::kKT : 1], vs[Q8 ? R::kKT : 1];
+  const auto multiply = [&](const u32x4 (&kf)[R::kKC][R::kKT]) __attribute__((always_inline)) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
@@ -101,7 +106,7 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
     for (int c = 0; c < R::kKC; ++c) {
 #pragma unroll
       for (int tt = 0; tt < R::kKT; ++tt) {
-        const u32x4 k = kr[c * 4 * T::kStage + tt * 16];
+        const u32x4 k = kf[c][tt];
         if constexpr (Q8) {
           const bf16x8 lo = codes8(k[0], k[1]), hi = codes8(k[2], k[3]);
 #pragma unroll
@@ -118,30 +123,15 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
     }
   };
   // .. and what they add to the rows.
-  const auto finish = [&](const u32x4* ring, int sd, int t) __attribute__((always_inline)) {
-    // (8 bits: two groups of 8 tokens share a piece.)
-    const u32x4* vr = ring + T::kPieces / 2 + (Q8 ? sd * 2 + (W.g >> 1) : sd * 4 + W.g) * D + W.r16;
-    f32x4 ks[Q8 ? R::kKT : 1], vs[Q8 ? R::kKT : 1];
-    if constexpr (Q8) {
-      const f32x4* scales = reinterpret_cast<const f32x4*>(ring + T::kPieces) + sd * 8 + W.g * 2;
-#pragma unroll
-      for (int tt = 0; tt < R::kKT; ++tt) {
-        ks[tt] = scales[tt];
-        vs[tt] = scales[T::kStage / 4 + tt];
-      }
-    }
+  const auto finish = [&](int t) __attribute__((always_inline)) {
     bf16x8 p[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) W.softmax(t, qt, s[qt], ks, vs, &p[qt]);
 #pragma unroll
     for (int dt = 0; dt < R::kVT; ++dt) {
       bf16x8 v;
-      if constexpr (Q8) {
-        const u32x2 codes = reinterpret_cast<const u32x2*>(vr + dt * 16)[W.g & 1];
-        v = codes8(codes[0], codes[1]);
-      } else {
-        v = as_bf16x8(vr[dt * 16]);
-      }
+      if constexpr (Q8) v = codes8(vf[dt][0], vf[dt][1]);
+      else v = as_bf16x8(vf[dt]);
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) W.o[qt][dt] = paged_mma(v, p[qt], W.o[qt][dt]);
       if (Q8 && dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
@@ -156,7 +146,16 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   const int key_token = lane % T::kStage / R::kStep * R::kStep + 8 * ((lane & 15) >> 2) + 4 * (lane / 16 % R::kKT) + (lane & 3);
   constexpr int kScaleLanes = T::kStage / 4;
   constexpr int kKeyPieces = 64 / T::kStage;  // pieces of keys in one load
-  const uint32_t key_offset = ((uint32_t)(lane / T::kStage) << (shift + 4)) + key_token * 16;
+  // A wave's loads: neighbouring kilobytes of the stage's keys (the lower half of the waves) or of its values (the last ones of
+  // either again where they do not divide). Its lanes' places in a page, those of a token on, and of a load on.
+  const int mine_chunk = wave / (kWaves / 2) * (T::kChunks / 2) +
+                         min(wave % (kWaves / 2) * T::kChunkLoads, T::kChunks / 2 - T::kChunkLoads);
+  const bool mine_keys = wave < kWaves / 2;
+  const char* mine_base = mine_keys ? keys + ((int64_t)mine_chunk * kKeyPieces << (shift + 4))
+                                    : values + (mine_chunk - T::kChunks / 2) * 1024;
+  const int mine_token = mine_keys ? 16 : D * 16 / E, mine_stride = mine_keys ? kKeyPieces << (shift + 4) : 1024;
+  const uint32_t mine_offset = mine_keys ? ((uint32_t)(lane / T::kStage) << (shift + 4)) + key_token * 16 : lane * 16;
+  const int64_t page_bytes = (int64_t)D * 16 / E << shift;  // (of one head)
   const auto page_at = [&](int tok) { return W.valid_page(constant_table[min(tok, W.length - 1) >> shift]); };
   for (int base = begin & ~page_mask; base < end; base += segment) {
     const int from = max(begin, base), to = min(end, base > (1 << 30) - segment ? end : base + segment);
@@ -181,15 +180,11 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
         const int64_t head = (int64_t)next_page * S.cache.heads + W.h;
         const int off = t & page_mask;
         next_page = page_at(t + T::kStage);
-        const char* kp = keys + ((head * (D / E) << shift) + off) * 16;
-        const char* vp = values + ((head << shift) + off) / E * (D * 16);
+        const char* src = mine_base + head * page_bytes + off * mine_token;
 #pragma unroll
-        for (int j = 0; j < T::kChunkLoads; ++j) {
-          const int chunk = min(wave + kWaves * j, T::kChunks - 1);  // (the last one again where they do not divide)
-          const char* src = chunk < T::kChunks / 2 ? kp + ((int64_t)chunk * kKeyPieces << (shift + 4)) : vp + (chunk - T::kChunks / 2) * 1024;
-          const uint32_t mine = chunk < T::kChunks / 2 ? key_offset : lane * 16;
-          __builtin_amdgcn_global_load_lds((global_ptr)(src + mine), (lds_ptr)(ring + chunk * 1024), 16, 0, 0);
-        }
+        for (int j = 0; j < T::kChunkLoads; ++j)
+          __builtin_amdgcn_global_load_lds((global_ptr)(src + j * mine_stride + mine_offset),
+                                           (lds_ptr)(ring + (mine_chunk + j) * 1024), 16, 0, 0);
         if constexpr (Q8) {
           // 4 tokens a lane: key scales, value scales, and both again (every lane of a load writes).
           const float* src = (lane & kScaleLanes ? S.cache.value_scales : S.cache.key_scales) + (head << shift) + off;
@@ -202,7 +197,7 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
       const char* kp = keys + ((head_of(grp) * (D / E) << shift) + (grp & page_mask) + (key_token & 7)) * 16;
 #pragma unroll
       for (int j = 0; j < T::kChunkLoads; ++j) {
-        const int chunk = min(wave + kWaves * j, T::kChunks - 1);  // (the last one again where they do not divide)
+        const int chunk = mine_chunk + j;
         const char* src;
         if (chunk < T::kChunks / 2) {
           src = kp + ((int64_t)(chunk * kKeyPieces + lane / T::kStage) << (shift + 4));
@@ -246,10 +241,39 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
 #pragma unroll 1
     for (int st = 0; st <= stages; ++st) {
       if (late && st < stages) arrive(st);
-      if (active && st > 0 && token_of(st - 1) < to) finish(ring_of(st - 1), side, token_of(st - 1));
-      if (!late && st < stages) arrive(st);
+      if (active && st > 0 && token_of(st - 1) < to) finish(token_of(st - 1));
+      if (st == stages) break;
+      if (!late) arrive(st);
+      // (Its keys are on their way while the loads ahead are made, its values while the products run.)
+      const u32x4* ring = ring_of(st);
+      const u32x4* kr = ring + W.g * T::kStage + side * R::kStep + W.r16;
+      constexpr bool kEarly = R::kKC * R::kKT <= 8;  // (or too many registers)
+      u32x4 kf[R::kKC][R::kKT];
+      const auto read_keys = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < R::kKC; ++c)
+#pragma unroll
+          for (int tt = 0; tt < R::kKT; ++tt) kf[c][tt] = kr[c * 4 * T::kStage + tt * 16];
+      };
+      if (kEarly) read_keys();
       if (st + T::kAhead < stages) load(st + T::kAhead);
-      if (active && st < stages) multiply(ring_of(st), side);
+      if (!active) continue;
+      if (!kEarly) read_keys();
+      multiply(kf);
+      __builtin_amdgcn_sched_barrier(0);
+      // (8 bits: two groups of 8 tokens share a piece.)
+      const Piece* vr = reinterpret_cast<const Piece*>(ring + T::kPieces / 2 + (Q8 ? side * 2 + (W.g >> 1) : side * 4 + W.g) * D + W.r16) +
+                        (Q8 ? W.g & 1 : 0);
+#pragma unroll
+      for (int dt = 0; dt < R::kVT; ++dt) vf[dt] = vr[dt * (Q8 ? 32 : 16)];
+      if constexpr (Q8) {
+        const f32x4* scales = reinterpret_cast<const f32x4*>(ring + T::kPieces) + side * 8 + W.g * 2;
+#pragma unroll
+        for (int tt = 0; tt < R::kKT; ++tt) {
+          ks[tt] = scales[tt];
+          vs[tt] = scales[T::kStage / 4 + tt];
+        }
+      }
     }
     // (Every load has been waited for: the ring is free behind the next barrier.)
     __syncthreads();
