@@ -185,64 +185,80 @@ struct PagedRows {
 
   // The probabilities of a step's tokens from t, whose products are s, as the second operand of the values' product; m, l and
   // o move with them. 8 bits: kscale multiplies the products, vscale the probabilities.
-  __device__ __forceinline__ void softmax(int t, int qt, f32x4 (&s)[kKT], const f32x4* kscale, const f32x4* vscale,
-                                          bf16x8* p) {
+  __device__ __forceinline__ void softmax(int t, f32x4 (&s)[QT][kKT], const f32x4* kscale, const f32x4* vscale,
+                                          bf16x8 (&p)[QT]) {
     const bool masked = t + kStep > context;
     if constexpr (Q8) {
 #pragma unroll
-      for (int tt = 0; tt < kKT; ++tt) s[tt] *= kscale[tt];
+      for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+        for (int tt = 0; tt < kKT; ++tt) s[qt][tt] *= kscale[tt];
     }
     if (masked) {
 #pragma unroll
-      for (int tt = 0; tt < kKT; ++tt)
+      for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[tt][i] = sees(qt, t + 8 * g + 4 * tt + i) ? s[tt][i] : -__builtin_inff();
+        for (int tt = 0; tt < kKT; ++tt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[qt][tt][i] = sees(qt, t + 8 * g + 4 * tt + i) ? s[qt][tt][i] : -__builtin_inff();
     }
     // Arguments of the exponentials beside the present maximum, which stays where none passes it by more than kSlack.
-    float e[8];
-    const auto arguments = [&](float ref) __attribute__((always_inline)) {
+    float e[QT][8];
+    const auto arguments = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int tt = 0; tt < kKT; ++tt)
+      for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[tt * 4 + i] = __builtin_fmaf(s[tt][i], unit, -ref);
+        for (int j = 0; j < 8; ++j) e[qt][j] = __builtin_fmaf(s[qt][j / 4][j % 4], unit, -m[qt]);
     };
-    arguments(m[qt]);
-    const float top = max3(max3(e[0], e[1], e[2]), max3(e[3], e[4], e[5]), max3(e[6], e[7], e[7]));
+    arguments();
+    float top = kNone;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      top = max3(top, max3(e[qt][0], e[qt][1], e[qt][2]), max3(e[qt][3], e[qt][4], e[qt][5]));
+      top = max3(top, e[qt][6], e[qt][7]);
+    }
     if (__any(top > kSlack)) {
-      float now = s[0][0];
 #pragma unroll
-      for (int tt = 0; tt < kKT; ++tt)
+      for (int qt = 0; qt < QT; ++qt) {
+        float now = s[qt][0][0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) now = fmaxf(now, s[tt][i]);
-      now *= unit;
-      now = fmaxf(now, __shfl_xor(now, 16));
-      now = fmaxf(fmaxf(now, __shfl_xor(now, 32)), m[qt]);
-      const float f = __builtin_amdgcn_exp2f(m[qt] - now);
-      l[qt] *= f;
+        for (int j = 1; j < 8; ++j) now = fmaxf(now, s[qt][j / 4][j % 4]);
+        now *= unit;
+        now = fmaxf(now, __shfl_xor(now, 16));
+        now = fmaxf(fmaxf(now, __shfl_xor(now, 32)), m[qt]);
+        const float f = __builtin_amdgcn_exp2f(m[qt] - now);
+        l[qt] *= f;
 #pragma unroll
-      for (int dt = 0; dt < kVT; ++dt) o[qt][dt] *= f;
-      m[qt] = now;
-      arguments(now);
+        for (int dt = 0; dt < kVT; ++dt) o[qt][dt] *= f;
+        m[qt] = now;
+      }
+      arguments();
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(e[j]);
-    float sum[4];
+    for (int qt = 0; qt < QT; ++qt) {
+      float sum[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] = e[j] + e[j + 4];
-    l[qt] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      for (int j = 0; j < 8; ++j) e[qt][j] = __builtin_amdgcn_exp2f(e[qt][j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] = e[qt][j] + e[qt][j + 4];
+      l[qt] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
     if constexpr (Q8) {
 #pragma unroll
-      for (int tt = 0; tt < kKT; ++tt)
+      for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = e[tt * 4 + i] * vscale[tt][i];
-          e[tt * 4 + i] = masked && !sees(qt, t + 8 * g + 4 * tt + i) ? 0.0f : x;
+        for (int j = 0; j < 8; ++j) {
+          const float x = e[qt][j] * vscale[j / 4][j % 4];
+          e[qt][j] = masked && !sees(qt, t + 8 * g + j) ? 0.0f : x;
         }
     }
-    u32x4 w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
-    *p = as_bf16x8(w);
+    for (int qt = 0; qt < QT; ++qt) {
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(e[qt][2 * i], e[qt][2 * i + 1]);
+      p[qt] = as_bf16x8(w);
+    }
   }
 
   // What those values add to o for the rows that see them: the wave's steps t, t + stride, .. again, token by token.

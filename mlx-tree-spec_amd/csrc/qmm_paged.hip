@@ -76,18 +76,18 @@ struct PagedWave : PagedRows<D, 1, Q8> {
   // on return those of t + 2 stride).
   template <bool MORE>
   __device__ __forceinline__ void step(int t, int stride, int* kp, int* vp) {
-    f32x4 s[R::kKT], kscale[Q8 ? R::kKT : 1], vscale[Q8 ? R::kKT : 1];
+    f32x4 s[1][R::kKT], kscale[Q8 ? R::kKT : 1], vscale[Q8 ? R::kKT : 1];
 #pragma unroll
-    for (int tt = 0; tt < R::kKT; ++tt) s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int tt = 0; tt < R::kKT; ++tt) s[0][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < R::kKC; ++c) {
 #pragma unroll
       for (int tt = 0; tt < R::kKT; ++tt) {
         if constexpr (Q8) {
-          s[tt] = paged_mma(codes8(kf[tt][c][0], kf[tt][c][1]), this->q[0][2 * c], s[tt]);
-          s[tt] = paged_mma(codes8(kf[tt][c][2], kf[tt][c][3]), this->q[0][2 * c + 1], s[tt]);
+          s[0][tt] = paged_mma(codes8(kf[tt][c][0], kf[tt][c][1]), this->q[0][2 * c], s[0][tt]);
+          s[0][tt] = paged_mma(codes8(kf[tt][c][2], kf[tt][c][3]), this->q[0][2 * c + 1], s[0][tt]);
         } else {
-          s[tt] = paged_mma(as_bf16x8(kf[tt][c]), this->q[0][c], s[tt]);
+          s[0][tt] = paged_mma(as_bf16x8(kf[tt][c]), this->q[0][c], s[0][tt]);
         }
       }
       if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);  // (few codes at a time in registers)
@@ -109,8 +109,8 @@ struct PagedWave : PagedRows<D, 1, Q8> {
       *vp = page(t + 2 * stride + 8 * this->g);
     }
     __builtin_amdgcn_sched_barrier(0);
-    bf16x8 p;
-    this->softmax(t, 0, s, kscale, vscale, &p);
+    bf16x8 p[1];
+    this->softmax(t, s, kscale, vscale, p);
     if constexpr (!Q8) {
       if (t + R::kStep > this->context) {
 #pragma unroll
@@ -119,8 +119,8 @@ struct PagedWave : PagedRows<D, 1, Q8> {
     }
 #pragma unroll
     for (int dt = 0; dt < R::kVT; ++dt) {
-      if constexpr (Q8) this->o[0][dt] = paged_mma(codes8(vf[dt][0], vf[dt][1]), p, this->o[0][dt]);
-      else this->o[0][dt] = paged_mma(as_bf16x8(vf[dt]), p, this->o[0][dt]);
+      if constexpr (Q8) this->o[0][dt] = paged_mma(codes8(vf[dt][0], vf[dt][1]), p[0], this->o[0][dt]);
+      else this->o[0][dt] = paged_mma(as_bf16x8(vf[dt]), p[0], this->o[0][dt]);
       if (Q8 && dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_sched_barrier(0);

@@ -125,8 +125,7 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   // .. and what they add to the rows.
   const auto finish = [&](int t) __attribute__((always_inline)) {
     bf16x8 p[QT];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) W.softmax(t, qt, s[qt], ks, vs, &p[qt]);
+    W.softmax(t, s, ks, vs, p);
 #pragma unroll
     for (int dt = 0; dt < R::kVT; ++dt) {
       bf16x8 v;
