@@ -25,6 +25,7 @@ extern "C" {
 
 #define QMM4_CACHE_MAX_REQUESTS 2048
 #define QMM4_CACHE_MAX_ROWS (1 << 22)
+#define QMM4_CACHE_MAX_KEEP (1 << 16)
 
 /*
  * One step of the tables. For request r of R, with page = page_size:
@@ -40,8 +41,8 @@ extern "C" {
  *   are free; keep: one byte per row [total], or null; slots, positions, request: int32 [total].
  *   plan: int32 [qmm4_cache_plan_words(..)] for qmm4_paged_attention_bf16 on this step, 16-byte aligned, or null where there
  *   is none (with keep: none is made).
- *   Requires R <= QMM4_CACHE_MAX_REQUESTS, total <= QMM4_CACHE_MAX_ROWS, max_rows >= 0, pages * page_size and capacity *
- *   page_size <= 2^30, heads % kv_heads == 0, heads <= 1024. Numbers in the tables that cannot be (lengths past the table,
+ *   Requires R <= QMM4_CACHE_MAX_REQUESTS, total <= QMM4_CACHE_MAX_ROWS (with keep QMM4_CACHE_MAX_KEEP), max_rows >= 0, capacity
+ *   <= 2^22, pages * page_size and capacity * page_size <= 2^30, heads % kv_heads == 0, heads <= 1024. Numbers in the tables that cannot be (lengths past the table,
  *   a count past the list) are taken as the nearest that can.
  */
 int64_t qmm4_cache_plan_words(int64_t R, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_rows);

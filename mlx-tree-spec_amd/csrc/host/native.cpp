@@ -452,7 +452,7 @@ PyObject* cache_step(PyObject*, PyObject* const* a, Py_ssize_t na) {
       !integers(a, 12, most) || len->dim() != 1 || tab->dim() != 2 || fp->dim() != 1)
     return none();
   const int64_t r = len->size(0), capacity = tab->size(1), pages = fp->size(0), total = v[0];
-  if (total <= 0 || !is_table(*len, at::kInt, {r}) || !is_table(*tab, at::kInt, {r, capacity}) || !is_table(*fp, at::kInt, {pages}) ||
+  if (total < 0 || !is_table(*len, at::kInt, {r}) || !is_table(*tab, at::kInt, {r, capacity}) || !is_table(*fp, at::kInt, {pages}) ||
       !is_table(*fc, at::kInt, {1}) || !is_table(*rows, at::kInt, {r}) || (base && !is_table(*base, at::kInt, {r})) ||
       (keep && !is_table(*keep, at::kBool, {total})) ||
       (v[4] != 64 && v[4] != 96 && v[4] != 128 && v[4] != 192 && v[4] != 256))
@@ -461,14 +461,14 @@ PyObject* cache_step(PyObject*, PyObject* const* a, Py_ssize_t na) {
     if (t && t->device() != len->device()) return none();
   if (!same_current_device(*len, {tab, fp, fc, rows})) return none();
   const int64_t words = p_plan_words(r, v[2], v[3], v[4], most[0]);
-  if (words < 0 || total > QMM4_CACHE_MAX_ROWS) return none();  // (the Python form raises)
+  if (words < 0 || total > (keep ? QMM4_CACHE_MAX_KEEP : QMM4_CACHE_MAX_ROWS)) return none();  // (the Python form raises)
   at::Tensor slots = fresh({total}, at::kInt, *len), positions = fresh({total}, at::kInt, *len),
              request = fresh({total}, at::kInt, *len), plan;
   if (!keep) plan = fresh({words}, at::kInt, *len);
   auto i32 = [](const at::Tensor* t) { return t ? static_cast<int32_t*>(ptr(*t)) : nullptr; };
   auto out = [](const at::Tensor& t) { return static_cast<int32_t*>(out_ptr(t)); };
   int32_t *sp = out(slots), *pp = out(positions), *rp = out(request), *plp = keep ? nullptr : out(plan);
-  if (!sp || !pp || !rp || (!keep && !plp)) return none();
+  if ((total > 0 && (!sp || !pp || !rp)) || (!keep && !plp)) return none();
   int32_t *lenp = i32(len), *tabp = i32(tab), *fpp = i32(fp), *fcp = i32(fc), *rowsp = i32(rows), *basep = i32(base);
   const uint8_t* keepp = keep ? static_cast<const uint8_t*>(ptr(*keep)) : nullptr;
   void* st = stream_of(*len);

@@ -41,6 +41,8 @@ int current_cus(int* cus) {
   return QMM4_OK;
 }
 
+int64_t clamp_rows(int64_t max_rows) { return max_rows < QMM4_CACHE_MAX_ROWS ? max_rows : QMM4_CACHE_MAX_ROWS; }
+
 int check_pages(int64_t pages, int64_t page_size, int64_t capacity) {
   if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0)
     return set_error(QMM4_ERR_INVALID, "page_size=%lld must be a power of two from 16 to 1024", (long long)page_size);
@@ -62,6 +64,14 @@ int check_requests(int64_t R, int64_t rows, int64_t max_rows) {
   if (R < 0 || R > QMM4_CACHE_MAX_REQUESTS || rows < 0 || rows > QMM4_CACHE_MAX_ROWS || max_rows < 0)
     return set_error(QMM4_ERR_INVALID, "%lld requests, %lld rows, at most %lld each: up to %d requests and %d rows are supported",
                      (long long)R, (long long)rows, (long long)max_rows, QMM4_CACHE_MAX_REQUESTS, QMM4_CACHE_MAX_ROWS);
+  return QMM4_OK;
+}
+
+// The most rows of a request, where their query rows to a key head can be counted.
+int check_query_rows(int64_t heads, int64_t kv_heads, int64_t max_rows) {
+  if (clamp_rows(max_rows) * (heads / kv_heads) > (1LL << 30))
+    return set_error(QMM4_ERR_INVALID, "up to %lld rows of a request of %lld query heads to a key head: up to 2^30 of both are supported",
+                     (long long)max_rows, (long long)(heads / kv_heads));
   return QMM4_OK;
 }
 
@@ -88,8 +98,6 @@ int log2_of(int64_t v) {
   return s;
 }
 
-int64_t clamp_rows(int64_t max_rows) { return max_rows < QMM4_CACHE_MAX_ROWS ? max_rows : QMM4_CACHE_MAX_ROWS; }
-
 int shape_of(int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_rows, qmm4::PagedShape* out) {
   int cus = 0;
   if (int rc = current_cus(&cus)) return rc;
@@ -108,6 +116,7 @@ int64_t qmm4_cache_plan_words(int64_t R, int64_t heads, int64_t kv_heads, int64_
   const int rc = guarded([&] {
     if (int bad = check_heads(heads, kv_heads)) return bad;
     if (int bad = check_requests(R, 0, max_rows)) return bad;
+    if (int bad = check_query_rows(heads, kv_heads, max_rows)) return bad;
     qmm4::PagedShape s;
     if (int bad = shape_of(heads, kv_heads, head_dim, clamp_rows(max_rows), &s)) return bad;
     words = qmm4::CachePlan::kHead + qmm4::CachePlan::kRecord * (2 * R + s.splits);
@@ -124,6 +133,11 @@ int qmm4_cache_step(int32_t* lengths, int32_t* block_table, int32_t* free_pages,
     if (int rc = check_pages(pages, page_size, capacity)) return rc;
     if (int rc = check_heads(heads, kv_heads)) return rc;
     if (int rc = check_requests(R, total, max_rows)) return rc;
+    if (int rc = check_query_rows(heads, kv_heads, max_rows)) return rc;
+    if (capacity > (1LL << 22))
+      return set_error(QMM4_ERR_INVALID, "%lld pages per request: up to 2^22 are supported", (long long)capacity);
+    if (keep && total > QMM4_CACHE_MAX_KEEP)
+      return set_error(QMM4_ERR_INVALID, "%lld rows with keep: up to %d are supported", (long long)total, QMM4_CACHE_MAX_KEEP);
     if (R == 0 && total == 0 && !plan) return (int)QMM4_OK;
     if ((R > 0 && (!lengths || !rows || (capacity > 0 && !block_table))) || !free_count || (pages > 0 && !free_pages) ||
         (total > 0 && (!slots || !positions || !request)))
@@ -172,6 +186,7 @@ int64_t qmm4_paged_workspace(int64_t M, int64_t R, int64_t Hq, int64_t Hk, int64
   const int rc = guarded([&] {
     if (int bad = check_heads(Hq, Hk)) return bad;
     if (int bad = check_requests(R, M, max_rows)) return bad;
+    if (int bad = check_query_rows(Hq, Hk, max_rows)) return bad;
     if (int bad = check_format(D, 16, nullptr, nullptr)) return bad;
     qmm4::PagedShape s;
     if (int bad = shape_of(Hq, Hk, D, clamp_rows(max_rows), &s)) return bad;
@@ -192,6 +207,7 @@ int qmm4_paged_attention_bf16(const void* q, int64_t q_row, int64_t q_head, cons
     if (int rc = check_pages(pages, page_size, capacity)) return rc;
     if (int rc = check_heads(Hq, Hk)) return rc;
     if (int rc = check_requests(R, M, max_rows)) return rc;
+    if (int rc = check_query_rows(Hq, Hk, max_rows)) return rc;
     if (!std::isfinite(scale)) return set_error(QMM4_ERR_INVALID, "scale must be finite");
     if (M == 0) return (int)QMM4_OK;
     if (!q || !keys || !values || !request || !plan || !out || !workspace || (R > 0 && !block_table))
@@ -204,9 +220,6 @@ int qmm4_paged_attention_bf16(const void* q, int64_t q_row, int64_t q_head, cons
     if (pages == 0 || capacity == 0)
       return set_error(QMM4_ERR_INVALID, "a cache without pages has nothing to attend to");
     const int64_t most = clamp_rows(max_rows);
-    if (most * (Hq / Hk) > (1LL << 30))
-      return set_error(QMM4_ERR_INVALID, "%lld rows of %lld query heads to a key head: up to 2^30 of both are supported",
-                       (long long)most, (long long)(Hq / Hk));
     qmm4::PagedShape s;
     if (int rc = shape_of(Hq, Hk, D, most, &s)) return rc;
     float* part = static_cast<float*>(workspace);

@@ -24,7 +24,7 @@ struct PagedItem {
   int32_t request, first, rows, length;
   int32_t begin, end;  // its tokens
   int32_t part;        // its first partial row, or -1: it is the request's only one
-  int32_t unused;
+  int32_t page;        // the page of its first token
 };
 struct CachePlan {
   int32_t* words;

@@ -3,7 +3,10 @@
 //
 // All of it is prefix sums over the requests (rows, pages back, pages taken, splits) and work over their flat results: item i of
 // a sum belongs to the last request whose prefix is at most i, found by a binary search in LDS. One workgroup does it, since
-// every part waits for a sum over all requests; only rows past kInOne go to a second launch of many workgroups.
+// every part waits for a sum over all requests; only rows past kInOne go to a second launch of many workgroups. Bound by
+// latency: a chain of four prefix sums, and of two loads (the requests' numbers, then page numbers), which is why a row's page is
+// read from where this step finds it (the table, or the free list) and not out of the table behind its update, and why the
+// first page numbers are on their way while the plan is made.
 #include <hip/hip_runtime.h>
 
 #include "qmm_cache.h"
@@ -13,34 +16,47 @@ namespace qmm4 {
 
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
-constexpr int kMaxRequests = QMM4_CACHE_MAX_REQUESTS;
-constexpr int kPer = (kMaxRequests + kThreads - 1) / kThreads;  // requests of a thread, neighbours
+constexpr int kPer = 2;  // requests of a thread, neighbours
+constexpr int kMost = 1024;
 // Rows that the one workgroup places itself.
 constexpr int kInOne = 4096;
+static_assert(kMost * kPer >= QMM4_CACHE_MAX_REQUESTS && kMost * 64 >= QMM4_CACHE_MAX_KEEP, "requests, words of kept rows");
 
-// Exclusive prefix sum over the workgroup's threads, and the total. s: kWaves + 1 words, free again after the next barrier.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s, int64_t* total) {
+// Sums over a wave's lanes up to and with each: shifts by 1, 2, 4 and 8 within rows of 16, then the rows' totals.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+  return x;
+}
+
+// Exclusive prefix sums over the workgroup's threads of N numbers (below 2^31 in a wave), and their totals. One barrier; s: the
+// waves' totals, of two sets in turn (a set is written again behind the next sum's barrier).
+template <int N, int WAVES>
+__device__ __forceinline__ void block_scan(const int (&v)[N], int64_t (&before)[N], int64_t (&total)[N], int (*s)[WAVES]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t x = v;
+  int x[N];
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t y = __shfl_up(x, off);
-    if (lane >= off) x += y;
+  for (int n = 0; n < N; ++n) x[n] = wave_scan(v[n]);
+  if (lane == 63) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) s[n][wave] = x[n];
   }
   __syncthreads();
-  if (lane == 63) s[wave] = x;
-  __syncthreads();
-  int64_t before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const int64_t t = s[w];
-    before += w < wave ? t : 0;
-    all += t;
+  for (int n = 0; n < N; ++n) {
+    before[n] = x[n] - v[n];
+    total[n] = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const int t = s[n][w];
+      before[n] += w < wave ? t : 0;
+      total[n] += t;
+    }
   }
-  *total = all;
-  return before + x - v;
 }
 
 // The last of R (> 0) rising numbers that is at most i (s[0] <= i).
@@ -54,215 +70,233 @@ __device__ __forceinline__ int last_at_most(const int* s, int R, int i) {
   return lo;
 }
 
+__device__ __forceinline__ int slot_of(int shift, int page, int position) {
+  return (int)(((uint32_t)page << shift) + (uint32_t)(position & ((1 << shift) - 1)));
+}
+
 __device__ __forceinline__ void place(const CacheStepParams& S, int m, int slot, int position, int request) {
   S.slots[m] = slot;
   S.positions[m] = position;
   S.request[m] = request;
 }
 
-__device__ __forceinline__ int slot_of(const CacheStepParams& S, int r, int position) {
-  const uint32_t page = S.table[(int64_t)r * S.capacity + (position >> S.page_shift)];
-  return (int)((page << S.page_shift) + (uint32_t)(position & ((1 << S.page_shift) - 1)));
-}
-
-__global__ __launch_bounds__(kThreads) void cache_step_kernel(CacheStepParams S) {
-  __shared__ int64_t s_scan[kWaves];
-  __shared__ int s_first[kMaxRequests], s_rows[kMaxRequests], s_base[kMaxRequests], s_off[kMaxRequests], s_left[kMaxRequests],
-      s_kept[kMaxRequests];
-  const int tid = threadIdx.x, R = S.R, page = 1 << S.page_shift;
-  const auto pages_of = [&](int64_t tokens) { return (int)((tokens + page - 1) >> S.page_shift); };
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void cache_step_kernel(CacheStepParams S) {
+  constexpr int kWaves = THREADS / 64, kRequests = THREADS * kPer;
+  __shared__ int s_scan[2][4][kWaves];
+  __shared__ int s_first[kRequests], s_rows[kRequests], s_base[kRequests], s_left[kRequests], s_back[kRequests], s_took[kRequests];
+  __shared__ uint64_t s_bits[THREADS];  // kept rows, and how many there are before each 64
+  __shared__ int s_kept[THREADS];
+  const int tid = threadIdx.x, lane = tid & 63, R = S.R, shift = S.page_shift, page = 1 << shift;
+  const auto pages_of = [&](int tokens) { return (tokens + page - 1) >> shift; };
   int n[kPer], had[kPer], base[kPer];
-  int64_t total;
+  int64_t total3[3], before3[3], total1[1], before1[1], total2[2], before2[2];
 
-  // Kept rows before each row (into positions for now).
-  if (S.keep) {
-    int64_t before = 0;
-    for (int m0 = 0; m0 < S.total; m0 += kThreads) {
-      const int m = m0 + tid;
-      const int v = m < S.total && S.keep[m] != 0;
-      const int64_t at = before + block_scan(v, s_scan, &total);
-      if (m < S.total) S.positions[m] = (int)at;
-      before += total;
-      __syncthreads();
-    }
-    if (tid == 0) s_scan[0] = before;
-    __syncthreads();
-  }
-  const int all_kept = S.keep ? (int)s_scan[0] : 0;
-
-  // Rows, bases and the pages that go back.
-  int64_t sum_n = 0, sum_back = 0;
+  const int in_list = *S.free_count;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     const int r = tid * kPer + e;
     n[e] = had[e] = base[e] = 0;
     if (r < R) {
-      const int64_t most = S.capacity << S.page_shift;
-      const int length = (int)max((int64_t)0, min((int64_t)S.lengths[r], most));
+      const int most = (int)(S.capacity << shift), length = max(0, min(S.lengths[r], most));
       base[e] = S.base ? max(0, min(S.base[r], length)) : length;
       n[e] = max(0, min(S.rows[r], min(S.max_rows, S.total)));
       had[e] = pages_of(length);
-      s_left[r] = pages_of(base[e]);
-      s_base[r] = base[e];
-      sum_back += had[e] - s_left[r];
-      sum_n += n[e];
     }
   }
-  int64_t at_n = block_scan(sum_n, s_scan, &total);
-  int64_t at_back = block_scan(sum_back, s_scan, &total);
-  const int64_t back = total;
+  const int words = S.keep ? (S.total + 63) / 64 : 0;
+  for (int w = tid >> 6; w < words; w += kWaves) {
+    const int m = w * 64 + lane;
+    const uint64_t kept = __ballot(m < S.total && S.keep[m] != 0);
+    if (lane == 0) s_bits[w] = kept;
+  }
+  if (S.keep) __syncthreads();
+
+  // Rows, the pages that go back, kept rows.
+  int sums[3] = {0, 0, tid < words ? __builtin_popcountll(s_bits[tid]) : 0};
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    sums[0] += n[e];
+    sums[1] += had[e] - pages_of(base[e]);
+  }
+  block_scan<3, kWaves>(sums, before3, total3, s_scan[0]);
+  if (tid < words) s_kept[tid] = (int)before3[2];
+  const int64_t back = total3[1];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     const int r = tid * kPer + e;
     if (r < R) {
-      const int64_t first = min(at_n, (int64_t)S.total);
-      at_n += n[e];
-      n[e] = (int)(min(at_n, (int64_t)S.total) - first);
-      s_first[r] = (int)first;
+      const int first = (int)min(before3[0], (int64_t)S.total);
+      before3[0] += n[e];
+      n[e] = (int)min(before3[0], (int64_t)S.total) - first;
+      s_first[r] = first;
       s_rows[r] = n[e];
-      s_off[r] = (int)min(at_back, (int64_t)1 << 30);
-      at_back += had[e] - s_left[r];
+      s_base[r] = base[e];
+      s_left[r] = pages_of(base[e]);
+      s_back[r] = (int)min(before3[1], (int64_t)1 << 30);
+      before3[1] += had[e] - s_left[r];
     }
   }
-  const int count = max(0, min(*S.free_count, S.pages));
-  __syncthreads();
-
   // (Pages of broken tables past the list's room are dropped.)
-  const int room = (int)min(back, (int64_t)(S.pages - count));
-  for (int i = tid; i < (int)min(back, (int64_t)1 << 30); i += kThreads) {
-    const int r = last_at_most(s_off, R, i);
-    int32_t* entry = S.table + (int64_t)r * S.capacity + s_left[r] + (i - s_off[r]);
-    if (i < room) S.free_pages[count + room - 1 - i] = *entry;
-    *entry = -1;
-  }
-  const int available = count + room;
+  const int count = max(0, min(in_list, S.pages)), room = (int)min(back, (int64_t)(S.pages - count)), available = count + room;
   __syncthreads();
+  if (back > 0) {
+    for (int i = tid; i < (int)min(back, (int64_t)1 << 30); i += THREADS) {
+      const int r = last_at_most(s_back, R, i);
+      int32_t* entry = S.table + (int64_t)r * S.capacity + s_left[r] + (i - s_back[r]);
+      if (i < room) S.free_pages[count + room - 1 - i] = *entry;
+      *entry = -1;
+    }
+    __syncthreads();
+  }
 
+  // Kept rows before row m.
+  const auto kept_before = [&](int m) {
+    if (m >= S.total) return (int)total3[2];
+    return s_kept[m >> 6] + __builtin_popcountll(s_bits[m >> 6] & ((1ull << (m & 63)) - 1));
+  };
   // Pages to take. a: rows that get a place, refused requests have none.
-  int a[kPer], need[kPer];
-  int64_t sum_need = 0;
+  int a[kPer], need[kPer], sum_need[1] = {0};
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     const int r = tid * kPer + e;
     a[e] = need[e] = 0;
     if (r < R) {
-      a[e] = n[e];
-      if (S.keep) {
-        const int first = s_first[r], end = first + n[e];
-        const int kept = first < S.total ? S.positions[first] : all_kept;
-        a[e] = (end < S.total ? S.positions[end] : all_kept) - kept;
-        s_kept[r] = kept;
-      }
-      const int64_t want = ((int64_t)base[e] + a[e] + page - 1) >> S.page_shift;
+      a[e] = S.keep ? kept_before(s_first[r] + n[e]) - kept_before(s_first[r]) : n[e];
+      const int want = pages_of(base[e] + a[e]);
       if (want > S.capacity) a[e] = -1;
-      else need[e] = (int)want - s_left[r];
-      sum_need += need[e];
+      else need[e] = want - s_left[r];
+      sum_need[0] += need[e];
     }
   }
-  int64_t at_need = block_scan(sum_need, s_scan, &total);
-  int64_t cost = 0, blocks = 0, taken = 0;
+  block_scan<1, kWaves>(sum_need, before1, total1, s_scan[1]);
+  int64_t cost = 0;
+  int taken[1] = {0}, blocks = 0;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     const int r = tid * kPer + e;
     if (r < R) {
-      s_off[r] = (int)min(at_need, (int64_t)available);
-      at_need += need[e];
-      if (need[e] > 0 && at_need > available) a[e] = -1;
-      else taken += need[e];
       // (Behind a refused request no other takes pages: the flat index below ends at what is taken.)
+      s_took[r] = (int)min(before1[0], (int64_t)available);
+      before1[0] += need[e];
+      if (need[e] > 0 && before1[0] > available) a[e] = -1;
+      else taken[0] += need[e];
       if (a[e] < 0) {
         a[e] = 0;
         s_rows[r] = -1 - n[e];
       }
       S.lengths[r] = base[e] + a[e];
-      if (S.plan.words) {
-        const int64_t rows = s_rows[r] > 0 ? (int64_t)s_rows[r] * S.G : 0;
-        blocks += (rows + kPagedRows - 1) / kPagedRows;
+      if (S.plan.words && s_rows[r] > 0) {
+        const int64_t rows = (int64_t)s_rows[r] * S.G;
+        blocks += (int)((rows + kPagedRows - 1) / kPagedRows);
         cost += (int64_t)(base[e] + a[e]) * ((rows + kPagedRows - 1) / kPagedRows);
       }
     }
   }
-  block_scan(taken, s_scan, &total);
-  const int took = (int)total;
-  __syncthreads();
-  if (tid == 0) *S.free_count = available - took;
-  for (int i = tid; i < took; i += kThreads) {
-    const int r = last_at_most(s_off, R, i);
-    S.table[(int64_t)r * S.capacity + s_left[r] + (i - s_off[r])] = S.free_pages[available - 1 - i];
+  int took = (int)total1[0];
+  if (total1[0] > available) {
+    block_scan<1, kWaves>(taken, before1, total1, s_scan[0]);
+    took = (int)total1[0];
+    __syncthreads();
   }
-  __syncthreads();
+  // The sum of the costs, in parts of 22 bits, whose sums in a wave stay below 2^31 (a cost is below 2^54).
+  const int parts[4] = {blocks, (int)(cost & 0x3FFFFF), (int)(cost >> 22 & 0x3FFFFF), (int)(cost >> 44)};
+  int64_t total4[4], before4[4];
+  block_scan<4, kWaves>(parts, before4, total4, s_scan[0]);
 
-  // The rows' places.
-  if (S.total <= kInOne || S.keep) {
-    for (int m = tid; m < S.total; m += kThreads) {
-      int slot = -1, position = -1, request = -1;
-      const int r = R > 0 ? last_at_most(s_first, R, m) : 0;
-      if (R > 0 && m - s_first[r] < s_rows[r] && (!S.keep || S.keep[m])) {
-        request = r;
-        position = s_base[r] + (S.keep ? S.positions[m] - s_kept[r] : m - s_first[r]);
-        slot = slot_of(S, r, position);
+  // A request's page, new ones from the list.
+  const auto page_of = [&](int r, int column) {
+    const int fresh = column - s_left[r];
+    return fresh < 0 ? S.table[(int64_t)r * S.capacity + column] : S.free_pages[available - 1 - (s_took[r] + fresh)];
+  };
+  const auto take = [&](int i, int* r, int* column) {
+    *r = last_at_most(s_took, R, i);
+    *column = s_left[*r] + (i - s_took[*r]);
+    return S.free_pages[available - 1 - i];
+  };
+  const auto locate = [&](int m, int* slot, int* position, int* request) {
+    *slot = *position = *request = -1;
+    const int r = R > 0 ? last_at_most(s_first, R, m) : 0;
+    if (R > 0 && m - s_first[r] < s_rows[r] && (!S.keep || (s_bits[m >> 6] >> (m & 63) & 1))) {
+      *request = r;
+      *position = s_base[r] + (S.keep ? kept_before(m) - kept_before(s_first[r]) : m - s_first[r]);
+      *slot = slot_of(shift, page_of(r, *position >> shift), *position);
+    }
+  };
+  // The first page and the first row of each thread: loaded here, stored behind the plan.
+  const bool place_here = S.total <= kInOne || S.keep;
+  int take_r = 0, take_column = 0, take_page = 0, slot, position, request;
+  if (tid < took) take_page = take(tid, &take_r, &take_column);
+  if (place_here && tid < S.total) locate(tid, &slot, &position, &request);
+
+  if (S.plan.words) {
+    // The attention's splits: as many tokens each as leave S.splits in all (a request of several row blocks counts as often). Every
+    // request ends in a split that is not full; where those are few, their number is taken off, so that the splits do not pass
+    // S.splits by them (one workgroup more than the GPU holds at once takes as long again).
+    const int64_t all = total4[1] + (total4[2] << 22) + (total4[3] << 44);
+    const int64_t aim = S.splits > 2 * total4[0] ? S.splits - total4[0] : S.splits;
+    const int64_t chunk = max((int64_t)kPagedUnit, ((all + aim - 1) / aim + kPagedUnit - 1) / kPagedUnit * kPagedUnit);
+    PagedRequest q[kPer];
+    int sum_splits[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int r = tid * kPer + e;
+      q[e] = {0, 0, 0, kPagedUnit, 0, 0, {0, 0}};
+      if (r < R) {
+        q[e].first = s_first[r];
+        q[e].rows = max(0, s_rows[r]);
+        q[e].length = base[e] + a[e];
+        if (q[e].rows > 0) {
+          const int pieces = chunk >= q[e].length ? 1 : (q[e].length + (int)chunk - 1) / (int)chunk;
+          q[e].per = ((q[e].length + pieces - 1) / pieces + kPagedUnit - 1) / kPagedUnit * kPagedUnit;
+          q[e].splits = (q[e].length + q[e].per - 1) / q[e].per;
+        }
+        sum_splits[0] += q[e].splits;
+        sum_splits[1] += q[e].splits > 1 ? q[e].splits * q[e].rows : 0;
       }
+    }
+    block_scan<2, kWaves>(sum_splits, before2, total2, s_scan[1]);
+    // (s_back has served: from here on the requests' first items.)
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int r = tid * kPer + e;
+      if (r < R) {
+        q[e].part = (int)before2[1];
+        S.plan.requests()[r] = q[e];
+        before2[1] += q[e].splits > 1 ? q[e].splits * q[e].rows : 0;
+        s_back[r] = (int)before2[0];
+        before2[0] += q[e].splits;
+      }
+    }
+    if (tid == 0) S.plan.words[0] = (int)total2[0];
+    __syncthreads();
+    for (int i = tid; i < (int)total2[0]; i += THREADS) {
+      const int r = last_at_most(s_back, R, i), split = i - s_back[r];
+      const PagedRequest t = S.plan.requests()[r];
+      S.plan.items()[i] = {r, t.first, t.rows, t.length, split * t.per, min(t.length, (split + 1) * t.per),
+                           t.splits > 1 ? t.part + split * t.rows : -1, page_of(r, split * t.per >> shift)};
+    }
+  }
+
+  if (tid == 0) *S.free_count = available - took;
+  for (int i = tid; i < took; i += THREADS) {
+    if (i != tid) take_page = take(i, &take_r, &take_column);
+    S.table[(int64_t)take_r * S.capacity + take_column] = take_page;
+  }
+  if (place_here) {
+    for (int m = tid; m < S.total; m += THREADS) {
+      if (m != tid) locate(m, &slot, &position, &request);
       place(S, m, slot, position, request);
     }
-  }
-  if (!S.plan.words) return;
-
-  // The attention's splits: as many tokens each as leave S.splits in all (a request of several row blocks counts as often). Every
-  // request ends in a split that is not full; where those are few, their number is taken off, so that the splits do not pass
-  // S.splits by them (one workgroup more than the GPU holds at once takes as long again).
-  block_scan(cost, s_scan, &total);
-  int64_t all_blocks;
-  block_scan(blocks, s_scan, &all_blocks);
-  const int64_t aim = S.splits > 2 * all_blocks ? S.splits - all_blocks : S.splits;
-  const int64_t chunk = max((int64_t)kPagedUnit, ((total + aim - 1) / aim + kPagedUnit - 1) / kPagedUnit * kPagedUnit);
-  PagedRequest q[kPer];
-  int64_t sum_splits = 0, sum_part = 0;
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    const int r = tid * kPer + e;
-    q[e] = {0, 0, 0, kPagedUnit, 0, 0, {0, 0}};
-    if (r < R) {
-      q[e].first = s_first[r];
-      q[e].rows = max(0, s_rows[r]);
-      q[e].length = base[e] + a[e];
-      if (q[e].rows > 0) {
-        const int64_t pieces = (q[e].length + chunk - 1) / chunk;
-        q[e].per = (int)(((q[e].length + pieces - 1) / pieces + kPagedUnit - 1) / kPagedUnit * kPagedUnit);
-        q[e].splits = (q[e].length + q[e].per - 1) / q[e].per;
-      }
-      sum_splits += q[e].splits;
-      sum_part += q[e].splits > 1 ? (int64_t)q[e].splits * q[e].rows : 0;
-    }
-  }
-  int64_t at_part = block_scan(sum_part, s_scan, &total);
-  int64_t at_splits = block_scan(sum_splits, s_scan, &total);
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    const int r = tid * kPer + e;
-    if (r < R) {
-      q[e].part = (int)at_part;
-      S.plan.requests()[r] = q[e];
-      at_part += q[e].splits > 1 ? (int64_t)q[e].splits * q[e].rows : 0;
-      s_off[r] = (int)at_splits;
-      at_splits += q[e].splits;
-    }
-  }
-  if (tid == 0) S.plan.words[0] = (int)total;
-  __syncthreads();
-  for (int i = tid; i < (int)total; i += kThreads) {
-    const int r = last_at_most(s_off, R, i), split = i - s_off[r];
-    const PagedRequest& t = S.plan.requests()[r];
-    S.plan.items()[i] = {r, t.first, t.rows, t.length, split * t.per, min(t.length, (split + 1) * t.per),
-                         t.splits > 1 ? t.part + split * t.rows : -1, 0};
   }
 }
 
 // The places of many rows, from the plan.
-__global__ __launch_bounds__(kThreads) void cache_rows_kernel(CacheStepParams S) {
-  __shared__ int s_first[kMaxRequests];
-  for (int r = threadIdx.x; r < S.R; r += kThreads) s_first[r] = S.plan.requests()[r].first;
+__global__ __launch_bounds__(kMost) void cache_rows_kernel(CacheStepParams S) {
+  __shared__ int s_first[QMM4_CACHE_MAX_REQUESTS];
+  for (int r = threadIdx.x; r < S.R; r += kMost) s_first[r] = S.plan.requests()[r].first;
   __syncthreads();
-  const int m = blockIdx.x * kThreads + threadIdx.x;
+  const int m = blockIdx.x * kMost + threadIdx.x;
   if (m >= S.total) return;
   int slot = -1, position = -1, request = -1;
   if (S.R > 0) {
@@ -270,7 +304,7 @@ __global__ __launch_bounds__(kThreads) void cache_rows_kernel(CacheStepParams S)
     if (m - s_first[r] < n) {
       request = r;
       position = S.plan.requests()[r].length - n + (m - s_first[r]);
-      slot = slot_of(S, r, position);
+      slot = slot_of(S.page_shift, S.table[(int64_t)r * S.capacity + (position >> S.page_shift)], position);
     }
   }
   place(S, m, slot, position, request);
@@ -279,9 +313,13 @@ __global__ __launch_bounds__(kThreads) void cache_rows_kernel(CacheStepParams S)
 }  // namespace
 
 hipError_t launch_cache_step(const CacheStepParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL(cache_step_kernel, dim3(1), dim3(kThreads), 0, stream, p);
+  // Fewer threads, whose barriers and sums are shorter, where two rows each are enough.
+  const int n = p.R > p.total ? p.R : p.total;
+  if (n <= 512) hipLaunchKernelGGL(cache_step_kernel<256>, dim3(1), dim3(256), 0, stream, p);
+  else if (n <= 1024) hipLaunchKernelGGL(cache_step_kernel<512>, dim3(1), dim3(512), 0, stream, p);
+  else hipLaunchKernelGGL(cache_step_kernel<kMost>, dim3(1), dim3(kMost), 0, stream, p);
   if (p.total > kInOne && !p.keep)
-    hipLaunchKernelGGL(cache_rows_kernel, dim3((p.total + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL(cache_rows_kernel, dim3((p.total + kMost - 1) / kMost), dim3(kMost), 0, stream, p);
   return hipGetLastError();
 }
 

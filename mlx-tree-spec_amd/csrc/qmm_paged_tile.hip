@@ -161,7 +161,7 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
     const int stages = (to - from + T::kStage - 1) / T::kStage;
     int next_page = 0;
     if (wide) {
-      next_page = page_at(from);
+      next_page = from == begin ? W.valid_page(I.page) : page_at(from);
     } else {
       __syncthreads();
       for (int i = threadIdx.x; i < kIds; i += kThreads) {

@@ -27,6 +27,8 @@ from .qmm import _check_device
 
 MAX_REQUESTS = 2048
 MAX_ROWS = 1 << 22
+MAX_KEEP = 1 << 16
+MAX_CAPACITY = 1 << 22
 MAX_TOKENS = 1 << 30
 HEAD_DIMS = (64, 96, 128, 192, 256)
 
@@ -118,7 +120,8 @@ def step_tables_(lengths: torch.Tensor, block_table: torch.Tensor, free_pages: t
 
     lengths, rows, base int32 [R]; block_table int32 [R, capacity]; free_pages int32 [pages], the first free_count (int32
     [1]) of which are free. Rows without a place (not kept, refused, padding) have -1 as slot, position and request. heads,
-    kv_heads, head_dim: those of the layers whose attention takes this step. Up to 2048 requests, 2^22 rows and 2^30 tokens.
+    kv_heads, head_dim: those of the layers whose attention takes this step. Up to 2048 requests, 2^22 rows (2^16 with keep), 2^22 pages per request
+    and 2^30 tokens.
     """
     what = "step_tables_"
     max_rows = total if max_rows is None else min(max_rows, total)
@@ -147,6 +150,10 @@ def _step_tables(what, lengths, block_table, free_pages, free_count, rows, total
     if r > MAX_REQUESTS or not 0 <= total <= MAX_ROWS or max_rows < 0:
         raise ValueError(f"[{what}] {r} requests, {total} rows, at most {max_rows} each: up to {MAX_REQUESTS} requests and "
                          f"{MAX_ROWS} rows are supported")
+    if keep is not None and total > MAX_KEEP:
+        raise ValueError(f"[{what}] {total} rows with keep: up to {MAX_KEEP} are supported")
+    if capacity > MAX_CAPACITY:
+        raise ValueError(f"[{what}] {capacity} pages per request: up to {MAX_CAPACITY} are supported")
     if max(capacity, pages) * page_size > MAX_TOKENS:
         raise ValueError(f"[{what}] {pages} pages, {capacity} per request, of {page_size} tokens: up to 2^30 tokens are supported")
     _table(what, "lengths", lengths, (r,))

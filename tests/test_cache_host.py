@@ -62,9 +62,14 @@ def test_table_refusals(change, error, msg):
 
 def test_tables_of_too_many_tokens():
     args = table_args()
-    args["block_table"] = torch.empty(3, 1 << 27, dtype=I32, device="meta")
+    args["block_table"] = torch.empty(3, (1 << 22) + 1, dtype=I32, device="meta")
+    with pytest.raises(ValueError, match="4194305 pages per request"):
+        step_tables_(**args)
+    args["block_table"], args["page_size"] = torch.empty(3, (1 << 20) + 1, dtype=I32, device="meta"), 1024
     with pytest.raises(ValueError, match="up to 2\\^30 tokens"):
         step_tables_(**args)
+    with pytest.raises(ValueError, match="65537 rows with keep"):
+        step_tables_(**{**table_args(total=65537), "keep": z(65537, dtype=torch.bool)})
 
 
 def cache(pages=4, page=16, heads=2, dim=64, bits=16):
@@ -169,7 +174,7 @@ def c_step(**kw):
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(page=17), "page_size=17"), (dict(page=0), "page_size=0"), (dict(pages=-1), "-1 pages"),
-    (dict(capacity=1 << 40), "up to 2^30"), (dict(pages=(1 << 26) + 1), "up to 2^30"), (dict(heads=9), "9 query heads"),
+    (dict(capacity=1 << 40), "up to 2^30"), (dict(capacity=(1 << 22) + 1), "up to 2^22"), (dict(keep=P, total=65537), "65537 rows with keep"), (dict(pages=(1 << 26) + 1), "up to 2^30"), (dict(heads=9), "9 query heads"),
     (dict(R=2049), "2049 requests"), (dict(total=-2), "-2 rows"), (dict(max_rows=-1), "at most -1"), (dict(lengths=None), "null"),
     (dict(table=None), "null"), (dict(count=None), "null"), (dict(free=None), "null"), (dict(slots=None), "null"),
     (dict(rows=P + 2), "aligned"), (dict(plan=P + 1), "aligned")])
