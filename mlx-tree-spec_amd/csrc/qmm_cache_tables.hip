@@ -85,6 +85,7 @@ __global__ __launch_bounds__(THREADS) void cache_step_kernel(CacheStepParams S) 
   constexpr int kWaves = THREADS / 64, kRequests = THREADS * kPer;
   __shared__ int s_scan[2][4][kWaves];
   __shared__ int s_first[kRequests], s_rows[kRequests], s_base[kRequests], s_left[kRequests], s_back[kRequests], s_took[kRequests];
+  static_assert(sizeof(uint64_t) * THREADS == sizeof(int) * kRequests, "s_part below");
   __shared__ uint64_t s_bits[THREADS];  // kept rows, and how many there are before each 64
   __shared__ int s_kept[THREADS];
   const int tid = threadIdx.x, lane = tid & 63, R = S.R, shift = S.page_shift, page = 1 << shift;
@@ -236,32 +237,34 @@ __global__ __launch_bounds__(THREADS) void cache_step_kernel(CacheStepParams S) 
     const int64_t all = total4[1] + (total4[2] << 22) + (total4[3] << 44);
     const int64_t aim = S.splits > 2 * total4[0] ? S.splits - total4[0] : S.splits;
     const int64_t chunk = max((int64_t)kPagedUnit, ((all + aim - 1) / aim + kPagedUnit - 1) / kPagedUnit * kPagedUnit);
+    // A request's record up to its partial rows. (Without keep every row of a request that is not refused has a place.)
+    const auto record = [&](int r) {
+      PagedRequest q = {s_first[r], max(0, s_rows[r]), 0, kPagedUnit, 0, 0, {0, 0}};
+      q.length = s_base[r] + q.rows;
+      if (q.rows > 0) {
+        const uint32_t length = q.length, pieces = chunk >= length ? 1 : (length + (uint32_t)chunk - 1) / (uint32_t)chunk;
+        q.per = ((length + pieces - 1) / pieces + kPagedUnit - 1) / kPagedUnit * kPagedUnit;
+        q.splits = (length + (uint32_t)q.per - 1) / (uint32_t)q.per;
+      }
+      return q;
+    };
     PagedRequest q[kPer];
     int sum_splits[2] = {0, 0};
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      const int r = tid * kPer + e;
-      q[e] = {0, 0, 0, kPagedUnit, 0, 0, {0, 0}};
-      if (r < R) {
-        q[e].first = s_first[r];
-        q[e].rows = max(0, s_rows[r]);
-        q[e].length = base[e] + a[e];
-        if (q[e].rows > 0) {
-          const int pieces = chunk >= q[e].length ? 1 : (q[e].length + (int)chunk - 1) / (int)chunk;
-          q[e].per = ((q[e].length + pieces - 1) / pieces + kPagedUnit - 1) / kPagedUnit * kPagedUnit;
-          q[e].splits = (q[e].length + q[e].per - 1) / q[e].per;
-        }
-        sum_splits[0] += q[e].splits;
-        sum_splits[1] += q[e].splits > 1 ? q[e].splits * q[e].rows : 0;
-      }
+      q[e] = {0, 0, 0, 0, 0, 0, {0, 0}};
+      if (tid * kPer + e < R) q[e] = record(tid * kPer + e);
+      sum_splits[0] += q[e].splits;
+      sum_splits[1] += q[e].splits > 1 ? q[e].splits * q[e].rows : 0;
     }
     block_scan<2, kWaves>(sum_splits, before2, total2, s_scan[1]);
-    // (s_back has served: from here on the requests' first items.)
+    // (s_back has served, and without keep s_bits does not: the requests' first items and partial rows.)
+    int* s_part = reinterpret_cast<int*>(s_bits);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       const int r = tid * kPer + e;
       if (r < R) {
-        q[e].part = (int)before2[1];
+        s_part[r] = q[e].part = (int)before2[1];
         S.plan.requests()[r] = q[e];
         before2[1] += q[e].splits > 1 ? q[e].splits * q[e].rows : 0;
         s_back[r] = (int)before2[0];
@@ -272,9 +275,10 @@ __global__ __launch_bounds__(THREADS) void cache_step_kernel(CacheStepParams S) 
     __syncthreads();
     for (int i = tid; i < (int)total2[0]; i += THREADS) {
       const int r = last_at_most(s_back, R, i), split = i - s_back[r];
-      const PagedRequest t = S.plan.requests()[r];
-      S.plan.items()[i] = {r, t.first, t.rows, t.length, split * t.per, min(t.length, (split + 1) * t.per),
-                           t.splits > 1 ? t.part + split * t.rows : -1, page_of(r, split * t.per >> shift)};
+      const PagedRequest t = record(r);
+      const int begin = split * t.per;
+      S.plan.items()[i] = {r, t.first, t.rows, t.length, begin, min(t.length, begin + t.per),
+                           t.splits > 1 ? s_part[r] + split * t.rows : -1, page_of(r, begin >> shift)};
     }
   }
 

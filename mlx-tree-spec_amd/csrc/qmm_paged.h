@@ -55,9 +55,8 @@ __device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi) {
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
 
 // x * sigmoid(gate) of 4 neighbouring dimensions, rounded.
-__device__ __forceinline__ u32x2 gated_bf16(f32x4 x, const uint16_t* gate) {
-  if (gate) {
-    const u32x2 y = *reinterpret_cast<const u32x2*>(gate);
+__device__ __forceinline__ u32x2 gated_bf16(f32x4 x, bool gated, u32x2 y) {
+  if (gated) {
     x[0] *= sigmoid(bf16_to_f32(y[0] & 0xFFFFu));
     x[1] *= sigmoid(bf16_to_f32(y[0] >> 16));
     x[2] *= sigmoid(bf16_to_f32(y[1] & 0xFFFFu));
@@ -351,7 +350,8 @@ struct PagedRows {
         const uint16_t* gate = S.gate.x ? S.gate.x + (int64_t)(I.first + i) * S.gate.row + (int64_t)hq * S.gate.head + 4 * g : nullptr;
 #pragma unroll
         for (int dt = 0; dt < kVT; ++dt)
-          *reinterpret_cast<u32x2*>(out + dt * 16) = gated_bf16(o[qt][dt] * inv, gate ? gate + dt * 16 : nullptr);
+          *reinterpret_cast<u32x2*>(out + dt * 16) =
+              gated_bf16(o[qt][dt] * inv, gate != nullptr, gate ? *reinterpret_cast<const u32x2*>(gate + dt * 16) : u32x2{0u, 0u});
       } else {
         const int64_t part = ((int64_t)I.part + i) * heads + hq;
 #pragma unroll

@@ -132,8 +132,10 @@ struct PagedWave : PagedRows<D, 1, Q8> {
   __device__ __forceinline__ void run(int t, int end, int stride) {
     const bool any = t < end;
     if (any) {
-      const int vpage = page(t + 8 * this->g);
-      load_keys(t, page(t + 8 * (this->r16 >> 2)));
+      // (The first tokens' page came with the item: one load less to wait for.)
+      const bool known = this->S.cache.page_shift >= 6 && t < this->I.begin + kPagedUnit;
+      const int vpage = known ? this->valid_page(this->I.page) : page(t + 8 * this->g);
+      load_keys(t, known ? vpage : page(t + 8 * (this->r16 >> 2)));
       load_scales(t, vpage);
       load_values(t, vpage);
     }
@@ -158,9 +160,11 @@ __global__ __launch_bounds__((RowsTraits<D, Q8>::kWaves * 64)) void paged_rows_k
   W.run(t, I.end, stride);
   W.add_odd_values(t, I.end, stride, 0);
   W.sum_lanes();
-  // The upper half of the waves hands over to the lower.
+  // The upper half of the waves hands over to the lower (where it has anything).
+  const int steps = (I.end - I.begin + R::kStep - 1) / R::kStep;
 #pragma unroll
   for (int half = T::kWaves / 2; half > 0; half /= 2) {
+    if (half >= steps) continue;
     __syncthreads();
     if (wave >= half && wave < 2 * half) W.hand_over(s_join + (wave - half) * R::kHandBytes);
     __syncthreads();
@@ -182,6 +186,8 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedParams S,
   const int hq = blockIdx.x, c = threadIdx.x % kLanes, slice = threadIdx.x / kLanes;
   const int r = S.request[row];
   uint16_t* out = S.out + (row * heads_q + hq) * D + c * 4;
+  u32x2 gate = {0u, 0u};  // (loaded here: nothing has to wait for it at the end)
+  if (S.gate.x && c * 4 < D) gate = *reinterpret_cast<const u32x2*>(S.gate.x + row * S.gate.row + (int64_t)hq * S.gate.head + c * 4);
   if (r < 0) {
     if (slice == 0 && c * 4 < D) *reinterpret_cast<u32x2*>(out) = u32x2{0u, 0u};
     return;
@@ -237,8 +243,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedParams S,
     o += s_o[s][c] * f;
   }
   o *= paged_empty(S.ancestors, row, Q.length, Q.rows) ? 0.0f : 1.0f / l;
-  *reinterpret_cast<u32x2*>(out) =
-      gated_bf16(o, S.gate.x ? S.gate.x + row * S.gate.row + (int64_t)hq * S.gate.head + c * 4 : nullptr);
+  *reinterpret_cast<u32x2*>(out) = gated_bf16(o, S.gate.x != nullptr, gate);
 }
 
 template <int D, bool Q8>
