@@ -152,7 +152,7 @@ int qmm4_cache_step(int32_t* lengths, int32_t* block_table, int32_t* free_pages,
     if (int rc = shape_of(heads, kv_heads, head_dim, most, &s)) return rc;
     const qmm4::CacheStepParams p{lengths, block_table, free_pages, free_count, rows, base, keep, slots, positions, request,
                                   {keep ? nullptr : plan, (int)R}, capacity, (int)R, (int)pages, (int)total, (int)most,
-                                  log2_of(page_size), s.G, s.splits};
+                                  log2_of(page_size), s.G, s.round, s.splits};
     const hipError_t e = qmm4::launch_cache_step(p, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return hip_error(e, "cache table kernel launch");
     return (int)QMM4_OK;

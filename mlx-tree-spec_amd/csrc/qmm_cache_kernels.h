@@ -38,7 +38,8 @@ static_assert(sizeof(PagedRequest) == CachePlan::kRecord * 4 && sizeof(PagedItem
 // How a step's attention is cut: at most `splits` + R items.
 struct PagedShape {
   int G;           // query heads of a key head
-  int64_t splits;  // pieces of the whole that are aimed at, for each key head
+  int64_t round;   // pieces for each key head whose workgroups the GPU holds at once
+  int64_t splits;  // pieces of the whole that are aimed at, at most
 };
 PagedShape paged_shape(int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_rows, int cus);
 // Query rows of all partial results, for each key head, at most.
@@ -52,7 +53,7 @@ struct CacheStepParams {
   CachePlan plan;  // (words null: none)
   int64_t capacity;
   int R, pages, total, max_rows, page_shift, G;
-  int64_t splits;
+  int64_t round, splits;
 };
 hipError_t launch_cache_step(const CacheStepParams& p, hipStream_t stream);
 

@@ -232,10 +232,10 @@ __global__ __launch_bounds__(THREADS) void cache_step_kernel(CacheStepParams S) 
 
   if (S.plan.words) {
     // The attention's splits: as many tokens each as leave S.splits in all (a request of several row blocks counts as often). Every
-    // request ends in a split that is not full; where those are few, their number is taken off, so that the splits do not pass
-    // S.splits by them (one workgroup more than the GPU holds at once takes as long again).
+    // request ends in a split that is not full; where they are few beside one round, one round less their number is aimed at
+    // (one workgroup more than the GPU holds at once takes as long again).
     const int64_t all = total4[1] + (total4[2] << 22) + (total4[3] << 44);
-    const int64_t aim = S.splits > 2 * total4[0] ? S.splits - total4[0] : S.splits;
+    const int64_t aim = S.round > 2 * total4[0] ? S.round - total4[0] : S.splits;
     const int64_t chunk = max((int64_t)kPagedUnit, ((all + aim - 1) / aim + kPagedUnit - 1) / kPagedUnit * kPagedUnit);
     // A request's record up to its partial rows. (Without keep every row of a request that is not refused has a place.)
     const auto record = [&](int r) {
