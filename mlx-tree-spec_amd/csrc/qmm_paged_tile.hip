@@ -57,7 +57,8 @@ __device__ __forceinline__ void bare_barrier() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-template <int D, int QT, int SIDES, bool Q8>
+// WIDE: pages of a stage's tokens and more.
+template <int D, int QT, int SIDES, bool Q8, bool WIDE>
 __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int block0, int blocks) {
   using T = TileTraits<D, QT, SIDES, Q8>;
   using R = PagedRows<D, QT, Q8>;
@@ -137,10 +138,9 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
     }
   };
 
-  // Pages of a stage's tokens and more: one page for a stage, addresses that only the scalar unit makes.
+  // WIDE: one page for a stage, addresses that only the scalar unit makes.
   static_assert(kPagedUnit % T::kStage == 0, "a stage begins at a multiple of its tokens");
-  const bool wide = page_mask + 1 >= T::kStage;
-  const int segment = wide ? 1 << 30 : kIds << shift;  // tokens whose pages are known at once
+  const int segment = WIDE ? 1 << 30 : kIds << shift;  // tokens whose pages are known at once
   // A lane's token of a key's piece, in the order of the tiles' rows.
   const int key_token = lane % T::kStage / R::kStep * R::kStep + 8 * ((lane & 15) >> 2) + 4 * (lane / 16 % R::kKT) + (lane & 3);
   constexpr int kScaleLanes = T::kStage / 4;
@@ -155,13 +155,13 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   const int mine_token = mine_keys ? 16 : D * 16 / E, mine_stride = mine_keys ? kKeyPieces << (shift + 4) : 1024;
   const uint32_t mine_offset = mine_keys ? ((uint32_t)(lane / T::kStage) << (shift + 4)) + key_token * 16 : lane * 16;
   const int64_t page_bytes = (int64_t)D * 16 / E << shift;  // (of one head)
-  const auto page_at = [&](int tok) { return W.valid_page(constant_table[min(tok, W.length - 1) >> shift]); };
+  const auto page_at = [&](int tok) { return constant_table[min(tok, W.length - 1) >> shift]; };
   for (int base = begin & ~page_mask; base < end; base += segment) {
     const int from = max(begin, base), to = min(end, base > (1 << 30) - segment ? end : base + segment);
     const int stages = (to - from + T::kStage - 1) / T::kStage;
-    int next_page = 0;
-    if (wide) {
-      next_page = from == begin ? W.valid_page(I.page) : page_at(from);
+    int next_page = 0;  // (as the table has it: made valid where it is used, a stage later)
+    if constexpr (WIDE) {
+      next_page = from == begin ? I.page : page_at(from);
     } else {
       __syncthreads();
       for (int i = threadIdx.x; i < kIds; i += kThreads) {
@@ -175,8 +175,8 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
     auto load = [&](int st) __attribute__((always_inline)) {
       const int t = from + st * T::kStage;
       char* ring = s_ring + (st % T::kStages) * T::kStageBytes;
-      if (wide) {
-        const int64_t head = (int64_t)next_page * S.cache.heads + W.h;
+      if constexpr (WIDE) {
+        const int64_t head = (int64_t)W.valid_page(next_page) * S.cache.heads + W.h;
         const int off = t & page_mask;
         next_page = page_at(t + T::kStage);
         const char* src = mine_base + head * page_bytes + off * mine_token;
@@ -189,28 +189,28 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
           const float* src = (lane & kScaleLanes ? S.cache.value_scales : S.cache.key_scales) + (head << shift) + off;
           __builtin_amdgcn_global_load_lds((global_ptr)(src + (lane & (kScaleLanes - 1)) * 4), (lds_ptr)(ring + T::kPieces * 16), 16, 0, 0);
         }
-        return;
-      }
-      const auto head_of = [&](int tok) { return (int64_t)s_ids[(tok - base) >> shift] * S.cache.heads + W.h; };
-      const int grp = min(W.group(t + (key_token & ~7)), base + segment - 8);
-      const char* kp = keys + ((head_of(grp) * (D / E) << shift) + (grp & page_mask) + (key_token & 7)) * 16;
+      } else {
+        const auto head_of = [&](int tok) { return (int64_t)s_ids[(tok - base) >> shift] * S.cache.heads + W.h; };
+        const int grp = min(W.group(t + (key_token & ~7)), base + segment - 8);
+        const char* kp = keys + ((head_of(grp) * (D / E) << shift) + (grp & page_mask) + (key_token & 7)) * 16;
 #pragma unroll
-      for (int j = 0; j < T::kChunkLoads; ++j) {
-        const int chunk = mine_chunk + j;
-        const char* src;
-        if (chunk < T::kChunks / 2) {
-          src = kp + ((int64_t)(chunk * kKeyPieces + lane / T::kStage) << (shift + 4));
-        } else {
-          const int f = (chunk - T::kChunks / 2) * 64 + lane, at = f / D, d = f - at * D;
-          const int tok = min(W.group(t + at * E), base + segment - E) & ~(E - 1);
-          src = values + (((head_of(tok) << shift) + (tok & page_mask)) / E * D + d) * 16;
+        for (int j = 0; j < T::kChunkLoads; ++j) {
+          const int chunk = mine_chunk + j;
+          const char* src;
+          if (chunk < T::kChunks / 2) {
+            src = kp + ((int64_t)(chunk * kKeyPieces + lane / T::kStage) << (shift + 4));
+          } else {
+            const int f = (chunk - T::kChunks / 2) * 64 + lane, at = f / D, d = f - at * D;
+            const int tok = min(W.group(t + at * E), base + segment - E) & ~(E - 1);
+            src = values + (((head_of(tok) << shift) + (tok & page_mask)) / E * D + d) * 16;
+          }
+          __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(ring + chunk * 1024), 16, 0, 0);
         }
-        __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(ring + chunk * 1024), 16, 0, 0);
-      }
-      if constexpr (Q8) {
-        const int tok = min(W.group(t + (lane & (kScaleLanes - 2)) * 4), base + segment - 8) + (lane & 1) * 4;
-        const float* src = (lane & kScaleLanes ? S.cache.value_scales : S.cache.key_scales) + (head_of(tok) << shift) + (tok & page_mask);
-        __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(ring + T::kPieces * 16), 16, 0, 0);
+        if constexpr (Q8) {
+          const int tok = min(W.group(t + (lane & (kScaleLanes - 2)) * 4), base + segment - 8) + (lane & 1) * 4;
+          const float* src = (lane & kScaleLanes ? S.cache.value_scales : S.cache.key_scales) + (head_of(tok) << shift) + (tok & page_mask);
+          __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(ring + T::kPieces * 16), 16, 0, 0);
+        }
       }
     };
 
@@ -290,19 +290,25 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   if (side == 0 && active) W.write(mine);
 }
 
-template <int D, int QT, int SIDES, bool Q8>
-hipError_t launch_tile(const PagedParams& p, hipStream_t stream) {
+template <int D, int QT, int SIDES, bool Q8, bool WIDE>
+hipError_t launch_pages(const PagedParams& p, hipStream_t stream) {
   using T = TileTraits<D, QT, SIDES, Q8>;
   static LdsAllowance allowance;
-  if (hipError_t e = allowance.allow(reinterpret_cast<const void*>(&paged_tile_kernel<D, QT, SIDES, Q8>), T::kLds)) return e;
+  if (hipError_t e = allowance.allow(reinterpret_cast<const void*>(&paged_tile_kernel<D, QT, SIDES, Q8, WIDE>), T::kLds)) return e;
   const int64_t units = ((int64_t)p.items * p.cache.heads + 7) / 8 * 8, blocks = ((int64_t)p.max_rows * p.G + T::kRows - 1) / T::kRows;
   const int64_t most = std::max<int64_t>(1, (int64_t{1} << 22) / units);  // (a grid may have 2^32 threads)
   for (int64_t b0 = 0; b0 < blocks; b0 += most) {
     const int64_t count = std::min(most, blocks - b0);
-    hipLaunchKernelGGL((paged_tile_kernel<D, QT, SIDES, Q8>), dim3((unsigned)(units * count)), dim3(kThreads), T::kLds, stream, p,
-                       (int)b0, (int)count);
+    hipLaunchKernelGGL((paged_tile_kernel<D, QT, SIDES, Q8, WIDE>), dim3((unsigned)(units * count)), dim3(kThreads), T::kLds, stream,
+                       p, (int)b0, (int)count);
   }
   return hipGetLastError();
+}
+
+template <int D, int QT, int SIDES, bool Q8>
+hipError_t launch_tile(const PagedParams& p, hipStream_t stream) {
+  if (1 << p.cache.page_shift >= TileTraits<D, QT, SIDES, Q8>::kStage) return launch_pages<D, QT, SIDES, Q8, true>(p, stream);
+  return launch_pages<D, QT, SIDES, Q8, false>(p, stream);
 }
 
 template <int D, bool Q8>
