@@ -7,9 +7,8 @@
 // a ring of stages in LDS without registers (1 KB an instruction), kAhead stages ahead, in the order in which the waves read
 // them: a fragment is then 256 neighbouring bytes for 16 lanes, without bank conflicts. One barrier a stage, behind an exact
 // count of the loads that may still be on their way.
-//
-// The barrier would have all waves multiply and exponentiate at the same time. Waves 4 to 7, which share the SIMDs with 0 to 3,
-// are half a stage late: they end the stage before (exponentials, values' product) while the others begin with this one's keys.
+// (Half of the waves half a stage late, so that a SIMD's two would multiply and exponentiate in turn, measured the same; so did
+// priorities.)
 #include <algorithm>
 #include <type_traits>
 
@@ -216,7 +215,6 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
 
     const auto ring_of = [&](int st) { return reinterpret_cast<const u32x4*>(s_ring + (st % T::kStages) * T::kStageBytes); };
     const auto token_of = [&](int st) { return from + st * T::kStage + side * R::kStep; };
-    const bool late = wave >= kWaves / 2;
     // The values of a stage past the context made clean in place, by all waves (once: a branch around products of clean and other
     // values would have every sum in registers twice).
     const auto clean = [&](int st) {
@@ -236,13 +234,9 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
       if (!Q8 && from + (st + 1) * T::kStage > W.context) clean(st);
     };
     for (int st = 0; st < T::kAhead && st < stages; ++st) load(st);
-    // Late waves meet the others at a stage's barrier before they end the stage before it.
 #pragma unroll 1
-    for (int st = 0; st <= stages; ++st) {
-      if (late && st < stages) arrive(st);
-      if (active && st > 0 && token_of(st - 1) < to) finish(token_of(st - 1));
-      if (st == stages) break;
-      if (!late) arrive(st);
+    for (int st = 0; st < stages; ++st) {
+      arrive(st);
       // (Its keys are on their way while the loads ahead are made, its values while the products run.)
       const u32x4* ring = ring_of(st);
       const u32x4* kr = ring + W.g * T::kStage + side * R::kStep + W.r16;
@@ -273,6 +267,7 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
           vs[tt] = scales[T::kStage / 4 + tt];
         }
       }
+      if (token_of(st) < to) finish(token_of(st));
     }
     // (Every load has been waited for: the ring is free behind the next barrier.)
     __syncthreads();
