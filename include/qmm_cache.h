@@ -37,8 +37,8 @@ extern "C" {
  * is every one that needs pages from the first on for which too few are left: a refused one has a = 0.
  *   lengths[r] becomes b + a; the k-th of its a rows gets position b + k, its slot, and request r; rows without a place
  *   (not kept, refused, behind the last request) get -1 in all three.
- *   lengths, rows, base: int32 [R]; block_table: int32 [R, capacity]; free_pages: int32 [pages], whose first free_count[0]
- *   are free; keep: one byte per row [total], or null; slots, positions, request: int32 [total].
+ *   lengths, rows, base: int32 [R]; block_table: int32 [R, capacity]; free_pages: int32 [pages] (room for every page of the
+ *   cache), whose first free_count[0] are free; keep: one byte per row [total], or null; slots, positions, request: int32 [total].
  *   plan: int32 [qmm4_cache_plan_words(..)] for qmm4_paged_attention_bf16 on this step, 16-byte aligned, or null where there
  *   is none (with keep: none is made).
  *   Requires R <= QMM4_CACHE_MAX_REQUESTS, total <= QMM4_CACHE_MAX_ROWS (with keep QMM4_CACHE_MAX_KEEP), max_rows >= 0, capacity

@@ -190,7 +190,7 @@ int64_t qmm4_paged_workspace(int64_t M, int64_t R, int64_t Hq, int64_t Hk, int64
     if (int bad = check_format(D, 16, nullptr, nullptr)) return bad;
     qmm4::PagedShape s;
     if (int bad = shape_of(Hq, Hk, D, clamp_rows(max_rows), &s)) return bad;
-    bytes = qmm4::paged_partial_rows(s, M, R, clamp_rows(max_rows)) * Hk * (D + 2) * (int64_t)sizeof(float);
+    bytes = std::max<int64_t>(16, qmm4::paged_partial_rows(s, M, R, clamp_rows(max_rows)) * Hk * (D + 2) * (int64_t)sizeof(float));
     return (int)QMM4_OK;
   });
   return rc ? rc : bytes;

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(kThreads) void store_kv_kernel(StoreParams S) {
   // Where runs begin among the block's rows and those behind it (a run has at most 16; past the last row: one more).
   const int64_t m = m0 + lane;
   const int slot = m < S.M ? S.slots[m] : -1, before = m > 0 && m < S.M ? S.slots[m - 1] : -1;
-  const uint64_t begins = __ballot(m == 0 || m >= S.M || (slot & (E - 1)) == 0 || before != slot - 1 || lane >= 48);
+  const uint64_t begins = __ballot(m == 0 || m >= S.M || (slot & (E - 1)) == 0 || (uint32_t)before + 1 != (uint32_t)slot || lane >= 48);
   const int last = S.block + __builtin_ctzll(begins >> S.block);
   for (int a = __builtin_ctzll(begins); a < last;) {
     // Whole runs of up to 16 rows.

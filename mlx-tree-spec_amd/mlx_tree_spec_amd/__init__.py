@@ -15,7 +15,7 @@ from .lora import LoRALinear, quantized_matmul_lora, stack_adapters
 from .packed_linear import STATS, QuantizedLinear, QuantizedMLP, eligible, install
 from .qmm import dequantize, gate_up_silu, pack_nax, quantized_matmul, unpack_nax
 from .sampling import sample
-from .verify import AttentionInputs, GraphedTail, MLPLayer, attention_inputs, layer_tail, next_tokens, stack_tail
+from .verify import AttentionInputs, GraphedTail, MLPLayer, attention_inputs, cached_attention, layer_tail, next_tokens, stack_tail
 
 __all__ = [
     "quantized_matmul", "gate_up_silu", "dequantize", "pack_nax", "unpack_nax", "add_rms_norm",
@@ -23,5 +23,6 @@ __all__ = [
     "quantized_matmul_lora", "stack_adapters", "LoRALinear", "qk_norm_rope", "sample", "eligible", "install",
     "STATS", "MLPLayer", "layer_tail", "stack_tail", "GraphedTail", "AttentionInputs", "attention_inputs", "next_tokens",
     "KVCache", "CacheTables", "CacheStep", "step_tables_", "store_kv_", "paged_attention",
+    "cached_attention",
 ]
 __version__ = "0.1.0"

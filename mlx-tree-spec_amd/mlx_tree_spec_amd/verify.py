@@ -8,11 +8,13 @@ once over all rows, and each residual add is fused with the RMS norm that follow
     nxt  = next layer's input_layernorm, or the model's final norm # 445
     h, x = add_rms_norm(h, layer.mlp(x), nxt)                      # 446
 
-`r` is the attention (or GatedDeltaNet) output of the layer, which this package does not compute. What lies before
-it, and behind the last layer, is here as well:
+`r` is the attention (or GatedDeltaNet) output of the layer. What lies before it, attention over a paged cache, and what
+lies behind the last layer are here as well:
 
     q, k, v, gate = attention_inputs(x, layer, positions, adapters)  # tree_verify.py:311-328: projections (with each
                                                                      # row's adapter), head norms, rotation
+    a, k, v = cached_attention(x, layer, cache, step, ...)           # tree_verify.py:311-402: the same, the rows stored, and
+                                                                     # attention over all that their requests hold
     tokens, logprobs = next_tokens(x, lm_head, uniform, ...)         # tree_verify.py:447: vocabulary head, sampling
 
 When the MLP is a QuantizedMLP, the first norm is folded into its gate+up projection
@@ -31,6 +33,7 @@ from __future__ import annotations
 
 import torch
 
+from .cache import CacheStep, KVCache, paged_attention, store_kv_
 from .fused_ops import _norm_eps, add_rms_norm, add_rms_norm_gate_up
 from .heads import qk_norm_rope
 from .lora import LoRALinear
@@ -105,6 +108,27 @@ def attention_inputs(x: torch.Tensor, layer: AttentionInputs, positions: torch.T
     q, k = qk_norm_rope(q[..., :d] if layer.gated else q, k, layer.q_norm.weight, layer.k_norm.weight,
                         _norm_eps(layer.q_norm), positions, layer.inv_freq, interleaved=layer.interleaved)
     return q, k, v, gate
+
+
+def cached_attention(x: torch.Tensor, layer: AttentionInputs, cache: KVCache, step: CacheStep,
+                     positions: torch.Tensor | None = None, adapters: torch.Tensor | None = None,
+                     ancestors: torch.Tensor | None = None, scale: float | None = None):
+    """(a, k, v) of a step's rows x (M, K): attention_inputs at `positions`, their keys and values stored into the layer's cache at
+    the step's places, and their attention a (M, heads * D) over it, times sigmoid(gate) where the layer is gated: what its
+    output projection takes.
+
+    positions: the step's by default (rows in a line); a tree's rows have that of their depth. ancestors as in
+    paged_attention. k and v (M, kv_heads, D) are what was stored: once a tree's accepted nodes are known, a step of the
+    tables with base and keep gives their places in a line, and store_kv_(k, v, cache, step.slots) puts them there.
+    """
+    if x.dim() != 2:
+        raise ValueError(f"[cached_attention] x must be (rows, K), got {tuple(x.shape)}")
+    if (layer.heads, layer.kv_heads, layer.head_dim) != (step.heads, step.kv_heads, step.head_dim):
+        raise ValueError(f"[cached_attention] a layer of {layer.heads} and {layer.kv_heads} heads of {layer.head_dim}, but the step "
+                         f"was made for {step.heads} and {step.kv_heads} heads of {step.head_dim}")
+    q, k, v, gate = attention_inputs(x, layer, step.positions if positions is None else positions, adapters)
+    store_kv_(k, v, cache, step.slots)
+    return paged_attention(q, cache, step, scale=scale, ancestors=ancestors, gate=gate).reshape(len(x), layer.heads * layer.head_dim), k, v
 
 
 def next_tokens(x: torch.Tensor, head: torch.nn.Module, uniform: torch.Tensor, adapters: torch.Tensor | None = None,

@@ -257,3 +257,27 @@ def test_plain_and_native_calls_agree(monkeypatch):
     monkeypatch.setattr(_lib, "_native", _lib._NoNative)
     for c, w in zip(cases, want):
         assert torch.equal(c.run(), w)
+
+
+def test_no_rows_and_no_requests():
+    case = Case([5, 9], [0, 0], 6, 2, 64, pad=3, seed=13)
+    case.check(case.run())
+    case = Case([5, 9], [2, 1], 6, 2, 64, seed=14, max_rows=0)
+    assert case.step.request.tolist() == [-1] * 3 and not case.run().any()
+    case = Case([5], [0], 6, 2, 64, seed=15)
+    assert case.run().shape == (0, 6, 64)
+    step = step_tables_(i32([]), torch.empty((0, 2), dtype=torch.int32, device=DEV), i32([0]), i32([1]), i32([]), 2, 64, 6, 2, 64)
+    q = torch.randn(2, 6, 64, device=DEV).to(torch.bfloat16)
+    assert not case.run(q=q, step=step).any()
+
+
+def test_nan_queries_stay_in_their_rows():
+    for rows, max_rows in ((1, 1), (9, None)):
+        case = Case([200, 50, 70], [rows] * 3, 6, 2, 128, seed=16, max_rows=max_rows)
+        want = case.run()
+        case.q[rows, 4, 7] = float("nan")
+        case.q[2 * rows, 1, 3] = float("inf")
+        out = case.run()
+        assert torch.isnan(out[rows, 4].float()).all() and not torch.isfinite(out[2 * rows, 1].float()).all()
+        out[rows, 4], out[2 * rows, 1] = want[rows, 4], want[2 * rows, 1]
+        assert torch.equal(out, want)
