@@ -39,11 +39,11 @@ extern "C" {
  *   (not kept, refused, behind the last request) get -1 in all three.
  *   lengths, rows, base: int32 [R]; block_table: int32 [R, capacity]; free_pages: int32 [pages] (room for every page of the
  *   cache), whose first free_count[0] are free; keep: one byte per row [total], or null; slots, positions, request: int32 [total].
- *   plan: int32 [qmm4_cache_plan_words(..)] for qmm4_paged_attention_bf16 on this step, 16-byte aligned, or null where there
- *   is none (with keep: none is made).
+ *   plan: int32 [qmm4_cache_plan_words(..)] for qmm4_paged_attention_bf16 on this step, 16-byte aligned, or null where no
+ *   attention follows (with keep none is made).
  *   Requires R <= QMM4_CACHE_MAX_REQUESTS, total <= QMM4_CACHE_MAX_ROWS (with keep QMM4_CACHE_MAX_KEEP), max_rows >= 0, capacity
- *   <= 2^22, pages * page_size and capacity * page_size <= 2^30, heads % kv_heads == 0, heads <= 1024. Numbers in the tables that cannot be (lengths past the table,
- *   a count past the list) are taken as the nearest that can.
+ *   <= 2^22, pages * page_size and capacity * page_size <= 2^30, heads % kv_heads == 0, heads <= 1024. Numbers in the tables
+ *   that cannot be (lengths past the table, a count past the list) are taken as the nearest that can.
  */
 int64_t qmm4_cache_plan_words(int64_t R, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_rows);
 int qmm4_cache_step(int32_t* lengths, int32_t* block_table, int32_t* free_pages, int32_t* free_count, const int32_t* rows,

@@ -3,7 +3,8 @@
 //
 // All of it is prefix sums over the requests (rows, pages back, pages taken, splits) and work over their flat results: item i of
 // a sum belongs to the last request whose prefix is at most i, found by a binary search in LDS. One workgroup does it, since
-// every part waits for a sum over all requests; only rows past kInOne go to a second launch of many workgroups. Bound by
+// every part waits for a sum over all requests; only rows past kInOne go to a second launch of many workgroups, which finds its
+// requests in the plan (without one, as with kept rows, the first places all). Bound by
 // latency: a chain of four prefix sums, and of two loads (the requests' numbers, then page numbers), which is why a row's page is
 // read from where this step finds it (the table, or the free list) and not out of the table behind its update, and why the
 // first page numbers are on their way while the plan is made.
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(THREADS) void cache_step_kernel(CacheStepParams S) 
     }
   };
   // The first page and the first row of each thread: loaded here, stored behind the plan.
-  const bool place_here = S.total <= kInOne || S.keep;
+  const bool place_here = S.total <= kInOne || !S.plan.words;
   int take_r = 0, take_column = 0, take_page = 0, slot, position, request;
   if (tid < took) take_page = take(tid, &take_r, &take_column);
   if (place_here && tid < S.total) locate(tid, &slot, &position, &request);
@@ -322,7 +323,7 @@ hipError_t launch_cache_step(const CacheStepParams& p, hipStream_t stream) {
   if (n <= 512) hipLaunchKernelGGL(cache_step_kernel<256>, dim3(1), dim3(256), 0, stream, p);
   else if (n <= 1024) hipLaunchKernelGGL(cache_step_kernel<512>, dim3(1), dim3(512), 0, stream, p);
   else hipLaunchKernelGGL(cache_step_kernel<kMost>, dim3(1), dim3(kMost), 0, stream, p);
-  if (p.total > kInOne && !p.keep)
+  if (p.total > kInOne && p.plan.words)
     hipLaunchKernelGGL(cache_rows_kernel, dim3((p.total + kMost - 1) / kMost), dim3(kMost), 0, stream, p);
   return hipGetLastError();
 }

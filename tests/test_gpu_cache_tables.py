@@ -8,7 +8,7 @@ import torch
 
 import cache_refs as R
 from cache_refs import i32
-from mlx_tree_spec_amd import CacheTables, step_tables_
+from mlx_tree_spec_amd import CacheTables, _lib, step_tables_
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -66,6 +66,28 @@ def test_many_rows(total, keep):
     rows = [total // 10, 0, total // 3, 1, 0, total // 4, 17]
     b.step(rows, total, keep=[rng.random() < 0.6 for _ in range(total)] if keep else None)
     b.step([0] * 7, 3, base=[0] * 7)
+
+
+@pytest.mark.parametrize("total", [100, 4096, 4097, 20000])
+def test_steps_without_a_plan(total):
+    """At the C entry a step whose plan nobody needs places its rows like one with a plan."""
+    requests, page, capacity, pages = 9, 32, 800, 1500
+    lib, rows = _lib.load(), i32([total // 9 - 3] * 8 + [total // 3])
+    out = []
+    for planned in (True, False):
+        tables = [i32([0, 40, 7, 0, 31, 32, 33, 1, 5]), torch.full((requests, capacity), -1, dtype=torch.int32, device=DEV),
+                  i32(list(range(pages))), i32([pages - 10])]
+        tables[1][:, :2] = torch.arange(pages - 18, pages, dtype=torch.int32, device=DEV).reshape(9, 2)
+        places = [torch.full((total,), -7, dtype=torch.int32, device=DEV) for _ in range(3)]
+        plan = torch.empty(lib.qmm4_cache_plan_words(requests, 24, 4, 128, total), dtype=torch.int32, device=DEV) if planned else None
+        rc = lib.qmm4_cache_step(*(t.data_ptr() for t in tables), rows.data_ptr(), None, None, *(t.data_ptr() for t in places),
+                                 plan.data_ptr() if planned else None, requests, capacity, pages, total, total, page, 24, 4, 128,
+                                 torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, _lib.last_error()
+        out.append(places + tables)
+    for a, b in zip(*out):
+        assert torch.equal(a, b) and a.min() > -7
+    assert (out[0][2] >= 0).sum() == min(total, int(rows.sum()))
 
 
 def test_pages_given_back_are_taken_again():
