@@ -555,6 +555,7 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t na) {
     if (t && t->device() != q->device()) return none();
   int64_t mq, qr, qh, gr = 0, gh = 0;
   if (!heads(*q, &mq, &qr, &qh) || (gate && !heads(*gate, &mq, &gr, &gh))) return none();
+  if (plan->dim() != 1 || plan->size(0) != p_plan_words(r, v[0], v[1], v[2], v[3])) return none();
   const int64_t bytes = p_paged_workspace(m, r, v[0], v[1], v[2], v[3]);
   if (bytes < 0) return PyLong_FromLong((long)bytes);
   at::Tensor out = fresh(q->sizes(), at::kBFloat16, *q), ws = fresh({bytes}, at::kByte, *q);

@@ -291,14 +291,25 @@ def paged_attention(q: torch.Tensor, cache: KVCache, step: CacheStep, scale: flo
         raise ValueError(f"[{what}] scale={scale} must be finite")
     if ancestors is not None:
         _table(what, "ancestors", ancestors, (m,), torch.int64)
+    if step.block_table.dim() != 2:
+        raise ValueError(f"[{what}] the step's block_table must have 2 dimensions, got {tuple(step.block_table.shape)}")
+    for name, t, shape in (("block_table", step.block_table, tuple(step.block_table.shape)), ("request", step.request, (m,)),
+                           ("plan", step.plan, tuple(step.plan.shape))):
+        _table(what, f"the step's {name}", t, shape)
+        if not t.is_contiguous():
+            raise ValueError(f"[{what}] the step's {name} must be contiguous")
     dev = _check_device(what, q, step.block_table, step.request, step.plan, *(t for t in cache if t is not None),
                         *(t for t in (ancestors, gate) if t is not None))
     r, capacity = step.block_table.shape
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        words = lib.qmm4_cache_plan_words(r, step.heads, kv_heads, dim, step.max_rows)
+    _lib.check(min(words, 0), what)
+    _table(what, "the step's plan", step.plan, (words,))
     q3 = _head_rows(q)
     g3 = None if gate is None else _head_rows(gate)
     ancestors = ancestors if ancestors is None else ancestors.contiguous()
     out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
-    lib = _lib.load()
     with torch.cuda.device(dev):
         size = lib.qmm4_paged_workspace(m, r, step.heads, kv_heads, dim, step.max_rows)
         _lib.check(min(size, 0), what)

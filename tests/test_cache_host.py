@@ -162,6 +162,20 @@ def test_attention_refusals(change, msg):
         paged_attention(**args)
 
 
+@pytest.mark.parametrize("change,msg", [
+    (dict(block_table=z(12, dtype=I32)), "block_table must have 2 dimensions"),
+    (dict(block_table=z(3, 4, dtype=torch.int64)), "block_table must be"),
+    (dict(block_table=z(3, 8, dtype=I32)[:, :4]), "block_table must be contiguous"),
+    (dict(request=z(10, dtype=I32)[::2]), "request must be contiguous"),
+    (dict(request=z(5, dtype=torch.int64)), "request must be"),
+    (dict(plan=z(40)), "plan must be"),
+    (dict(plan=z(80, dtype=I32)[::2]), "plan must be contiguous"),
+])
+def test_attention_of_a_changed_step(change, msg):
+    with pytest.raises(ValueError, match=msg):
+        paged_attention(z(5, 8, 64), cache(), step()._replace(**change))
+
+
 P = 0x10000
 
 

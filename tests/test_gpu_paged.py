@@ -271,6 +271,15 @@ def test_no_rows_and_no_requests():
     assert not case.run(q=q, step=step).any()
 
 
+def test_plans_of_other_steps_are_refused():
+    """A plan whose size is not that of the step's requests and heads is refused before anything is launched."""
+    c = Case([100, 40], [1, 1], 8, 2, 64)
+    for change in (dict(plan=c.step.plan[:-8]), dict(plan=torch.cat((c.step.plan, c.step.plan[:8]))),
+                   dict(block_table=c.step.block_table[:1])):
+        with pytest.raises(ValueError, match="the step's plan must be"):
+            paged_attention(c.q, c.cache, c.step._replace(**change))
+
+
 def test_nan_queries_stay_in_their_rows():
     for rows, max_rows in ((1, 1), (9, None)):
         case = Case([200, 50, 70], [rows] * 3, 6, 2, 128, seed=16, max_rows=max_rows)
