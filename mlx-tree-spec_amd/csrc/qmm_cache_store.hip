@@ -4,7 +4,8 @@
 // the cache hold one dimension of E neighbouring tokens. Rows whose tokens share such a piece are a run, and a run is stored by
 // one workgroup: in whole pieces where all E tokens are there (prompts), in single elements where not (decode); lines of the
 // cache are not written in parts by several XCDs. A workgroup takes the runs that begin in its block of rows, up to 16 rows at a
-// time, for some 256 values of each, of keys or of values. Bound by latency up to some hundred rows, by HBM past that.
+// time, for some 256 values of each, of keys or of values. Bound by latency up to some hundred rows (16 rows of 4 heads of 256:
+// 3.2 us), by HBM past that (4096 rows of 8 heads of 128, 34 MB in and out: 9.7 us, 3.5 TB/s; 1500 of 4 heads of 256 into 8 bits: 8.2).
 #include "qmm4_common.h"
 #include "qmm_cache_kernels.h"
 
@@ -201,7 +202,8 @@ __global__ __launch_bounds__(kThreads) void store_kv_kernel(StoreParams S) {
 
 hipError_t launch_store_kv(const CacheRows& k, const CacheRows& v, const int32_t* slots, const CacheArrays& cache, int64_t M,
                            int D, bool q8, hipStream_t stream) {
-  // A row to a block where there are few.
+  // A row to a block where there are few: 16 of as many requests 4.1 us (7.4 with blocks of 16), 200 5.8 (8.3); 512 of a prompt 4.7
+  // with blocks of 16 (8.2 with blocks of one), 4096 10 (42).
   const int block = M <= 256 ? 1 : 16, heads = kWidth / D;
   const StoreParams p{k, v, slots, cache, M, D, block, heads};
   const dim3 grid((unsigned)((M + block - 1) / block), (unsigned)((cache.heads + heads - 1) / heads * 2));
