@@ -2,11 +2,12 @@
 // (include/qmm_cache.h). With G query heads to a key head, a request of n rows has n G query rows for each key head:
 //   s = scale q . k_t,   m = max s,   l = sum exp(s - m),   o = sum exp(s - m) v_t,   out = o / l  (* sigmoid(gate))
 //
-// This file: up to 16 query rows to a key head (decode), the join of splits, and the choice. Every byte of the cache is used
-// once, for 16 rows at most: bound by HBM. A wave loads its operands from memory to registers, 1 KB an instruction in whole
-// runs of 64 bytes and more, without LDS, and takes every KW-th step of its workgroup's split; while a step's probabilities
-// are made the next step's keys are on their way, and its values while the products with the present ones run. Waves join
-// through LDS, splits through memory (fp32) and a second kernel.
+// This file: up to 16 query rows to a key head (decode) of heads up to 128 or 8 bits, the join of splits, and the choice. Every
+// byte of the cache is used once, for 16 rows at most: bound by HBM (64 requests of up to 16000 tokens, 8 key heads of 128, 2.4 GB:
+// 416 us, 5.8 TB/s; 16 of up to 40000 in 8 bits, 4 of 256: 133 us, 5.7 TB/s). A wave loads its operands from memory to registers,
+// 1 KB an instruction in whole runs of 64 bytes and more, without LDS, and takes every 8th step of its workgroup's split; while
+// a step's probabilities are made the next step's keys are on their way, and its values while the products with the present ones
+// run. Waves join through LDS, splits through memory (fp32) and a second kernel (4.7 us for 64 splits).
 #include <type_traits>
 
 #include "qmm4_lds.h"
@@ -16,14 +17,7 @@ namespace qmm4 {
 
 namespace {
 
-template <int D, bool Q8>
-struct RowsTraits {
-  using R = PagedRows<D, 1, Q8>;
-  // Registers of o, q, s, keys, values and scales; with what else there is more than 256: one wave to a SIMD.
-  static constexpr int kRegisters = 4 * (R::kVT + R::kQK + R::kKT + R::kKT * R::kKC + (Q8 ? R::kVT / 2 + 3 * R::kKT : R::kVT));
-  static constexpr int kWaves = kRegisters > 200 ? 4 : 8;
-  static constexpr size_t kLds = (size_t)(kWaves / 2) * R::kHandBytes;
-};
+constexpr int kRowsWaves = 8;
 
 template <int D, bool Q8>
 struct PagedWave : PagedRows<D, 1, Q8> {
@@ -148,22 +142,21 @@ struct PagedWave : PagedRows<D, 1, Q8> {
 };
 
 template <int D, bool Q8>
-__global__ __launch_bounds__((RowsTraits<D, Q8>::kWaves * 64)) void paged_rows_kernel(PagedParams S) {
-  using T = RowsTraits<D, Q8>;
+__global__ __launch_bounds__(kRowsWaves * 64) void paged_rows_kernel(PagedParams S) {
   using R = PagedRows<D, 1, Q8>;
   extern __shared__ __attribute__((aligned(16))) char s_join[];
   const int item = blockIdx.x / S.cache.heads;
   const PagedItem I = S.plan.items()[item];
   if (item >= S.plan.words[0]) return;
   PagedWave<D, Q8> W(S, I, blockIdx.x - item * S.cache.heads);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = I.begin + wave * R::kStep, stride = T::kWaves * R::kStep;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = I.begin + wave * R::kStep, stride = kRowsWaves * R::kStep;
   W.run(t, I.end, stride);
   W.add_odd_values(t, I.end, stride, 0);
   W.sum_lanes();
   // The upper half of the waves hands over to the lower (where it has anything).
   const int steps = (I.end - I.begin + R::kStep - 1) / R::kStep;
 #pragma unroll
-  for (int half = T::kWaves / 2; half > 0; half /= 2) {
+  for (int half = kRowsWaves / 2; half > 0; half /= 2) {
     if (half >= steps) continue;
     __syncthreads();
     if (wave >= half && wave < 2 * half) W.hand_over(s_join + (wave - half) * R::kHandBytes);
@@ -175,11 +168,11 @@ __global__ __launch_bounds__((RowsTraits<D, Q8>::kWaves * 64)) void paged_rows_k
 
 constexpr int kJoinThreads = 256;
 
-// The splits of each row and head joined; zeros for rows without a request. kLanes lanes of 4 dimensions to a split, kAhead
-// splits of each loaded together.
+// The splits of each row and head joined; zeros for rows without a request. kLanes lanes of 4 dimensions to a split, up to 8 splits
+// of each loaded together.
 template <int D>
 __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedParams S, int64_t m0) {
-  constexpr int kLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, kSlices = kJoinThreads / kLanes, kAhead = 8;
+  constexpr int kLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, kSlices = kJoinThreads / kLanes;
   __shared__ f32x4 s_o[kSlices][kLanes];
   __shared__ float s_m[kSlices], s_l[kSlices];
   const int64_t row = m0 + blockIdx.y, heads_q = gridDim.x;
@@ -197,33 +190,39 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedParams S,
   const int64_t part = ((int64_t)Q.part + (row - Q.first)) * heads_q + hq, stride = (int64_t)Q.rows * heads_q;
   float m = -__builtin_inff(), l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s0 = slice; s0 < Q.splits; s0 += kSlices * kAhead) {
-    float m2[kAhead], l2[kAhead];
-    f32x4 o2[kAhead];
+  const auto gather = [&](auto ahead) __attribute__((always_inline)) {
+    constexpr int kAhead = decltype(ahead)::value;
+    for (int s0 = slice; s0 < Q.splits; s0 += kSlices * kAhead) {
+      float m2[kAhead], l2[kAhead];
+      f32x4 o2[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      // (Past the last: the first again, with nothing in it.)
-      const bool here = s0 + j * kSlices < Q.splits;
-      const int64_t at = part + (here ? s0 + j * kSlices : s0) * stride;
-      m2[j] = here ? S.part_ml[at * 2] : -__builtin_inff();
-      l2[j] = S.part_ml[at * 2 + 1];
-      o2[j] = *reinterpret_cast<const f32x4*>(S.part + at * D + (c * 4 < D ? c * 4 : 0));
+      for (int j = 0; j < kAhead; ++j) {
+        // (Past the last: the first again, with nothing in it.)
+        const bool here = s0 + j * kSlices < Q.splits;
+        const int64_t at = part + (here ? s0 + j * kSlices : s0) * stride;
+        m2[j] = here ? S.part_ml[at * 2] : -__builtin_inff();
+        l2[j] = S.part_ml[at * 2 + 1];
+        o2[j] = *reinterpret_cast<const f32x4*>(S.part + at * D + (c * 4 < D ? c * 4 : 0));
+      }
+      float top = m;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) top = fmaxf(top, m2[j]);
+      const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      l *= f;
+      o *= f;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (m2[j] == -__builtin_inff()) continue;
+        const float f2 = __builtin_amdgcn_exp2f(m2[j] - top);
+        l += l2[j] * f2;
+        o += o2[j] * f2;
+      }
     }
-    float top = m;
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) top = fmaxf(top, m2[j]);
-    const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-    m = top;
-    l *= f;
-    o *= f;
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      if (m2[j] == -__builtin_inff()) continue;
-      const float f2 = __builtin_amdgcn_exp2f(m2[j] - top);
-      l += l2[j] * f2;
-      o += o2[j] * f2;
-    }
-  }
+  };
+  if (Q.splits <= 2 * kSlices) gather(std::integral_constant<int, 2>{});
+  else if (Q.splits <= 4 * kSlices) gather(std::integral_constant<int, 4>{});
+  else gather(std::integral_constant<int, 8>{});
   s_o[slice][c] = o;
   if (c == 0) {
     s_m[slice] = m;
@@ -248,20 +247,12 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedParams S,
 
 template <int D, bool Q8>
 hipError_t launch_rows(const PagedParams& p, hipStream_t stream) {
-  using T = RowsTraits<D, Q8>;
+  constexpr size_t kLds = (size_t)(kRowsWaves / 2) * PagedRows<D, 1, Q8>::kHandBytes;
   static LdsAllowance allowance;
-  if (T::kLds > 64 * 1024)
-    if (hipError_t e = allowance.allow(reinterpret_cast<const void*>(&paged_rows_kernel<D, Q8>), T::kLds)) return e;
-  hipLaunchKernelGGL((paged_rows_kernel<D, Q8>), dim3((unsigned)p.items * p.cache.heads), dim3(T::kWaves * 64), T::kLds, stream, p);
+  if (kLds > 64 * 1024)
+    if (hipError_t e = allowance.allow(reinterpret_cast<const void*>(&paged_rows_kernel<D, Q8>), kLds)) return e;
+  hipLaunchKernelGGL((paged_rows_kernel<D, Q8>), dim3((unsigned)p.items * p.cache.heads), dim3(kRowsWaves * 64), kLds, stream, p);
   return hipGetLastError();
-}
-
-template <int D>
-hipError_t launch_dim(const PagedParams& p, bool q8, hipStream_t stream) {
-  if constexpr (D % 64 == 0) {
-    if (q8) return launch_rows<D, true>(p, stream);
-  }
-  return launch_rows<D, false>(p, stream);
 }
 
 template <int D>
@@ -292,18 +283,23 @@ int64_t paged_partial_rows(const PagedShape& s, int64_t M, int64_t R, int64_t ma
 
 static hipError_t launch_paged_rows(const PagedParams& p, int D, bool q8, hipStream_t stream) {
   switch (D) {
-    case 64: return launch_dim<64>(p, q8, stream);
-    case 96: return launch_dim<96>(p, q8, stream);
-    case 128: return launch_dim<128>(p, q8, stream);
-    case 192: return launch_dim<192>(p, q8, stream);
-    default: return launch_dim<256>(p, q8, stream);
+    case 64: return q8 ? launch_rows<64, true>(p, stream) : launch_rows<64, false>(p, stream);
+    case 96: return launch_rows<96, false>(p, stream);
+    case 128: return q8 ? launch_rows<128, true>(p, stream) : launch_rows<128, false>(p, stream);
+    case 192: return launch_rows<192, true>(p, stream);
+    default: return launch_rows<256, true>(p, stream);
   }
 }
 
 hipError_t launch_paged_attention(const PagedParams& p, int64_t M, int D, bool q8, hipStream_t stream) {
   const int64_t rows = (int64_t)p.max_rows * p.G;
   if (p.plan.R > 0 && rows > 0) {
-    const hipError_t e = rows <= 16 ? launch_paged_rows(p, D, q8, stream) : launch_paged_tile(p, D, q8, stream);
+    // bf16 heads of 192 and more take the tile kernel from the first row on: their step is more than 8 waves' registers hold, while one
+    // wave that multiplies keeps up with the loads of 8 into LDS (one request of 2000 tokens, 6 heads of 256 to a key head: 6.3 us, 7.6
+    // with waves of their own; 16 of up to 8000: 63, 65). Smaller heads do not (64 of up to 16000, 4 of 128: 433 us, 428; one of
+    // 2000 7.0, 5.9), and codes have to be converted by all waves (16 of up to 40000, 6 of 256: 357, 133).
+    const bool tile = rows > 16 || (D > 128 && !q8);
+    const hipError_t e = tile ? launch_paged_tile(p, D, q8, stream) : launch_paged_rows(p, D, q8, stream);
     if (e != hipSuccess) return e;
   }
   switch (D) {

@@ -1,14 +1,18 @@
-// Paged attention of more than 16 query rows to a key head: tree verify and prompt rows (qmm_paged.h has the products and the
-// softmax). Each byte of the cache serves up to 128 query rows of a workgroup: bound by HBM up to about that many, past it by the
-// matrix instructions and what feeds them.
+// Paged attention of more than 16 query rows to a key head, tree verify and prompt rows, and of all rows of bf16 heads of 192 and
+// more (qmm_paged.h has the products and the softmax). Each byte of the cache serves up to 128 query rows of a workgroup: bound by
+// HBM up to some 64 rows (one row of 6 heads over 200000 tokens, 4 key heads of 256: 137 us, 6.0 TB/s), past that by the matrix
+// instructions and the softmax's vector instructions (64 nodes of 4 heads over 32000 tokens, 8 key heads of 128: 51.6 us, 650 TFLOP/s;
+// 1000 rows over 8000: 174 us, 800 TFLOP/s).
 //
 // A workgroup takes up to kPagedRows query rows of one key head over one split: 8 waves with 16 QT rows each, or with two SIDES
 // 4 of them on the even steps and the others with the same rows on the odd ones. The steps' keys and values go from memory to
-// a ring of stages in LDS without registers (1 KB an instruction), kAhead stages ahead, in the order in which the waves read
-// them: a fragment is then 256 neighbouring bytes for 16 lanes, without bank conflicts. One barrier a stage, behind an exact
-// count of the loads that may still be on their way.
+// a ring of stages in LDS without registers (1 KB an instruction), two stages ahead, in the order in which the waves read
+// them: a fragment is then 256 neighbouring bytes for 16 lanes, without bank conflicts. One barrier a stage, in front of the
+// softmax, behind an exact count of the loads that may still be on their way: the softmax covers the reads of its own values and of the
+// next step's keys (1000 rows 181 -> 174 us, 4 x 16 nodes of 6 heads of 256 28.4 -> 26.6).
 // (Half of the waves half a stage late, so that a SIMD's two would multiply and exponentiate in turn, measured the same; so did
-// priorities.)
+// priorities, 4 waves to a workgroup and two of those to a CU, and the values' products among the next step's exponentials: with
+// heads of 256 those took more registers than there are.)
 #include <algorithm>
 #include <type_traits>
 
@@ -34,21 +38,25 @@ struct TileTraits {
   static constexpr int kStageBytes = kPieces * 16 + (Q8 ? 1024 : 0);  // (scales, over and over)
   static constexpr int kChunkLoads = (kChunks / 2 + kWaves / 2 - 1) / (kWaves / 2);
   static constexpr int kLoads = kChunkLoads + (Q8 ? 1 : 0);  // a wave's loads of a stage
-  static constexpr int kRoom = 160 * 1024 - kIds * 4 - 512;
-  static constexpr int kStages = kRoom / kStageBytes < 4 ? kRoom / kStageBytes : 4;
-  static constexpr int kAhead = kStages - 1;              // (a stage is read between its barrier and the next)
+  // A stage that is multiplied, whose values are read while the next one's keys are, and two on their way.
+  static constexpr int kStages = 4;
+  // A step's keys are read while the softmax before it runs, or where registers are short piece by piece in place of values.
+  static constexpr bool kEarly = R::kKC * R::kKT <= 8;
+  static_assert(kEarly || SIDES == 1, "every wave has a step of each stage");
   static constexpr size_t kRing = (size_t)kStages * kStageBytes;
   static constexpr size_t kJoin = SIDES > 1 ? (size_t)kAcross * R::kHandBytes : 0;
   static constexpr size_t kLds = (kRing > kJoin ? kRing : kJoin) + kIds * 4 + 16;
-  static_assert(kAhead >= 1 && kLds <= 160 * 1024, "LDS");
+  static_assert(kLds <= 160 * 1024, "LDS");
 };
 
-// Waits until at most N of the wave's loads into LDS are on their way, and none of its reads out of LDS (what it has read may be
-// written over behind the next barrier).
+// Waits until at most N of the wave's loads into LDS are on their way.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+
+// Waits for the wave's reads out of LDS.
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 __device__ __forceinline__ void bare_barrier() {
   __builtin_amdgcn_sched_barrier(0);
@@ -123,7 +131,7 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
     }
   };
   // .. and what they add to the rows.
-  const auto finish = [&](int t) __attribute__((always_inline)) {
+  const auto finish = [&](int t, auto&& between) __attribute__((always_inline)) {
     bf16x8 p[QT];
     W.softmax(t, s, ks, vs, p);
 #pragma unroll
@@ -133,6 +141,7 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
       else v = as_bf16x8(vf[dt]);
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) W.o[qt][dt] = paged_mma(v, p[qt], W.o[qt][dt]);
+      between(dt);
       if (Q8 && dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -227,47 +236,75 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       bare_barrier();
     };
+    // Stage `st` is in the ring for every wave, where those up to st + 1 are loaded or on their way.
     const auto arrive = [&](int st) __attribute__((always_inline)) {
-      if (st + T::kAhead - 1 < stages) wait_loads<(T::kAhead - 1) * T::kLoads>();
+      if (st + 1 < stages) wait_loads<T::kLoads>();
       else wait_loads<0>();
       bare_barrier();
       if (!Q8 && from + (st + 1) * T::kStage > W.context) clean(st);
     };
-    for (int st = 0; st < T::kAhead && st < stages; ++st) load(st);
+    u32x4 kf[R::kKC][R::kKT];
+    const auto read_key = [&](int st, int c, int tt) __attribute__((always_inline)) {
+      kf[c][tt] = (ring_of(st) + W.g * T::kStage + side * R::kStep + W.r16)[c * 4 * T::kStage + tt * 16];
+    };
+    const auto read_keys = [&](int st) __attribute__((always_inline)) {
+#pragma unroll
+      for (int c = 0; c < R::kKC; ++c)
+#pragma unroll
+        for (int tt = 0; tt < R::kKT; ++tt) read_key(st, c, tt);
+    };
+    // The next stage, and one behind those on their way into the place of the one before `st`.
+    const auto advance = [&](int st, auto&& then) __attribute__((always_inline)) {
+      if (st + 1 >= stages) return;
+      arrive(st + 1);
+      then();
+      if (st + 3 < stages) load(st + 3);
+    };
+    load(0);
+    if (1 < stages) load(1);
+    arrive(0);
+    if (active) read_keys(0);
+    if (2 < stages) load(2);
+    if (!active) {
 #pragma unroll 1
-    for (int st = 0; st < stages; ++st) {
-      arrive(st);
-      // (Its keys are on their way while the loads ahead are made, its values while the products run.)
-      const u32x4* ring = ring_of(st);
-      const u32x4* kr = ring + W.g * T::kStage + side * R::kStep + W.r16;
-      constexpr bool kEarly = R::kKC * R::kKT <= 8;  // (or too many registers)
-      u32x4 kf[R::kKC][R::kKT];
-      const auto read_keys = [&]() __attribute__((always_inline)) {
+      for (int st = 0; st < stages; ++st) advance(st, [] {});
+    } else {
+#pragma unroll 1
+      for (int st = 0; st < stages; ++st) {
+        // (The keys, and all that was read before them: behind the next barrier the place of the stage before is loaded again.)
+        wait_reads();
+        multiply(kf);
+        __builtin_amdgcn_sched_barrier(0);
+        const u32x4* ring = ring_of(st);
+        // (8 bits: two groups of 8 tokens share a piece.)
+        const Piece* vr = reinterpret_cast<const Piece*>(ring + T::kPieces / 2 + (Q8 ? side * 2 + (W.g >> 1) : side * 4 + W.g) * D + W.r16) +
+                          (Q8 ? W.g & 1 : 0);
 #pragma unroll
-        for (int c = 0; c < R::kKC; ++c)
+        for (int dt = 0; dt < R::kVT; ++dt) vf[dt] = vr[dt * (Q8 ? 32 : 16)];
+        if constexpr (Q8) {
+          const f32x4* scales = reinterpret_cast<const f32x4*>(ring + T::kPieces) + side * 8 + W.g * 2;
 #pragma unroll
-          for (int tt = 0; tt < R::kKT; ++tt) kf[c][tt] = kr[c * 4 * T::kStage + tt * 16];
-      };
-      if (kEarly) read_keys();
-      if (st + T::kAhead < stages) load(st + T::kAhead);
-      if (!active) continue;
-      if (!kEarly) read_keys();
-      multiply(kf);
-      __builtin_amdgcn_sched_barrier(0);
-      // (8 bits: two groups of 8 tokens share a piece.)
-      const Piece* vr = reinterpret_cast<const Piece*>(ring + T::kPieces / 2 + (Q8 ? side * 2 + (W.g >> 1) : side * 4 + W.g) * D + W.r16) +
-                        (Q8 ? W.g & 1 : 0);
+          for (int tt = 0; tt < R::kKT; ++tt) {
+            ks[tt] = scales[tt];
+            vs[tt] = scales[T::kStage / 4 + tt];
+          }
+        }
+        const int next = st + 1 < stages ? st + 1 : st;
+        advance(st, [&]() __attribute__((always_inline)) {
+          if constexpr (T::kEarly) read_keys(next);
+        });
+        if constexpr (T::kEarly) {
+          if (SIDES == 1 || token_of(st) < to) finish(token_of(st), [](int) {});
+        } else {
+          constexpr int kEach = R::kKC * R::kKT / R::kVT;
+          static_assert(kEach * R::kVT == R::kKC * R::kKT, "keys in place of values");
+          finish(token_of(st), [&](int dt) __attribute__((always_inline)) {
 #pragma unroll
-      for (int dt = 0; dt < R::kVT; ++dt) vf[dt] = vr[dt * (Q8 ? 32 : 16)];
-      if constexpr (Q8) {
-        const f32x4* scales = reinterpret_cast<const f32x4*>(ring + T::kPieces) + side * 8 + W.g * 2;
-#pragma unroll
-        for (int tt = 0; tt < R::kKT; ++tt) {
-          ks[tt] = scales[tt];
-          vs[tt] = scales[T::kStage / 4 + tt];
+            for (int i = 0; i < kEach; ++i) read_key(next, (dt * kEach + i) / R::kKT, (dt * kEach + i) % R::kKT);
+            __builtin_amdgcn_sched_barrier(0);
+          });
         }
       }
-      if (token_of(st) < to) finish(token_of(st));
     }
     // (Every load has been waited for: the ring is free behind the next barrier.)
     __syncthreads();
@@ -308,8 +345,9 @@ hipError_t launch_tile(const PagedParams& p, hipStream_t stream) {
 
 template <int D, bool Q8>
 hipError_t launch_rows(const PagedParams& p, hipStream_t stream) {
-  // Two sides of 4 waves; 16 rows to a wave where those hold a request's, else 32. Heads of 192 and more, whose sums and queries
-  // would not leave room for 32 rows in 256 registers (nor their stages of 64 tokens for 3 of them in LDS): 16 rows to each of 8.
+  // Two sides of 4 waves; 16 rows to a wave where those hold a request's (16 nodes of 4 heads to a key head over 32000 tokens:
+  // 33.7 us, 35.9 with 32 rows), else 32 (64 nodes: 58 us, 68 with 16 rows). Heads of 192 and more, whose sums and queries would not
+  // leave room for 32 rows in 256 registers (nor their stages of 64 tokens for 4 of them in LDS): 16 rows to each of 8.
   if constexpr (D > 128) return launch_tile<D, 1, 1, Q8>(p, stream);
   else if ((int64_t)p.max_rows * p.G <= 64) return launch_tile<D, 1, 2, Q8>(p, stream);
   else return launch_tile<D, 2, 2, Q8>(p, stream);
