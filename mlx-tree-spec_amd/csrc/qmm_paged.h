@@ -173,7 +173,7 @@ struct PagedRows {
   // The first token of a group of 8, within the request's.
   __device__ __forceinline__ int group(int token) const { return min(token, (length - 1) & ~7); }
   // A page of the cache, whatever the table holds.
-  __device__ __forceinline__ int valid_page(int page) const { return max(0, min(page, (int)S.cache.pages - 1)); }
+  __device__ __forceinline__ int valid_page(int page) const { return (int)min((uint32_t)page, (uint32_t)S.cache.pages - 1); }
 
   // Whether the row sees a token: all of the context, and of what follows up to `seen` what its bits say. (Without branches:
   // hipcc 7.2 has lost the selected value of nested divergent ones here.)

@@ -162,8 +162,9 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
                                     : values + (mine_chunk - T::kChunks / 2) * 1024;
   const int mine_token = mine_keys ? 16 : D * 16 / E, mine_stride = mine_keys ? kKeyPieces << (shift + 4) : 1024;
   const uint32_t mine_offset = mine_keys ? ((uint32_t)(lane / T::kStage) << (shift + 4)) + key_token * 16 : lane * 16;
-  const int64_t page_bytes = (int64_t)D * 16 / E << shift;  // (of one head)
-  const auto page_at = [&](int tok) { return constant_table[min(tok, W.length - 1) >> shift]; };
+  const uint32_t head_bytes = D * 16 / E << shift, page_bytes = S.cache.heads * head_bytes;  // of a page (at most 2^29)
+  const char* mine_head = mine_base + (int64_t)W.h * head_bytes;
+  const auto page_at = [&](int tok) { return constant_table[(uint32_t)min(tok, W.length - 1) >> shift]; };
   for (int base = begin & ~page_mask; base < end; base += segment) {
     const int from = max(begin, base), to = min(end, base > (1 << 30) - segment ? end : base + segment);
     const int stages = (to - from + T::kStage - 1) / T::kStage;
@@ -184,17 +185,17 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
       const int t = from + st * T::kStage;
       char* ring = s_ring + (st % T::kStages) * T::kStageBytes;
       if constexpr (WIDE) {
-        const int64_t head = (int64_t)W.valid_page(next_page) * S.cache.heads + W.h;
-        const int off = t & page_mask;
+        const uint32_t page = W.valid_page(next_page), off = t & page_mask;
         next_page = page_at(t + T::kStage);
-        const char* src = mine_base + head * page_bytes + off * mine_token;
+        const char* src = mine_head + (uint64_t)page * page_bytes + off * mine_token;
 #pragma unroll
         for (int j = 0; j < T::kChunkLoads; ++j)
           __builtin_amdgcn_global_load_lds((global_ptr)(src + j * mine_stride + mine_offset),
                                            (lds_ptr)(ring + (mine_chunk + j) * 1024), 16, 0, 0);
         if constexpr (Q8) {
           // 4 tokens a lane: key scales, value scales, and both again (every lane of a load writes).
-          const float* src = (lane & kScaleLanes ? S.cache.value_scales : S.cache.key_scales) + (head << shift) + off;
+          const float* src = (lane & kScaleLanes ? S.cache.value_scales : S.cache.key_scales) +
+                             (((int64_t)page * S.cache.heads + W.h) << shift) + off;
           __builtin_amdgcn_global_load_lds((global_ptr)(src + (lane & (kScaleLanes - 1)) * 4), (lds_ptr)(ring + T::kPieces * 16), 16, 0, 0);
         }
       } else {
