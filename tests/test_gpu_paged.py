@@ -134,6 +134,15 @@ def test_rows_of_a_prompt():
     case.check(case.run())
 
 
+@pytest.mark.parametrize("hq,hk,dim,bits", [(8, 2, 64, 16), (4, 2, 256, 16), (8, 2, 128, 8)])
+def test_most_requests(hq, hk, dim, bits):
+    """As many requests as a step takes, of a few tokens each."""
+    rng = random.Random(7)
+    case = Case([rng.randrange(0, 4) for _ in range(2048)], [rng.choice([0, 1, 1]) for _ in range(2048)], hq, hk, dim, page=16,
+                bits=bits, max_rows=1, seed=11)
+    case.check(case.run())
+
+
 def test_rows_that_see_nothing():
     """Masks of zero without a context give zeros, with one the context; bits of rows that are not there see nothing."""
     case = Case([0, 9, 0], [4, 3, 2], 6, 2, 64, tree=True, gated=True, seed=2)
