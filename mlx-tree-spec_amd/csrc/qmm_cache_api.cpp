@@ -190,7 +190,7 @@ int64_t qmm4_paged_workspace(int64_t M, int64_t R, int64_t Hq, int64_t Hk, int64
     if (int bad = check_format(D, 16, nullptr, nullptr)) return bad;
     qmm4::PagedShape s;
     if (int bad = shape_of(Hq, Hk, D, clamp_rows(max_rows), &s)) return bad;
-    bytes = std::max<int64_t>(16, qmm4::paged_partial_rows(s, M, R, clamp_rows(max_rows)) * Hk * (D + 2) * (int64_t)sizeof(float));
+    bytes = std::max<int64_t>(16, qmm4::paged_partial_rows(s, R, clamp_rows(max_rows)) * Hk * (D + 2) * (int64_t)sizeof(float));
     return (int)QMM4_OK;
   });
   return rc ? rc : bytes;
@@ -223,7 +223,7 @@ int qmm4_paged_attention_bf16(const void* q, int64_t q_row, int64_t q_head, cons
     qmm4::PagedShape s;
     if (int rc = shape_of(Hq, Hk, D, most, &s)) return rc;
     float* part = static_cast<float*>(workspace);
-    const int64_t rows = qmm4::paged_partial_rows(s, M, R, most) * Hk;
+    const int64_t rows = qmm4::paged_partial_rows(s, R, most) * Hk;
     const qmm4::PagedParams p{rows_of(q, q_row, q_head), rows_of(gate, gate_row, gate_head),
                               {const_cast<void*>(keys), const_cast<void*>(values), const_cast<float*>(key_scales),
                                const_cast<float*>(value_scales), pages, log2_of(page_size), (int)Hk},

@@ -42,8 +42,8 @@ struct PagedShape {
   int64_t splits;  // pieces of the whole that are aimed at, at most
 };
 PagedShape paged_shape(int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_rows, int cus);
-// Query rows of all partial results, for each key head, at most.
-int64_t paged_partial_rows(const PagedShape& s, int64_t M, int64_t R, int64_t max_rows);
+// Query rows of all partial results (of requests that are cut), for each key head, at most.
+int64_t paged_partial_rows(const PagedShape& s, int64_t R, int64_t max_rows);
 
 struct CacheStepParams {
   int32_t *lengths, *table, *free_pages, *free_count;

@@ -8,6 +8,7 @@
 // 1 KB an instruction in whole runs of 64 bytes and more, without LDS, and takes every 8th step of its workgroup's split; while
 // a step's probabilities are made the next step's keys are on their way, and its values while the products with the present ones
 // run. Waves join through LDS, splits through memory (fp32) and a second kernel (4.7 us for 64 splits).
+#include <algorithm>
 #include <type_traits>
 
 #include "qmm4_lds.h"
@@ -276,9 +277,10 @@ PagedShape paged_shape(int64_t heads, int64_t kv_heads, int64_t head_dim, int64_
   return {G, round, max_rows * G > 16 ? round : (2 * cus + kv_heads - 1) / kv_heads};
 }
 
-int64_t paged_partial_rows(const PagedShape& s, int64_t M, int64_t R, int64_t max_rows) {
-  const int64_t items = s.splits + R, by_block = kPagedRows * items + M * s.G, by_rows = items * max_rows * s.G;
-  return by_block < by_rows ? by_block : by_rows;
+int64_t paged_partial_rows(const PagedShape& s, int64_t R, int64_t max_rows) {
+  // A request of n row blocks and L tokens that is cut has more than `chunk` tokens, so fewer than 2 L / chunk splits; chunk is at
+  // least the sum of all n L over s.splits. So the blocks of all splits of such requests are below 2 s.splits.
+  return std::min<int64_t>(2 * kPagedRows * s.splits, (s.splits + R) * max_rows * s.G);
 }
 
 static hipError_t launch_paged_rows(const PagedParams& p, int D, bool q8, hipStream_t stream) {

@@ -8,7 +8,7 @@ import torch
 
 import cache_refs as R
 from cache_refs import i32
-from mlx_tree_spec_amd import KVCache, paged_attention, step_tables_
+from mlx_tree_spec_amd import KVCache, _lib, paged_attention, step_tables_
 from request_refs import f64
 
 pytestmark = pytest.mark.gpu
@@ -141,6 +141,33 @@ def test_most_requests(hq, hk, dim, bits):
     case = Case([rng.randrange(0, 4) for _ in range(2048)], [rng.choice([0, 1, 1]) for _ in range(2048)], hq, hk, dim, page=16,
                 bits=bits, max_rows=1, seed=11)
     case.check(case.run())
+
+
+@pytest.mark.parametrize("hq,hk,dim", [(6, 1, 256), (24, 4, 256), (32, 8, 128), (16, 16, 64), (40, 2, 64), (129, 1, 64)])
+def test_partial_results_fit_the_workspace(hq, hk, dim):
+    """Plans of all kinds of batches: the partial rows and items that a plan names fit what is set aside for them."""
+    lib, rng, page = _lib.load(), random.Random(hq), 64
+    for _ in range(40):
+        n = rng.choice([1, 2, 3, 17, 300])
+        most = rng.choice([1, 2, 5, 22, 64, 200])
+        rows = [rng.choice([0, 1, most, rng.randrange(most + 1)]) for _ in range(n)]
+        longest = rng.choice([70, 1000, 30000, 1 << 19])
+        cached = [min(longest, (1 << 24) // n) if rng.random() < 0.3 else rng.randrange(longest // 8 + 1) for _ in range(n)]
+        held = [R.ceil(c + k, page) for c, k in zip(cached, rows)]
+        lengths, table = i32([c + k for c, k in zip(cached, rows)]), torch.zeros(n, max(held) + 1, dtype=torch.int32, device=DEV)
+        step = step_tables_(lengths, table, torch.zeros(sum(held) + 1, dtype=torch.int32, device=DEV), i32([0]), i32(rows), sum(rows), page,
+                            hq, hk, dim, base=i32(cached), max_rows=most)
+        words = step.plan.tolist()
+        size = lib.qmm4_paged_workspace(sum(rows), n, hq, hk, dim, step.max_rows)
+        room = size // (4 * (dim + 2) * hq)  # rows of the step, each with all its heads
+        items = 0
+        for r, (c, k) in enumerate(zip(cached, rows)):
+            first, count, length, per, splits, part = words[8 + 8 * r:14 + 8 * r]
+            assert count == k and (k == 0 or (first, length) == (sum(rows[:r]), c + k))
+            items += splits
+            if splits > 1:
+                assert per * (splits - 1) < length <= per * splits and 0 <= part and part + splits * k <= room
+        assert words[0] == items and 8 * (1 + n + items) <= len(words)
 
 
 def test_rows_that_see_nothing():
