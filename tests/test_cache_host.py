@@ -2,11 +2,12 @@
 
 import os
 import re
+import types
 
 import pytest
 import torch
 
-from mlx_tree_spec_amd import CacheStep, CacheTables, KVCache, _lib, paged_attention, step_tables_, store_kv_
+from mlx_tree_spec_amd import CacheStep, CacheTables, KVCache, _lib, cached_attention, paged_attention, step_tables_, store_kv_
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 BF, I32 = torch.bfloat16, torch.int32
@@ -174,6 +175,13 @@ def test_attention_refusals(change, msg):
 def test_attention_of_a_changed_step(change, msg):
     with pytest.raises(ValueError, match=msg):
         paged_attention(z(5, 8, 64), cache(), step()._replace(**change))
+
+
+def test_cached_attention_wants_a_plan():
+    """A step of kept rows is refused before anything is computed or stored."""
+    layer = types.SimpleNamespace(heads=8, kv_heads=2, head_dim=64)
+    with pytest.raises(ValueError, match="no plan"):
+        cached_attention(z(5, 32), layer, cache(), step(plan=False))
 
 
 P = 0x10000
