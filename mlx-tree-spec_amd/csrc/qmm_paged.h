@@ -87,12 +87,14 @@ __device__ __forceinline__ bool paged_empty(const int64_t* ancestors, int64_t ro
   return ((uint64_t)ancestors[row] & (n < 64 ? (1ull << n) - 1 : ~0ull)) == 0;
 }
 
-template <int D, int QT, bool Q8>
+// Q8: a cache of codes with scales. CODES: the products' operands are read as codes (else as bf16 numbers, which codes may have been
+// made before).
+template <int D, int QT, bool Q8, bool CODES = Q8>
 struct PagedRows {
-  static constexpr int E = Q8 ? 16 : 8;  // elements of 16 bytes
+  static constexpr int E = Q8 ? 16 : 8;  // elements of 16 bytes of the cache
   static constexpr int kStep = 32;       // tokens of a wave's step
   static constexpr int kKT = 2;          // tiles of 16 tokens
-  static constexpr int kKC = D / (4 * E);  // 16-byte pieces of a key for each lane
+  static constexpr int kKC = D / (CODES ? 64 : 32);  // 16-byte pieces of a key's operands for each lane
   static constexpr int kQK = D / 32;     // matrix instructions along D
   static constexpr int kVT = D / 16;     // tiles of 16 dimensions
   // LDS of a wave that hands over its results.
@@ -150,7 +152,7 @@ struct PagedRows {
       }
 #pragma unroll
       for (int c = 0; c < kQK; ++c) {
-        const int d = Q8 ? (c / 2) * 64 + g * 16 + (c & 1) * 8 : c * 32 + g * 8;
+        const int d = CODES ? (c / 2) * 64 + g * 16 + (c & 1) * 8 : c * 32 + g * 8;
         u32x4 v = {0u, 0u, 0u, 0u};
         if (x) v = *reinterpret_cast<const u32x4*>(x + d);
         q[qt][c] = as_bf16x8(v);
@@ -246,10 +248,13 @@ struct PagedRows {
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float x = e[qt][j] * vscale[j / 4][j % 4];
-          e[qt][j] = masked && !sees(qt, t + 8 * g + j) ? 0.0f : x;
-        }
+        for (int j = 0; j < 8; ++j) e[qt][j] *= vscale[j / 4][j % 4];
+      if (masked) {  // (what is not there may have a scale that is not a number)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[qt][j] = sees(qt, t + 8 * g + j) ? e[qt][j] : 0.0f;
+      }
     }
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {

@@ -10,6 +10,9 @@
 // them: a fragment is then 256 neighbouring bytes for 16 lanes, without bank conflicts. One barrier a stage, in front of the
 // softmax, behind an exact count of the loads that may still be on their way: the softmax covers the reads of its own values and of the
 // next step's keys (1000 rows 181 -> 174 us, 4 x 16 nodes of 6 heads of 256 28.4 -> 26.6).
+// 8 bits: the waves together make a stage's codes bf16 numbers, in LDS, one stage ahead and behind the products of keys; each wave
+// for itself would make them all again (1000 rows over 8000 tokens, 8 heads of 128: 308 -> 208 us, 4 of 256 over 4000: 426 -> 232; 4 x 16
+// nodes of 6 heads of 256 over 8000: 28.6 -> 20.2).
 // (Half of the waves half a stage late, so that a SIMD's two would multiply and exponentiate in turn, measured the same; so did
 // priorities, 4 waves to a workgroup and two of those to a CU, and the values' products among the next step's exponentials: with
 // heads of 256 those took more registers than there are.)
@@ -29,7 +32,7 @@ constexpr int kIds = 1024;  // page numbers held in LDS at once
 
 template <int D, int QT, int SIDES, bool Q8>
 struct TileTraits {
-  using R = PagedRows<D, QT, Q8>;
+  using R = PagedRows<D, QT, Q8, false>;
   static constexpr int kAcross = kWaves / SIDES;          // waves side by side along the rows
   static constexpr int kRows = kAcross * 16 * QT;
   static constexpr int kStage = SIDES * R::kStep;         // tokens
@@ -41,9 +44,9 @@ struct TileTraits {
   // A stage that is multiplied, whose values are read while the next one's keys are, and two on their way.
   static constexpr int kStages = 4;
   // A step's keys are read while the softmax before it runs, or where registers are short piece by piece in place of values.
-  static constexpr bool kEarly = R::kKC * R::kKT <= 8;
-  static_assert(kEarly || SIDES == 1, "every wave has a step of each stage");
-  static constexpr size_t kRing = (size_t)kStages * kStageBytes;
+  static constexpr bool kEarly = R::kKC * R::kKT <= 8 && !(Q8 && QT * D >= 256);
+  static constexpr int kBf16 = D * kStage * 2 / 8;  // pieces of a stage as bf16 numbers
+  static constexpr size_t kRing = (size_t)kStages * kStageBytes + (Q8 ? 2 * kBf16 * 16 : 0);
   static constexpr size_t kJoin = SIDES > 1 ? (size_t)kAcross * R::kHandBytes : 0;
   static constexpr size_t kLds = (kRing > kJoin ? kRing : kJoin) + kIds * 4 + 16;
   static_assert(kLds <= 160 * 1024, "LDS");
@@ -68,7 +71,7 @@ __device__ __forceinline__ void bare_barrier() {
 template <int D, int QT, int SIDES, bool Q8, bool WIDE>
 __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int block0, int blocks) {
   using T = TileTraits<D, QT, SIDES, Q8>;
-  using R = PagedRows<D, QT, Q8>;
+  using R = PagedRows<D, QT, Q8, false>;
   constexpr int E = R::E;
   typedef __attribute__((address_space(1))) const void* global_ptr;
   typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -101,9 +104,8 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   const char* values = static_cast<const char*>(S.cache.values);
 
   // A step from a stage in LDS: its products with the queries ..
-  using Piece = std::conditional_t<Q8, u32x2, u32x4>;  // 8 tokens of a dimension
   f32x4 s[QT][R::kKT];
-  Piece vf[R::kVT];
+  u32x4 vf[R::kVT];  // 8 tokens of a dimension each
   f32x4 ks[Q8 ? R::kKT : 1], vs[Q8 ? R::kKT : 1];
   const auto multiply = [&](const u32x4 (&kf)[R::kKC][R::kKT]) __attribute__((always_inline)) {
 #pragma unroll
@@ -114,20 +116,9 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
     for (int c = 0; c < R::kKC; ++c) {
 #pragma unroll
       for (int tt = 0; tt < R::kKT; ++tt) {
-        const u32x4 k = kf[c][tt];
-        if constexpr (Q8) {
-          const bf16x8 lo = codes8(k[0], k[1]), hi = codes8(k[2], k[3]);
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt) {
-            s[qt][tt] = paged_mma(lo, W.q[qt][2 * c], s[qt][tt]);
-            s[qt][tt] = paged_mma(hi, W.q[qt][2 * c + 1], s[qt][tt]);
-          }
-        } else {
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) s[qt][tt] = paged_mma(as_bf16x8(k), W.q[qt][c], s[qt][tt]);
-        }
+        for (int qt = 0; qt < QT; ++qt) s[qt][tt] = paged_mma(as_bf16x8(kf[c][tt]), W.q[qt][c], s[qt][tt]);
       }
-      if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);  // (few codes at a time in registers)
     }
   };
   // .. and what they add to the rows.
@@ -136,13 +127,9 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
     W.softmax(t, s, ks, vs, p);
 #pragma unroll
     for (int dt = 0; dt < R::kVT; ++dt) {
-      bf16x8 v;
-      if constexpr (Q8) v = codes8(vf[dt][0], vf[dt][1]);
-      else v = as_bf16x8(vf[dt]);
 #pragma unroll
-      for (int qt = 0; qt < QT; ++qt) W.o[qt][dt] = paged_mma(v, p[qt], W.o[qt][dt]);
+      for (int qt = 0; qt < QT; ++qt) W.o[qt][dt] = paged_mma(as_bf16x8(vf[dt]), p[qt], W.o[qt][dt]);
       between(dt);
-      if (Q8 && dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   };
 
@@ -223,30 +210,55 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
       }
     };
 
-    const auto ring_of = [&](int st) { return reinterpret_cast<const u32x4*>(s_ring + (st % T::kStages) * T::kStageBytes); };
+    const auto ring_of = [&](int st) { return reinterpret_cast<u32x4*>(s_ring + (st % T::kStages) * T::kStageBytes); };
+    // Its keys and values as bf16 numbers.
+    const auto stage_of = [&](int st) {
+      if constexpr (Q8) return reinterpret_cast<u32x4*>(s_ring + T::kStages * T::kStageBytes) + (st & 1) * T::kBf16;
+      else return ring_of(st);
+    };
+    // (Splits begin and end at whole stages, but for the last token that is seen: past that a step has no effect.)
     const auto token_of = [&](int st) { return from + st * T::kStage + side * R::kStep; };
     // The values of a stage past the context made clean in place, by all waves (once: a branch around products of clean and other
     // values would have every sum in registers twice).
     const auto clean = [&](int st) {
-      u32x4* values = reinterpret_cast<u32x4*>(s_ring + (st % T::kStages) * T::kStageBytes) + T::kPieces / 2;
+      u32x4* values = ring_of(st) + T::kPieces / 2;
       for (int f = threadIdx.x; f < T::kPieces / 2; f += kThreads) {
         bool odd = false;
         values[f] = clean_values(values[f], from + st * T::kStage + f / D * 8 - W.length, &odd);
         if (odd) *s_odd = 1;
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      bare_barrier();
     };
-    // Stage `st` is in the ring for every wave, where those up to st + 1 are loaded or on their way.
+    // 8 bits: a stage's codes as bf16 numbers, by all waves (once, and not by each wave that multiplies them).
+    const auto convert = [&](int st) __attribute__((always_inline)) {
+      const u32x4* from_codes = ring_of(st);
+      u32x4* to_bf16 = stage_of(st);
+#pragma unroll
+      for (int f0 = 0; f0 < T::kPieces; f0 += kThreads) {
+        const int f = f0 + threadIdx.x;
+        if (T::kPieces % kThreads != 0 && f >= T::kPieces) break;
+        // (16 dimensions of a token, or 16 tokens of a dimension: two pieces, a row of tokens or of dimensions apart.)
+        const int v = f - T::kPieces / 2, row = v < 0 ? T::kStage : D, at = v < 0 ? f / T::kStage : v / D, i = v < 0 ? f % T::kStage : v % D;
+        u32x4* to = to_bf16 + (v < 0 ? 0 : T::kBf16 / 2) + 2 * at * row + i;
+        const u32x4 x = from_codes[f];
+        to[0] = __builtin_bit_cast(u32x4, codes8(x[0], x[1]));
+        to[row] = __builtin_bit_cast(u32x4, codes8(x[2], x[3]));
+      }
+    };
+    // Behind it stage `st` can be read by every wave (8 bits: and the codes of the next be converted), where all up to kOnWay behind
+    // `st` are loaded or on their way.
+    constexpr int kOnWay = Q8 ? 2 : 1;
     const auto arrive = [&](int st) __attribute__((always_inline)) {
-      if (st + 1 < stages) wait_loads<T::kLoads>();
+      if (st + kOnWay < stages) wait_loads<T::kLoads>();
       else wait_loads<0>();
       bare_barrier();
-      if (!Q8 && from + (st + 1) * T::kStage > W.context) clean(st);
+      if (Q8 || from + (st + 1) * T::kStage <= W.context) return;
+      clean(st);
+      wait_reads();
+      bare_barrier();
     };
     u32x4 kf[R::kKC][R::kKT];
     const auto read_key = [&](int st, int c, int tt) __attribute__((always_inline)) {
-      kf[c][tt] = (ring_of(st) + W.g * T::kStage + side * R::kStep + W.r16)[c * 4 * T::kStage + tt * 16];
+      kf[c][tt] = (stage_of(st) + W.g * T::kStage + side * R::kStep + W.r16)[c * 4 * T::kStage + tt * 16];
     };
     const auto read_keys = [&](int st) __attribute__((always_inline)) {
 #pragma unroll
@@ -254,18 +266,29 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
 #pragma unroll
         for (int tt = 0; tt < R::kKT; ++tt) read_key(st, c, tt);
     };
-    // The next stage, and one behind those on their way into the place of the one before `st`.
+    // The next stage, and one behind those on their way into the place of one that is done.
     const auto advance = [&](int st, auto&& then) __attribute__((always_inline)) {
       if (st + 1 >= stages) return;
+      if constexpr (Q8) {
+        convert(st + 1);
+        wait_reads();
+      }
       arrive(st + 1);
       then();
-      if (st + 3 < stages) load(st + 3);
+      if (st + 2 + kOnWay < stages) load(st + 2 + kOnWay);
     };
-    load(0);
-    if (1 < stages) load(1);
+    for (int st = 0; st < 1 + kOnWay && st < stages; ++st) load(st);
+    if constexpr (Q8) {
+      if (stages > 2) wait_loads<2 * T::kLoads>();
+      else if (stages > 1) wait_loads<T::kLoads>();
+      else wait_loads<0>();
+      bare_barrier();
+      convert(0);
+      wait_reads();
+    }
     arrive(0);
     if (active) read_keys(0);
-    if (2 < stages) load(2);
+    if (1 + kOnWay < stages) load(1 + kOnWay);
     if (!active) {
 #pragma unroll 1
       for (int st = 0; st < stages; ++st) advance(st, [] {});
@@ -276,14 +299,11 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
         wait_reads();
         multiply(kf);
         __builtin_amdgcn_sched_barrier(0);
-        const u32x4* ring = ring_of(st);
-        // (8 bits: two groups of 8 tokens share a piece.)
-        const Piece* vr = reinterpret_cast<const Piece*>(ring + T::kPieces / 2 + (Q8 ? side * 2 + (W.g >> 1) : side * 4 + W.g) * D + W.r16) +
-                          (Q8 ? W.g & 1 : 0);
+        const u32x4* vr = stage_of(st) + T::kBf16 / 2 + (side * 4 + W.g) * D + W.r16;
 #pragma unroll
-        for (int dt = 0; dt < R::kVT; ++dt) vf[dt] = vr[dt * (Q8 ? 32 : 16)];
+        for (int dt = 0; dt < R::kVT; ++dt) vf[dt] = vr[dt * 16];
         if constexpr (Q8) {
-          const f32x4* scales = reinterpret_cast<const f32x4*>(ring + T::kPieces) + side * 8 + W.g * 2;
+          const f32x4* scales = reinterpret_cast<const f32x4*>(ring_of(st) + T::kPieces) + side * 8 + W.g * 2;
 #pragma unroll
           for (int tt = 0; tt < R::kKT; ++tt) {
             ks[tt] = scales[tt];
@@ -295,7 +315,7 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
           if constexpr (T::kEarly) read_keys(next);
         });
         if constexpr (T::kEarly) {
-          if (SIDES == 1 || token_of(st) < to) finish(token_of(st), [](int) {});
+          finish(token_of(st), [](int) {});
         } else {
           constexpr int kEach = R::kKC * R::kKT / R::kVT;
           static_assert(kEach * R::kVT == R::kKC * R::kKT, "keys in place of values");
