@@ -298,8 +298,8 @@ hipError_t launch_paged_attention(const PagedParams& p, int64_t M, int D, bool q
   if (p.plan.R > 0 && rows > 0) {
     // bf16 heads of 192 and more take the tile kernel from the first row on: their step is more than 8 waves' registers hold, while one
     // wave that multiplies keeps up with the loads of 8 into LDS (one request of 2000 tokens, 6 heads of 256 to a key head: 6.3 us, 7.6
-    // with waves of their own; 16 of up to 8000: 63, 65). Smaller heads do not (64 of up to 16000, 4 of 128: 433 us, 428; one of
-    // 2000 7.0, 5.9), and codes have to be converted by all waves (16 of up to 40000, 6 of 256: 357, 133).
+    // with waves of their own; 16 of up to 8000: 63, 65). Smaller heads and codes are fewer bytes beside as much work for that wave
+    // (64 of up to 16000, 4 of 128: 434 us, 428; 16 of up to 8000, one of 64: 60, 56; 8 bits, 16 of up to 40000, 6 of 256: 210, 140).
     const bool tile = rows > 16 || (D > 128 && !q8);
     const hipError_t e = tile ? launch_paged_tile(p, D, q8, stream) : launch_paged_rows(p, D, q8, stream);
     if (e != hipSuccess) return e;
