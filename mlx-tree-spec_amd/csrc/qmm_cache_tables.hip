@@ -235,10 +235,13 @@ __global__ __launch_bounds__(THREADS) void cache_step_kernel(CacheStepParams S) 
 
   if (S.plan.words) {
     // The attention's splits: as many tokens each as leave S.splits in all (a request of several row blocks counts as often). Every
-    // request ends in a split that is not full; where they are few beside one round, one round less their number is aimed at
-    // (one workgroup more than the GPU holds at once takes as long again).
+    // request ends in a split that is not full; up to half a round of row blocks, less than their number beside what fills one round
+    // is aimed at (one workgroup more than the GPU holds at once takes as long again). More blocks, where one round is aimed at: as
+    // many splits as blocks, since twice as many would be two rounds (a prompt of one request is not cut, and has no partial sums).
     const int64_t all = total4[1] + (total4[2] << 22) + (total4[3] << 44);
-    const int64_t aim = S.round > 2 * total4[0] ? S.round - total4[0] : S.splits;
+    const int64_t aim = S.round >= 2 * total4[0]   ? S.round - total4[0] + 1
+                        : S.splits > S.round ? S.splits
+                                             : min(S.splits, total4[0]);
     const int64_t chunk = max((int64_t)kPagedUnit, ((all + aim - 1) / aim + kPagedUnit - 1) / kPagedUnit * kPagedUnit);
     // A request's record up to its partial rows. (Without keep every row of a request that is not refused has a place.)
     const auto record = [&](int r) {

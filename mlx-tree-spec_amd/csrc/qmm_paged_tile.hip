@@ -78,10 +78,24 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   extern __shared__ __attribute__((aligned(16))) char s_ring[];
   int* s_ids = reinterpret_cast<int*>(s_ring + T::kLds - kIds * 4 - 16);
   int* s_odd = s_ids + kIds;  // a value that is not finite was left out
-  // The row blocks of one split and key head follow each other on one XCD (workgroups go round the 8 of them): the later
+  // The row blocks of one split and key head (a unit) follow each other on one XCD (workgroups go round the 8 of them): the later
   // ones find the cache's bytes in its L2.
-  const int unit = blockIdx.x / (8 * blocks) * 8 + (blockIdx.x & 7), block = block0 + blockIdx.x / 8 % blocks;
-  const int item = unit / S.cache.heads;
+  int unit = blockIdx.x / (8 * blocks) * 8 + (blockIdx.x & 7), in_unit = blockIdx.x / 8 % blocks;
+  if (blocks > 2) {
+    // Prompts: most of the grid, made for as many splits as there may be, ends here, before anything else. Units that are few and not
+    // a multiple of 8 are shared out, so that every XCD has as many blocks (1000 rows, 47 blocks of one request, over 4 key heads of 256:
+    // 182 us, 343 on 4 XCDs).
+    const int units = S.plan.words[0] * S.cache.heads;
+    if (blockIdx.x >= (uint32_t)((units + 7) / 8 * 8) * (blocks + 7)) return;
+    if (units < 64 && units % 8 != 0) {
+      const int share = min(blocks, units % 4 == 0 ? 2 : units % 2 == 0 ? 4 : 8), each = (blocks + share - 1) / share;
+      const int place = blockIdx.x / (8 * each) * 8 + (blockIdx.x & 7);
+      unit = place / share;
+      in_unit = place % share * each + blockIdx.x / 8 % each;
+      if (in_unit >= blocks) return;
+    }
+  }
+  const int item = unit / S.cache.heads, block = block0 + in_unit;
   const PagedItem I = S.plan.items()[item < S.items ? item : 0];
   if (item >= S.plan.words[0]) return;
   R W(S, I, unit - item * S.cache.heads);
@@ -348,7 +362,8 @@ hipError_t launch_pages(const PagedParams& p, hipStream_t stream) {
   using T = TileTraits<D, QT, SIDES, Q8>;
   static LdsAllowance allowance;
   if (hipError_t e = allowance.allow(reinterpret_cast<const void*>(&paged_tile_kernel<D, QT, SIDES, Q8, WIDE>), T::kLds)) return e;
-  const int64_t units = ((int64_t)p.items * p.cache.heads + 7) / 8 * 8, blocks = ((int64_t)p.max_rows * p.G + T::kRows - 1) / T::kRows;
+  // (At least 128: units that are shared out, fewer than 64, take up to twice as many places.)
+  const int64_t units = std::max<int64_t>(128, ((int64_t)p.items * p.cache.heads + 7) / 8 * 8), blocks = ((int64_t)p.max_rows * p.G + T::kRows - 1) / T::kRows;
   const int64_t most = std::max<int64_t>(1, (int64_t{1} << 22) / units);  // (a grid may have 2^32 threads)
   for (int64_t b0 = 0; b0 < blocks; b0 += most) {
     const int64_t count = std::min(most, blocks - b0);

@@ -134,6 +134,15 @@ def test_rows_of_a_prompt():
     case.check(case.run())
 
 
+@pytest.mark.parametrize("hq,hk,dim,bits", [(4, 1, 64, 16), (4, 2, 128, 16), (12, 4, 256, 16), (9, 3, 64, 8), (5, 5, 96, 16),
+                                            (4, 1, 256, 8)])
+@pytest.mark.parametrize("cached,rows", [([0], [230]), ([70, 5, 0], [100, 1, 150])])
+def test_row_blocks_of_few_heads(cached, rows, hq, hk, dim, bits):
+    """Several row blocks of so few requests and heads that each is shared out."""
+    case = Case(cached, rows, hq, hk, dim, bits=bits, gated=True, pad=1, seed=hk)
+    case.check(case.run())
+
+
 @pytest.mark.parametrize("hq,hk,dim,bits", [(8, 2, 64, 16), (4, 2, 256, 16), (8, 2, 128, 8)])
 def test_most_requests(hq, hk, dim, bits):
     """As many requests as a step takes, of a few tokens each."""
