@@ -363,7 +363,8 @@ hipError_t launch_pages(const PagedParams& p, hipStream_t stream) {
   static LdsAllowance allowance;
   if (hipError_t e = allowance.allow(reinterpret_cast<const void*>(&paged_tile_kernel<D, QT, SIDES, Q8, WIDE>), T::kLds)) return e;
   // (At least 128: units that are shared out, fewer than 64, take up to twice as many places.)
-  const int64_t units = std::max<int64_t>(128, ((int64_t)p.items * p.cache.heads + 7) / 8 * 8), blocks = ((int64_t)p.max_rows * p.G + T::kRows - 1) / T::kRows;
+  const int64_t units = std::max<int64_t>(128, ((int64_t)p.items * p.cache.heads + 7) / 8 * 8);
+  const int64_t blocks = ((int64_t)p.max_rows * p.G + T::kRows - 1) / T::kRows;
   const int64_t most = std::max<int64_t>(1, (int64_t{1} << 22) / units);  // (a grid may have 2^32 threads)
   for (int64_t b0 = 0; b0 < blocks; b0 += most) {
     const int64_t count = std::min(most, blocks - b0);

@@ -119,9 +119,10 @@ def step_tables_(lengths: torch.Tensor, block_table: torch.Tensor, free_pages: t
     a tree verify stores all nodes, and then, with base the length before and `keep` the accepted nodes, these alone.
 
     lengths, rows, base int32 [R]; block_table int32 [R, capacity]; free_pages int32 [pages] (room for every page of the
-    cache), the first free_count (int32 [1]) of which are free. Rows without a place (not kept, refused, padding) have -1 as slot, position and request. heads,
-    kv_heads, head_dim: those of the layers whose attention takes this step. Up to 2048 requests, 2^22 rows (2^16 with keep), 2^22 pages per request
-    and 2^30 tokens.
+    cache), the first free_count (int32 [1]) of which are free. Rows without a place (not kept, refused, padding) have -1 as
+    slot, position and request. heads, kv_heads, head_dim: those of the layers whose attention takes this step. max_rows
+    (total by default): the fewer, the better the attention's kernels fit (1 for a decode step). Up to 2048 requests, 2^22
+    rows (2^16 with keep), 2^22 pages per request and 2^30 tokens.
     """
     what = "step_tables_"
     max_rows = total if max_rows is None else min(max_rows, total)

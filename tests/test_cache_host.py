@@ -196,7 +196,9 @@ def c_step(**kw):
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(page=17), "page_size=17"), (dict(page=0), "page_size=0"), (dict(pages=-1), "-1 pages"),
-    (dict(capacity=1 << 40), "up to 2^30"), (dict(capacity=(1 << 22) + 1), "up to 2^22"), (dict(keep=P, total=65537), "65537 rows with keep"), (dict(pages=(1 << 26) + 1), "up to 2^30"), (dict(heads=9), "9 query heads"),
+    (dict(capacity=1 << 40), "up to 2^30"), (dict(capacity=(1 << 22) + 1), "up to 2^22"),
+    (dict(keep=P, total=65537), "65537 rows with keep"),
+    (dict(pages=(1 << 26) + 1), "up to 2^30"), (dict(heads=9), "9 query heads"),
     (dict(R=2049), "2049 requests"), (dict(total=-2), "-2 rows"), (dict(max_rows=-1), "at most -1"), (dict(lengths=None), "null"),
     (dict(table=None), "null"), (dict(count=None), "null"), (dict(free=None), "null"), (dict(slots=None), "null"),
     (dict(rows=P + 2), "aligned"), (dict(plan=P + 1), "aligned")])
