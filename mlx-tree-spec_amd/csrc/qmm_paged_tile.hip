@@ -58,7 +58,7 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// Waits for the wave's reads out of LDS.
+// Waits for the wave's reads out of LDS and its writes to it.
 __device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 __device__ __forceinline__ void bare_barrier() {
@@ -106,7 +106,9 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
   const bool active = mine < rows;
   W.load_rows(mine);
 
-  if (threadIdx.x == 0) *s_odd = 0;  // (read and written behind the barrier of a stage at least)
+  // (Waited for here: the barriers in front of a stage's reads are bare, and the first stage may set it.)
+  if (threadIdx.x == 0) *s_odd = 0;
+  wait_reads();
   const int begin = I.begin;
   int end = I.end;
   // (Without ancestors nothing past the block's last row is seen.)

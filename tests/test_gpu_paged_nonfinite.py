@@ -1,0 +1,67 @@
+"""Infinities and NaN in the paged cache (needs an MI355X): each row has what the formula gives of the tokens that it sees, in 64
+bits: NaN and infinities of the same sign where that has them, and finite values within the attention's bound elsewhere."""
+
+import numpy as np
+import pytest
+import torch
+
+import cache_refs as R
+from request_refs import f64
+from test_gpu_paged import Case
+
+pytestmark = pytest.mark.gpu
+KINDS = (float("nan"), float("inf"), -float("inf"))
+
+
+def put(case, request, token, which, head, d, x):
+    """x as dimension d of a token's key or value."""
+    page = case.step.page_size
+    p, o = int(case.table[request, token // page]), token % page
+    if which == "keys":
+        case.cache.keys[p, head, d // 8, o, d % 8] = x
+    else:
+        case.cache.values[p, head, o // 8, d, o % 8] = x
+
+
+def poison_values(case, request, tokens):
+    """A dimension of its own that is not finite in the value of each of the tokens, in the last key head."""
+    head, dim = case.cache.keys.shape[1] - 1, case.q.shape[2]
+    assert len(set(tokens)) == len(tokens) < dim
+    for i, t in enumerate(tokens):
+        put(case, request, t, "values", head, i * 5 % dim, KINDS[i % 3])
+
+
+def check(case, out):
+    k, v = R.token_rows(case.cache)
+    q, got, page, row = f64(case.q), f64(out), case.step.page_size, 0
+    for r, (c, n) in enumerate(zip(case.cached, case.rows)):
+        if n == 0:
+            continue
+        t = np.arange(c + n)
+        at = case.table[r, t // page].astype(np.int64) * page + t % page
+        masks = None if case.ancestors is None else case.ancestors[row:row + n].tolist()
+        with np.errstate(all="ignore"):
+            want, mag, delta = R.attention(q[row:row + n], k[at], v[at], case.scale, R.visible(c, n, masks))
+            if case.gate is not None:
+                s = 1 / (1 + np.exp(-f64(case.gate[row:row + n])))
+                want, mag = want * s, mag * s
+            bound = R.attention_bound(want, mag, delta, c + n)
+            here = got[row:row + n]
+            assert np.array_equal(np.isnan(here), np.isnan(want)), (r, c, n)
+            inf = np.isinf(want)
+            assert np.array_equal(np.isinf(here), inf) and (here[inf] == want[inf]).all(), (r, c, n)
+            finite = np.isfinite(want)
+            assert (np.abs(here - want)[finite] <= bound[finite]).all(), (r, c, n)
+        row += n
+    assert not got[row:].any()
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("rows", [20, 40])
+def test_values_of_the_first_stage(rows, dim, tree):
+    """Requests of one stage and no context: what is not finite in it is known from the first barrier on."""
+    case = Case([0, 0], [rows, 7], 6, 2, dim, tree=tree, gated=tree, seed=dim + rows)
+    poison_values(case, 0, [0, 5, 13, rows - 1])
+    poison_values(case, 1, [1, 6])
+    check(case, case.run())
