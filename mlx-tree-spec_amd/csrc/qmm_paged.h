@@ -265,13 +265,14 @@ struct PagedRows {
     }
   }
 
-  // What those values add to o for the rows that see them: the wave's steps t, t + stride, .. again, token by token.
-  __device__ __forceinline__ void add_odd_values(int t, int end, int stride, int row0) {
+  // What those values add to o for the rows that see them: the wave's steps t, t + stride, .. again, token by token, where what
+  // was made clean, `reach` tokens from the step's first on, ends past the context.
+  __device__ __forceinline__ void add_odd_values(int t, int end, int stride, int reach, int row0) {
     if (Q8 || !__any(odd)) return;
     odd = false;
     const int shift = S.cache.page_shift;
     for (; t < end; t += stride) {
-      if (t + kStep <= context) continue;
+      if (t + reach <= context) continue;
       for (int tok = t; tok < min(t + kStep, length); ++tok) {
         const int64_t head = (int64_t)valid_page(table[tok >> shift]) * S.cache.heads + h;
         const int off = tok & ((1 << shift) - 1);

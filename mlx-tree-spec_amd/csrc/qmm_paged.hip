@@ -152,7 +152,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void paged_rows_kernel(PagedParams
   PagedWave<D, Q8> W(S, I, blockIdx.x - item * S.cache.heads);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = I.begin + wave * R::kStep, stride = kRowsWaves * R::kStep;
   W.run(t, I.end, stride);
-  W.add_odd_values(t, I.end, stride, 0);
+  W.add_odd_values(t, I.end, stride, R::kStep, 0);
   W.sum_lanes();
   // The upper half of the waves hands over to the lower (where it has anything).
   const int steps = (I.end - I.begin + R::kStep - 1) / R::kStep;

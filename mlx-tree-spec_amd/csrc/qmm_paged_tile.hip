@@ -346,7 +346,8 @@ __global__ __launch_bounds__(kThreads) void paged_tile_kernel(PagedParams S, int
     // (Every load has been waited for: the ring is free behind the next barrier.)
     __syncthreads();
     W.odd = *s_odd != 0;
-    if (active) W.add_odd_values(from + side * R::kStep, to, SIDES * R::kStep, mine);
+    // (A whole stage was made clean, both sides' steps of it.)
+    if (active) W.add_odd_values(from + side * R::kStep, to, T::kStage, T::kStage - side * R::kStep, mine);
   }
 
   W.sum_lanes();

@@ -65,3 +65,59 @@ def test_values_of_the_first_stage(rows, dim, tree):
     poison_values(case, 0, [0, 5, 13, rows - 1])
     poison_values(case, 1, [1, 6])
     check(case, case.run())
+
+
+CONTEXTS = [40, 10, 31, 100, 63, 64, 700, 5030]
+# Query rows of a key head: up to 16 (one wave's), up to 64 and more (trees; 16 and 32 rows to a wave of the narrower heads).
+FORMS = [(1, 3), (5, 3), (20, 3), (40, 3), (64, 1)]
+
+
+def interesting(c, n):
+    """Tokens in and in front of the stage that the context ends in, in both of its halves, and among the step's."""
+    stage = c // 64 * 64
+    return sorted({t for t in (0, 3, stage - 33, stage - 1, stage, stage + 10, stage + 31, stage + 32, c - 1, c, c + 1, c + n // 2,
+                               c + n - 1) if 0 <= t < c + n})
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("rows,group", FORMS)
+def test_values(rows, group, dim, page, tree):
+    """Cached tokens' values and the step's own, in every kernel's form, in requests of one split and of many."""
+    case = Case(CONTEXTS, [rows] * len(CONTEXTS), 2 * group, 2, dim, page=page, tree=tree, gated=tree, seed=dim + rows, max_rows=rows)
+    for r, c in enumerate(CONTEXTS):
+        poison_values(case, r, interesting(c, rows))
+    check(case, case.run())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 192])
+@pytest.mark.parametrize("rows,group", FORMS)
+def test_keys(rows, group, dim):
+    """A key that is not finite in each request, at another place."""
+    case = Case(CONTEXTS, [rows] * len(CONTEXTS), 2 * group, 2, dim, tree=True, seed=dim + rows, max_rows=rows)
+    for r, c in enumerate(CONTEXTS):
+        tokens = interesting(c, rows)
+        put(case, r, tokens[-1 - r % len(tokens)], "keys", r % 2, r * 7, KINDS[r % 3])
+    check(case, case.run())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows,group", FORMS)
+def test_scales_of_8_bits(rows, group, dim):
+    """A token of each request whose scale is NaN, as a head that was not finite is stored: of its keys, or of its values."""
+    case = Case(CONTEXTS, [rows] * len(CONTEXTS), 2 * group, 2, dim, bits=8, tree=True, gated=True, seed=dim + rows, max_rows=rows)
+    for r, c in enumerate(CONTEXTS):
+        tokens = interesting(c, rows)
+        for h, (scales, t) in enumerate(((case.cache.key_scales, tokens[-1 - r % len(tokens)]), (case.cache.value_scales, tokens[r % len(tokens)]))):
+            scales[int(case.table[r, t // 64]), h, t % 64] = float("nan")
+    check(case, case.run())
+
+
+def test_cut_and_whole_requests_agree_about_every_context():
+    """Contexts of all lengths modulo a stage, each with an infinite value in the stage it ends in."""
+    cached = list(range(64, 128))
+    case = Case(cached, [7] * 64, 6, 2, 64, tree=True, seed=3, max_rows=7)
+    for r, c in enumerate(cached):
+        poison_values(case, r, [64 + r // 2, 63] if r else [63])
+    check(case, case.run())
