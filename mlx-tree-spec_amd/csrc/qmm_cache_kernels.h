@@ -8,6 +8,8 @@ namespace qmm4 {
 
 // Query rows (rows of the step x query heads of a key head) of one workgroup of the attention.
 constexpr int kPagedRows = 128;
+// How far (in powers of two) a logit may pass the largest one before it without moving the running maximum.
+constexpr int kPagedSlack = 8;
 // Tokens at which a request's cache may be cut into splits.
 constexpr int kPagedUnit = 64;
 
@@ -78,9 +80,10 @@ struct PagedParams {
   CachePlan plan;
   const int64_t* ancestors;
   uint16_t* out;
-  float *part, *part_ml;  // partial sums [rows, Hq, D]; their largest logit and sum of exponentials [rows, Hq, 2]
+  float *part, *part_ml;  // partial sums [rows, Hq, D]; their running maximum and sum of exponentials [rows, Hq, 2]
   int64_t capacity;
   float scale;
+  float above, enough;  // the running maximum's place above the largest logit; an argument past which it moves
   int G, max_rows;
   int items;  // records of items in the plan
 };

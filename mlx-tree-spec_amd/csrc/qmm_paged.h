@@ -8,8 +8,11 @@
 // tokens within a step of 32 is chosen (row 4 g + i of tile tt is token 8 g + 4 tt + i, g = lane / 16) so that they are the
 // second operand of O^T without a move between lanes.
 //
-// The running maximum moves only where a logit passes it by more than 2^8: probabilities up to 256 lose nothing in fp32, and
-// most steps need no exchange between lanes.
+// The running maximum moves only where a logit passes it by more than 2^8, so that most steps need no exchange between lanes. It
+// is held above the largest logit by those 2^8 and by the tokens that a request may have: all its probabilities together stay
+// below 1, and no sum of finite values overflows, whatever their size, nor does a probability times a scale of 8 bits. What this takes
+// is as many powers of two of how small a probability may be (2^-126). (Both bounds come with the call: the widest kernels have no
+// vector register for them.)
 #pragma once
 
 #include "qmm4_common.h"
@@ -18,8 +21,6 @@
 namespace qmm4 {
 
 constexpr float kLog2e = 1.44269504f;
-// How far (in powers of two) a logit may pass the running maximum.
-constexpr float kSlack = 8.0f;
 // The running maximum before any token is seen: below every finite logit (in powers of two), finite itself, so that no difference
 // of two is NaN.
 constexpr float kNone = -0x1p127f;
@@ -203,7 +204,7 @@ struct PagedRows {
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[qt][tt][i] = sees(qt, t + 8 * g + 4 * tt + i) ? s[qt][tt][i] : -__builtin_inff();
     }
-    // Arguments of the exponentials beside the present maximum, which stays where none passes it by more than kSlack.
+    // Arguments of the exponentials beside the present maximum, which stays where none passes the largest logit by more than kPagedSlack.
     float e[QT][8];
     const auto arguments = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -218,13 +219,13 @@ struct PagedRows {
       top = max3(top, max3(e[qt][0], e[qt][1], e[qt][2]), max3(e[qt][3], e[qt][4], e[qt][5]));
       top = max3(top, e[qt][6], e[qt][7]);
     }
-    if (__any(top > kSlack)) {
+    if (__any(top > S.enough)) {
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
         float now = s[qt][0][0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) now = fmaxf(now, s[qt][j / 4][j % 4]);
-        now *= unit;
+        now = __builtin_fmaf(now, unit, S.above);
         now = fmaxf(now, __shfl_xor(now, 16));
         now = fmaxf(fmaxf(now, __shfl_xor(now, 32)), m[qt]);
         const float f = __builtin_amdgcn_exp2f(m[qt] - now);
