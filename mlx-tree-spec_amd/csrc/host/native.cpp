@@ -24,6 +24,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdint>
 
 #include "qmm4.h"
@@ -534,28 +535,33 @@ PyObject* store_kv(PyObject*, PyObject* const* a, Py_ssize_t na) {
 }
 
 // paged(q, keys, values, key_scales, value_scales, block_table, request, plan, heads, kv_heads, head_dim, max_rows, page_size,
-// scale, ancestors, gate): paged_attention's output.
+// scale, ancestors, gate): paged_attention's output. Without q (None): True where a call with the step's rows would be made.
 PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t na) {
   HANDLE_TH_ERRORS
   if (na != 16 || !PyFloat_CheckExact(a[13])) return none();
-  const at::Tensor *q = strided(a[0], 16), *tab = plain(a[5], 4), *req = plain(a[6], 4), *plan = plain(a[7], 4), *anc;
+  const bool ask = a[0] == Py_None;
+  const at::Tensor *q = ask ? nullptr : strided(a[0], 16), *tab = plain(a[5], 4), *req = plain(a[6], 4), *plan = plain(a[7], 4), *anc;
   const at::Tensor* gate = a[15] == Py_None ? nullptr : strided(a[15], 16);
   Cache c;
   int64_t v[5];  // heads, kv_heads, head_dim, max_rows, page_size
-  if (!q || !tab || !req || !plan || (a[15] != Py_None && !gate) || !c.read(a + 1) || !optional(a[14], 8, &anc) ||
-      !integers(a, 8, v) || !is_bf16(*q) || q->dim() != 3 || tab->dim() != 2)
+  if ((!q && !ask) || !tab || !req || !plan || (a[15] != Py_None && !gate) || !c.read(a + 1) || !optional(a[14], 8, &anc) ||
+      !integers(a, 8, v) || (q && (!is_bf16(*q) || q->dim() != 3)) || tab->dim() != 2 || req->dim() != 1)
     return none();
-  const int64_t m = q->size(0), r = tab->size(0), capacity = tab->size(1);
-  if (q->size(1) != v[0] || q->size(2) != c.dim || v[1] != c.heads || v[2] != c.dim || v[4] != c.page ||
-      !is_table(*tab, at::kInt, {r, capacity}) || !is_table(*req, at::kInt, {m}) || plan->scalar_type() != at::kInt ||
-      (anc && !is_table(*anc, at::kLong, {m})) || (gate && (!is_bf16(*gate) || gate->sizes() != q->sizes())) ||
-      !same_current_device(*q, {tab, req, plan, c.keys, c.values}) || wants_gradient({q, gate}))
+  const int64_t m = req->size(0), r = tab->size(0), capacity = tab->size(1);
+  if (v[1] != c.heads || v[2] != c.dim || v[4] != c.page || !is_table(*tab, at::kInt, {r, capacity}) ||
+      req->scalar_type() != at::kInt || plan->scalar_type() != at::kInt || (anc && !is_table(*anc, at::kLong, {m})) ||
+      !same_current_device(*req, {tab, plan, c.keys, c.values}) || (anc && anc->device() != req->device()))
     return none();
-  for (const at::Tensor* t : {anc, gate})
-    if (t && t->device() != q->device()) return none();
+  if (plan->dim() != 1 || plan->size(0) != p_plan_words(r, v[0], v[1], v[2], v[3])) return none();
+  if (ask) {
+    if (!std::isfinite((float)PyFloat_AS_DOUBLE(a[13])) || (m > 0 && (c.pages == 0 || capacity == 0))) return none();
+    Py_RETURN_TRUE;
+  }
+  if (q->size(0) != m || q->size(1) != v[0] || q->size(2) != c.dim || q->device() != req->device() ||
+      (gate && (!is_bf16(*gate) || gate->sizes() != q->sizes() || gate->device() != q->device())) || wants_gradient({q, gate}))
+    return none();
   int64_t mq, qr, qh, gr = 0, gh = 0;
   if (!heads(*q, &mq, &qr, &qh) || (gate && !heads(*gate, &mq, &gr, &gh))) return none();
-  if (plan->dim() != 1 || plan->size(0) != p_plan_words(r, v[0], v[1], v[2], v[3])) return none();
   const int64_t bytes = p_paged_workspace(m, r, v[0], v[1], v[2], v[3]);
   if (bytes < 0) return PyLong_FromLong((long)bytes);
   at::Tensor out = fresh(q->sizes(), at::kBFloat16, *q), ws = fresh({bytes}, at::kByte, *q);

@@ -15,7 +15,6 @@ device; there is no CPU path, and no gradient.
 
 from __future__ import annotations
 
-import math
 from typing import NamedTuple
 
 import torch
@@ -248,6 +247,51 @@ def store_kv_(k: torch.Tensor, v: torch.Tensor, cache: KVCache, slots: torch.Ten
     _lib.check(rc, what)
 
 
+def _check_step(what: str, cache: KVCache, step: CacheStep, scale: float, ancestors: torch.Tensor | None) -> tuple[int, int]:
+    """(pages, bits) of a cache that a step's rows can attend to."""
+    pages, kv_heads, dim, page_size, bits = _check_cache(what, cache)
+    if (kv_heads, dim, page_size) != (step.kv_heads, step.head_dim, step.page_size):
+        raise ValueError(f"[{what}] a cache of {kv_heads} heads of {dim} in pages of {page_size}, but the step was made for "
+                         f"{step.kv_heads} heads of {step.head_dim} in pages of {step.page_size}")
+    m = step.request.shape[0]
+    if not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"[{what}] scale={scale} must be finite")
+    if ancestors is not None:
+        _table(what, "ancestors", ancestors, (m,), torch.int64)
+    if step.block_table.dim() != 2:
+        raise ValueError(f"[{what}] the step's block_table must have 2 dimensions, got {tuple(step.block_table.shape)}")
+    for name, t, shape in (("block_table", step.block_table, tuple(step.block_table.shape)), ("request", step.request, (m,)),
+                           ("plan", step.plan, tuple(step.plan.shape))):
+        _table(what, f"the step's {name}", t, shape)
+        if not t.is_contiguous():
+            raise ValueError(f"[{what}] the step's {name} must be contiguous")
+    if m > 0 and (pages == 0 or step.block_table.shape[1] == 0):
+        raise ValueError(f"[{what}] a cache without pages has nothing to attend to")
+    return pages, bits
+
+
+def _check_plan(what: str, cache: KVCache, step: CacheStep, *others: torch.Tensor | None) -> torch.device:
+    """The device of all of them, where the step's plan has the size of one for its requests and heads."""
+    dev = _check_device(what, step.block_table, step.request, step.plan, *(t for t in (*cache, *others) if t is not None))
+    with torch.cuda.device(dev):
+        words = _lib.load().qmm4_cache_plan_words(step.block_table.shape[0], step.heads, step.kv_heads, step.head_dim, step.max_rows)
+    _lib.check(min(words, 0), what)
+    _table(what, "the step's plan", step.plan, (words,))
+    return dev
+
+
+def check_attention(what: str, cache: KVCache, step: CacheStep, scale: float | None, ancestors: torch.Tensor | None) -> None:
+    """Raises where paged_attention would, whatever its rows are."""
+    if step.plan is None:
+        raise ValueError(f"[{what}] the step has no plan: it was made with keep")
+    scale = 1.0 if scale is None else scale
+    if cache.keys.is_cuda and _lib.native().paged(None, *cache, step.block_table, step.request, step.plan, step.heads, step.kv_heads,
+                                                  step.head_dim, step.max_rows, step.page_size, float(scale), ancestors, None) is True:
+        return
+    _check_step(what, cache, step, scale, ancestors)
+    _check_plan(what, cache, step, ancestors)
+
+
 def paged_attention(q: torch.Tensor, cache: KVCache, step: CacheStep, scale: float | None = None,
                     ancestors: torch.Tensor | None = None, gate: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of a step's rows over their requests' cached tokens, their own among them (stored before): bf16 (M, Hq, D)
@@ -276,11 +320,8 @@ def paged_attention(q: torch.Tensor, cache: KVCache, step: CacheStep, scale: flo
             return out
     no_gradient(what, q=q, gate=gate, keys=cache.keys, values=cache.values, key_scales=cache.key_scales,
                 value_scales=cache.value_scales)
-    pages, kv_heads, dim, page_size, bits = _check_cache(what, cache)
-    if (kv_heads, dim, page_size) != (step.kv_heads, step.head_dim, step.page_size):
-        raise ValueError(f"[{what}] a cache of {kv_heads} heads of {dim} in pages of {page_size}, but the step was made for "
-                         f"{step.kv_heads} heads of {step.head_dim} in pages of {step.page_size}")
-    m = step.request.shape[0]
+    pages, bits = _check_step(what, cache, step, scale, ancestors)
+    m, r, capacity, kv_heads, dim = step.request.shape[0], *step.block_table.shape, step.kv_heads, step.head_dim
     for name, t in (("q", q), ("gate", gate)):
         if t is None:
             continue
@@ -288,29 +329,12 @@ def paged_attention(q: torch.Tensor, cache: KVCache, step: CacheStep, scale: flo
             raise ValueError(f"[{what}] {name} must be bfloat16, got {t.dtype}")
         if tuple(t.shape) != (m, step.heads, dim):
             raise ValueError(f"[{what}] {name} must be the step's ({m}, {step.heads}, {dim}), got {tuple(t.shape)}")
-    if not math.isfinite(scale):
-        raise ValueError(f"[{what}] scale={scale} must be finite")
-    if ancestors is not None:
-        _table(what, "ancestors", ancestors, (m,), torch.int64)
-    if step.block_table.dim() != 2:
-        raise ValueError(f"[{what}] the step's block_table must have 2 dimensions, got {tuple(step.block_table.shape)}")
-    for name, t, shape in (("block_table", step.block_table, tuple(step.block_table.shape)), ("request", step.request, (m,)),
-                           ("plan", step.plan, tuple(step.plan.shape))):
-        _table(what, f"the step's {name}", t, shape)
-        if not t.is_contiguous():
-            raise ValueError(f"[{what}] the step's {name} must be contiguous")
-    dev = _check_device(what, q, step.block_table, step.request, step.plan, *(t for t in cache if t is not None),
-                        *(t for t in (ancestors, gate) if t is not None))
-    r, capacity = step.block_table.shape
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        words = lib.qmm4_cache_plan_words(r, step.heads, kv_heads, dim, step.max_rows)
-    _lib.check(min(words, 0), what)
-    _table(what, "the step's plan", step.plan, (words,))
+    dev = _check_plan(what, cache, step, ancestors, q, gate)
     q3 = _head_rows(q)
     g3 = None if gate is None else _head_rows(gate)
     ancestors = ancestors if ancestors is None else ancestors.contiguous()
     out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+    lib = _lib.load()
     with torch.cuda.device(dev):
         size = lib.qmm4_paged_workspace(m, r, step.heads, kv_heads, dim, step.max_rows)
         _lib.check(min(size, 0), what)
@@ -319,7 +343,7 @@ def paged_attention(q: torch.Tensor, cache: KVCache, step: CacheStep, scale: flo
                                            _ptr(cache.key_scales), _ptr(cache.value_scales), step.block_table.data_ptr(),
                                            step.request.data_ptr(), step.plan.data_ptr(), _ptr(ancestors), _ptr(g3),
                                            *((0, 0) if g3 is None else _strides(g3)), out.data_ptr(), workspace.data_ptr(),
-                                           float(scale), m, r, step.heads, kv_heads, dim, pages, page_size, capacity,
+                                           float(scale), m, r, step.heads, kv_heads, dim, pages, step.page_size, capacity,
                                            step.max_rows, bits, torch.cuda.current_stream(dev).cuda_stream)
     _lib.check(rc, what)
     return out

@@ -33,7 +33,7 @@ from __future__ import annotations
 
 import torch
 
-from .cache import CacheStep, KVCache, paged_attention, store_kv_
+from .cache import CacheStep, KVCache, check_attention, paged_attention, store_kv_
 from .fused_ops import _norm_eps, add_rms_norm, add_rms_norm_gate_up
 from .heads import qk_norm_rope
 from .lora import LoRALinear
@@ -126,8 +126,7 @@ def cached_attention(x: torch.Tensor, layer: AttentionInputs, cache: KVCache, st
     if (layer.heads, layer.kv_heads, layer.head_dim) != (step.heads, step.kv_heads, step.head_dim):
         raise ValueError(f"[cached_attention] a layer of {layer.heads} and {layer.kv_heads} heads of {layer.head_dim}, but the step "
                          f"was made for {step.heads} and {step.kv_heads} heads of {step.head_dim}")
-    if step.plan is None:
-        raise ValueError("[cached_attention] the step has no plan: it was made with keep")
+    check_attention("cached_attention", cache, step, scale, ancestors)  # (nothing is stored for a step that is refused)
     q, k, v, gate = attention_inputs(x, layer, step.positions if positions is None else positions, adapters)
     store_kv_(k, v, cache, step.slots)
     return paged_attention(q, cache, step, scale=scale, ancestors=ancestors, gate=gate).reshape(len(x), layer.heads * layer.head_dim), k, v
