@@ -115,7 +115,9 @@ def step_tables_(lengths: torch.Tensor, block_table: torch.Tensor, free_pages: t
       requests, it takes pages for b + a tokens from the list's end. The tokens get positions b, b + 1, .. and their slots.
     A request whose tokens would not fit its row of block_table is refused (no row of it gets a place, its length becomes b);
     so is every request that needs pages, from the first on for which too few are left. base 0 and rows 0 release a request;
-    a tree verify stores all nodes, and then, with base the length before and `keep` the accepted nodes, these alone.
+    a tree verify stores all nodes, and then, with base the length before and `keep` the accepted nodes, these alone. A request
+    that was refused for all nodes may fit with the kept ones, which have attended to nothing: keep & (step.request >= 0) leaves
+    them out.
 
     lengths, rows, base int32 [R]; block_table int32 [R, capacity]; free_pages int32 [pages] (room for every page of the
     cache), the first free_count (int32 [1]) of which are free. Rows without a place (not kept, refused, padding) have -1 as

@@ -119,7 +119,8 @@ def cached_attention(x: torch.Tensor, layer: AttentionInputs, cache: KVCache, st
 
     positions: the step's by default (rows in a line); a tree's rows have that of their depth. ancestors as in
     paged_attention. k and v (M, kv_heads, D) are what was stored: once a tree's accepted nodes are known, a step of the
-    tables with base and keep gives their places in a line, and store_kv_(k, v, cache, step.slots) puts them there.
+    tables with base and keep gives their places in a line, and store_kv_(k, v, cache, step.slots) puts them there. Rows of a
+    request that the step refused (step.request < 0) are not stored and have an attention of zeros: they are not to be kept.
     """
     if x.dim() != 2:
         raise ValueError(f"[cached_attention] x must be (rows, K), got {tuple(x.shape)}")
