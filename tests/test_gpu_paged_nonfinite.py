@@ -121,3 +121,12 @@ def test_cut_and_whole_requests_agree_about_every_context():
     for r, c in enumerate(cached):
         poison_values(case, r, [64 + r // 2, 63] if r else [63])
     check(case, case.run())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_rows_of_prompts(dim):
+    """Several row blocks of a request, each of which ends in a stage of its own."""
+    case = Case([0, 100, 40], [300, 150, 90], 4, 2, dim, gated=True, seed=dim)
+    for r, (c, n) in enumerate(zip(case.cached, case.rows)):
+        poison_values(case, r, sorted({*interesting(c, n), *(t for t in (c + 63, c + 70, c + 130, c + 200) if t < c + n)}))
+    check(case, case.run())
