@@ -72,7 +72,7 @@ int qmm4_store_kv_bf16(const void* k, int64_t k_row, int64_t k_head, const void*
  * Rows that see nothing, and rows without a request, give zeros. What is not finite in a token that a row does not see does not
  * reach it. Products and sums are fp32, probabilities are rounded to bf16 for their product with the values (8 bits: with
  * the scale in them), the result is rounded once. No sum of finite values overflows, whatever their size; probabilities below
- * 2^-118 capacity page_size of a row's largest may count as zero.
+ * 2^-117 capacity page_size of a row's largest may count as zero.
  *   q, gate: bf16 with strides as for k above; out: bf16 [M, Hq, D] contiguous, overlapping no input; block_table, request,
  *   plan: those of qmm4_cache_step, made with the same R, total = M, heads, kv_heads, D and max_rows on this device;
  *   ancestors: int64 [M] or null. Requires D as above, Hq % Hk == 0, scale finite.

@@ -224,13 +224,12 @@ int qmm4_paged_attention_bf16(const void* q, int64_t q_row, int64_t q_head, cons
     if (int rc = shape_of(Hq, Hk, D, most, &s)) return rc;
     float* part = static_cast<float*>(workspace);
     const int64_t rows = qmm4::paged_partial_rows(s, R, most) * Hk;
-    const float tokens = (float)log2_of(capacity * page_size);
     const qmm4::PagedParams p{rows_of(q, q_row, q_head), rows_of(gate, gate_row, gate_head),
                               {const_cast<void*>(keys), const_cast<void*>(values), const_cast<float*>(key_scales),
                                const_cast<float*>(value_scales), pages, log2_of(page_size), (int)Hk},
                               block_table, request, {const_cast<int32_t*>(plan), (int)R}, ancestors,
-                              static_cast<uint16_t*>(out), part, part + rows * D, capacity, scale,
-                              qmm4::kPagedSlack + tokens, -tokens, s.G, (int)most, (int)(s.splits + R)};
+                              static_cast<uint16_t*>(out), part, part + rows * D, (int32_t)capacity, scale,
+                              (float)log2_of(capacity * page_size), s.G, (int)most, (int)(s.splits + R)};
     const hipError_t e = qmm4::launch_paged_attention(p, M, (int)D, bits == 8, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return hip_error(e, "paged attention kernel launch");
     return (int)QMM4_OK;

@@ -11,8 +11,8 @@
 // The running maximum moves only where a logit passes it by more than 2^8, so that most steps need no exchange between lanes. It
 // is held above the largest logit by those 2^8 and by the tokens that a request may have: all its probabilities together stay
 // below 1, and no sum of finite values overflows, whatever their size, nor does a probability times a scale of 8 bits. What this takes
-// is as many powers of two of how small a probability may be (2^-126). (Both bounds come with the call: the widest kernels have no
-// vector register for them.)
+// is as many powers of two of how small a probability may be (2^-126). (The bound on the tokens comes with the call: the widest kernels
+// have no vector register for a request's own.)
 #pragma once
 
 #include "qmm4_common.h"
@@ -219,15 +219,15 @@ struct PagedRows {
       top = max3(top, max3(e[qt][0], e[qt][1], e[qt][2]), max3(e[qt][3], e[qt][4], e[qt][5]));
       top = max3(top, e[qt][6], e[qt][7]);
     }
-    if (__any(top > S.enough)) {
+    if (__any(top > -S.tokens)) {
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
         float now = s[qt][0][0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) now = fmaxf(now, s[qt][j / 4][j % 4]);
-        now = __builtin_fmaf(now, unit, S.above);
+        now = __builtin_fmaf(now, unit, S.tokens);
         now = fmaxf(now, __shfl_xor(now, 16));
-        now = fmaxf(fmaxf(now, __shfl_xor(now, 32)), m[qt]);
+        now = fmaxf(fmaxf(now, __shfl_xor(now, 32)) + kPagedSlack, m[qt]);
         const float f = __builtin_amdgcn_exp2f(m[qt] - now);
         l[qt] *= f;
 #pragma unroll
