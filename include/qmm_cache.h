@@ -30,7 +30,8 @@ extern "C" {
 /*
  * One step of the tables. For request r of R, with page = page_size:
  *   b = base[r] (null: lengths[r]) within 0 .. lengths[r];   n = rows[r] within 0 .. max_rows, cut where the n so far reach
- *   `total`: the request's rows lie behind those of the requests before it;   a = n, or those of the n with keep != 0.
+ *   `total`: the request's rows lie behind the n of each request before it (so max_rows has to be at least every one's rows);
+ *   a = n, or those of the n with keep != 0.
  * Every request gives back its pages past ceil(b / page) (their entries of block_table become -1); then pages for
  * ceil((b + a) / page) are taken from the end of the free list in the order of requests, so that pages given back and taken
  * again by the same requests are the same ones. A request whose tokens would not fit its row of block_table is refused, and so

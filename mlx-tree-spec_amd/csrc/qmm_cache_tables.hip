@@ -8,7 +8,7 @@
 // latency: a chain of four prefix sums, and of two loads (the requests' numbers, then page numbers), which is why a row's page is
 // read from where this step finds it (the table, or the free list) and not out of the table behind its update, and why the
 // first page numbers are on their way while the plan is made.
-// 16 requests of one row: 5.9 us, of which an empty launch takes 1.8; 100 of 16 rows 7.9; 24 of 50000 rows 9.3, and 3.4 for the rows.
+// 16 requests of one row: 5.4 us, of which an empty launch takes 1.8; 100 of 16 rows 7.9; 24 of 50000 rows 9.4-10.3, and 3.3-4.0 for the rows.
 #include <hip/hip_runtime.h>
 
 #include "qmm_cache.h"

@@ -257,6 +257,8 @@ struct PagedRows {
           for (int j = 0; j < 8; ++j) e[qt][j] = sees(qt, t + 8 * g + j) ? e[qt][j] : 0.0f;
       }
     }
+    // (bf16, as the values are: the matrix instructions of 32 bits are a sixteenth as fast. Half a step each, 2^-8, beside a sum of them
+    // that stays in 32 bits: against 64 bits 1.3 to 1.4 times the error of products in fp32, whose result is rounded to bf16 as well.)
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       u32x4 w;

@@ -4,10 +4,11 @@
 //
 // This file: up to 16 query rows to a key head (decode) of heads up to 128 or 8 bits, the join of splits, and the choice. Every
 // byte of the cache is used once, for 16 rows at most: bound by HBM (64 requests of up to 16000 tokens, 8 key heads of 128, 2.4 GB:
-// 416 us, 5.8 TB/s; 16 of up to 40000 in 8 bits, 4 of 256: 133 us, 5.7 TB/s). A wave loads its operands from memory to registers,
+// 415 us, 5.8 TB/s; 16 of up to 40000 in 8 bits, 4 of 256: 140-144 us, 5.4 TB/s). A wave loads its operands from memory to registers,
 // 1 KB an instruction in whole runs of 64 bytes and more, without LDS, and takes every 8th step of its workgroup's split; while
 // a step's probabilities are made the next step's keys are on their way, and its values while the products with the present ones
-// run. Waves join through LDS, splits through memory (fp32) and a second kernel (4.7 us for 64 splits).
+// run. Waves join through LDS, splits through memory (fp32) and a second kernel (5.3 us for 64 splits of 24 heads of 256).
+// That one looks at every row and head, whether they were cut or not (a prompt of 4096 rows of 32 heads, which is not: 47 us of 420).
 #include <algorithm>
 #include <type_traits>
 

@@ -2,7 +2,7 @@
 // more (qmm_paged.h has the products and the softmax). Each byte of the cache serves up to 128 query rows of a workgroup: bound by
 // HBM up to some 64 rows (one row of 6 heads over 200000 tokens, 4 key heads of 256: 137 us, 6.0 TB/s), past that by the matrix
 // instructions and the softmax's vector instructions (64 nodes of 4 heads over 32000 tokens, 8 key heads of 128: 51.6 us, 650 TFLOP/s;
-// 1000 rows over 8000: 167 us, 830 TFLOP/s).
+// 1000 rows over 8000: 168 us, 830 TFLOP/s).
 //
 // A workgroup takes up to kPagedRows query rows of one key head over one split: 8 waves with 16 QT rows each, or with two SIDES
 // 4 of them on the even steps and the others with the same rows on the odd ones. The steps' keys and values go from memory to

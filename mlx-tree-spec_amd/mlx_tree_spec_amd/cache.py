@@ -107,7 +107,8 @@ def step_tables_(lengths: torch.Tensor, block_table: torch.Tensor, free_pages: t
                  rows: torch.Tensor, total: int, page_size: int, heads: int, kv_heads: int, head_dim: int,
                  base: torch.Tensor | None = None, keep: torch.Tensor | None = None, max_rows: int | None = None) -> CacheStep:
     """One step of the tables, in place, and the new rows' places. `total` rows are packed one request behind the other,
-    rows[r] of request r (none below 0, at most max_rows; those past `total` are cut off), padding behind the last.
+    rows[r] of request r (none below 0, at most max_rows; those past `total` are cut off), padding behind the last. max_rows has to
+    be at least the most rows of a request: a longer one is cut, and the next request's rows are taken to begin where it was cut.
 
     For each of R requests, with b = base[r] (by default its length; never more than that) and a = its rows, or with `keep`
     (bool [total]) those of them that are kept:
@@ -301,8 +302,8 @@ def paged_attention(q: torch.Tensor, cache: KVCache, step: CacheStep, scale: flo
         out[m, h] = softmax(scale * q[m, h] . keys of what the row sees) values  (* sigmoid(gate[m, h])),
 
     query head h over key head h // (Hq // Hk). A row sees every token before the step's, and of its request's rows those up
-    to its own; with `ancestors` (int64 [M], a tree's masks) row j of its request where bit j is set, itself included. Rows
-    that see nothing, and rows without a request, give zeros.
+    to its own; with `ancestors` (int64 [M], a tree's masks) row j of its request where bit j is set, itself included (the
+    64 rows that have a bit: those behind them are seen by none). Rows that see nothing, and rows without a request, give zeros.
 
     q and gate bf16 (M, Hq, D): projections, or views of one (strided rows and heads are read in place). scale: D ** -0.5 by
     default. step: of step_tables_ with as many rows, these heads and this cache's page size, without `keep`.
