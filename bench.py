@@ -14,6 +14,9 @@ TFLOP/s against MI355X peaks (8 TB/s; 2.5 PFLOP/s dense bf16). The `roofline` ob
 dominant kernel of the headline: algorithmic bytes per launch / mean launch duration, measured
 with per-launch HIP events on the launch stream in a second pass of K steps.
 
+The JSON line on stdout holds these; what else is measured (DETAIL) is a JSON line of its own on stderr before it, since a
+line of all of it, over 20 KB, does not survive in logs that keep the end of an output.
+
 cpu_baseline: the oracle's C restatement (OpenMP, fp32 accumulation) on the host cores, on a
 bounded, time-boxed sample of the same decode steps.
 """
@@ -87,6 +90,16 @@ DESCR = {
     "c3": "vocab head: x bf16 [32, 5120] @ packed 4-bit [151936, 5120]",
     "c4": "chunked prefill: x bf16 [4096, 5120] @ packed 4-bit [17408, 5120]",
 }
+
+
+# Measurements beside the headline and the workloads.
+DETAIL = ("mid_m", "model_linears", "fallback_kernels", "shard8", "fused")
+
+
+def emit(line: dict) -> None:
+    """The details to stderr, the headline to stdout, a JSON line each."""
+    log("[bench] detail " + json.dumps({k: line[k] for k in DETAIL if k in line}))
+    print(json.dumps({k: v for k, v in line.items() if k not in DETAIL}), flush=True)
 
 
 def log(msg: str) -> None:
@@ -740,7 +753,7 @@ def main() -> int:
     if not args.no_cpu:
         log("[bench] cpu baseline")
         line["cpu_baseline"] = cpu_baseline(wl.rows, wl.k, wl.n, args.cpu_seconds)
-    print(json.dumps(line), flush=True)
+    emit(line)
     return 0
 
 
